@@ -486,7 +486,7 @@ def _run_own(st):
     qs, ks, seqs = st["qs"].data_ptr(), st["ks"].data_ptr(), len(st["ql"])
     if case["kind"] == "select":
         if case["index"]:
-            s3dx.block_index(st["k"].data_ptr(), dt, st["k"].shape[0], case["kv"], d, ks, seqs, case["block"], st["rows_k"],
+            s3dx.block_index(st["k"].data_ptr(), dt, st["k"].shape[0], case["kv"], d, ks, seqs, case["block"],
                              st["codes"].data_ptr(), st["scale"].data_ptr(), k_stride=st["k"].stride(0), stream=stream)
         s3dx.block_select(st["q"].data_ptr(), dt, n, st["k"].shape[0], h, case["kv"], d, qs, ks, seqs, case["block"],
                           case["top"], st["rows_k"], st["codes"].data_ptr(), st["scale"].data_ptr(), st["selected"].data_ptr(),
