@@ -139,7 +139,7 @@ def _voxels(n, seed):
         xyz = np.argwhere(mask).astype(np.int32)
         parts.append(np.concatenate([np.full((xyz.shape[0], 1), b, np.int32), xyz], 1))
         have, b = have + xyz.shape[0], b + 1
-    return np.concatenate(parts, 0)[:n]
+    return np.ascontiguousarray(np.concatenate(parts, 0)[:n])
 
 
 def _gen(seed, tag):
