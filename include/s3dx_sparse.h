@@ -469,6 +469,131 @@ S3DX_API s3dx_status s3dx_convert(const void *x, int32_t x_dtype, int64_t count,
                                   int32_t y_dtype, s3dx_stream stream, char *error,
                                   uint64_t error_capacity);
 
+/* ------------------------------------------------------------------------
+ * Attention over voxel rows: what stands between the SLat flow's sparse
+ * input and output blocks (its transformer blocks over the coarse rows,
+ * slat_flow_graph.cpp:304-434) and in the decoders' windows
+ * (gs_decoder_graph.cpp:93-121), where the reference runs stock GGML
+ * attention (graph_builder.cpp:121-153).  Inference only, like the rest.
+ *
+ * Rows of heads: x[r][h][d] lies at x + r*stride + h*head_dim + d, strides in
+ * elements, so that the heads of a packed qkv projection are read where they
+ * are.  dtype S3DX_F32 or S3DX_BF16; sums, norms, softmax statistics and
+ * accumulators are float32 or wider.
+ *
+ * Sequences are packed: starts is a DEVICE int32 [sequences + 1], rising, and
+ * sequence s holds rows [starts[s], starts[s+1]); sequences may be empty, and
+ * rows behind the last one are neither read nor written.  Query i of a
+ * sequence of lq queries and lk keys stands at key place i + lk - lq (the
+ * last query at the last key).  Starts outside [0, total] are cut to it.
+ *
+ * Nothing here allocates device memory or synchronizes: the calls can be
+ * captured into a graph, and the buffers belong to the current device.  Zero
+ * rows are valid and do nothing.
+ * ---------------------------------------------------------------------- */
+
+/* Rotary positions with several axes, e.g. (x, y, z) of voxels or (time,
+ * height, width) of video.  Pair j turns by
+ * positions[row][host_axis[j]] * host_frequency[j] radians: (a, b) ->
+ * (a cos - b sin, a sin + b cos).  The usual choice is a geometric series for
+ * each axis, frequency base^(-j/m) for the j-th of the axis' m pairs; any
+ * other (one series over all pairs, axes taking turns) is a table as well.
+ * S3DX_ROTARY_ADJACENT pairs channels (2j, 2j+1), S3DX_ROTARY_HALVES (j,
+ * j + pairs); channels from 2*pairs on are not turned.  The angle is reduced
+ * to a part of a turn in 64-bit integers, so far positions (any int32) cost no
+ * accuracy.  Requires 1 <= head_dim <= 256, 1 <= axes <= 8,
+ * 1 <= pairs <= head_dim / 2, |frequency| <= 1e6.  The object is host memory
+ * alone and may be used by any number of calls at once. */
+#define S3DX_ROTARY_ADJACENT 0
+#define S3DX_ROTARY_HALVES 1
+typedef struct s3dx_rotary s3dx_rotary;
+S3DX_API s3dx_status s3dx_rotary_create(int32_t head_dim, int32_t axes, int32_t pairs, const int32_t *host_axis,
+                                        const double *host_frequency, int32_t pairing, s3dx_rotary **out,
+                                        char *error, uint64_t error_capacity);
+S3DX_API void s3dx_rotary_free(s3dx_rotary *rotary);
+/* y = x turned by its rows' positions; inverse 1 turns back (the transpose,
+ * hence also the gradient's way).  positions: int32, axis a of row r at
+ * positions[r*position_stride + a] (voxel coordinates: coords + 1, stride 4).
+ * y may be x with the same dtype and stride, and otherwise must not overlap it. */
+S3DX_API s3dx_status s3dx_rotary_apply(const s3dx_rotary *rotary, int32_t inverse, const void *x, int32_t x_dtype,
+                                       int64_t n, int32_t heads, int64_t x_stride, const int32_t *positions,
+                                       int64_t position_stride, void *y, int32_t y_dtype, int64_t y_stride,
+                                       s3dx_stream stream, char *error, uint64_t error_capacity);
+/* Queries and keys on their way to the attention, in one launch: every head's
+ * channels over their root mean square, x / sqrt(mean(x^2) + eps), times an
+ * optional gain (DEVICE float32: [heads][head_dim] with gain_per_head 1, else
+ * [head_dim], which all heads share), then turned as by s3dx_rotary_apply, rounded
+ * once.  rotary and positions NULL: the norm alone.  k NULL with k_heads 0:
+ * queries alone.  eps > 0.  Outputs alias inputs as in s3dx_rotary_apply. */
+S3DX_API s3dx_status s3dx_qk_norm_rotary(const s3dx_rotary *rotary, const int32_t *positions, int64_t position_stride,
+                                         const void *q, int32_t q_heads, int64_t q_stride, const float *q_gain,
+                                         const void *k, int32_t k_heads, int64_t k_stride, const float *k_gain,
+                                         int32_t gain_per_head, int32_t dtype, int64_t n, int32_t head_dim, float eps,
+                                         void *q_out, int64_t q_out_stride, void *k_out, int64_t k_out_stride,
+                                         int32_t out_dtype, s3dx_stream stream, char *error, uint64_t error_capacity);
+
+/* Attention over blocks that a cheap score selects for each query.
+ *
+ * Key block j of a sequence is its rows [j*block, (j+1)*block) (the last may be
+ * short); block is 32, 64 or 128, head_dim 32, 64, 96 or 128, heads a multiple
+ * of kv_heads (query head h reads key head h / (heads / kv_heads)); pointers
+ * 16-byte aligned, strides whole 16-byte pieces below 2^22 elements.
+ *
+ * The index holds each block's mean key in 8 bits: of the mean m (over the
+ * block's rows, in 64 bits), with 2^e <= max|m_d| < 2^(e+1), the codes
+ * round(m_d * 2^(6-e)), halves to even, cut to +-127, and the scale 2^(e-6).
+ * Largest values below 2^-100 and rows with a NaN or an infinity get codes
+ * and scale 0.  Sequence s' block j is index row starts[s]/block + s + j of
+ * s3dx_block_index_rows rows; rows between are left as they are.
+ *   codes  int8 [kv_heads][rows][head_dim], 16-byte aligned
+ *   scale  float32 [kv_heads][rows] */
+#define S3DX_BLOCK_CAUSAL 1 /* a query sees the keys up to its own place */
+#define S3DX_BLOCK_NEAR 2   /* selection: the block at the query's own place always is one of the chosen */
+S3DX_API s3dx_status s3dx_block_index_rows(int64_t total_k, int64_t sequences, int32_t block, int64_t *rows,
+                                           char *error, uint64_t error_capacity);
+S3DX_API s3dx_status s3dx_block_index(const void *k, int32_t dtype, int64_t total_k, int32_t kv_heads, int32_t head_dim,
+                                      int64_t k_stride, const int32_t *k_starts, int64_t sequences, int32_t block,
+                                      int8_t *codes, float *scale, s3dx_stream stream, char *error,
+                                      uint64_t error_capacity);
+/* The best `top` blocks (1 to 4096) of each query row and key head, into
+ * selected int32 [total_q][kv_heads][top], ascending, -1 behind the last.  A
+ * block's score is the integer product of its codes with the codes of the
+ * query (the sum of the heads that share the key head, in 64 bits, coded in the
+ * same way), times its scale: exact, so the choice depends on no order of
+ * sums; equal scores go to the lower block.  With S3DX_BLOCK_CAUSAL blocks
+ * that begin behind the query's place are not chosen.  max_k: at least the keys of
+ * the longest sequence, at most 32768 * block; blocks behind it are not looked at. */
+S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t total_q, int64_t total_k, int32_t heads,
+                                       int32_t kv_heads, int32_t head_dim, int64_t q_stride, const int32_t *q_starts,
+                                       const int32_t *k_starts, int64_t sequences, int32_t block, int32_t top,
+                                       int64_t max_k, const int8_t *codes, const float *scale, int32_t flags,
+                                       int32_t *selected, s3dx_stream stream, char *error, uint64_t error_capacity);
+/* o = softmax(softmax_scale * q k^T) v over the keys of each row's chosen blocks
+ * (selected as above; any order, entries outside the sequence's blocks count
+ * for nothing, a block that stands twice counts twice), or over all keys of
+ * its sequence where selected is NULL and top 0.  o [total_q][heads][head_dim] in
+ * dtype by o_stride; lse (may be NULL): float32 [total_q][heads], the natural
+ * logarithm of the row's sum of exp(score).  A row that sees no key, or only
+ * scores of -inf, gets zeros and lse -inf; keys and values that a row does not
+ * see do not reach it, whatever they hold.  BF16 weights are rounded to bfloat16
+ * before they meet the values, FP32 ones are not.  Rows whose result is not
+ * finite are computed a second time key by key, more slowly.
+ * The workspace holds partial results where there are too few rows to fill the GPU
+ * (s3dx_block_attention_workspace_size, 0 bytes where none are needed); the
+ * pieces are joined in a fixed order: results are deterministic. */
+S3DX_API s3dx_status s3dx_block_attention_workspace_size(int64_t total_q, int32_t heads, int32_t kv_heads,
+                                                         int32_t head_dim, int64_t sequences, int32_t block,
+                                                         int32_t top, int64_t max_k, uint64_t *bytes, char *error,
+                                                         uint64_t error_capacity);
+S3DX_API s3dx_status s3dx_block_attention(const void *q, const void *k, const void *v, int32_t dtype, int64_t total_q,
+                                          int64_t total_k, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                          int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                          const int32_t *q_starts, const int32_t *k_starts, int64_t sequences,
+                                          int32_t block, int64_t max_k, const int32_t *selected, int32_t top,
+                                          float softmax_scale, int32_t flags, void *o, int64_t o_stride, float *lse,
+                                          void *workspace, uint64_t workspace_bytes, s3dx_stream stream, char *error,
+                                          uint64_t error_capacity);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,8 @@ operator interface for this path:
   MeshSubdivideTables.build(parents)   sparse_ops.hpp:77
   SparseConv(...).run(...)             slat_flow_graph.cpp:112-155 conv lambda,
                                        mesh_decoder_graph.cpp:81-103 convolution
+  Rotary, qk_norm_rotary, block_*      the attention over voxel rows between
+                                       the sparse blocks (slat_flow_graph.cpp:304-434)
 
 Device memory is plain device pointers owned by DeviceArray.  There is no
 fallback: if the HIP library cannot be loaded, import fails loudly.
@@ -29,6 +31,10 @@ F32 = 0
 BF16 = 1
 WEIGHT_SLAT = 0
 WEIGHT_MESH = 1
+ROTARY_ADJACENT = 0
+ROTARY_HALVES = 1
+BLOCK_CAUSAL = 1
+BLOCK_NEAR = 2
 
 OK, INVALID_ARGUMENT, OUT_OF_MEMORY, INTERNAL_ERROR = 0, 1, 2, 3
 
@@ -98,6 +104,19 @@ SIGNATURES = {
     "s3dx_upsample_nearest": (_u32, [_vp, _i32, _i64, _i32, _vp, _i64, _vp, _vp], True),
     "s3dx_concat_rows": (_u32, [_vp, _i32, _vp, _i32, _i32, _i64, _vp, _i64, _vp, _vp], True),
     "s3dx_convert": (_u32, [_vp, _i32, _i64, _vp, _i32, _vp], True),
+    "s3dx_rotary_create": (_u32, [_i32, _i32, _i32, _vp, _vp, _i32, C.POINTER(_vp)], True),
+    "s3dx_rotary_free": (None, [_vp], False),
+    "s3dx_rotary_apply": (_u32, [_vp, _i32, _vp, _i32, _i64, _i32, _i64, _vp, _i64, _vp, _i32, _i64, _vp], True),
+    "s3dx_qk_norm_rotary": (_u32, [_vp, _vp, _i64, _vp, _i32, _i64, _vp, _vp, _i32, _i64, _vp, _i32, _i32, _i64, _i32,
+                                   _f32, _vp, _i64, _vp, _i64, _i32, _vp], True),
+    "s3dx_block_index_rows": (_u32, [_i64, _i64, _i32, C.POINTER(_i64)], True),
+    "s3dx_block_index": (_u32, [_vp, _i32, _i64, _i32, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _vp], True),
+    "s3dx_block_select": (_u32, [_vp, _i32, _i64, _i64, _i32, _i32, _i32, _i64, _vp, _vp, _i64, _i32, _i32, _i64, _vp,
+                                 _vp, _i32, _vp, _vp], True),
+    "s3dx_block_attention_workspace_size": (_u32, [_i64, _i32, _i32, _i32, _i64, _i32, _i32, _i64, C.POINTER(_u64)],
+                                            True),
+    "s3dx_block_attention": (_u32, [_vp, _vp, _vp, _i32, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _vp, _vp, _i64,
+                                    _i32, _i64, _vp, _i32, _f32, _i32, _vp, _i64, _vp, _vp, _u64, _vp], True),
 }
 
 _lib = None
@@ -622,6 +641,110 @@ def concat_rows(a, ca, b, cb, dtype, n_src, rows, n, y, stream=None):
 
 def convert(x, x_dtype, count, y, y_dtype, stream=None):
     call("s3dx_convert", _dptr(x), _i32(x_dtype), _i64(count), _dptr(y), _i32(y_dtype), _sptr(stream))
+
+
+# ---------------------------------------------------------------------------
+# Attention over voxel rows
+# ---------------------------------------------------------------------------
+class Rotary:
+    """Rotary positions with several axes (s3dx_rotary): pair j turns by
+    position[axis[j]] * frequency[j] radians."""
+
+    def __init__(self, head_dim: int, axis, frequency, axes: int = None, pairing: int = ROTARY_ADJACENT):
+        self.handle = None
+        ax = np.ascontiguousarray(axis, dtype=np.int32)
+        fr = np.ascontiguousarray(frequency, dtype=np.float64)
+        if ax.ndim != 1 or ax.shape != fr.shape:
+            raise ValueError("axis and frequency are lists of the same length")
+        self.axes = axes if axes is not None else (int(ax.max()) + 1 if ax.size else 0)
+        p = _vp()
+        call("s3dx_rotary_create", _i32(head_dim), _i32(self.axes), _i32(ax.size), ax.ctypes.data_as(_vp),
+             fr.ctypes.data_as(_vp), _i32(pairing), C.byref(p))
+        self.handle = p.value
+        self.head_dim, self.pairs, self.pairing = head_dim, int(ax.size), pairing
+
+    @classmethod
+    def per_axis(cls, head_dim: int, sections, base: float = 10000.0, pairing: int = ROTARY_ADJACENT) -> "Rotary":
+        """sections[a] pairs for axis a, each axis its own series base^(-j/sections[a])."""
+        return cls(head_dim, [a for a, m in enumerate(sections) for _ in range(m)],
+                   [base ** (-j / m) for m in sections for j in range(m)], len(sections), pairing)
+
+    def apply(self, x, dtype, n, heads, positions, y=None, position_stride=None, inverse=False, x_stride=None,
+              y_dtype=None, y_stride=None, stream=None):
+        """y (default: x itself) = x turned by positions, back with inverse (s3dx_rotary_apply)."""
+        row = heads * self.head_dim
+        xs = row if x_stride is None else x_stride
+        ys = y_stride if y_stride is not None else (xs if y is None else row)
+        call("s3dx_rotary_apply", self.handle, int(inverse), _dptr(x), dtype, n, heads, xs, _dptr(positions),
+             self.axes if position_stride is None else position_stride, _dptr(x if y is None else y),
+             dtype if y_dtype is None else y_dtype, ys, _sptr(stream))
+
+    def __del__(self):
+        try:
+            if self.handle:
+                lib().s3dx_rotary_free(_vp(self.handle))
+        except Exception:
+            pass
+
+
+def qk_norm_rotary(q, k, dtype, n, q_heads, k_heads, head_dim, eps, q_out=None, k_out=None, rotary: Rotary = None,
+                   positions=None, position_stride=None, q_gain=None, k_gain=None, gain_per_head=True, q_stride=None,
+                   k_stride=None, q_out_stride=None, k_out_stride=None, out_dtype=None, stream=None):
+    """Per-head RMS norms of q and k and their rotation in one pass (s3dx_qk_norm_rotary);
+    without q_out / k_out in place."""
+    qs, ks = q_heads * head_dim if q_stride is None else q_stride, k_heads * head_dim if k_stride is None else k_stride
+    qo = q_out_stride if q_out_stride is not None else (qs if q_out is None else q_heads * head_dim)
+    ko = k_out_stride if k_out_stride is not None else (ks if k_out is None else k_heads * head_dim)
+    ps = position_stride if position_stride is not None else (rotary.axes if rotary is not None else 0)
+    call("s3dx_qk_norm_rotary", rotary.handle if rotary is not None else None, _dptr(positions), ps, _dptr(q), q_heads,
+         qs, _dptr(q_gain), _dptr(k), k_heads, ks, _dptr(k_gain), int(gain_per_head), dtype, n, head_dim, eps,
+         _dptr(q if q_out is None else q_out), qo, _dptr(k if k_out is None else k_out), ko,
+         dtype if out_dtype is None else out_dtype, _sptr(stream))
+
+
+def block_index_rows(total_k: int, sequences: int, block: int) -> int:
+    rows = _i64(0)
+    call("s3dx_block_index_rows", total_k, sequences, block, C.byref(rows))
+    return int(rows.value)
+
+
+def block_index(k, dtype, total_k, kv_heads, head_dim, k_starts, sequences, block, codes, scale, k_stride=None,
+                stream=None):
+    """The 8-bit index of the key blocks' means (s3dx_block_index)."""
+    call("s3dx_block_index", _dptr(k), dtype, total_k, kv_heads, head_dim,
+         kv_heads * head_dim if k_stride is None else k_stride, _dptr(k_starts), sequences, block, _dptr(codes),
+         _dptr(scale), _sptr(stream))
+
+
+def block_select(q, dtype, total_q, total_k, heads, kv_heads, head_dim, q_starts, k_starts, sequences, block, top, max_k,
+                 codes, scale, selected, q_stride=None, causal=False, near=False, stream=None):
+    """The `top` best key blocks of each query row and key head (s3dx_block_select)."""
+    call("s3dx_block_select", _dptr(q), dtype, total_q, total_k, heads, kv_heads, head_dim,
+         heads * head_dim if q_stride is None else q_stride, _dptr(q_starts), _dptr(k_starts), sequences, block, top,
+         max_k, _dptr(codes), _dptr(scale), (BLOCK_CAUSAL if causal else 0) | (BLOCK_NEAR if near else 0),
+         _dptr(selected), _sptr(stream))
+
+
+def block_attention_workspace_size(total_q, heads, kv_heads, head_dim, sequences, block, top, max_k) -> int:
+    b = _u64(0)
+    call("s3dx_block_attention_workspace_size", total_q, heads, kv_heads, head_dim, sequences, block, top, max_k,
+         C.byref(b))
+    return int(b.value)
+
+
+def block_attention(q, k, v, dtype, total_q, total_k, heads, kv_heads, head_dim, q_starts, k_starts, sequences, block,
+                    max_k, o, lse=None, selected=None, top=0, q_stride=None, k_stride=None, v_stride=None, o_stride=None,
+                    scale=None, causal=False, workspace=None, workspace_bytes=None, stream=None):
+    """softmax(scale q k^T) v over the selected blocks, or all keys of each sequence (s3dx_block_attention);
+    scale: head_dim^-0.5 unless given."""
+    if workspace_bytes is None:
+        workspace_bytes = workspace.nbytes if isinstance(workspace, DeviceArray) else 0
+    call("s3dx_block_attention", _dptr(q), _dptr(k), _dptr(v), dtype, total_q, total_k, heads, kv_heads, head_dim,
+         heads * head_dim if q_stride is None else q_stride, kv_heads * head_dim if k_stride is None else k_stride,
+         kv_heads * head_dim if v_stride is None else v_stride, _dptr(q_starts), _dptr(k_starts), sequences, block, max_k,
+         _dptr(selected), top, head_dim ** -0.5 if scale is None else scale, BLOCK_CAUSAL if causal else 0, _dptr(o),
+         heads * head_dim if o_stride is None else o_stride, _dptr(lse), _dptr(workspace), workspace_bytes,
+         _sptr(stream))
 
 
 def synchronize(stream=None):

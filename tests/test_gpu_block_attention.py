@@ -1,0 +1,463 @@
+"""GPU: the 8-bit block index, the selection (both exact) and the attention over
+selected blocks or all keys, against 64-bit references."""
+import numpy as np
+import pytest
+
+import attention_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+def starts(s3dx, lens):
+    return R.dev(s3dx, np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+
+
+def rows(rng, n, heads, d, scale=1.0):
+    return (rng.standard_normal((n, heads, d)) * scale).astype(np.float32)
+
+
+def wide(s3dx, a, dtype, pad):
+    """Rows of heads with `pad` elements behind each (NaN, which nothing may read), and their values and stride."""
+    n, h, d = a.shape
+    w = np.full((n, h * d + pad), np.nan, np.float32)
+    w[:, : h * d] = a.reshape(n, -1)
+    st, v = R.stored(s3dx, w, dtype)
+    return R.dev(s3dx, st), v[:, : h * d].reshape(n, h, d), h * d + pad
+
+
+# ---------------------------------------------------------------------------
+# Index
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("lens,kv,d,block,pad", [
+    ([1], 1, 32, 32, 0), ([200], 3, 64, 64, 64), ([0, 65, 0, 1, 64, 130, 0], 2, 128, 64, 0), ([1000, 31], 4, 96, 128, 8),
+    ([33, 32, 31], 5, 32, 32, 16), ([5000], 16, 64, 64, 0)])
+def test_block_index(s3dx, dtype, lens, kv, d, block, pad):
+    rng = np.random.default_rng(sum(lens) + d)
+    total = sum(lens)
+    k = rows(rng, total + 3, kv, d) * np.exp(3 * rng.standard_normal((total + 3, kv, 1))).astype(np.float32)
+    dk, kv64, stride = wide(s3dx, k, dtype, pad)
+    n = s3dx.block_index_rows(total, len(lens), block)
+    codes, scale = R.filled(s3dx, (kv, n, d), np.int8, 0x5A), R.filled(s3dx, (kv, n), np.float32, 0x5A)
+    s3dx.block_index(dk, dtype, total, kv, d, starts(s3dx, lens), len(lens), block, codes, scale, k_stride=stride)
+    want, power, used = R.index_of(kv64[:total], lens, block)
+    c, s = codes.download(), scale.download()
+    assert np.array_equal(c[:, used], want[:, used]) and np.array_equal(s[:, used], power[:, used].astype(np.float32))
+    assert np.all(c[:, ~used] == 0x5A) and np.all(np.ascontiguousarray(s[:, ~used]).view(np.uint8) == 0x5A)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_block_index_of_what_has_no_codes(s3dx, dtype):
+    # zeros, values too small, NaN and infinities: codes and scale 0, their neighbours untouched by them; halves round to even
+    rng = np.random.default_rng(2)
+    kv, d, block = 2, 64, 32
+    k = rows(rng, 32 * 7, kv, d)
+    k[0:32] = 0.0
+    k[32:64] = 2.0 ** -110
+    k[70, 0, 5] = np.nan
+    k[100, 1, 63] = -np.inf
+    k[128:160] = 0.0
+    k[128:160, :, 0], k[128:160, :, 1], k[128:160, :, 2] = 64.0, 2.5, -3.5   # e = 6: codes 64, 2, -4
+    k[160:192] = 1.9921875 * 2.0 ** 40                                       # 127.5: cut to 127
+    dk, v, _ = wide(s3dx, k, dtype, 0)
+    n = s3dx.block_index_rows(k.shape[0], 1, block)
+    codes, scale = R.filled(s3dx, (kv, n, d), np.int8, 0), R.filled(s3dx, (kv, n), np.float32, 0)
+    s3dx.block_index(dk, dtype, k.shape[0], kv, d, starts(s3dx, [k.shape[0]]), 1, block, codes, scale)
+    with np.errstate(invalid="ignore"):
+        want, power, _ = R.index_of(v, [k.shape[0]], block)
+    c, s = codes.download(), scale.download()
+    assert np.array_equal(c, want) and np.array_equal(s, power.astype(np.float32))
+    assert not c[:, 0:2].any() and not c[0, 2].any() and c[1, 2].any() and not c[1, 3].any() and c[0, 3].any()
+    assert c[0, 4, :3].tolist() == [64, 2, -4] and s[0, 4] == 1.0 and np.all(c[:, 5] == 127)
+
+
+# ---------------------------------------------------------------------------
+# Selection
+# ---------------------------------------------------------------------------
+def run_select(s3dx, q, k, dtype, ql, kl, block, top, causal, near, pad=0):
+    (heads, d), kv = q.shape[1:], k.shape[1]
+    dq, q64, qst = wide(s3dx, q, dtype, pad)
+    dk, k64, kst = wide(s3dx, k, dtype, pad)
+    total_q, total_k = sum(ql), sum(kl)
+    codes, scale, _ = R.index_of(k64[:total_k], kl, block)
+    n = codes.shape[1]
+    dc, ds = s3dx.DeviceArray((kv, n, d), np.int8), s3dx.DeviceArray((kv, n), np.float32)
+    ks, qs = starts(s3dx, kl), starts(s3dx, ql)
+    s3dx.block_index(dk, dtype, total_k, kv, d, ks, len(kl), block, dc, ds, k_stride=kst)
+    out = R.filled(s3dx, (q.shape[0], kv, top), np.int32, 0x5A)
+    s3dx.block_select(dq, dtype, total_q, total_k, heads, kv, d, qs, ks, len(kl), block, top, max(kl), dc, ds, out, q_stride=qst,
+                      causal=causal, near=near)
+    got = out.download()
+    assert np.all(got[total_q:] == 0x5A5A5A5A)
+    return got[:total_q], R.select(q64[:total_q], codes, scale, ql, kl, block, top, causal, near)
+
+
+SELECT = [
+    # ql, kl, heads, kv, d, block, top, causal, near
+    ([1], [1], 1, 1, 64, 64, 1, False, False),
+    ([100], [100], 4, 4, 64, 32, 3, False, True),
+    ([300], [300], 6, 2, 32, 32, 4, True, True),
+    ([70, 0, 1, 130], [70, 0, 1, 130], 8, 8, 128, 64, 2, True, False),
+    ([5, 3, 0], [400, 0, 50], 10, 2, 96, 32, 5, True, True),        # keys without queries and the reverse
+    ([40], [20], 2, 1, 64, 32, 3, True, True),                      # queries before the first key see nothing
+    ([1, 1, 1], [3000, 1, 777], 16, 2, 64, 64, 8, True, True),      # one new row each
+    ([33], [500], 5, 1, 64, 32, 40, False, False),                  # more than there are
+    ([260], [260], 2, 2, 64, 128, 1, False, True),
+    ([17], [6000], 3, 3, 64, 32, 20, False, False),                 # 188 blocks
+]
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("case", range(len(SELECT)))
+def test_block_select(s3dx, dtype, case):
+    ql, kl, heads, kv, d, block, top, causal, near = SELECT[case]
+    rng = np.random.default_rng(case)
+    got, want = run_select(s3dx, rows(rng, sum(ql) + 2, heads, d), rows(rng, sum(kl) + 2, kv, d), dtype, ql, kl, block, top, causal,
+                           near, pad=16)
+    assert np.array_equal(got, want)
+
+
+def test_block_select_long(s3dx):
+    # more blocks than a workgroup's usual share: 2,500 and 20,000 of them
+    rng = np.random.default_rng(3)
+    for lk, n in ((80_000, 3), (640_000, 1)):
+        print(f"select over {lk} keys", flush=True)
+        got, want = run_select(s3dx, rows(rng, n, 4, 32), rows(rng, lk, 2, 32), s3dx.BF16, [n], [lk], 32, 300, True, True)
+        assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("top", [1, 5, 7, 4096])
+def test_block_select_ties_go_to_the_lower_block(s3dx, top):
+    # equal blocks, blocks without codes (score 0) and a query of zeros
+    rng = np.random.default_rng(4)
+    q, k = rows(rng, 40, 2, 64), np.tile(rows(rng, 32, 2, 64), (9, 1, 1))
+    k[64:96] = 0.0
+    k[130, 0, 3] = np.nan
+    k[190] *= 3.0
+    q[7] = 0.0
+    q[9, :, 5] = np.nan
+    with np.errstate(invalid="ignore"):
+        got, want = run_select(s3dx, q, k, s3dx.F32, [40], [288], 32, top, False, False)
+    assert np.array_equal(got, want)
+    assert got[7, 0, : min(top, 9)].tolist() == list(range(min(top, 9)))
+
+
+def test_block_select_looks_at_no_block_behind_max_k(s3dx):
+    rng = np.random.default_rng(5)
+    k, q = rows(rng, 640, 1, 64), rows(rng, 10, 1, 64)
+    dk, k64, _ = wide(s3dx, k, s3dx.F32, 0)
+    n = s3dx.block_index_rows(640, 1, 64)
+    dc, ds = s3dx.DeviceArray((1, n, 64), np.int8), s3dx.DeviceArray((1, n), np.float32)
+    ks, qs = starts(s3dx, [640]), starts(s3dx, [10])
+    s3dx.block_index(dk, s3dx.F32, 640, 1, 64, ks, 1, 64, dc, ds)
+    out = s3dx.DeviceArray((10, 1, 12), np.int32)
+    s3dx.block_select(R.dev(s3dx, q), s3dx.F32, 10, 640, 1, 1, 64, qs, ks, 1, 64, 12, 200, dc, ds, out)
+    assert np.array_equal(out.download()[:, 0], np.tile([0, 1, 2, 3] + [-1] * 8, (10, 1)))
+    s3dx.block_select(R.dev(s3dx, q), s3dx.F32, 10, 640, 1, 1, 64, qs, ks, 1, 64, 12, 0, dc, ds, out)
+    assert np.all(out.download() == -1)
+
+
+# ---------------------------------------------------------------------------
+# Attention
+# ---------------------------------------------------------------------------
+def choose(rng, ql, kl, kv, block, top):
+    """A random choice, ascending, some rows' shorter than others and some empty."""
+    out = np.full((sum(ql), kv, top), -1, np.int32)
+    at = 0
+    for lq, lk in zip(ql, kl):
+        nb = -(-lk // block)
+        for i in range(lq):
+            for h in range(kv):
+                take = min(nb, int(rng.integers(0, top + 1)) if rng.random() < 0.2 else top)
+                out[at + i, h, :take] = np.sort(rng.permutation(nb)[:take])
+        at += lq
+    return out
+
+
+def run_attend(s3dx, q, k, v, dtype, ql, kl, block, selected=None, causal=False, scale=None, pad=0, behind=0, stream=None):
+    """The call's o and lse with the references and bounds; `behind`: rows behind the last sequence."""
+    heads, d = q.shape[1:]
+    kv = k.shape[1]
+    tq, tk = sum(ql) + behind, sum(kl) + behind
+    (dq, q64, qst), (dk, k64, kst), (dv, v64, vst) = (wide(s3dx, a, dtype, pad) for a in (q, k, v))
+    ost = heads * d + pad
+    o = R.filled(s3dx, (tq, ost), R.store_type(s3dx, dtype), 0x5A)
+    lse = R.filled(s3dx, (tq, heads), np.float32, 0x5A)
+    top = 0 if selected is None else selected.shape[2]
+    if top and behind:
+        selected = np.concatenate([selected, np.zeros((behind, kv, top), np.int32)])
+    ds = None if selected is None else R.dev(s3dx, selected)
+    ws = R.filled(s3dx, max(1, s3dx.block_attention_workspace_size(tq, heads, kv, d, len(ql), block, top, max(kl))), np.uint8, 0xFF)
+    qs, ks = starts(s3dx, ql), starts(s3dx, kl)
+    s3dx.block_attention(dq, dk, dv, dtype, tq, tk, heads, kv, d, qs, ks, len(ql), block, max(kl), o, lse, ds, top, qst, kst, vst,
+                         ost, scale, causal, ws, stream=stream)
+    if stream is not None:
+        stream.synchronize()
+    n = sum(ql)
+    got, g_lse = R.values(s3dx, o, dtype), lse.download()
+    assert np.all(o.download()[n:].view(np.uint8) == 0x5A) and np.all(g_lse[n:].view(np.uint8) == 0x5A)
+    assert np.all(np.ascontiguousarray(o.download()[:, heads * d:]).view(np.uint8) == 0x5A)
+    want = R.attend(q64[:n], k64[: sum(kl)], v64[: sum(kl)], ql, kl, block, selected, d ** -0.5 if scale is None else scale, causal,
+                    dtype == s3dx.BF16)
+    return got[:n, : heads * d].reshape(n, heads, d), g_lse[:n].astype(np.float64), want
+
+
+def check(s3dx, dtype, got, lse, want, what=""):
+    o, l, off, l_off = want
+    fine = np.isfinite(o)
+    assert np.array_equal(np.isnan(got), np.isnan(o)) and np.array_equal(got[~fine & ~np.isnan(o)], o[~fine & ~np.isnan(o)]), what
+    err = np.abs(got - o)[fine]
+    bound = (off + R.half_step(s3dx, dtype) * (np.abs(o) + off))[fine]
+    rel = float(np.linalg.norm(err) / max(np.linalg.norm(o[fine]), 1e-30))
+    print(f"  {what} worst share of the bound {np.max(err / np.maximum(bound, 1e-37), initial=0):.3f}, rel-L2 {rel:.2e}", flush=True)
+    assert np.all(err <= bound + 1e-37), what
+    # Over many elements the errors do not all reach their bounds: rounding to bfloat16 is off by 2^-8 / sqrt(3) of the
+    # value at most in the mean square, once for the weights and once for the output.  A key left out of a few hundred shows.
+    if dtype == s3dx.BF16 and err.size > 2000:
+        assert rel <= 2 * R.UBF / np.sqrt(3) * 1.5, (what, rel)
+    fine = np.isfinite(l)
+    assert np.array_equal(lse[~fine & ~np.isnan(l)], l[~fine & ~np.isnan(l)]) and np.array_equal(np.isnan(lse), np.isnan(l)), what
+    assert np.all(np.abs(lse - l)[fine] <= l_off[fine] + R.U32 * np.abs(l[fine])), what
+
+
+ATTEND = [
+    # ql, kl, heads, kv, d, block, top (0: all), causal
+    ([1], [1], 1, 1, 64, 64, 0, False),
+    ([1], [1], 2, 2, 128, 32, 1, True),
+    ([100], [100], 3, 3, 64, 64, 0, False),
+    ([257], [257], 2, 2, 64, 64, 0, True),
+    ([90], [130], 2, 2, 32, 32, 0, False),
+    ([65], [200], 4, 4, 96, 128, 0, True),
+    ([200], [330], 4, 2, 128, 64, 0, True),
+    ([37, 0, 1, 64, 33, 5], [37, 0, 1, 64, 33, 5], 2, 2, 64, 64, 0, False),   # windows
+    ([17, 3, 0, 40], [5, 0, 50, 90], 3, 1, 64, 32, 0, True),                  # more queries than keys, none of either
+    ([150], [150], 4, 4, 64, 32, 2, False),
+    ([300], [300], 2, 2, 64, 64, 3, True),
+    ([129], [500], 5, 1, 64, 32, 4, False),      # five heads on a key head: rows of a tile are not whole groups
+    ([100], [400], 8, 2, 128, 64, 3, True),
+    ([80], [513], 16, 1, 96, 128, 2, True),
+    ([40], [256], 40, 1, 64, 64, 2, False),      # a group that is wider than a tile
+    ([60, 1, 0, 90], [60, 300, 33, 90], 6, 3, 32, 32, 2, True),
+    ([1, 1, 1], [3000, 1, 900], 8, 2, 128, 64, 12, True),    # one new row each
+    ([1, 1], [2500, 64], 12, 12, 64, 64, 0, True),           # ... over everything
+    ([2], [4000], 4, 4, 64, 128, 0, False),
+    ([3], [2000], 4, 1, 64, 32, 30, True),
+]
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("case", range(len(ATTEND)))
+def test_block_attention(s3dx, dtype, case):
+    ql, kl, heads, kv, d, block, top, causal = ATTEND[case]
+    rng = np.random.default_rng(100 + case)
+    q, k, v = rows(rng, sum(ql) + 3, heads, d, 1.5), rows(rng, sum(kl) + 3, kv, d), rows(rng, sum(kl) + 3, kv, d)
+    sel = choose(rng, ql, kl, kv, block, top) if top else None
+    got, lse, want = run_attend(s3dx, q, k, v, dtype, ql, kl, block, sel, causal, pad=24 if case % 2 else 0, behind=3)
+    check(s3dx, dtype, got, lse, want, f"case {case}")
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_lists_in_any_order(s3dx, dtype):
+    # unsorted, with blocks twice (they count twice) and entries that name no block
+    rng = np.random.default_rng(7)
+    q, k, v = rows(rng, 70, 2, 64), rows(rng, 300, 2, 64), rows(rng, 300, 2, 64)
+    sel = rng.integers(-3, 14, (70, 2, 9)).astype(np.int32)   # 10 blocks of 32
+    sel[5] = -1
+    sel[6], sel[7] = 2 ** 31 - 1, -2 ** 31
+    sel[8] = 3
+    got, lse, want = run_attend(s3dx, q, k, v, dtype, [70], [300], 32, sel)
+    check(s3dx, dtype, got, lse, want)
+    assert np.all(got[5:8] == 0) and np.all(lse[5:8] == -np.inf)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n,lk,top,late", [(90, 200, 2, 0), (1, 1500, 9, 0), (70, 200, 0, 0), (70, 200, 0, 130)])
+def test_what_a_row_does_not_see_does_not_reach_it(s3dx, dtype, n, lk, top, late):
+    rng = np.random.default_rng(n)
+    q, k, v = rows(rng, n, 4, 64), rows(rng, lk, 2, 64), rows(rng, lk, 2, 64)
+    sel = choose(rng, [n], [lk], 2, 32, top) if top else None
+    # with all keys and without `late` every row sees the first of them
+    bad = [late + 1, late + 40, lk - n + 1 + late // 6, lk - 2] if n > 1 else [33, 700, 1400]
+    if n == 1:
+        sel[sel == 1] = 2
+        sel[(sel == 700 // 32) | (sel == 1400 // 32)] = 5
+    for j, what in zip(bad, (np.nan, np.inf, -np.inf, np.nan)):
+        v[j, :, 3:9], k[j, 1] = what, what
+    with np.errstate(invalid="ignore"):
+        got, lse, want = run_attend(s3dx, q, k, v, dtype, [n], [lk], 32, sel, causal=True)
+    print("rows with NaN:", int(np.isnan(want[0]).any(-1).sum()), "of", want[0].shape[0] * 4, flush=True)
+    assert np.isfinite(want[0]).all(-1).any() or not (top or late)
+    check(s3dx, dtype, got, lse, want)
+
+
+def test_scores_of_any_size(s3dx):
+    # scores of thousands (one key takes all), of the type's lowest value, and infinities
+    rng = np.random.default_rng(12)
+    q, k, v = rows(rng, 40, 1, 64, 40.0), rows(rng, 150, 1, 64, 40.0), rows(rng, 150, 1, 64)
+    got, lse, want = run_attend(s3dx, q, k, v, s3dx.F32, [40], [150], 64)
+    check(s3dx, s3dx.F32, got, lse, want, "large")
+    q[:, :, :], k[:, :, :] = 1.0, 0.0
+    k[:150, 0, 0] = -3e38
+    got, lse, want = run_attend(s3dx, q, k, v, s3dx.F32, [40], [150], 64, scale=1.0)
+    check(s3dx, s3dx.F32, got, lse, want, "lowest")
+    k[:150, 0, 0] = -np.inf
+    got, lse, want = run_attend(s3dx, q, k, v, s3dx.F32, [40], [150], 64, scale=1.0)
+    check(s3dx, s3dx.F32, got, lse, want, "none left")
+    assert np.all(got == 0)
+    k[3, 0, 0] = 1.0
+    got, lse, want = run_attend(s3dx, q, k, v, s3dx.F32, [40], [150], 64, scale=1.0)
+    assert np.array_equal(got[:, 0], np.tile(v[3, 0], (40, 1)))
+
+
+def test_lse_may_be_left_out_and_results_repeat(s3dx):
+    rng = np.random.default_rng(13)
+    for n, lk, top in ((3, 2000, 20), (500, 500, 4)):
+        q, k, v = rows(rng, n, 4, 64), rows(rng, lk, 4, 64), rows(rng, lk, 4, 64)
+        sel = choose(rng, [n], [lk], 4, 64, top)
+        d = [R.dev(s3dx, R.stored(s3dx, a, s3dx.BF16)[0]) for a in (q, k, v)]
+        qs, ks, ds = starts(s3dx, [n]), starts(s3dx, [lk]), R.dev(s3dx, sel)
+        size = s3dx.block_attention_workspace_size(n, 4, 4, 64, 1, 64, top, lk)
+        outs = []
+        for byte, lse in ((0, None), (0xFF, s3dx.DeviceArray((n, 4), np.float32)), (0x7F, None)):
+            o, ws = s3dx.DeviceArray((n, 4, 64), np.uint16), R.filled(s3dx, max(size, 1), np.uint8, byte)
+            s3dx.block_attention(*d, s3dx.BF16, n, lk, 4, 4, 64, qs, ks, 1, 64, lk, o, lse, ds, top, workspace=ws)
+            outs.append(o.download())
+        assert all(np.array_equal(outs[0], o) for o in outs[1:])
+
+
+def test_workspace_too_small_is_refused(s3dx):
+    rng = np.random.default_rng(14)
+    d = [R.dev(s3dx, R.stored(s3dx, rows(rng, n, 2, 64), s3dx.BF16)[0]) for n in (1, 5000, 5000)]
+    size = s3dx.block_attention_workspace_size(1, 2, 2, 64, 1, 64, 0, 5000)
+    o, ws = R.filled(s3dx, (1, 2, 64), np.uint16, 0x5A), s3dx.DeviceArray(max(1, size), np.uint8)
+    args = (*d, s3dx.BF16, 1, 5000, 2, 2, 64, starts(s3dx, [1]), starts(s3dx, [5000]), 1, 64, 5000, o)
+    if size:
+        with pytest.raises(s3dx.S3dxError, match="workspace"):
+            s3dx.block_attention(*args, workspace=ws, workspace_bytes=size - 1)
+        with pytest.raises(s3dx.S3dxError, match="workspace"):
+            s3dx.block_attention(*args, workspace=None, workspace_bytes=size)
+        assert np.all(o.download().view(np.uint8) == 0x5A)
+    s3dx.block_attention(*args, workspace=ws)
+
+
+def test_a_long_cache_past_32_bit_offsets(s3dx):
+    # rows 2^21 elements apart: 1,200 of them span 5 GB; the chosen blocks lie at both ends
+    rng = np.random.default_rng(15)
+    lk, stride, d = 1200, 2 ** 21, 64
+    (kb, k64), (vb, v64), (qb, q64) = (R.stored(s3dx, rows(rng, n, 1, d), s3dx.BF16) for n in (lk, lk, 5))
+    kd = s3dx.DeviceArray((lk * stride,), np.uint16)
+    for r in range(lk):
+        pair = np.concatenate([kb[r, 0], vb[r, 0]])
+        s3dx.call("s3dx_memcpy_h2d", s3dx._vp(kd.ptr + 2 * r * stride), pair.ctypes.data_as(s3dx._vp), 4 * d, None)
+    qs, ks = starts(s3dx, [5]), starts(s3dx, [lk])
+    n = s3dx.block_index_rows(lk, 1, 64)
+    codes, scale = s3dx.DeviceArray((1, n, d), np.int8), s3dx.DeviceArray((1, n), np.float32)
+    s3dx.block_index(kd, s3dx.BF16, lk, 1, d, ks, 1, 64, codes, scale, k_stride=stride)
+    want, power, used = R.index_of(k64, [lk], 64)
+    assert np.array_equal(codes.download()[:, used], want[:, used])
+    sel = np.array([[0, 18], [17, 18], [3, 9], [18, -1], [1, 16]], np.int32).reshape(5, 1, 2)
+    for chosen in (sel, None):
+        o, lse = s3dx.DeviceArray((5, 1, d), np.uint16), s3dx.DeviceArray((5, 1), np.float32)
+        top = 0 if chosen is None else 2
+        ws = s3dx.DeviceArray(max(1, s3dx.block_attention_workspace_size(5, 1, 1, d, 1, 64, top, lk)), np.uint8)
+        s3dx.block_attention(R.dev(s3dx, qb), kd, kd.ptr + 2 * d, s3dx.BF16, 5, lk, 1, 1, d, qs, ks, 1, 64, lk, o, lse,
+                             None if chosen is None else R.dev(s3dx, chosen), top, k_stride=stride, v_stride=stride, workspace=ws)
+        check(s3dx, s3dx.BF16, R.values(s3dx, o, s3dx.BF16), lse.download().astype(np.float64),
+              R.attend(q64, k64, v64, [5], [lk], 64, chosen, d ** -0.5, False, True))
+    kd.free()
+
+
+# ---------------------------------------------------------------------------
+# The operators together
+# ---------------------------------------------------------------------------
+class Layer:
+    """A block's attention over voxel rows from the packed projection: norm and turn, index, select, attend."""
+
+    def __init__(self, s3dx, lens, heads, kv, d, block, top, dtype):
+        self.__dict__.update(s3dx=s3dx, lens=lens, heads=heads, kv=kv, d=d, block=block, top=top, dtype=dtype)
+        self.n = n = sum(lens)
+        self.row = (heads + 2 * kv) * d
+        st = R.store_type(s3dx, dtype)
+        self.qkv, self.pos = s3dx.DeviceArray((n, self.row), st), s3dx.DeviceArray((n, 4), np.int32)
+        self.gq, self.gk = s3dx.DeviceArray((heads, d), np.float32), s3dx.DeviceArray((kv, d), np.float32)
+        self.rotary = s3dx.Rotary.per_axis(d, [10, 10, 10])
+        rows = s3dx.block_index_rows(n, len(lens), block)
+        self.codes, self.scale = s3dx.DeviceArray((kv, rows, d), np.int8), s3dx.DeviceArray((kv, rows), np.float32)
+        self.sel, self.o = s3dx.DeviceArray((n, kv, top), np.int32), s3dx.DeviceArray((n, heads, d), st)
+        self.lse = s3dx.DeviceArray((n, heads), np.float32)
+        self.ws = s3dx.DeviceArray(max(1, s3dx.block_attention_workspace_size(n, heads, kv, d, len(lens), block, top, max(lens))), np.uint8)
+        self.starts = starts(s3dx, lens)
+
+    def fill(self, rng):
+        s, n = self.s3dx, self.n
+        st, self.x = R.stored(s, rng.standard_normal((n, self.row)), self.dtype)
+        self.qkv.upload(st)
+        self.places = rng.integers(0, 64, (n, 4)).astype(np.int32)
+        self.pos.upload(self.places)
+        self.g = [(1 + 0.1 * rng.standard_normal((h, self.d))).astype(np.float32) for h in (self.heads, self.kv)]
+        self.gq.upload(self.g[0])
+        self.gk.upload(self.g[1])
+
+    def run(self, stream=None):
+        s, n, h, kv, d, e = self.s3dx, self.n, self.heads, self.kv, self.d, 2 if self.dtype == 1 else 4
+        q, k, v = self.qkv.ptr, self.qkv.ptr + h * d * e, self.qkv.ptr + (h + kv) * d * e
+        s.qk_norm_rotary(q, k, self.dtype, n, h, kv, d, 1e-6, rotary=self.rotary, positions=self.pos.ptr + 4, position_stride=4,
+                         q_gain=self.gq, k_gain=self.gk, q_stride=self.row, k_stride=self.row, stream=stream)
+        s.block_index(k, self.dtype, n, kv, d, self.starts, len(self.lens), self.block, self.codes, self.scale, self.row, stream)
+        s.block_select(q, self.dtype, n, n, h, kv, d, self.starts, self.starts, len(self.lens), self.block, self.top, max(self.lens),
+                       self.codes, self.scale, self.sel, self.row, near=True, stream=stream)
+        s.block_attention(q, k, v, self.dtype, n, n, h, kv, d, self.starts, self.starts, len(self.lens), self.block, max(self.lens),
+                          self.o, self.lse, self.sel, self.top, self.row, self.row, self.row, workspace=self.ws, stream=stream)
+
+    def check(self):
+        s, n, h, kv, d = self.s3dx, self.n, self.heads, self.kv, self.d
+        got = R.values(s, self.qkv, self.dtype)   # in place: normed and turned
+        axis, freq = [a for a in range(3) for _ in range(10)], [10000.0 ** (-j / 10) for _ in range(3) for j in range(10)]
+        for at, heads, g in ((0, h, self.g[0]), (h * d, kv, self.g[1])):
+            want, size = R.turn(R.rms(self.x[:, at: at + heads * d].reshape(n, heads, d), g, 1e-6), self.places[:, 1:], axis, freq, True)
+            off = np.abs(got[:, at: at + heads * d].reshape(n, heads, d) - want)
+            assert np.all(off <= ((d + 2) / 2 + 16) * R.U32 * size + R.half_step(s, self.dtype) * np.abs(want))
+        q, k, v = (got[:, a * d: b * d].reshape(n, b - a, d) for a, b in ((0, h), (h, h + kv), (h + kv, h + 2 * kv)))
+        codes, scale, used = R.index_of(k, self.lens, self.block)
+        assert np.array_equal(self.codes.download()[:, used], codes[:, used])
+        sel = self.sel.download()
+        assert np.array_equal(sel, R.select(q, codes, scale, self.lens, self.lens, self.block, self.top, False, True))
+        check(s, self.dtype, R.values(s, self.o, self.dtype), self.lse.download().astype(np.float64),
+              R.attend(q, k, v, self.lens, self.lens, self.block, sel, d ** -0.5, False, self.dtype == s.BF16))
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("lens,heads,kv,d,block,top", [([250], 4, 4, 64, 32, 3), ([100, 0, 170], 6, 2, 64, 64, 2)])
+def test_layer(s3dx, dtype, lens, heads, kv, d, block, top):
+    layer = Layer(s3dx, lens, heads, kv, d, block, top, dtype)
+    layer.fill(np.random.default_rng(20))
+    layer.run()
+    layer.check()
+
+
+def test_two_layers_on_two_streams_and_in_graphs(s3dx):
+    rng = np.random.default_rng(21)
+    layers = [Layer(s3dx, lens, 4, 2, 64, 32, 3, s3dx.BF16) for lens in ([200], [3, 120])]
+    streams = [s3dx.Stream(), s3dx.Stream()]
+    for l in layers:
+        l.fill(rng)
+    for l, s in zip(layers, streams):
+        l.run(s)
+    for l, s in zip(layers, streams):
+        s.synchronize()
+        l.check()
+    graphs = [R.Graph(s3dx, s, lambda l=l, s=s: l.run(s)) for l, s in zip(layers, streams)]
+    for _ in range(3):
+        for l in layers:
+            l.fill(rng)
+        for g in graphs:
+            g.launch()
+        for l, s in zip(layers, streams):
+            s.synchronize()
+            l.check()
+        layers[0].fill(rng)   # the program's own eager work between replays
+        layers[0].run()
+        s3dx.synchronize()
+        layers[0].check()
+    for g in graphs:
+        g.close()
