@@ -214,50 +214,68 @@ struct AttendArgs {
     float *lse;
     const int32_t *q_starts, *k_starts, *selected;
     int64_t total_q, total_k, q_stride, k_stride, v_stride, o_stride, sequences;
-    int32_t heads, group, kv_heads, d, block, top, flags;
+    int32_t heads, group, kv_heads, block, block_log2, top, causal, splits, tile_groups;
     float scale;
+    float *part_o;   // [splits][total_q][heads][d]: unnormalized
+    float2 *part_ml; // [splits][total_q][heads]: maximum (natural units), sum
 };
 
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLog2e = 1.44269504088896341f;
 
-// One wave per (query row, head), key by key: scores with a key per lane, the
-// running maximum and sum, values with a channel pair per lane.  Only keys that the
-// row sees are multiplied.
-template <class T>
-__global__ void __launch_bounds__(64) attend_row_kernel(AttendArgs a) {
-    __shared__ float qf[128];
-    const int lane = threadIdx.x;
-    const int64_t row = blockIdx.x / a.heads;
-    const int head = static_cast<int>(blockIdx.x - row * a.heads);
-    const int64_t s = sequence_of_row(a.q_starts, a.sequences, row);
-    if (s < 0) return;
-    const Span qs = sequence_span(a.q_starts, s, a.total_q), ks = sequence_span(a.k_starts, s, a.total_k);
-    const int kvh = head / a.group;
-    const T *q = static_cast<const T *>(a.q) + row * a.q_stride + static_cast<int64_t>(head) * a.d;
-    for (int c = lane; c < a.d; c += 64) qf[c] = load_as_f32<T>(q + c) * a.scale;
-    __syncthreads();
-    int32_t seen = ks.rows;
-    if (a.flags & S3DX_BLOCK_CAUSAL)
-        seen = max(0, min(seen, static_cast<int32_t>(row - qs.begin) + ks.rows - qs.rows + 1));
-    const int32_t nb = (ks.rows + a.block - 1) / a.block;
-    const int32_t *list = a.selected ? a.selected + (row * a.kv_heads + kvh) * a.top : nullptr;
-    float m = -__builtin_inff(), l = 0.0f, o[2] = {0.0f, 0.0f};
-    for (int t = 0; t < (list ? a.top : nb); ++t) {
-        const int32_t b = list ? list[t] : t;
-        if (b < 0 || b >= nb) continue;
-        for (int k0 = b * a.block; k0 < min((b + 1) * a.block, seen); k0 += 64) {
-            const int count = min(64, min((b + 1) * a.block, seen) - k0);
-            const T *kr = static_cast<const T *>(a.k) + (ks.begin + k0) * a.k_stride + static_cast<int64_t>(kvh) * a.d;
-            const T *vr = static_cast<const T *>(a.v) + (ks.begin + k0) * a.v_stride + static_cast<int64_t>(kvh) * a.d;
-            float sc = -__builtin_inff();
-            if (lane < count) {
-                sc = 0.0f;
-                for (int c = 0; c < a.d; ++c) sc += qf[c] * load_as_f32<T>(kr + lane * a.k_stride + c);
-            }
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+
+// Largest over the lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float max_over_groups(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const float m = fmaxf(__builtin_bit_cast(float, a[0]), __builtin_bit_cast(float, a[1]));
+    const uint32_t w = __builtin_bit_cast(uint32_t, m);
+    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return fmaxf(__builtin_bit_cast(float, b[0]), __builtin_bit_cast(float, b[1]));
+}
+
+// Smallest over lanes 0..31, in every lane.
+__device__ __forceinline__ int min_of_32(int v) {
+    constexpr int kMax = 0x7fffffff;
+    v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x111, 0xf, 0xf, false));  // row_shr:1
+    v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x112, 0xf, 0xf, false));
+    v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x114, 0xf, 0xf, false));
+    v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x118, 0xf, 0xf, false));
+    return min(__builtin_amdgcn_readlane(v, 15), __builtin_amdgcn_readlane(v, 31));
+}
+
+// One row by the whole wave, key by key: scores with a key per lane, the running
+// maximum and sum, values with a channel pair per lane.  Only keys that the row
+// sees, [0, seen), are multiplied, so nothing else reaches it.  For rows whose tile gave
+// no finite result.  With a list its entries [first, last), else the keys [first, last).
+// Gives this lane's channels lane, lane + 64, and the maximum and the sum in every lane.
+template <class T, int D>
+__device__ void attend_row(const T *q, const T *k, const T *v, const AttendArgs &a, const int32_t *list, int seen, int first,
+                           int last, float (&o)[2], float *m_out, float *l_out) {
+    const int lane = threadIdx.x & 63;
+    float qv[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) qv[w] = lane + 64 * w < D ? load_as_f32<T>(q + lane + 64 * w) * a.scale : 0.0f;
+    float m = neg_inf(), l = 0.0f;
+    o[0] = o[1] = 0.0f;
+    const auto keys = [&](int begin, int end) {
+        for (int k0 = begin; k0 < end; k0 += 64) {
+            const int count = min(64, end - k0);
+            const T *kr = k + static_cast<int64_t>(k0 + min(lane, count - 1)) * a.k_stride;
+            const T *vr = v + static_cast<int64_t>(k0) * a.v_stride;
+            float sc = 0.0f;
+            for (int c = 0; c < D; ++c) sc += __shfl(c < 64 ? qv[0] : qv[1], c & 63, 64) * load_as_f32<T>(kr + c);
+            if (lane >= count) sc = neg_inf();
             float mx = sc;
             for (int w = 1; w < 64; w <<= 1) mx = fmaxf(mx, __shfl_xor(mx, w, 64));
-            const float mn = fmaxf(m, mx), base = mn == -__builtin_inff() ? 0.0f : mn;
+            const float mn = fmaxf(m, mx), base = mn == neg_inf() ? 0.0f : mn;
             // the difference first: scores of the type's lowest value stay finite
             const float alpha = exp2f((m - base) * kLog2e), p = exp2f((sc - base) * kLog2e);
             l = l * alpha + (lane < count ? p : 0.0f);
@@ -266,18 +284,437 @@ __global__ void __launch_bounds__(64) attend_row_kernel(AttendArgs a) {
             m = mn;
             for (int j = 0; j < count; ++j) {
                 const float pj = __shfl(p, j, 64);
+#pragma unroll
                 for (int w = 0; w < 2; ++w)
-                    if (lane + 64 * w < a.d) o[w] += pj * load_as_f32<T>(vr + j * a.v_stride + lane + 64 * w);
+                    if (lane + 64 * w < D) o[w] += pj * load_as_f32<T>(vr + j * a.v_stride + lane + 64 * w);
+            }
+        }
+    };
+    if (list) {
+        for (int t = first; t < last; ++t) {
+            const int b = list[t];
+            if (b >= 0 && seen > 0 && b <= (seen - 1) >> a.block_log2)
+                keys(b << a.block_log2, min((b << a.block_log2) + a.block, seen));
+        }
+    } else {
+        keys(first, min(last, seen));
+    }
+    for (int w = 1; w < 64; w <<= 1) l += __shfl_xor(l, w, 64);
+    *m_out = m;
+    *l_out = l;
+}
+
+// N dwords at byte offset `at` of a buffer; zeros from its end on.
+template <int N>
+__device__ __forceinline__ void buffer_dwords(__amdgpu_buffer_rsrc_t r, int at, uint32_t *out) {
+    static_assert(N >= 1 && N <= 4 || N == 6 || N == 8);
+    if constexpr (N == 1) {
+        out[0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
+    } else if constexpr (N == 2) {
+        const u32x2 t = __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0);
+        out[0] = t[0], out[1] = t[1];
+    } else if constexpr (N == 3) {
+        const u32x3 t = __builtin_amdgcn_raw_buffer_load_b96(r, at, 0, 0);
+        out[0] = t[0], out[1] = t[1], out[2] = t[2];
+    } else if constexpr (N == 4) {
+        const u32x4 t = __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0);
+        out[0] = t[0], out[1] = t[1], out[2] = t[2], out[3] = t[3];
+    } else {
+        buffer_dwords<N / 2>(r, at, out);
+        buffer_dwords<N / 2>(r, at + 2 * N, out + N / 2);
+    }
+}
+
+// Rows [first, first + rows) of a head as a buffer; reads behind the last row's
+// channels give zeros.
+template <class T, int D>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void *x, int64_t row, int64_t stride, int head,
+                                                              int rows) {
+    const T *p = static_cast<const T *>(x) + row * stride + static_cast<int64_t>(head) * D;
+    const int bytes = static_cast<int>(((rows - 1) * stride + D) * static_cast<int64_t>(sizeof(T)));
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(p), static_cast<short>(0), bytes, 0x00020000);
+}
+
+// Attention of a tile of 32 rows (query rows times the heads that share a key head)
+// by one wave, on matrix units, without LDS: the wave computes S^T = K Q^T and
+// O^T = V^T P^T, so that what one product leaves in a lane is what the next one wants
+// there.  A 16x16 product leaves lane (c, g) = (lane & 15, lane >> 4) with rows
+// 4g..4g+3 of column c: of S^T four keys of query c, and two such (keys 4g.. of one
+// 16-key group and of the next) are the eight k-values that lane (c, g) holds of the
+// operand P^T.  V^T's operand wants the same eight keys of one channel: the lane
+// reads D/16 channels of eight rows and pairs them up by byte permutes; channel
+// c*(D/16) + t goes with product t, so O^T leaves each lane D/4 channels that lie
+// side by side.  Statistics, scales and masks are per query, hence per lane.
+//
+// The keys of a tile are those of any of its rows' blocks: its rows' lists (a row per
+// lane) are merged on the way, the next block being the smallest that heads a list;
+// rows that did not choose it are masked.  Neighbouring rows choose alike, which is what
+// makes tiles of them pay.
+template <class T, int D, int KC, bool LISTED>
+__global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
+    constexpr bool BF = sizeof(T) == 2;
+    constexpr int NS = 2, ROWS = 16 * NS;
+    constexpr int KT = KC / 16;              // 16-key groups of a step
+    constexpr int QV = BF ? D / 32 : D / 16; // 16-byte pieces of a lane's K or Q row
+    constexpr int C = D / 16;                // channels of a lane's V row
+    constexpr int VW = C * static_cast<int>(sizeof(T)) / 4;
+    constexpr int E = static_cast<int>(sizeof(T));
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    // Consecutive workgroups of one XCD run neighbouring tiles of a head: its L2 holds
+    // their keys.
+    const int id = xcd_tile(blockIdx.x, gridDim.x);
+    const int split = id / a.tile_groups % a.splits, kvh = id / a.tile_groups / a.splits;
+    int tg = id % a.tile_groups;
+    if (a.causal) tg = a.tile_groups - 1 - tg;  // longest rows first
+    const int64_t tile = static_cast<int64_t>(tg) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, a.group, ROWS, tile);
+    const Span qs = sequence_span(a.q_starts, s, a.total_q), ks = sequence_span(a.k_starts, s, a.total_k);
+    const int64_t first_row = (tile - (qs.begin * a.group / ROWS + s)) * ROWS;
+    const int nrows = qs.rows * a.group;  // total_q * heads < 2^31
+    if (first_row < 0 || first_row >= nrows) return;
+    const int r0 = static_cast<int>(first_row);
+    const int tok0 = r0 / a.group, ntok = (min(r0 + ROWS, nrows) - 1) / a.group - tok0 + 1;
+    const int lag = ks.rows - qs.rows;
+
+    // this lane's query of each set of 16
+    int tok[NS], lim[NS];
+    bool valid[NS];
+    const T *qrow[NS];
+    uint32_t qf[NS][QV][4];
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+        const int r = min(r0 + 16 * n + c, nrows - 1);
+        valid[n] = r0 + 16 * n + c < nrows;
+        tok[n] = r / a.group - tok0;
+        lim[n] = a.causal ? max(0, min(ks.rows, tok0 + tok[n] + lag + 1)) : ks.rows;
+        qrow[n] = static_cast<const T *>(a.q) + (qs.begin + tok0 + tok[n]) * a.q_stride +
+                  static_cast<int64_t>(kvh * a.group + r % a.group) * D;
+#pragma unroll
+        for (int j = 0; j < QV; ++j) {
+            const u32x4 t = *reinterpret_cast<const u32x4 *>(qrow[n] + (BF ? 32 * j + 8 * g : 16 * j + 4 * g));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qf[n][j][i] = t[i];
+        }
+    }
+    const int most = a.causal ? max(0, min(ks.rows, tok0 + ntok + lag)) : ks.rows;  // keys that some row sees
+
+    // ---- the tile's steps of KC keys
+    int slot = 0, slots = 0;           // this lane's list (lane < ntok)
+    const int32_t *list = nullptr;
+    int ahead[4] = {-1, -1, -1, -1}, left = 0, cur = 0x7fffffff;
+    uint32_t members = ~0u;
+    int first = 0, end = 0;            // the step's first key, the end of its block
+    const auto refill = [&]() __attribute__((always_inline)) {
+        left = min(4, slots - slot);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ahead[i] = i < left ? list[slot + i] : -1;
+        slot += left;
+    };
+    const auto pop = [&]() __attribute__((always_inline)) {  // cur = the next entry that names a block in reach
+        cur = 0x7fffffff;
+        while (left > 0) {
+            const int b = ahead[0];
+            ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
+            if (--left == 0) refill();
+            if (b >= 0 && b <= (most - 1) >> a.block_log2) {
+                cur = b;
+                break;
+            }
+        }
+    };
+    // the next step; false: none
+    const auto next = [&]() __attribute__((always_inline)) {
+        if constexpr (LISTED) {
+            first += KC;
+            if (first < end) return true;
+            const int b = min_of_32(cur);
+            if (b == 0x7fffffff) return false;
+            members = static_cast<uint32_t>(__ballot(cur == b));
+            if (cur == b) pop();
+            first = b << a.block_log2;
+            end = min(first + a.block, most);
+            return true;
+        } else {
+            first += KC;
+            return first < end;
+        }
+    };
+    if constexpr (LISTED) {
+        first = -KC;
+        end = 0;
+        if (lane < ntok && most > 0) {
+            list = a.selected + ((qs.begin + tok0 + lane) * a.kv_heads + kvh) * a.top;
+            slot = static_cast<int>(static_cast<int64_t>(a.top) * split / a.splits);
+            slots = static_cast<int>(static_cast<int64_t>(a.top) * (split + 1) / a.splits);
+            if (slots > slot) {
+                refill();
+                pop();
+            }
+        }
+    } else {
+        const int steps = (most + KC - 1) / KC;
+        first = static_cast<int>(static_cast<int64_t>(steps) * split / a.splits) * KC - KC;
+        end = min(static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / a.splits) * KC, most);
+    }
+
+    // this piece of the rows' lists, or of the keys
+    const int piece_lo = LISTED ? static_cast<int>(static_cast<int64_t>(a.top) * split / a.splits) : first + KC;
+    const int piece_hi = LISTED ? static_cast<int>(static_cast<int64_t>(a.top) * (split + 1) / a.splits) : end;
+
+    // ---- state
+    f32x4 acc[NS][C], sum[NS];
+    float top[NS];  // running maximum of the raw products
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+        top[n] = neg_inf();
+        sum[n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < C; ++t) acc[n][t] = f32x4{0, 0, 0, 0};
+    }
+    const float cs = a.scale * kLog2e;
+    const int kstep = static_cast<int>(a.k_stride) * E, vstep = static_cast<int>(a.v_stride) * E;
+    uint32_t kf[KT][QV][4];
+    const auto load_k = [&]() __attribute__((always_inline)) {
+        const auto r = rows_buffer<T, D>(a.k, ks.begin + first, a.k_stride, kvh, min(KC, ks.rows - first));
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int j = 0; j < QV; ++j)
+                buffer_dwords<4>(r, (16 * t + c) * kstep + 64 * j + 16 * g, kf[t][j]);
+    };
+
+    bool more = next();
+    if (more) load_k();
+    while (more) {
+        const int at = first;
+        const uint32_t mem = members;
+        // ---- V of this step
+        uint32_t vf[KT][4][VW];  // rows 16t + 4g + i
+        {
+            const auto r = rows_buffer<T, D>(a.v, ks.begin + at, a.v_stride, kvh, min(KC, ks.rows - at));
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) buffer_dwords<VW>(r, (16 * t + 4 * g + i) * vstep + c * (C * E), vf[t][i]);
+        }
+        // ---- which rows see what
+        int see[NS];
+        bool any[NS], mask[NS];
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            see[n] = LISTED && !((mem >> tok[n]) & 1u) ? 0 : lim[n];
+            any[n] = __any(valid[n] && see[n] > at);
+            mask[n] = !__all(!valid[n] || see[n] >= at + KC);
+        }
+        // ---- S^T
+        f32x4 sc[NS][KT];
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            if (!any[n]) continue;
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                f32x4 d = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < QV; ++j) {
+                    if constexpr (BF) {
+                        const u32x4 x = {kf[t][j][0], kf[t][j][1], kf[t][j][2], kf[t][j][3]};
+                        const u32x4 y = {qf[n][j][0], qf[n][j][1], qf[n][j][2], qf[n][j][3]};
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x),
+                                                                    __builtin_bit_cast(bf16x8, y), d, 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            d = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kf[t][j][i]),
+                                                                     __builtin_bit_cast(float, qf[n][j][i]), d, 0, 0, 0);
+                    }
+                }
+                sc[n][t] = d;
+            }
+        }
+        more = next();
+        if (more) load_k();
+        // ---- softmax and O^T
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            if (!any[n]) continue;
+            if (mask[n]) {
+#pragma unroll
+                for (int t = 0; t < KT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (at + 16 * t + 4 * g + i >= see[n]) sc[n][t][i] = neg_inf();
+            }
+            float mx = neg_inf();
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[n][t][i]);
+            mx = max_over_groups(mx);
+            const float now = fmaxf(top[n], mx);
+            // nothing seen yet: any finite base leaves weights of 0
+            const float base = now == neg_inf() ? 0.0f : now * cs;
+            if (__any(now != top[n])) {
+                const float alpha = __builtin_amdgcn_exp2f(top[n] * cs - base);
+                sum[n] *= alpha;
+#pragma unroll
+                for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
+                top[n] = now;
+            }
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[n][t][i] = __builtin_amdgcn_exp2f(fmaf(sc[n][t][i], cs, -base));
+            if constexpr (BF) {
+                // Weights are rounded to bfloat16 for the product (2^-8 of each at most, of either sign); the sum
+                // is taken of the same rounded weights, by a product with ones.
+                const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+                for (int u = 0; u < KT / 2; ++u) {
+                    const f32x4 lo = sc[n][2 * u], hi = sc[n][2 * u + 1];
+                    const u32x4 pw = {pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
+                                      pack_bf16x2(hi[2], hi[3])};
+                    const bf16x8 p = __builtin_bit_cast(bf16x8, pw);
+                    sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, one), p, sum[n], 0, 0, 0);
+#pragma unroll
+                    for (int t = 0; t < C; ++t) {
+                        const uint32_t pick = t & 1 ? 0x07060302u : 0x05040100u;
+                        const u32x4 x = {__builtin_amdgcn_perm(vf[2 * u][1][t / 2], vf[2 * u][0][t / 2], pick),
+                                         __builtin_amdgcn_perm(vf[2 * u][3][t / 2], vf[2 * u][2][t / 2], pick),
+                                         __builtin_amdgcn_perm(vf[2 * u + 1][1][t / 2], vf[2 * u + 1][0][t / 2], pick),
+                                         __builtin_amdgcn_perm(vf[2 * u + 1][3][t / 2], vf[2 * u + 1][2][t / 2], pick)};
+                        acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), p, acc[n][t],
+                                                                            0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < KT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        sum[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, sc[n][t][i], sum[n], 0, 0, 0);
+#pragma unroll
+                        for (int w = 0; w < C; ++w)
+                            acc[n][w] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vf[t][i][w]),
+                                                                             sc[n][t][i], acc[n][w], 0, 0, 0);
+                    }
             }
         }
     }
-    for (int w = 1; w < 64; w <<= 1) l += __shfl_xor(l, w, 64);
-    // l == 0: nothing seen (a NaN is not 0 and stays)
+
+    // ---- out
+    const bool parts = a.splits > 1;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+        const float l = sum[n][0];
+        float odd = l * 0.0f;
+#pragma unroll
+        for (int t = 0; t < C; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) odd += acc[n][t][i] * 0.0f;
+        const bool bad = valid[n] && odd != 0.0f;  // a NaN
+        const int64_t token = qs.begin + tok0 + tok[n];
+        const int head = kvh * a.group + min(r0 + 16 * n + c, nrows - 1) % a.group;
+        const int64_t cell = (static_cast<int64_t>(split) * a.total_q + token) * a.heads + head;
+        if (valid[n]) {
+            const float natural = top[n] * a.scale;
+            if (parts) {
+                float *y = a.part_o + cell * D + 4 * g * C;
+#pragma unroll
+                for (int w = 0; w < 4 * C; w += 4)
+                    *reinterpret_cast<f32x4 *>(y + w) = f32x4{acc[n][w % C][w / C], acc[n][(w + 1) % C][(w + 1) / C],
+                                                              acc[n][(w + 2) % C][(w + 2) / C],
+                                                              acc[n][(w + 3) % C][(w + 3) / C]};
+                if (g == 0) a.part_ml[cell] = make_float2(natural, l);
+            } else {
+                const float r = l == 0.0f ? 0.0f : 1.0f / l;
+                T *y = static_cast<T *>(a.o) + token * a.o_stride + static_cast<int64_t>(head) * D + 4 * g * C;
+                if constexpr (BF) {
+#pragma unroll
+                    for (int w = 0; w < 4 * C; w += 8) {
+                        u32x4 d;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int e = w + 2 * i;
+                            d[i] = pack_bf16x2(acc[n][e % C][e / C] * r, acc[n][(e + 1) % C][(e + 1) / C] * r);
+                        }
+                        *reinterpret_cast<u32x4 *>(y + w) = d;
+                    }
+                } else {
+#pragma unroll
+                    for (int w = 0; w < 4 * C; w += 4)
+                        *reinterpret_cast<f32x4 *>(y + w) =
+                            f32x4{acc[n][w % C][w / C] * r, acc[n][(w + 1) % C][(w + 1) / C] * r,
+                                  acc[n][(w + 2) % C][(w + 2) / C] * r, acc[n][(w + 3) % C][(w + 3) / C] * r};
+                }
+                if (a.lse && g == 0)
+                    a.lse[token * a.heads + head] = l == 0.0f ? neg_inf() : natural + __builtin_amdgcn_logf(l) * kLn2;
+            }
+        }
+        // A weight of 0 times a value that is not finite is a NaN: rows that did not see that value are computed again,
+        // from the keys that they see alone.  The test costs nothing in the loop.
+        uint64_t again = __ballot(bad);
+        again = (again | again >> 16 | again >> 32 | again >> 48) & 0xffffu;
+        while (again) {
+            const int w = __builtin_ctzll(again);
+            again &= again - 1;
+            const int r = r0 + 16 * n + w, tk = r / a.group, hd = kvh * a.group + r % a.group;
+            const int64_t row = qs.begin + tk;
+            const int32_t seen = a.causal ? max(0, min(ks.rows, tk + lag + 1)) : ks.rows;
+            const T *q = static_cast<const T *>(a.q) + row * a.q_stride + static_cast<int64_t>(hd) * D;
+            const T *k = static_cast<const T *>(a.k) + ks.begin * a.k_stride + static_cast<int64_t>(kvh) * D;
+            const T *v = static_cast<const T *>(a.v) + ks.begin * a.v_stride + static_cast<int64_t>(kvh) * D;
+            float o[2], m, l2;
+            attend_row<T, D>(q, k, v, a, LISTED ? a.selected + (row * a.kv_heads + kvh) * a.top : nullptr, seen, piece_lo,
+                             piece_hi, o, &m, &l2);
+            const int64_t at = (static_cast<int64_t>(split) * a.total_q + row) * a.heads + hd;
+            const float rcp = l2 == 0.0f ? 0.0f : 1.0f / l2;
+            for (int e = 0; e < 2; ++e) {
+                const int d = lane + 64 * e;
+                if (d >= D) continue;
+                if (parts) a.part_o[at * D + d] = o[e];
+                else
+                    store_from_f32<T>(static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(hd) * D + d,
+                                      l2 == 0.0f ? 0.0f : o[e] * rcp);
+            }
+            if (lane == 0) {
+                if (parts) a.part_ml[at] = make_float2(m, l2);
+                else if (a.lse) a.lse[row * a.heads + hd] = l2 == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l2) * kLn2;
+            }
+        }
+    }
+}
+
+// Joins the pieces of each (row, head), in their order; a wave each.
+template <class T, int D>
+__global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t cell = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6), cells = a.total_q * a.heads;
+    if (cell >= cells) return;
+    const int64_t row = cell / a.heads;
+    const int head = static_cast<int>(cell - row * a.heads);
+    if (sequence_of_row(a.q_starts, a.sequences, row) < 0) return;
+    float m = neg_inf();
+    for (int p = 0; p < a.splits; ++p) {
+        const float2 ml = a.part_ml[p * cells + cell];
+        if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+    }
+    float l = 0.0f, o[2] = {0.0f, 0.0f};
+    for (int p = 0; p < a.splits; ++p) {
+        const float2 ml = a.part_ml[p * cells + cell];
+        if (ml.y == 0.0f) continue;  // a piece without keys (a NaN is not 0 and stays)
+        const float w = exp2f((ml.x - m) * kLog2e);
+        l += w * ml.y;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (lane + 64 * e < D) o[e] += w * a.part_o[(p * cells + cell) * D + lane + 64 * e];
+    }
     const float r = l == 0.0f ? 0.0f : 1.0f / l;
-    T *y = static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(head) * a.d;
-    for (int w = 0; w < 2; ++w)
-        if (lane + 64 * w < a.d) store_from_f32<T>(y + lane + 64 * w, l == 0.0f ? 0.0f : o[w] * r);
-    if (a.lse && lane == 0) a.lse[row * a.heads + head] = l == 0.0f ? -__builtin_inff() : m + log2f(l) * kLn2;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (lane + 64 * e < D)
+            store_from_f32<T>(static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(head) * D + lane + 64 * e,
+                              l == 0.0f ? 0.0f : o[e] * r);
+    if (a.lse && lane == 0) a.lse[cell] = l == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l) * kLn2;
 }
 
 // ---------------------------------------------------------------------------
@@ -307,6 +744,51 @@ void check_rows(const void *p, int64_t stride, int32_t heads, int32_t head_dim, 
 }
 void check_starts(const int32_t *p) { require(p && aligned(p, 4), "starts is NULL or not aligned"); }
 int64_t index_rows(int64_t total_k, int64_t sequences, int32_t block) { return total_k / block + sequences; }
+
+constexpr int kTileRows = 32;
+
+// How an attention call is cut: tiles of rows (an upper bound, as the lengths are on the
+// device), and each tile's blocks or keys into pieces where the tiles alone
+// are fewer than two waves for each SIMD, with at least 128 keys a piece.
+struct AttendCut {
+    int64_t tile_groups;
+    int32_t splits;
+};
+AttendCut attend_cut(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, int32_t block, int32_t top,
+                     int64_t max_k) {
+    constexpr int64_t kWaves = 256 * 4 * 2;
+    const int64_t tiles = total_q * (heads / kv_heads) / kTileRows + sequences;
+    const int64_t waves = tiles * kv_heads;
+    const int64_t keys = top ? std::min<int64_t>(top * static_cast<int64_t>(block), max_k) : max_k;
+    const int64_t most = top ? std::min<int64_t>(top, (keys + 127) / 128) : (keys + 127) / 128;
+    const int64_t splits = std::max<int64_t>(1, std::min(most, std::min<int64_t>(kWaves / std::max<int64_t>(waves, 1), 64)));
+    return {(tiles + 3) / 4, static_cast<int32_t>(splits)};
+}
+
+using AttendFn = void (*)(AttendArgs);
+// Steps of 64 keys where a lane's registers hold them (fewer reductions for each
+// key), else of 32, FP32's widest heads of 16.
+template <class T, int D>
+AttendFn pick_step(bool listed, int32_t block) {
+    constexpr bool BF = sizeof(T) == 2;
+    if constexpr (BF && D <= 64)
+        if (block >= 64 || !listed) return listed ? attend_kernel<T, D, 64, true> : attend_kernel<T, D, 64, false>;
+    constexpr int KC = !BF && D > 64 ? 16 : 32;
+    return listed ? attend_kernel<T, D, KC, true> : attend_kernel<T, D, KC, false>;
+}
+template <class T>
+AttendFn pick_attend(int32_t d, bool listed, int32_t block) {
+    switch (d) {
+        case 32: return pick_step<T, 32>(listed, block);
+        case 64: return pick_step<T, 64>(listed, block);
+        case 96: return pick_step<T, 96>(listed, block);
+        default: return pick_step<T, 128>(listed, block);
+    }
+}
+template <class T>
+AttendFn pick_join(int32_t d) {
+    return d == 32 ? join_kernel<T, 32> : d == 64 ? join_kernel<T, 64> : d == 96 ? join_kernel<T, 96> : join_kernel<T, 128>;
+}
 
 }  // namespace
 }  // namespace s3dx
@@ -390,7 +872,13 @@ S3DX_API s3dx_status s3dx_block_attention_workspace_size(int64_t total_q, int32_
         check_total(max_k);
         check_shape(S3DX_F32, heads, kv_heads, head_dim, sequences, block);
         require(top >= 0 && top <= kMaxTop, "top must be 0 to 4096");
+        const AttendCut cut = attend_cut(total_q, heads, kv_heads, sequences, block, top, max_k);
         *bytes = 0;
+        if (cut.splits == 1) return;
+        Sizer z;
+        z.take<float>(static_cast<uint64_t>(cut.splits) * total_q * heads * head_dim);
+        z.take<float2>(static_cast<uint64_t>(cut.splits) * total_q * heads);
+        *bytes = z.used;
     });
 }
 
@@ -421,15 +909,29 @@ S3DX_API s3dx_status s3dx_block_attention(const void *q, const void *k, const vo
         check_starts(k_starts);
         require(!selected || aligned(selected, 4), "selected is not aligned");
         require(!lse || aligned(lse, 4), "lse is not aligned");
-        (void)workspace;
-        (void)workspace_bytes;
-        const AttendArgs a = {q, k, v, o, lse, q_starts, k_starts, selected, total_q, total_k, q_stride, k_stride,
-                              v_stride, o_stride, sequences, heads, heads / kv_heads, kv_heads, head_dim, block, top,
-                              flags, softmax_scale};
         require(total_q * heads <= std::numeric_limits<int32_t>::max(), "total_q * heads is out of range");
-        (dtype == S3DX_BF16 ? attend_row_kernel<uint16_t> : attend_row_kernel<float>)<<<
-            dim3(static_cast<unsigned>(total_q * heads)), dim3(64), 0, as_stream(stream)>>>(a);
+        const AttendCut cut = attend_cut(total_q, heads, kv_heads, sequences, block, top, max_k);
+        AttendArgs a = {q, k, v, o, lse, q_starts, k_starts, selected, total_q, total_k, q_stride, k_stride, v_stride, o_stride,
+                        sequences, heads, heads / kv_heads, kv_heads, block, block == 32 ? 5 : block == 64 ? 6 : 7, top,
+                        flags & S3DX_BLOCK_CAUSAL, cut.splits, static_cast<int32_t>(cut.tile_groups), softmax_scale, nullptr,
+                        nullptr};
+        if (cut.splits > 1) {
+            require(workspace && aligned(workspace, 16), "workspace is NULL or not 16-byte aligned");
+            Carver w(workspace, workspace_bytes);
+            a.part_o = w.take<float>(static_cast<uint64_t>(cut.splits) * total_q * heads * head_dim);
+            a.part_ml = w.take<float2>(static_cast<uint64_t>(cut.splits) * total_q * heads);
+        }
+        const int64_t grid = cut.tile_groups * kv_heads * cut.splits;
+        require(grid <= std::numeric_limits<int32_t>::max(), "too many rows and sequences");
+        const bool bf = dtype == S3DX_BF16;
+        (bf ? pick_attend<uint16_t>(head_dim, selected, block) : pick_attend<float>(head_dim, selected, block))<<<
+            dim3(static_cast<unsigned>(grid)), dim3(256), 0, as_stream(stream)>>>(a);
         launch_check("block attention");
+        if (cut.splits > 1) {
+            (bf ? pick_join<uint16_t>(head_dim) : pick_join<float>(head_dim))<<<
+                dim3(static_cast<unsigned>((total_q * heads + 3) / 4)), dim3(256), 0, as_stream(stream)>>>(a);
+            launch_check("block attention join");
+        }
     });
 }
 
