@@ -216,7 +216,7 @@ struct AttendArgs {
     int64_t total_q, total_k, q_stride, k_stride, v_stride, o_stride, sequences;
     int32_t heads, group, kv_heads, block, block_log2, top, causal, splits, tile_groups;
     float scale;
-    float *part_o;   // [splits][total_q][heads][d]: unnormalized
+    float *part_o;   // [splits][total_q][heads][d]: not yet divided by the sum
     float2 *part_ml; // [splits][total_q][heads]: maximum (natural units), sum
 };
 
@@ -251,23 +251,42 @@ __device__ __forceinline__ int min_of_32(int v) {
     return min(__builtin_amdgcn_readlane(v, 15), __builtin_amdgcn_readlane(v, 31));
 }
 
-// One row by the whole wave, key by key: scores with a key per lane, the running
+// A tile's work is cut into `count` pieces, a power of two: piece `at` takes the keys' steps
+// at, at + count, ..., or of lists the blocks with those numbers modulo count, so that the
+// pieces of rows that choose alike do not share blocks.  Tiles of one or two query rows
+// take ranges of their lists instead, which come out even.
+struct Piece {
+    int at, count;
+    bool slots;
+    __device__ int slot_lo(int top) const { return slots ? static_cast<int>(static_cast<int64_t>(top) * at / count) : 0; }
+    __device__ int slot_hi(int top) const {
+        return slots ? static_cast<int>(static_cast<int64_t>(top) * (at + 1) / count) : top;
+    }
+    __device__ bool has(int block) const { return slots || (block & (count - 1)) == at; }
+};
+
+// A piece of one row by the whole wave, key by key: scores with a key per lane, the running
 // maximum and sum, values with a channel pair per lane.  Only keys that the row
 // sees, [0, seen), are multiplied, so nothing else reaches it.  For rows whose tile gave
-// no finite result.  With a list its entries [first, last), else the keys [first, last).
-// Gives this lane's channels lane, lane + 64, and the maximum and the sum in every lane.
-template <class T, int D>
-__device__ void attend_row(const T *q, const T *k, const T *v, const AttendArgs &a, const int32_t *list, int seen, int first,
-                           int last, float (&o)[2], float *m_out, float *l_out) {
+// no finite result.  Gives this lane's channels lane, lane + 64, and the maximum and the
+// sum in every lane.
+template <class T, int D, int KC>
+__device__ void attend_row(const T *q, const T *k, const T *v, const AttendArgs &a, const int32_t *list, int seen, Piece piece,
+                           float (&o)[2], float *m_out, float *l_out) {
     const int lane = threadIdx.x & 63;
     float qv[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) qv[w] = lane + 64 * w < D ? load_as_f32<T>(q + lane + 64 * w) * a.scale : 0.0f;
     float m = neg_inf(), l = 0.0f;
     o[0] = o[1] = 0.0f;
-    const auto keys = [&](int begin, int end) {
-        for (int k0 = begin; k0 < end; k0 += 64) {
-            const int count = min(64, end - k0);
+    // entry t of the list, or step t of the keys
+    const int first = list ? piece.slot_lo(a.top) : piece.at, by = list ? 1 : piece.count;
+    const int last = list ? piece.slot_hi(a.top) : (seen + KC - 1) / KC, width = list ? a.block : KC;
+    for (int t = first; t < last; t += by) {
+        const int b = list ? list[t] : t;
+        if (list && (b < 0 || seen == 0 || b > (seen - 1) >> a.block_log2 || !piece.has(b))) continue;
+        for (int k0 = b * width; k0 < min((b + 1) * width, seen); k0 += 64) {
+            const int count = min(64, min((b + 1) * width, seen) - k0);
             const T *kr = k + static_cast<int64_t>(k0 + min(lane, count - 1)) * a.k_stride;
             const T *vr = v + static_cast<int64_t>(k0) * a.v_stride;
             float sc = 0.0f;
@@ -289,15 +308,6 @@ __device__ void attend_row(const T *q, const T *k, const T *v, const AttendArgs 
                     if (lane + 64 * w < D) o[w] += pj * load_as_f32<T>(vr + j * a.v_stride + lane + 64 * w);
             }
         }
-    };
-    if (list) {
-        for (int t = first; t < last; ++t) {
-            const int b = list[t];
-            if (b >= 0 && seen > 0 && b <= (seen - 1) >> a.block_log2)
-                keys(b << a.block_log2, min((b << a.block_log2) + a.block, seen));
-        }
-    } else {
-        keys(first, min(last, seen));
     }
     for (int w = 1; w < 64; w <<= 1) l += __shfl_xor(l, w, 64);
     *m_out = m;
@@ -336,9 +346,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void *x, int
 }
 
 // Attention of a tile of 32 rows (query rows times the heads that share a key head)
-// by one wave, on matrix units, without LDS: the wave computes S^T = K Q^T and
-// O^T = V^T P^T, so that what one product leaves in a lane is what the next one wants
-// there.  A 16x16 product leaves lane (c, g) = (lane & 15, lane >> 4) with rows
+// on matrix units.  A wave computes S^T = K Q^T and O^T = V^T P^T, so that what one
+// product leaves in a lane is what the next one wants there and nothing goes through
+// LDS.  A 16x16 product leaves lane (c, g) = (lane & 15, lane >> 4) with rows
 // 4g..4g+3 of column c: of S^T four keys of query c, and two such (keys 4g.. of one
 // 16-key group and of the next) are the eight k-values that lane (c, g) holds of the
 // operand P^T.  V^T's operand wants the same eight keys of one channel: the lane
@@ -348,9 +358,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void *x, int
 //
 // The keys of a tile are those of any of its rows' blocks: its rows' lists (a row per
 // lane) are merged on the way, the next block being the smallest that heads a list;
-// rows that did not choose it are masked.  Neighbouring rows choose alike, which is what
-// makes tiles of them pay.
-template <class T, int D, int KC, bool LISTED>
+// rows that did not choose it take weights 0.  Neighbouring rows choose alike, which is
+// what makes tiles of them pay.
+//
+// WAVES 4: the workgroup's waves take a tile together, a piece of its keys each, and
+// join them through LDS: a quarter of the tiles' length, so that the last ones to run
+// leave fewer units idle.  WAVES 1: a tile each, for rows of few keys.
+template <class T, int D, int KC, bool LISTED, int WAVES>
 __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr bool BF = sizeof(T) == 2;
     constexpr int NS = 2, ROWS = 16 * NS;
@@ -359,14 +373,19 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr int C = D / 16;                // channels of a lane's V row
     constexpr int VW = C * static_cast<int>(sizeof(T)) / 4;
     constexpr int E = static_cast<int>(sizeof(T));
+    static_assert(WAVES == 1 || WAVES == 4);
+    // pieces of a workgroup: element (set n, i, t) of every lane, maxima and sums
+    __shared__ float part[WAVES == 4 ? 4 : 1][WAVES == 4 ? NS * 4 * C : 1][64];
+    __shared__ float2 part_ml[4][NS][16];
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Consecutive workgroups of one XCD run neighbouring tiles of a head: its L2 holds
     // their keys.
     const int id = xcd_tile(blockIdx.x, gridDim.x);
     const int split = id / a.tile_groups % a.splits, kvh = id / a.tile_groups / a.splits;
     int tg = id % a.tile_groups;
     if (a.causal) tg = a.tile_groups - 1 - tg;  // longest rows first
-    const int64_t tile = static_cast<int64_t>(tg) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t tile = WAVES == 4 ? tg : static_cast<int64_t>(tg) * 4 + wave;
     const int64_t s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, a.group, ROWS, tile);
     const Span qs = sequence_span(a.q_starts, s, a.total_q), ks = sequence_span(a.k_starts, s, a.total_k);
     const int64_t first_row = (tile - (qs.begin * a.group / ROWS + s)) * ROWS;
@@ -375,23 +394,23 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     const int r0 = static_cast<int>(first_row);
     const int tok0 = r0 / a.group, ntok = (min(r0 + ROWS, nrows) - 1) / a.group - tok0 + 1;
     const int lag = ks.rows - qs.rows;
+    const Piece piece = {WAVES == 4 ? split * 4 + wave : split, WAVES == 4 ? a.splits * 4 : a.splits, ntok <= 2};
 
     // this lane's query of each set of 16
-    int tok[NS], lim[NS];
+    int tok[NS], lim[NS], head[NS];
     bool valid[NS];
-    const T *qrow[NS];
     uint32_t qf[NS][QV][4];
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         const int r = min(r0 + 16 * n + c, nrows - 1);
         valid[n] = r0 + 16 * n + c < nrows;
         tok[n] = r / a.group - tok0;
+        head[n] = kvh * a.group + r % a.group;
         lim[n] = a.causal ? max(0, min(ks.rows, tok0 + tok[n] + lag + 1)) : ks.rows;
-        qrow[n] = static_cast<const T *>(a.q) + (qs.begin + tok0 + tok[n]) * a.q_stride +
-                  static_cast<int64_t>(kvh * a.group + r % a.group) * D;
+        const T *q = static_cast<const T *>(a.q) + (qs.begin + tok0 + tok[n]) * a.q_stride + static_cast<int64_t>(head[n]) * D;
 #pragma unroll
         for (int j = 0; j < QV; ++j) {
-            const u32x4 t = *reinterpret_cast<const u32x4 *>(qrow[n] + (BF ? 32 * j + 8 * g : 16 * j + 4 * g));
+            const u32x4 t = *reinterpret_cast<const u32x4 *>(q + (BF ? 32 * j + 8 * g : 16 * j + 4 * g));
 #pragma unroll
             for (int i = 0; i < 4; ++i) qf[n][j][i] = t[i];
         }
@@ -403,20 +422,20 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     const int32_t *list = nullptr;
     int ahead[4] = {-1, -1, -1, -1}, left = 0, cur = 0x7fffffff;
     uint32_t members = ~0u;
-    int first = 0, end = 0;            // the step's first key, the end of its block
+    int first, end;                    // the step's first key, the end of its block
     const auto refill = [&]() __attribute__((always_inline)) {
         left = min(4, slots - slot);
 #pragma unroll
         for (int i = 0; i < 4; ++i) ahead[i] = i < left ? list[slot + i] : -1;
         slot += left;
     };
-    const auto pop = [&]() __attribute__((always_inline)) {  // cur = the next entry that names a block in reach
+    const auto pop = [&]() __attribute__((always_inline)) {  // cur = the next entry that names a block of this piece
         cur = 0x7fffffff;
         while (left > 0) {
             const int b = ahead[0];
             ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
             if (--left == 0) refill();
-            if (b >= 0 && b <= (most - 1) >> a.block_log2) {
+            if (b >= 0 && b <= (most - 1) >> a.block_log2 && piece.has(b)) {
                 cur = b;
                 break;
             }
@@ -435,52 +454,58 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             end = min(first + a.block, most);
             return true;
         } else {
-            first += KC;
+            first += piece.count * KC;
             return first < end;
         }
     };
     if constexpr (LISTED) {
-        first = -KC;
-        end = 0;
+        first = end = 0;
         if (lane < ntok && most > 0) {
             list = a.selected + ((qs.begin + tok0 + lane) * a.kv_heads + kvh) * a.top;
-            slot = static_cast<int>(static_cast<int64_t>(a.top) * split / a.splits);
-            slots = static_cast<int>(static_cast<int64_t>(a.top) * (split + 1) / a.splits);
+            slot = piece.slot_lo(a.top);
+            slots = piece.slot_hi(a.top);
             if (slots > slot) {
                 refill();
                 pop();
             }
         }
     } else {
-        const int steps = (most + KC - 1) / KC;
-        first = static_cast<int>(static_cast<int64_t>(steps) * split / a.splits) * KC - KC;
-        end = min(static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / a.splits) * KC, most);
+        first = (piece.at - piece.count) * KC;
+        end = most;
     }
-
-    // this piece of the rows' lists, or of the keys
-    const int piece_lo = LISTED ? static_cast<int>(static_cast<int64_t>(a.top) * split / a.splits) : first + KC;
-    const int piece_hi = LISTED ? static_cast<int>(static_cast<int64_t>(a.top) * (split + 1) / a.splits) : end;
 
     // ---- state
     f32x4 acc[NS][C], sum[NS];
-    float top[NS];  // running maximum of the raw products
+    float top[NS], base[NS];  // what weights are relative to: a raw product, and the same as a power of two
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         top[n] = neg_inf();
+        base[n] = 0.0f;
         sum[n] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int t = 0; t < C; ++t) acc[n][t] = f32x4{0, 0, 0, 0};
     }
     const float cs = a.scale * kLog2e;
+    // Byte offsets of this lane's rows in a step: held where registers allow, else the first and the steps between.
+    constexpr bool HELD = D < 128;
     const int kstep = static_cast<int>(a.k_stride) * E, vstep = static_cast<int>(a.v_stride) * E;
+    const int kat = c * kstep + 16 * g, vat = 4 * g * vstep + c * (C * E);
+    int koff[HELD ? KT : 1], voff[HELD ? KT : 1][4];
+    if constexpr (HELD) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            koff[t] = kat + 16 * t * kstep;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) voff[t][i] = vat + (16 * t + i) * vstep;
+        }
+    }
     uint32_t kf[KT][QV][4];
     const auto load_k = [&]() __attribute__((always_inline)) {
         const auto r = rows_buffer<T, D>(a.k, ks.begin + first, a.k_stride, kvh, min(KC, ks.rows - first));
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int j = 0; j < QV; ++j)
-                buffer_dwords<4>(r, (16 * t + c) * kstep + 64 * j + 16 * g, kf[t][j]);
+            for (int j = 0; j < QV; ++j) buffer_dwords<4>(r, (HELD ? koff[HELD ? t : 0] : kat + 16 * t * kstep) + 64 * j, kf[t][j]);
     };
 
     bool more = next();
@@ -495,16 +520,15 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) buffer_dwords<VW>(r, (16 * t + 4 * g + i) * vstep + c * (C * E), vf[t][i]);
+                for (int i = 0; i < 4; ++i) buffer_dwords<VW>(r, HELD ? voff[HELD ? t : 0][i] : vat + (16 * t + i) * vstep, vf[t][i]);
         }
         // ---- which rows see what
-        int see[NS];
-        bool any[NS], mask[NS];
+        bool in[NS], any[NS], mask[NS];
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-            see[n] = LISTED && !((mem >> tok[n]) & 1u) ? 0 : lim[n];
-            any[n] = __any(valid[n] && see[n] > at);
-            mask[n] = !__all(!valid[n] || see[n] >= at + KC);
+            in[n] = valid[n] && lim[n] > at && (!LISTED || ((mem >> tok[n]) & 1u));
+            any[n] = __any(in[n]);
+            mask[n] = __any(in[n] && lim[n] < at + KC);
         }
         // ---- S^T
         f32x4 sc[NS][KT];
@@ -533,7 +557,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         }
         more = next();
         if (more) load_k();
-        // ---- softmax and O^T
+        // ---- softmax
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
             if (!any[n]) continue;
@@ -542,7 +566,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                 for (int t = 0; t < KT; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (at + 16 * t + 4 * g + i >= see[n]) sc[n][t][i] = neg_inf();
+                        if (at + 16 * t + 4 * g + i >= lim[n]) sc[n][t][i] = neg_inf();
             }
             float mx = neg_inf();
 #pragma unroll
@@ -550,43 +574,67 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[n][t][i]);
             mx = max_over_groups(mx);
-            const float now = fmaxf(top[n], mx);
-            // nothing seen yet: any finite base leaves weights of 0
-            const float base = now == neg_inf() ? 0.0f : now * cs;
-            if (__any(now != top[n])) {
-                const float alpha = __builtin_amdgcn_exp2f(top[n] * cs - base);
+            // What weights are relative to moves only where a weight would pass 2^8: far less often than the
+            // maximum, and floating point loses nothing by it.
+            const float now = in[n] ? fmaxf(top[n], mx) : top[n];
+            if (__any(now != top[n] && !(mx * cs <= base[n] + 8.0f && top[n] != neg_inf()))) {
+                // nothing seen yet: any finite base leaves weights of 0
+                const float to = now == neg_inf() ? 0.0f : now * cs;
+                const float alpha = __builtin_amdgcn_exp2f(top[n] * cs - to);
                 sum[n] *= alpha;
 #pragma unroll
                 for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
                 top[n] = now;
+                base[n] = to;
             }
+            const float off = in[n] ? -base[n] : neg_inf();  // rows that do not see the block: weights 2^-inf
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sc[n][t][i] = __builtin_amdgcn_exp2f(fmaf(sc[n][t][i], cs, -base));
-            if constexpr (BF) {
-                // Weights are rounded to bfloat16 for the product (2^-8 of each at most, of either sign); the sum
-                // is taken of the same rounded weights, by a product with ones.
-                const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+                for (int i = 0; i < 4; ++i) sc[n][t][i] = __builtin_amdgcn_exp2f(fmaf(sc[n][t][i], cs, off));
+        }
+        // ---- O^T
+        if constexpr (BF) {
+            // Weights are rounded to bfloat16 for the product (2^-8 of each at most, of either sign); the sum is taken of
+            // the same rounded weights, by a product with ones.
+            const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+            u32x4 pw[NS][KT / 2 > 0 ? KT / 2 : 1], x[KT / 2 > 0 ? KT / 2 : 1][C];
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int u = 0; u < KT / 2; ++u)
+                    if (any[n]) {
+                        const f32x4 lo = sc[n][2 * u], hi = sc[n][2 * u + 1];
+                        pw[n][u] = u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
+                                         pack_bf16x2(hi[2], hi[3])};
+                    }
+#pragma unroll
+            for (int u = 0; u < KT / 2; ++u)
+#pragma unroll
+                for (int t = 0; t < C; ++t) {
+                    const uint32_t pick = t & 1 ? 0x07060302u : 0x05040100u;
+                    x[u][t] = u32x4{__builtin_amdgcn_perm(vf[2 * u][1][t / 2], vf[2 * u][0][t / 2], pick),
+                                    __builtin_amdgcn_perm(vf[2 * u][3][t / 2], vf[2 * u][2][t / 2], pick),
+                                    __builtin_amdgcn_perm(vf[2 * u + 1][1][t / 2], vf[2 * u + 1][0][t / 2], pick),
+                                    __builtin_amdgcn_perm(vf[2 * u + 1][3][t / 2], vf[2 * u + 1][2][t / 2], pick)};
+                }
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                if (!any[n]) continue;
 #pragma unroll
                 for (int u = 0; u < KT / 2; ++u) {
-                    const f32x4 lo = sc[n][2 * u], hi = sc[n][2 * u + 1];
-                    const u32x4 pw = {pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
-                                      pack_bf16x2(hi[2], hi[3])};
-                    const bf16x8 p = __builtin_bit_cast(bf16x8, pw);
+                    const bf16x8 p = __builtin_bit_cast(bf16x8, pw[n][u]);
                     sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, one), p, sum[n], 0, 0, 0);
 #pragma unroll
-                    for (int t = 0; t < C; ++t) {
-                        const uint32_t pick = t & 1 ? 0x07060302u : 0x05040100u;
-                        const u32x4 x = {__builtin_amdgcn_perm(vf[2 * u][1][t / 2], vf[2 * u][0][t / 2], pick),
-                                         __builtin_amdgcn_perm(vf[2 * u][3][t / 2], vf[2 * u][2][t / 2], pick),
-                                         __builtin_amdgcn_perm(vf[2 * u + 1][1][t / 2], vf[2 * u + 1][0][t / 2], pick),
-                                         __builtin_amdgcn_perm(vf[2 * u + 1][3][t / 2], vf[2 * u + 1][2][t / 2], pick)};
-                        acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), p, acc[n][t],
+                    for (int t = 0; t < C; ++t)
+                        acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[u][t]), p, acc[n][t],
                                                                             0, 0, 0);
-                    }
                 }
-            } else {
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                if (!any[n]) continue;
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -603,57 +651,57 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 
     // ---- out
     const bool parts = a.splits > 1;
+    const auto cell_of = [&](int t, int h) __attribute__((always_inline)) {
+        return (static_cast<int64_t>(split) * a.total_q + qs.begin + tok0 + t) * a.heads + h;
+    };
+    // channels [ch, ch + N) of a row
+    const auto put = [&]<int N>(int t, int h, int ch, const float (&y)[N], float m, float l) __attribute__((always_inline)) {
+        static_assert(N % 4 == 0 || !BF);
+        if (parts) {
+            float *to = a.part_o + cell_of(t, h) * D + ch;
+#pragma unroll
+            for (int w = 0; w < N; w += 4) *reinterpret_cast<f32x4 *>(to + w) = f32x4{y[w], y[w + 1], y[w + 2], y[w + 3]};
+            if (ch == 0) a.part_ml[cell_of(t, h)] = make_float2(m, l);
+            return;
+        }
+        const float r = l == 0.0f ? 0.0f : 1.0f / l;
+        const int64_t token = qs.begin + tok0 + t;
+        T *to = static_cast<T *>(a.o) + token * a.o_stride + static_cast<int64_t>(h) * D + ch;
+        if constexpr (BF) {
+#pragma unroll
+            for (int w = 0; w < N; w += 4)
+                *reinterpret_cast<u32x2 *>(to + w) = u32x2{pack_bf16x2(y[w] * r, y[w + 1] * r), pack_bf16x2(y[w + 2] * r, y[w + 3] * r)};
+        } else {
+#pragma unroll
+            for (int w = 0; w < N; w += 4)
+                *reinterpret_cast<f32x4 *>(to + w) = f32x4{y[w] * r, y[w + 1] * r, y[w + 2] * r, y[w + 3] * r};
+        }
+        if (a.lse && ch == 0) a.lse[token * a.heads + h] = l == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l) * kLn2;
+    };
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-        const float l = sum[n][0];
+        const float l = sum[n][0], natural = top[n] * a.scale;
         float odd = l * 0.0f;
 #pragma unroll
         for (int t = 0; t < C; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) odd += acc[n][t][i] * 0.0f;
-        const bool bad = valid[n] && odd != 0.0f;  // a NaN
-        const int64_t token = qs.begin + tok0 + tok[n];
-        const int head = kvh * a.group + min(r0 + 16 * n + c, nrows - 1) % a.group;
-        const int64_t cell = (static_cast<int64_t>(split) * a.total_q + token) * a.heads + head;
-        if (valid[n]) {
-            const float natural = top[n] * a.scale;
-            if (parts) {
-                float *y = a.part_o + cell * D + 4 * g * C;
-#pragma unroll
-                for (int w = 0; w < 4 * C; w += 4)
-                    *reinterpret_cast<f32x4 *>(y + w) = f32x4{acc[n][w % C][w / C], acc[n][(w + 1) % C][(w + 1) / C],
-                                                              acc[n][(w + 2) % C][(w + 2) / C],
-                                                              acc[n][(w + 3) % C][(w + 3) / C]};
-                if (g == 0) a.part_ml[cell] = make_float2(natural, l);
-            } else {
-                const float r = l == 0.0f ? 0.0f : 1.0f / l;
-                T *y = static_cast<T *>(a.o) + token * a.o_stride + static_cast<int64_t>(head) * D + 4 * g * C;
-                if constexpr (BF) {
-#pragma unroll
-                    for (int w = 0; w < 4 * C; w += 8) {
-                        u32x4 d;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int e = w + 2 * i;
-                            d[i] = pack_bf16x2(acc[n][e % C][e / C] * r, acc[n][(e + 1) % C][(e + 1) / C] * r);
-                        }
-                        *reinterpret_cast<u32x4 *>(y + w) = d;
-                    }
-                } else {
-#pragma unroll
-                    for (int w = 0; w < 4 * C; w += 4)
-                        *reinterpret_cast<f32x4 *>(y + w) =
-                            f32x4{acc[n][w % C][w / C] * r, acc[n][(w + 1) % C][(w + 1) / C] * r,
-                                  acc[n][(w + 2) % C][(w + 2) / C] * r, acc[n][(w + 3) % C][(w + 3) / C] * r};
-                }
-                if (a.lse && g == 0)
-                    a.lse[token * a.heads + head] = l == 0.0f ? neg_inf() : natural + __builtin_amdgcn_logf(l) * kLn2;
-            }
-        }
         // A weight of 0 times a value that is not finite is a NaN: rows that did not see that value are computed again,
         // from the keys that they see alone.  The test costs nothing in the loop.
-        uint64_t again = __ballot(bad);
+        uint64_t again = __ballot(valid[n] && odd != 0.0f);
         again = (again | again >> 16 | again >> 32 | again >> 48) & 0xffffu;
+        if constexpr (WAVES == 4) {
+#pragma unroll
+            for (int t = 0; t < C; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[wave][(n * 4 + i) * C + t][lane] = acc[n][t][i];
+            if (g == 0) part_ml[wave][n][c] = make_float2(natural, l);
+        } else if (valid[n] && !((again >> c) & 1u)) {
+            float y[4 * C];
+#pragma unroll
+            for (int e = 0; e < 4 * C; ++e) y[e] = acc[n][e % C][e / C];
+            put(tok[n], head[n], 4 * g * C, y, natural, l);
+        }
         while (again) {
             const int w = __builtin_ctzll(again);
             again &= again - 1;
@@ -664,23 +712,46 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             const T *k = static_cast<const T *>(a.k) + ks.begin * a.k_stride + static_cast<int64_t>(kvh) * D;
             const T *v = static_cast<const T *>(a.v) + ks.begin * a.v_stride + static_cast<int64_t>(kvh) * D;
             float o[2], m, l2;
-            attend_row<T, D>(q, k, v, a, LISTED ? a.selected + (row * a.kv_heads + kvh) * a.top : nullptr, seen, piece_lo,
-                             piece_hi, o, &m, &l2);
-            const int64_t at = (static_cast<int64_t>(split) * a.total_q + row) * a.heads + hd;
+            attend_row<T, D, KC>(q, k, v, a, LISTED ? a.selected + (row * a.kv_heads + kvh) * a.top : nullptr, seen, piece, o,
+                                 &m, &l2);
             const float rcp = l2 == 0.0f ? 0.0f : 1.0f / l2;
             for (int e = 0; e < 2; ++e) {
                 const int d = lane + 64 * e;
                 if (d >= D) continue;
-                if (parts) a.part_o[at * D + d] = o[e];
+                if (WAVES == 4) part[wave][WAVES == 4 ? (n * 4 + d / C % 4) * C + d % C : 0][d / (4 * C) * 16 + w] = o[e];
+                else if (parts) a.part_o[cell_of(tk - tok0, hd) * D + d] = o[e];
                 else
                     store_from_f32<T>(static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(hd) * D + d,
                                       l2 == 0.0f ? 0.0f : o[e] * rcp);
             }
             if (lane == 0) {
-                if (parts) a.part_ml[at] = make_float2(m, l2);
+                if (WAVES == 4) part_ml[wave][n][w] = make_float2(m, l2);
+                else if (parts) a.part_ml[cell_of(tk - tok0, hd)] = make_float2(m, l2);
                 else if (a.lse) a.lse[row * a.heads + hd] = l2 == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l2) * kLn2;
             }
         }
+    }
+    if constexpr (WAVES == 4) {
+        __syncthreads();
+        // Wave w joins elements i = 2(w & 1), + 1 of set w >> 1: 2C channels of each row a lane.
+        const int n = wave >> 1, i0 = 2 * (wave & 1);
+        float m = neg_inf(), l = 0.0f, wgt[4], y[2 * C];
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+            if (part_ml[p][n][c].y != 0.0f) m = fmaxf(m, part_ml[p][n][c].x);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const float2 ml = part_ml[p][n][c];
+            wgt[p] = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((ml.x - m) * kLog2e);  // a piece without keys: 0
+            l += wgt[p] * ml.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 2 * C; ++e) {
+            y[e] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) y[e] += wgt[p] * part[p][(n * 4 + i0 + e / C) * C + e % C][lane];
+        }
+        if (valid[n]) put(tok[n], head[n], (4 * g + i0) * C, y, m, l);
     }
 }
 
@@ -748,41 +819,48 @@ int64_t index_rows(int64_t total_k, int64_t sequences, int32_t block) { return t
 constexpr int kTileRows = 32;
 
 // How an attention call is cut: tiles of rows (an upper bound, as the lengths are on the
-// device), and each tile's blocks or keys into pieces where the tiles alone
-// are fewer than two waves for each SIMD, with at least 128 keys a piece.
+// device), four waves to a tile where rows see 512 keys and more, else one; and each
+// tile's blocks or keys into pieces for several workgroups where the tiles alone are fewer than two waves
+// for each SIMD, with at least 128 keys a wave.
 struct AttendCut {
     int64_t tile_groups;
-    int32_t splits;
+    int32_t splits, waves;
 };
 AttendCut attend_cut(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, int32_t block, int32_t top,
                      int64_t max_k) {
     constexpr int64_t kWaves = 256 * 4 * 2;
-    const int64_t tiles = total_q * (heads / kv_heads) / kTileRows + sequences;
-    const int64_t waves = tiles * kv_heads;
     const int64_t keys = top ? std::min<int64_t>(top * static_cast<int64_t>(block), max_k) : max_k;
-    const int64_t most = top ? std::min<int64_t>(top, (keys + 127) / 128) : (keys + 127) / 128;
-    const int64_t splits = std::max<int64_t>(1, std::min(most, std::min<int64_t>(kWaves / std::max<int64_t>(waves, 1), 64)));
-    return {(tiles + 3) / 4, static_cast<int32_t>(splits)};
+    const int32_t per_tile = keys >= 512 ? 4 : 1;
+    const int64_t tiles = total_q * (heads / kv_heads) / kTileRows + sequences;
+    const int64_t waves = std::max<int64_t>(tiles * kv_heads * per_tile, 1);
+    int32_t splits = 1;
+    while (splits < 64 && waves * splits * 2 <= kWaves && keys >= 256 * splits * per_tile) splits *= 2;
+    return {per_tile == 4 ? tiles : (tiles + 3) / 4, splits, per_tile};
 }
 
 using AttendFn = void (*)(AttendArgs);
+template <class T, int D, int KC>
+AttendFn pick_form(bool listed, int32_t waves) {
+    if (listed) return waves == 4 ? attend_kernel<T, D, KC, true, 4> : attend_kernel<T, D, KC, true, 1>;
+    return waves == 4 ? attend_kernel<T, D, KC, false, 4> : attend_kernel<T, D, KC, false, 1>;
+}
 // Steps of 64 keys where a lane's registers hold them (fewer reductions for each
 // key), else of 32, FP32's widest heads of 16.
 template <class T, int D>
-AttendFn pick_step(bool listed, int32_t block) {
+AttendFn pick_step(bool listed, int32_t block, int32_t waves) {
     constexpr bool BF = sizeof(T) == 2;
     if constexpr (BF && D <= 64)
-        if (block >= 64 || !listed) return listed ? attend_kernel<T, D, 64, true> : attend_kernel<T, D, 64, false>;
+        if (block >= 64 || !listed) return pick_form<T, D, 64>(listed, waves);
     constexpr int KC = !BF && D > 64 ? 16 : 32;
-    return listed ? attend_kernel<T, D, KC, true> : attend_kernel<T, D, KC, false>;
+    return pick_form<T, D, KC>(listed, waves);
 }
 template <class T>
-AttendFn pick_attend(int32_t d, bool listed, int32_t block) {
+AttendFn pick_attend(int32_t d, bool listed, int32_t block, int32_t waves) {
     switch (d) {
-        case 32: return pick_step<T, 32>(listed, block);
-        case 64: return pick_step<T, 64>(listed, block);
-        case 96: return pick_step<T, 96>(listed, block);
-        default: return pick_step<T, 128>(listed, block);
+        case 32: return pick_step<T, 32>(listed, block, waves);
+        case 64: return pick_step<T, 64>(listed, block, waves);
+        case 96: return pick_step<T, 96>(listed, block, waves);
+        default: return pick_step<T, 128>(listed, block, waves);
     }
 }
 template <class T>
@@ -924,7 +1002,8 @@ S3DX_API s3dx_status s3dx_block_attention(const void *q, const void *k, const vo
         const int64_t grid = cut.tile_groups * kv_heads * cut.splits;
         require(grid <= std::numeric_limits<int32_t>::max(), "too many rows and sequences");
         const bool bf = dtype == S3DX_BF16;
-        (bf ? pick_attend<uint16_t>(head_dim, selected, block) : pick_attend<float>(head_dim, selected, block))<<<
+        (bf ? pick_attend<uint16_t>(head_dim, selected, block, cut.waves)
+            : pick_attend<float>(head_dim, selected, block, cut.waves))<<<
             dim3(static_cast<unsigned>(grid)), dim3(256), 0, as_stream(stream)>>>(a);
         launch_check("block attention");
         if (cut.splits > 1) {
