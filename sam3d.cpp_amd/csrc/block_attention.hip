@@ -241,14 +241,18 @@ __device__ __forceinline__ float max_over_groups(float v) {
     return fmaxf(__builtin_bit_cast(float, b[0]), __builtin_bit_cast(float, b[1]));
 }
 
-// Smallest over lanes 0..31, in every lane.
-__device__ __forceinline__ int min_of_32(int v) {
+// Smallest over the first N lanes (a multiple of 16), in every lane.
+template <int N>
+__device__ __forceinline__ int min_of(int v) {
     constexpr int kMax = 0x7fffffff;
     v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x111, 0xf, 0xf, false));  // row_shr:1
     v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x112, 0xf, 0xf, false));
     v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x114, 0xf, 0xf, false));
     v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x118, 0xf, 0xf, false));
-    return min(__builtin_amdgcn_readlane(v, 15), __builtin_amdgcn_readlane(v, 31));
+    int m = __builtin_amdgcn_readlane(v, 15);
+#pragma unroll
+    for (int l = 31; l < N; l += 16) m = min(m, __builtin_amdgcn_readlane(v, l));
+    return m;
 }
 
 // A tile's work is cut into `count` pieces, a power of two: piece `at` takes the keys' steps
@@ -345,7 +349,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void *x, int
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(p), static_cast<short>(0), bytes, 0x00020000);
 }
 
-// Attention of a tile of 32 rows (query rows times the heads that share a key head)
+// Attention of a tile of 16 NS rows (query rows times the heads that share a key head)
 // on matrix units.  A wave computes S^T = K Q^T and O^T = V^T P^T, so that what one
 // product leaves in a lane is what the next one wants there and nothing goes through
 // LDS.  A 16x16 product leaves lane (c, g) = (lane & 15, lane >> 4) with rows
@@ -364,10 +368,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void *x, int
 // WAVES 4: the workgroup's waves take a tile together, a piece of its keys each, and
 // join them through LDS: a quarter of the tiles' length, so that the last ones to run
 // leave fewer units idle.  WAVES 1: a tile each, for rows of few keys.
-template <class T, int D, int KC, bool LISTED, int WAVES>
+template <class T, int D, int KC, int NS, bool LISTED, int WAVES>
 __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr bool BF = sizeof(T) == 2;
-    constexpr int NS = 2, ROWS = 16 * NS;
+    constexpr int ROWS = 16 * NS;
     constexpr int KT = KC / 16;              // 16-key groups of a step
     constexpr int QV = BF ? D / 32 : D / 16; // 16-byte pieces of a lane's K or Q row
     constexpr int C = D / 16;                // channels of a lane's V row
@@ -421,7 +425,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     int slot = 0, slots = 0;           // this lane's list (lane < ntok)
     const int32_t *list = nullptr;
     int ahead[4] = {-1, -1, -1, -1}, left = 0, cur = 0x7fffffff;
-    uint32_t members = ~0u;
+    uint64_t members = ~UINT64_C(0);
     int first, end;                    // the step's first key, the end of its block
     const auto refill = [&]() __attribute__((always_inline)) {
         left = min(4, slots - slot);
@@ -446,9 +450,9 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         if constexpr (LISTED) {
             first += KC;
             if (first < end) return true;
-            const int b = min_of_32(cur);
+            const int b = min_of<ROWS>(cur);
             if (b == 0x7fffffff) return false;
-            members = static_cast<uint32_t>(__ballot(cur == b));
+            members = __ballot(cur == b);
             if (cur == b) pop();
             first = b << a.block_log2;
             end = min(first + a.block, most);
@@ -512,7 +516,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     if (more) load_k();
     while (more) {
         const int at = first;
-        const uint32_t mem = members;
+        const uint64_t mem = members;
         // ---- V of this step
         uint32_t vf[KT][4][VW];  // rows 16t + 4g + i
         {
@@ -522,19 +526,19 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) buffer_dwords<VW>(r, HELD ? voff[HELD ? t : 0][i] : vat + (16 * t + i) * vstep, vf[t][i]);
         }
-        // ---- which rows see what
-        bool in[NS], any[NS], mask[NS];
+        // ---- sets of 16 rows: S^T, weights
+        f32x4 w[NS][KT];
+        u32x4 pw[NS][KT / 2 > 0 ? KT / 2 : 1];
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-            in[n] = valid[n] && lim[n] > at && (!LISTED || ((mem >> tok[n]) & 1u));
-            any[n] = __any(in[n]);
-            mask[n] = __any(in[n] && lim[n] < at + KC);
-        }
-        // ---- S^T
-        f32x4 sc[NS][KT];
+            const bool in = valid[n] && lim[n] > at && (!LISTED || ((mem >> tok[n]) & 1u));
+            if (!__any(in)) {  // no row of the set sees the block: weights 0
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            if (!any[n]) continue;
+                for (int t = 0; t < KT; ++t) w[n][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < KT / 2; ++u) pw[n][u] = u32x4{0, 0, 0, 0};
+                continue;
+            }
 #pragma unroll
             for (int t = 0; t < KT; ++t) {
                 f32x4 d = {0, 0, 0, 0};
@@ -552,32 +556,25 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                                                                      __builtin_bit_cast(float, qf[n][j][i]), d, 0, 0, 0);
                     }
                 }
-                sc[n][t] = d;
+                w[n][t] = d;
             }
-        }
-        more = next();
-        if (more) load_k();
-        // ---- softmax
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            if (!any[n]) continue;
-            if (mask[n]) {
+            if (__any(in && lim[n] < at + KC)) {
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (at + 16 * t + 4 * g + i >= lim[n]) sc[n][t][i] = neg_inf();
+                        if (at + 16 * t + 4 * g + i >= lim[n]) w[n][t][i] = neg_inf();
             }
             float mx = neg_inf();
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[n][t][i]);
-            mx = max_over_groups(mx);
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, w[n][t][i]);
             // What weights are relative to moves only where a weight would pass 2^8: far less often than the
-            // maximum, and floating point loses nothing by it.
-            const float now = in[n] ? fmaxf(top[n], mx) : top[n];
-            if (__any(now != top[n] && !(mx * cs <= base[n] + 8.0f && top[n] != neg_inf()))) {
+            // maximum, and floating point loses nothing by it.  base is +0 and top -inf before the first key.
+            if (__any(in && mx > neg_inf() && !(mx * cs <= base[n] + 8.0f && top[n] > neg_inf()))) {
+                mx = max_over_groups(mx);
+                const float now = in ? fmaxf(top[n], mx) : top[n];
                 // nothing seen yet: any finite base leaves weights of 0
                 const float to = now == neg_inf() ? 0.0f : now * cs;
                 const float alpha = __builtin_amdgcn_exp2f(top[n] * cs - to);
@@ -587,65 +584,60 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                 top[n] = now;
                 base[n] = to;
             }
-            const float off = in[n] ? -base[n] : neg_inf();  // rows that do not see the block: weights 2^-inf
+            const float off = in ? -base[n] : neg_inf();  // rows that do not see the block: weights 2^-inf
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sc[n][t][i] = __builtin_amdgcn_exp2f(fmaf(sc[n][t][i], cs, off));
+                for (int i = 0; i < 4; ++i) w[n][t][i] = __builtin_amdgcn_exp2f(fmaf(w[n][t][i], cs, off));
+            if constexpr (BF) {
+                // Weights are rounded to bfloat16 for the product (2^-8 of each at most, of either sign); the sum is taken
+                // of the same rounded weights, by a product with ones.
+#pragma unroll
+                for (int u = 0; u < KT / 2; ++u) {
+                    const f32x4 lo = w[n][2 * u], hi = w[n][2 * u + 1];
+                    pw[n][u] = u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
+                                     pack_bf16x2(hi[2], hi[3])};
+                }
+            }
         }
+        more = next();
+        if (more) load_k();
         // ---- O^T
         if constexpr (BF) {
-            // Weights are rounded to bfloat16 for the product (2^-8 of each at most, of either sign); the sum is taken of
-            // the same rounded weights, by a product with ones.
             const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-            u32x4 pw[NS][KT / 2 > 0 ? KT / 2 : 1], x[KT / 2 > 0 ? KT / 2 : 1][C];
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
+            for (int u = 0; u < KT / 2; ++u) {
 #pragma unroll
-                for (int u = 0; u < KT / 2; ++u)
-                    if (any[n]) {
-                        const f32x4 lo = sc[n][2 * u], hi = sc[n][2 * u + 1];
-                        pw[n][u] = u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
-                                         pack_bf16x2(hi[2], hi[3])};
-                    }
-#pragma unroll
-            for (int u = 0; u < KT / 2; ++u)
+                for (int n = 0; n < NS; ++n)
+                    sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, one),
+                                                                     __builtin_bit_cast(bf16x8, pw[n][u]), sum[n], 0, 0, 0);
 #pragma unroll
                 for (int t = 0; t < C; ++t) {
                     const uint32_t pick = t & 1 ? 0x07060302u : 0x05040100u;
-                    x[u][t] = u32x4{__builtin_amdgcn_perm(vf[2 * u][1][t / 2], vf[2 * u][0][t / 2], pick),
-                                    __builtin_amdgcn_perm(vf[2 * u][3][t / 2], vf[2 * u][2][t / 2], pick),
-                                    __builtin_amdgcn_perm(vf[2 * u + 1][1][t / 2], vf[2 * u + 1][0][t / 2], pick),
-                                    __builtin_amdgcn_perm(vf[2 * u + 1][3][t / 2], vf[2 * u + 1][2][t / 2], pick)};
-                }
+                    const u32x4 x = {__builtin_amdgcn_perm(vf[2 * u][1][t / 2], vf[2 * u][0][t / 2], pick),
+                                     __builtin_amdgcn_perm(vf[2 * u][3][t / 2], vf[2 * u][2][t / 2], pick),
+                                     __builtin_amdgcn_perm(vf[2 * u + 1][1][t / 2], vf[2 * u + 1][0][t / 2], pick),
+                                     __builtin_amdgcn_perm(vf[2 * u + 1][3][t / 2], vf[2 * u + 1][2][t / 2], pick)};
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                if (!any[n]) continue;
-#pragma unroll
-                for (int u = 0; u < KT / 2; ++u) {
-                    const bf16x8 p = __builtin_bit_cast(bf16x8, pw[n][u]);
-                    sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, one), p, sum[n], 0, 0, 0);
-#pragma unroll
-                    for (int t = 0; t < C; ++t)
-                        acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[u][t]), p, acc[n][t],
+                    for (int n = 0; n < NS; ++n)
+                        acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x),
+                                                                            __builtin_bit_cast(bf16x8, pw[n][u]), acc[n][t],
                                                                             0, 0, 0);
                 }
             }
         } else {
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                if (!any[n]) continue;
+            for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int t = 0; t < KT; ++t)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        sum[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, sc[n][t][i], sum[n], 0, 0, 0);
+                    for (int n = 0; n < NS; ++n) {
+                        sum[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, w[n][t][i], sum[n], 0, 0, 0);
 #pragma unroll
-                        for (int w = 0; w < C; ++w)
-                            acc[n][w] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vf[t][i][w]),
-                                                                             sc[n][t][i], acc[n][w], 0, 0, 0);
+                        for (int x = 0; x < C; ++x)
+                            acc[n][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vf[t][i][x]), w[n][t][i],
+                                                                             acc[n][x], 0, 0, 0);
                     }
-            }
         }
     }
 
@@ -733,25 +725,30 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     }
     if constexpr (WAVES == 4) {
         __syncthreads();
-        // Wave w joins elements i = 2(w & 1), + 1 of set w >> 1: 2C channels of each row a lane.
-        const int n = wave >> 1, i0 = 2 * (wave & 1);
-        float m = neg_inf(), l = 0.0f, wgt[4], y[2 * C];
+        // (set, i) pairs, NS for each wave: C (or with few sets, more) channels of each row a lane.
+        constexpr int PER = NS >= 4 ? 4 : NS;  // i's of one set that a wave joins
 #pragma unroll
-        for (int p = 0; p < 4; ++p)
-            if (part_ml[p][n][c].y != 0.0f) m = fmaxf(m, part_ml[p][n][c].x);
+        for (int k = 0; k < NS / PER; ++k) {
+            const int pair = wave * NS + k * PER, n = pair >> 2, i0 = pair & 3;
+            float m = neg_inf(), l = 0.0f, wgt[4], y[PER * C];
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const float2 ml = part_ml[p][n][c];
-            wgt[p] = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((ml.x - m) * kLog2e);  // a piece without keys: 0
-            l += wgt[p] * ml.y;
+            for (int p = 0; p < 4; ++p)
+                if (part_ml[p][n][c].y != 0.0f) m = fmaxf(m, part_ml[p][n][c].x);
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const float2 ml = part_ml[p][n][c];
+                wgt[p] = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((ml.x - m) * kLog2e);  // a piece without keys: 0
+                l += wgt[p] * ml.y;
+            }
+#pragma unroll
+            for (int e = 0; e < PER * C; ++e) {
+                y[e] = 0.0f;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) y[e] += wgt[p] * part[p][(n * 4 + i0 + e / C) * C + e % C][lane];
+            }
+            const int r = r0 + 16 * n + c;
+            if (r < nrows) put(r / a.group - tok0, kvh * a.group + r % a.group, (4 * g + i0) * C, y, m, l);
         }
-#pragma unroll
-        for (int e = 0; e < 2 * C; ++e) {
-            y[e] = 0.0f;
-#pragma unroll
-            for (int p = 0; p < 4; ++p) y[e] += wgt[p] * part[p][(n * 4 + i0 + e / C) * C + e % C][lane];
-        }
-        if (valid[n]) put(tok[n], head[n], (4 * g + i0) * C, y, m, l);
     }
 }
 
@@ -816,8 +813,6 @@ void check_rows(const void *p, int64_t stride, int32_t heads, int32_t head_dim, 
 void check_starts(const int32_t *p) { require(p && aligned(p, 4), "starts is NULL or not aligned"); }
 int64_t index_rows(int64_t total_k, int64_t sequences, int32_t block) { return total_k / block + sequences; }
 
-constexpr int kTileRows = 32;
-
 // How an attention call is cut: tiles of rows (an upper bound, as the lengths are on the
 // device), four waves to a tile where rows see 512 keys and more, else one; and each
 // tile's blocks or keys into pieces for several workgroups where the tiles alone are fewer than two waves
@@ -826,42 +821,44 @@ struct AttendCut {
     int64_t tile_groups;
     int32_t splits, waves;
 };
-AttendCut attend_cut(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, int32_t block, int32_t top,
-                     int64_t max_k) {
+constexpr int tile_sets(bool bf, int32_t head_dim, int32_t waves) { return bf && waves == 4 && head_dim <= 64 ? 4 : 2; }
+AttendCut attend_cut(bool bf, int64_t total_q, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t sequences, int32_t block,
+                     int32_t top, int64_t max_k) {
     constexpr int64_t kWaves = 256 * 4 * 2;
     const int64_t keys = top ? std::min<int64_t>(top * static_cast<int64_t>(block), max_k) : max_k;
     const int32_t per_tile = keys >= 512 ? 4 : 1;
-    const int64_t tiles = total_q * (heads / kv_heads) / kTileRows + sequences;
-    const int64_t waves = std::max<int64_t>(tiles * kv_heads * per_tile, 1);
+    const int64_t rows = total_q * (heads / kv_heads), tiles = rows / (16 * tile_sets(bf, head_dim, per_tile)) + sequences;
+    // by tiles of 32 rows for either type, so that the workspace does not depend on it
+    const int64_t waves = std::max<int64_t>((rows / 32 + sequences) * kv_heads * per_tile, 1);
     int32_t splits = 1;
     while (splits < 64 && waves * splits * 2 <= kWaves && keys >= 256 * splits * per_tile) splits *= 2;
     return {per_tile == 4 ? tiles : (tiles + 3) / 4, splits, per_tile};
 }
 
 using AttendFn = void (*)(AttendArgs);
-template <class T, int D, int KC>
-AttendFn pick_form(bool listed, int32_t waves) {
-    if (listed) return waves == 4 ? attend_kernel<T, D, KC, true, 4> : attend_kernel<T, D, KC, true, 1>;
-    return waves == 4 ? attend_kernel<T, D, KC, false, 4> : attend_kernel<T, D, KC, false, 1>;
-}
-// Steps of 64 keys where a lane's registers hold them (fewer reductions for each
-// key), else of 32, FP32's widest heads of 16.
-template <class T, int D>
-AttendFn pick_step(bool listed, int32_t block, int32_t waves) {
+// Steps of keys as registers allow: of 64 for narrow heads and two sets of rows, of 32,
+// FP32's widest heads of 16.
+template <class T, int D, int WAVES>
+AttendFn pick_step(bool listed, int32_t block) {
     constexpr bool BF = sizeof(T) == 2;
-    if constexpr (BF && D <= 64)
-        if (block >= 64 || !listed) return pick_form<T, D, 64>(listed, waves);
+    constexpr int NS = tile_sets(BF, D, WAVES);
+    if constexpr (BF && D <= 64 && NS == 2)
+        if (block >= 64 || !listed) return listed ? attend_kernel<T, D, 64, NS, true, WAVES> : attend_kernel<T, D, 64, NS, false, WAVES>;
     constexpr int KC = !BF && D > 64 ? 16 : 32;
-    return pick_form<T, D, KC>(listed, waves);
+    return listed ? attend_kernel<T, D, KC, NS, true, WAVES> : attend_kernel<T, D, KC, NS, false, WAVES>;
+}
+template <class T, int WAVES>
+AttendFn pick_dim(int32_t d, bool listed, int32_t block) {
+    switch (d) {
+        case 32: return pick_step<T, 32, WAVES>(listed, block);
+        case 64: return pick_step<T, 64, WAVES>(listed, block);
+        case 96: return pick_step<T, 96, WAVES>(listed, block);
+        default: return pick_step<T, 128, WAVES>(listed, block);
+    }
 }
 template <class T>
 AttendFn pick_attend(int32_t d, bool listed, int32_t block, int32_t waves) {
-    switch (d) {
-        case 32: return pick_step<T, 32>(listed, block, waves);
-        case 64: return pick_step<T, 64>(listed, block, waves);
-        case 96: return pick_step<T, 96>(listed, block, waves);
-        default: return pick_step<T, 128>(listed, block, waves);
-    }
+    return waves == 4 ? pick_dim<T, 4>(d, listed, block) : pick_dim<T, 1>(d, listed, block);
 }
 template <class T>
 AttendFn pick_join(int32_t d) {
@@ -950,7 +947,7 @@ S3DX_API s3dx_status s3dx_block_attention_workspace_size(int64_t total_q, int32_
         check_total(max_k);
         check_shape(S3DX_F32, heads, kv_heads, head_dim, sequences, block);
         require(top >= 0 && top <= kMaxTop, "top must be 0 to 4096");
-        const AttendCut cut = attend_cut(total_q, heads, kv_heads, sequences, block, top, max_k);
+        const AttendCut cut = attend_cut(true, total_q, heads, kv_heads, head_dim, sequences, block, top, max_k);
         *bytes = 0;
         if (cut.splits == 1) return;
         Sizer z;
@@ -988,7 +985,7 @@ S3DX_API s3dx_status s3dx_block_attention(const void *q, const void *k, const vo
         require(!selected || aligned(selected, 4), "selected is not aligned");
         require(!lse || aligned(lse, 4), "lse is not aligned");
         require(total_q * heads <= std::numeric_limits<int32_t>::max(), "total_q * heads is out of range");
-        const AttendCut cut = attend_cut(total_q, heads, kv_heads, sequences, block, top, max_k);
+        const AttendCut cut = attend_cut(dtype == S3DX_BF16, total_q, heads, kv_heads, head_dim, sequences, block, top, max_k);
         AttendArgs a = {q, k, v, o, lse, q_starts, k_starts, selected, total_q, total_k, q_stride, k_stride, v_stride, o_stride,
                         sequences, heads, heads / kv_heads, kv_heads, block, block == 32 ? 5 : block == 64 ? 6 : 7, top,
                         flags & S3DX_BLOCK_CAUSAL, cut.splits, static_cast<int32_t>(cut.tile_groups), softmax_scale, nullptr,
