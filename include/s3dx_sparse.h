@@ -570,7 +570,7 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
                                        int32_t *selected, s3dx_stream stream, char *error, uint64_t error_capacity);
 /* o = softmax(softmax_scale * q k^T) v over the keys of each row's chosen blocks
  * (selected as above; any order, entries outside the sequence's blocks count
- * for nothing, a block that stands twice counts twice), or over all keys of
+ * for nothing, a block that stands twice counts once), or over all keys of
  * its sequence where selected is NULL and top 0.  o [total_q][heads][head_dim] in
  * dtype by o_stride; lse (may be NULL): float32 [total_q][heads], the natural
  * logarithm of the row's sum of exp(score).  A row that sees no key, or only

@@ -241,56 +241,32 @@ __device__ __forceinline__ float max_over_groups(float v) {
     return fmaxf(__builtin_bit_cast(float, b[0]), __builtin_bit_cast(float, b[1]));
 }
 
-// Smallest over the first N lanes (a multiple of 16), in every lane.
-template <int N>
-__device__ __forceinline__ int min_of(int v) {
-    constexpr int kMax = 0x7fffffff;
-    v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x111, 0xf, 0xf, false));  // row_shr:1
-    v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x112, 0xf, 0xf, false));
-    v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x114, 0xf, 0xf, false));
-    v = min(v, __builtin_amdgcn_update_dpp(kMax, v, 0x118, 0xf, 0xf, false));
-    int m = __builtin_amdgcn_readlane(v, 15);
-#pragma unroll
-    for (int l = 31; l < N; l += 16) m = min(m, __builtin_amdgcn_readlane(v, l));
-    return m;
-}
-
-// A tile's work is cut into `count` pieces, a power of two: piece `at` takes the keys' steps
-// at, at + count, ..., or of lists the blocks with those numbers modulo count, so that the
-// pieces of rows that choose alike do not share blocks.  Tiles of one or two query rows
-// take ranges of their lists instead, which come out even.
-struct Piece {
-    int at, count;
-    bool slots;
-    __device__ int slot_lo(int top) const { return slots ? static_cast<int>(static_cast<int64_t>(top) * at / count) : 0; }
-    __device__ int slot_hi(int top) const {
-        return slots ? static_cast<int>(static_cast<int64_t>(top) * (at + 1) / count) : top;
-    }
-    __device__ bool has(int block) const { return slots || (block & (count - 1)) == at; }
-};
-
-// A piece of one row by the whole wave, key by key: scores with a key per lane, the running
-// maximum and sum, values with a channel pair per lane.  Only keys that the row
-// sees, [0, seen), are multiplied, so nothing else reaches it.  For rows whose tile gave
-// no finite result.  Gives this lane's channels lane, lane + 64, and the maximum and the
-// sum in every lane.
-template <class T, int D, int KC>
-__device__ void attend_row(const T *q, const T *k, const T *v, const AttendArgs &a, const int32_t *list, int seen, Piece piece,
-                           float (&o)[2], float *m_out, float *l_out) {
-    const int lane = threadIdx.x & 63;
+// One row by the whole wave, key by key: scores with a key per lane, the running maximum
+// and sum, values with a channel pair per lane.  Only keys that the row sees are
+// multiplied, so nothing else reaches it: for rows whose tile gave no finite result.
+template <class T, int D>
+__device__ void attend_row(const AttendArgs &a, int64_t row, int head, Span qs, Span ks) {
+    const int lane = threadIdx.x & 63, kvh = head / a.group;
+    const T *q = static_cast<const T *>(a.q) + row * a.q_stride + static_cast<int64_t>(head) * D;
+    const T *k = static_cast<const T *>(a.k) + ks.begin * a.k_stride + static_cast<int64_t>(kvh) * D;
+    const T *v = static_cast<const T *>(a.v) + ks.begin * a.v_stride + static_cast<int64_t>(kvh) * D;
+    const int seen = a.causal ? max(0, min(ks.rows, static_cast<int>(row - qs.begin) + ks.rows - qs.rows + 1)) : ks.rows;
+    const int blocks = (seen + a.block - 1) >> a.block_log2;
+    const int32_t *list = a.selected ? a.selected + (row * a.kv_heads + kvh) * a.top : nullptr;
     float qv[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) qv[w] = lane + 64 * w < D ? load_as_f32<T>(q + lane + 64 * w) * a.scale : 0.0f;
-    float m = neg_inf(), l = 0.0f;
-    o[0] = o[1] = 0.0f;
-    // entry t of the list, or step t of the keys
-    const int first = list ? piece.slot_lo(a.top) : piece.at, by = list ? 1 : piece.count;
-    const int last = list ? piece.slot_hi(a.top) : (seen + KC - 1) / KC, width = list ? a.block : KC;
-    for (int t = first; t < last; t += by) {
+    float m = neg_inf(), l = 0.0f, o[2] = {0.0f, 0.0f};
+    for (int t = 0; t < (list ? a.top : blocks); ++t) {
         const int b = list ? list[t] : t;
-        if (list && (b < 0 || seen == 0 || b > (seen - 1) >> a.block_log2 || !piece.has(b))) continue;
-        for (int k0 = b * width; k0 < min((b + 1) * width, seen); k0 += 64) {
-            const int count = min(64, min((b + 1) * width, seen) - k0);
+        if (b < 0 || b >= blocks) continue;
+        if (list) {  // a block counts once
+            bool before = false;
+            for (int e = lane; e < t; e += 64) before = before || list[e] == b;
+            if (__any(before)) continue;
+        }
+        for (int k0 = b << a.block_log2; k0 < min((b + 1) << a.block_log2, seen); k0 += 64) {
+            const int count = min(64, min((b + 1) << a.block_log2, seen) - k0);
             const T *kr = k + static_cast<int64_t>(k0 + min(lane, count - 1)) * a.k_stride;
             const T *vr = v + static_cast<int64_t>(k0) * a.v_stride;
             float sc = 0.0f;
@@ -314,8 +290,12 @@ __device__ void attend_row(const T *q, const T *k, const T *v, const AttendArgs 
         }
     }
     for (int w = 1; w < 64; w <<= 1) l += __shfl_xor(l, w, 64);
-    *m_out = m;
-    *l_out = l;
+    const float r = l == 0.0f ? 0.0f : 1.0f / l;  // 0: nothing seen (a NaN is not 0 and stays)
+    T *y = static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(head) * D;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+        if (lane + 64 * w < D) store_from_f32<T>(y + lane + 64 * w, l == 0.0f ? 0.0f : o[w] * r);
+    if (a.lse && lane == 0) a.lse[row * a.heads + head] = l == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l) * kLn2;
 }
 
 // N dwords at byte offset `at` of a buffer; zeros from its end on.
@@ -360,14 +340,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void *x, int
 // c*(D/16) + t goes with product t, so O^T leaves each lane D/4 channels that lie
 // side by side.  Statistics, scales and masks are per query, hence per lane.
 //
-// The keys of a tile are those of any of its rows' blocks: its rows' lists (a row per
-// lane) are merged on the way, the next block being the smallest that heads a list;
-// rows that did not choose it take weights 0.  Neighbouring rows choose alike, which is
-// what makes tiles of them pay.
+// The keys of a tile are those of any of its rows' blocks: a table in LDS gets, for each
+// block, a bit for each row that chose it; rows that did not take weights 0.
+// Neighbouring rows choose alike, which is what makes tiles of them pay.
 //
-// WAVES 4: the workgroup's waves take a tile together, a piece of its keys each, and
-// join them through LDS: a quarter of the tiles' length, so that the last ones to run
-// leave fewer units idle.  WAVES 1: a tile each, for rows of few keys.
+// WAVES 4: the workgroup's waves take a tile together, every fourth step (of lists,
+// block) each, and join them through LDS: a quarter of the tiles' length, so that the last
+// ones to run leave fewer units idle.  WAVES 1: a tile each, for rows of few keys.
 template <class T, int D, int KC, int NS, bool LISTED, int WAVES>
 __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr bool BF = sizeof(T) == 2;
@@ -378,9 +357,14 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr int VW = C * static_cast<int>(sizeof(T)) / 4;
     constexpr int E = static_cast<int>(sizeof(T));
     static_assert(WAVES == 1 || WAVES == 4);
-    // pieces of a workgroup: element (set n, i, t) of every lane, maxima and sums
-    __shared__ float part[WAVES == 4 ? 4 : 1][WAVES == 4 ? NS * 4 * C : 1][64];
-    __shared__ float2 part_ml[4][NS][16];
+    // The table of blocks, TABLE of them at a time for each tile of the workgroup; after the last, its waves' results:
+    // element (set n, i, t) of every lane, maxima and sums.
+    constexpr int TABLE = WAVES == 4 ? 4096 : 1024, TILES = 4 / WAVES;
+    constexpr int PART = WAVES == 4 ? 4 * NS * 4 * C * 64 * 4 : 0;
+    constexpr int LDS = LISTED && TABLE * TILES * 8 > PART ? TABLE * TILES * 8 : PART;
+    __shared__ alignas(16) char lds[LDS > 0 ? LDS : 16];
+    __shared__ float2 part_ml[WAVES == 4 ? 4 : 1][NS][16];
+    auto part = reinterpret_cast<float (*)[NS * 4 * C][64]>(lds);
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Consecutive workgroups of one XCD run neighbouring tiles of a head: its L2 holds
@@ -398,20 +382,18 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     const int r0 = static_cast<int>(first_row);
     const int tok0 = r0 / a.group, ntok = (min(r0 + ROWS, nrows) - 1) / a.group - tok0 + 1;
     const int lag = ks.rows - qs.rows;
-    const Piece piece = {WAVES == 4 ? split * 4 + wave : split, WAVES == 4 ? a.splits * 4 : a.splits, ntok <= 2};
+    // this wave's share of the tile: every `pieces`-th step or chosen block, a power of two
+    const int piece = WAVES == 4 ? split * 4 + wave : split, pieces = WAVES == 4 ? a.splits * 4 : a.splits;
 
-    // this lane's query of each set of 16
-    int tok[NS], lim[NS], head[NS];
-    bool valid[NS];
+    // this lane's query of each set of 16, and the keys that it sees: [0, lim)
+    int lim[NS];
     uint32_t qf[NS][QV][4];
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-        const int r = min(r0 + 16 * n + c, nrows - 1);
-        valid[n] = r0 + 16 * n + c < nrows;
-        tok[n] = r / a.group - tok0;
-        head[n] = kvh * a.group + r % a.group;
-        lim[n] = a.causal ? max(0, min(ks.rows, tok0 + tok[n] + lag + 1)) : ks.rows;
-        const T *q = static_cast<const T *>(a.q) + (qs.begin + tok0 + tok[n]) * a.q_stride + static_cast<int64_t>(head[n]) * D;
+        const int r = min(r0 + 16 * n + c, nrows - 1), tok = r / a.group;
+        lim[n] = a.causal ? max(0, min(ks.rows, tok + lag + 1)) : ks.rows;
+        const T *q = static_cast<const T *>(a.q) + (qs.begin + tok) * a.q_stride +
+                     static_cast<int64_t>(kvh * a.group + r % a.group) * D;
 #pragma unroll
         for (int j = 0; j < QV; ++j) {
             const u32x4 t = *reinterpret_cast<const u32x4 *>(q + (BF ? 32 * j + 8 * g : 16 * j + 4 * g));
@@ -420,70 +402,73 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         }
     }
     const int most = a.causal ? max(0, min(ks.rows, tok0 + ntok + lag)) : ks.rows;  // keys that some row sees
+    const int least = a.causal ? max(0, min(ks.rows, tok0 + lag + 1)) : ks.rows;          // ... that all rows see
 
     // ---- the tile's steps of KC keys
-    int slot = 0, slots = 0;           // this lane's list (lane < ntok)
-    const int32_t *list = nullptr;
-    int ahead[4] = {-1, -1, -1, -1}, left = 0, cur = 0x7fffffff;
+    uint64_t *table = reinterpret_cast<uint64_t *>(lds) + (WAVES == 4 ? 0 : wave * TABLE);
+    const int blocks = (most + a.block - 1) >> a.block_log2;  // in reach of the tile
+    int w0 = 0, chunk = 0, rank = 0;  // the table's first block, the next 64 of it, chosen blocks before them
+    uint64_t todo = 0, mine = 0;      // this wave's blocks among the last 64; this lane's table entry of them
     uint64_t members = ~UINT64_C(0);
-    int first, end;                    // the step's first key, the end of its block
-    const auto refill = [&]() __attribute__((always_inline)) {
-        left = min(4, slots - slot);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ahead[i] = i < left ? list[slot + i] : -1;
-        slot += left;
-    };
-    const auto pop = [&]() __attribute__((always_inline)) {  // cur = the next entry that names a block of this piece
-        cur = 0x7fffffff;
-        while (left > 0) {
-            const int b = ahead[0];
-            ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
-            if (--left == 0) refill();
-            if (b >= 0 && b <= (most - 1) >> a.block_log2 && piece.has(b)) {
-                cur = b;
-                break;
-            }
-        }
-    };
-    // the next step; false: none
-    const auto next = [&]() __attribute__((always_inline)) {
+    int first, end;                   // the step's first key, the end of its block
+    const auto next = [&]() __attribute__((always_inline)) {  // false: no step left in the table
         if constexpr (LISTED) {
             first += KC;
             if (first < end) return true;
-            const int b = min_of<ROWS>(cur);
-            if (b == 0x7fffffff) return false;
-            members = __ballot(cur == b);
-            if (cur == b) pop();
-            first = b << a.block_log2;
+            while (todo == 0) {
+                const int count = min(TABLE, blocks - w0);
+                if (chunk >= count) return false;
+                mine = chunk + lane < count ? table[chunk + lane] : 0;
+                const uint64_t chosen = __ballot(mine != 0);
+                const int r = rank + __popcll(chosen & ((UINT64_C(1) << lane) - 1));
+                todo = __ballot(mine != 0 && (r & (pieces - 1)) == piece);
+                rank += __popcll(chosen);
+                chunk += 64;
+            }
+            const int bit = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            members = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), bit))) << 32 |
+                      static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), bit));
+            first = (w0 + chunk - 64 + bit) << a.block_log2;
             end = min(first + a.block, most);
             return true;
         } else {
-            first += piece.count * KC;
+            first += pieces * KC;
             return first < end;
         }
     };
-    if constexpr (LISTED) {
-        first = end = 0;
-        if (lane < ntok && most > 0) {
-            list = a.selected + ((qs.begin + tok0 + lane) * a.kv_heads + kvh) * a.top;
-            slot = piece.slot_lo(a.top);
-            slots = piece.slot_hi(a.top);
-            if (slots > slot) {
-                refill();
-                pop();
-            }
+    // The table's waves agree on it: the workgroup's, or this one alone.
+    const auto together = [&]() __attribute__((always_inline)) {
+        if constexpr (WAVES == 4) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    const auto fill_table = [&]() __attribute__((always_inline)) {
+        const int id0 = WAVES == 4 ? static_cast<int>(threadIdx.x) : lane, step = 64 * WAVES;
+        const int count = min(TABLE, blocks - w0);
+        for (int e = id0; e < count; e += step) table[e] = 0;
+        together();
+        const int32_t *list = a.selected + ((qs.begin + tok0) * a.kv_heads + kvh) * a.top;
+        const int64_t by = static_cast<int64_t>(a.kv_heads) * a.top;
+        for (uint32_t e = id0; e < static_cast<uint32_t>(ntok * a.top); e += step) {
+            const uint32_t t = e / static_cast<uint32_t>(a.top);
+            const int b = list[t * by + (e - t * a.top)];
+            if (b < w0 || b >= w0 + count) continue;
+            // the tile's rows of query t: [t * group, t * group + group), less what is outside
+            const int lo = max(static_cast<int>(t + tok0) * a.group - r0, 0);
+            const int hi = min(static_cast<int>(t + tok0 + 1) * a.group - r0, min(ROWS, nrows - r0));
+            __hip_atomic_fetch_or(&table[b - w0], (~UINT64_C(0) >> (64 - (hi - lo))) << lo, __ATOMIC_RELAXED,
+                                  __HIP_MEMORY_SCOPE_WORKGROUP);
         }
-    } else {
-        first = (piece.at - piece.count) * KC;
-        end = most;
-    }
+        together();
+    };
 
     // ---- state
     f32x4 acc[NS][C], sum[NS];
-    float top[NS], base[NS];  // what weights are relative to: a raw product, and the same as a power of two
+    // what weights are relative to: a raw product, and the same as a power of two; the product from which on it moves
+    float top[NS], base[NS], above[NS];
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-        top[n] = neg_inf();
+        top[n] = above[n] = neg_inf();
         base[n] = 0.0f;
         sum[n] = f32x4{0, 0, 0, 0};
 #pragma unroll
@@ -512,8 +497,25 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             for (int j = 0; j < QV; ++j) buffer_dwords<4>(r, (HELD ? koff[HELD ? t : 0] : kat + 16 * t * kstep) + 64 * j, kf[t][j]);
     };
 
-    bool more = next();
-    if (more) load_k();
+    if constexpr (LISTED) first = end = 0;
+    else first = (piece - pieces) * KC, end = most;
+    bool more;
+    const auto begin = [&]() __attribute__((always_inline)) {
+        if constexpr (LISTED) fill_table();
+        more = next();
+        if (more) load_k();
+    };
+    // what is left to see once this table is through; a workgroup's waves agree on it
+    const auto again = [&]() __attribute__((always_inline)) {
+        if constexpr (!LISTED) return false;
+        if (w0 + TABLE >= blocks) return false;
+        w0 += TABLE;
+        chunk = 0;
+        together();
+        return true;
+    };
+    do {
+    begin();
     while (more) {
         const int at = first;
         const uint64_t mem = members;
@@ -531,14 +533,17 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         u32x4 pw[NS][KT / 2 > 0 ? KT / 2 : 1];
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-            const bool in = valid[n] && lim[n] > at && (!LISTED || ((mem >> tok[n]) & 1u));
-            if (!__any(in)) {  // no row of the set sees the block: weights 0
+            // the set's rows, a bit each (all keys: all of them), and the same for the four lanes of each
+            const uint32_t rows = LISTED ? static_cast<uint32_t>(mem >> (16 * n)) & 0xffffu : r0 + 16 * n < nrows ? 0xffffu : 0u;
+            if (rows == 0) {  // none sees the block: weights 0
 #pragma unroll
                 for (int t = 0; t < KT; ++t) w[n][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int u = 0; u < KT / 2; ++u) pw[n][u] = u32x4{0, 0, 0, 0};
                 continue;
             }
+            const uint32_t twice = rows | rows << 16;
+            const uint64_t lanes = static_cast<uint64_t>(twice) << 32 | twice;
 #pragma unroll
             for (int t = 0; t < KT; ++t) {
                 f32x4 d = {0, 0, 0, 0};
@@ -558,7 +563,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                 }
                 w[n][t] = d;
             }
-            if (__any(in && lim[n] < at + KC)) {
+            if (at + KC > least) {
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -571,8 +576,9 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, w[n][t][i]);
             // What weights are relative to moves only where a weight would pass 2^8: far less often than the
-            // maximum, and floating point loses nothing by it.  base is +0 and top -inf before the first key.
-            if (__any(in && mx > neg_inf() && !(mx * cs <= base[n] + 8.0f && top[n] > neg_inf()))) {
+            // maximum, and floating point loses nothing by it.
+            if ((__builtin_amdgcn_ballot_w64(mx > above[n]) & lanes) != 0) {
+                const bool in = !LISTED || __builtin_amdgcn_inverse_ballot_w64(lanes);
                 mx = max_over_groups(mx);
                 const float now = in ? fmaxf(top[n], mx) : top[n];
                 // nothing seen yet: any finite base leaves weights of 0
@@ -583,8 +589,10 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                 for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
                 top[n] = now;
                 base[n] = to;
+                above[n] = now + 8.0f / cs;
             }
-            const float off = in ? -base[n] : neg_inf();  // rows that do not see the block: weights 2^-inf
+            // rows that do not see the block: weights 2^-inf
+            const float off = !LISTED || __builtin_amdgcn_inverse_ballot_w64(lanes) ? -base[n] : neg_inf();
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -641,23 +649,24 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         }
     }
 
+    } while (again());
+
     // ---- out
     const bool parts = a.splits > 1;
-    const auto cell_of = [&](int t, int h) __attribute__((always_inline)) {
-        return (static_cast<int64_t>(split) * a.total_q + qs.begin + tok0 + t) * a.heads + h;
-    };
-    // channels [ch, ch + N) of a row
+    // Channels [ch, ch + N) of a row.  A weight of 0 times a value that is not finite is a NaN: with `bad`, a set's rows
+    // that got one are left out, and computed again below from the keys that they see alone.  The test costs nothing in the loop.
     const auto put = [&]<int N>(int t, int h, int ch, const float (&y)[N], float m, float l) __attribute__((always_inline)) {
-        static_assert(N % 4 == 0 || !BF);
+        static_assert(N % 4 == 0);
+        const int64_t token = qs.begin + tok0 + t;
         if (parts) {
-            float *to = a.part_o + cell_of(t, h) * D + ch;
+            const int64_t cell = (static_cast<int64_t>(split) * a.total_q + token) * a.heads + h;
+            float *to = a.part_o + cell * D + ch;
 #pragma unroll
             for (int w = 0; w < N; w += 4) *reinterpret_cast<f32x4 *>(to + w) = f32x4{y[w], y[w + 1], y[w + 2], y[w + 3]};
-            if (ch == 0) a.part_ml[cell_of(t, h)] = make_float2(m, l);
+            if (ch == 0) a.part_ml[cell] = make_float2(m, l);
             return;
         }
         const float r = l == 0.0f ? 0.0f : 1.0f / l;
-        const int64_t token = qs.begin + tok0 + t;
         T *to = static_cast<T *>(a.o) + token * a.o_stride + static_cast<int64_t>(h) * D + ch;
         if constexpr (BF) {
 #pragma unroll
@@ -670,85 +679,58 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         }
         if (a.lse && ch == 0) a.lse[token * a.heads + h] = l == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l) * kLn2;
     };
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-        const float l = sum[n][0], natural = top[n] * a.scale;
+    const auto finish = [&](int n, const float (&y)[4 * C], float m, float l) __attribute__((always_inline)) {
+        const int r = r0 + 16 * n + c;
         float odd = l * 0.0f;
 #pragma unroll
-        for (int t = 0; t < C; ++t)
+        for (int e = 0; e < 4 * C; ++e) odd += y[e] * 0.0f;
+        uint64_t bad = parts ? 0 : __ballot(r < nrows && odd != 0.0f);  // pieces: the join looks
+        bad = (bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffffu;
+        if (r < nrows && !((bad >> c) & 1u)) put(r / a.group - tok0, kvh * a.group + r % a.group, 4 * g * C, y, m, l);
+        while (bad) {
+            const int w = r0 + 16 * n + __builtin_ctzll(bad);
+            bad &= bad - 1;
+            attend_row<T, D>(a, qs.begin + w / a.group, kvh * a.group + w % a.group, qs, ks);
+        }
+    };
+    if constexpr (WAVES == 1) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) odd += acc[n][t][i] * 0.0f;
-        // A weight of 0 times a value that is not finite is a NaN: rows that did not see that value are computed again,
-        // from the keys that they see alone.  The test costs nothing in the loop.
-        uint64_t again = __ballot(valid[n] && odd != 0.0f);
-        again = (again | again >> 16 | again >> 32 | again >> 48) & 0xffffu;
-        if constexpr (WAVES == 4) {
+        for (int n = 0; n < NS; ++n) {
+            float y[4 * C];
+#pragma unroll
+            for (int e = 0; e < 4 * C; ++e) y[e] = acc[n][e % C][e / C];
+            finish(n, y, top[n] * a.scale, sum[n][0]);
+        }
+    } else {
+        if constexpr (LISTED) __syncthreads();  // the table is through
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
 #pragma unroll
             for (int t = 0; t < C; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[wave][(n * 4 + i) * C + t][lane] = acc[n][t][i];
-            if (g == 0) part_ml[wave][n][c] = make_float2(natural, l);
-        } else if (valid[n] && !((again >> c) & 1u)) {
-            float y[4 * C];
-#pragma unroll
-            for (int e = 0; e < 4 * C; ++e) y[e] = acc[n][e % C][e / C];
-            put(tok[n], head[n], 4 * g * C, y, natural, l);
+            if (g == 0) part_ml[wave][n][c] = make_float2(top[n] * a.scale, sum[n][0]);
         }
-        while (again) {
-            const int w = __builtin_ctzll(again);
-            again &= again - 1;
-            const int r = r0 + 16 * n + w, tk = r / a.group, hd = kvh * a.group + r % a.group;
-            const int64_t row = qs.begin + tk;
-            const int32_t seen = a.causal ? max(0, min(ks.rows, tk + lag + 1)) : ks.rows;
-            const T *q = static_cast<const T *>(a.q) + row * a.q_stride + static_cast<int64_t>(hd) * D;
-            const T *k = static_cast<const T *>(a.k) + ks.begin * a.k_stride + static_cast<int64_t>(kvh) * D;
-            const T *v = static_cast<const T *>(a.v) + ks.begin * a.v_stride + static_cast<int64_t>(kvh) * D;
-            float o[2], m, l2;
-            attend_row<T, D, KC>(q, k, v, a, LISTED ? a.selected + (row * a.kv_heads + kvh) * a.top : nullptr, seen, piece, o,
-                                 &m, &l2);
-            const float rcp = l2 == 0.0f ? 0.0f : 1.0f / l2;
-            for (int e = 0; e < 2; ++e) {
-                const int d = lane + 64 * e;
-                if (d >= D) continue;
-                if (WAVES == 4) part[wave][WAVES == 4 ? (n * 4 + d / C % 4) * C + d % C : 0][d / (4 * C) * 16 + w] = o[e];
-                else if (parts) a.part_o[cell_of(tk - tok0, hd) * D + d] = o[e];
-                else
-                    store_from_f32<T>(static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(hd) * D + d,
-                                      l2 == 0.0f ? 0.0f : o[e] * rcp);
-            }
-            if (lane == 0) {
-                if (WAVES == 4) part_ml[wave][n][w] = make_float2(m, l2);
-                else if (parts) a.part_ml[cell_of(tk - tok0, hd)] = make_float2(m, l2);
-                else if (a.lse) a.lse[row * a.heads + hd] = l2 == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l2) * kLn2;
-            }
-        }
-    }
-    if constexpr (WAVES == 4) {
         __syncthreads();
-        // (set, i) pairs, NS for each wave: C (or with few sets, more) channels of each row a lane.
-        constexpr int PER = NS >= 4 ? 4 : NS;  // i's of one set that a wave joins
+        if (wave >= NS) return;
+        const int n = wave;  // a set for each wave
+        float m = neg_inf(), l = 0.0f, wgt[4], y[4 * C];
 #pragma unroll
-        for (int k = 0; k < NS / PER; ++k) {
-            const int pair = wave * NS + k * PER, n = pair >> 2, i0 = pair & 3;
-            float m = neg_inf(), l = 0.0f, wgt[4], y[PER * C];
+        for (int p = 0; p < 4; ++p)
+            if (part_ml[p][n][c].y != 0.0f) m = fmaxf(m, part_ml[p][n][c].x);
 #pragma unroll
-            for (int p = 0; p < 4; ++p)
-                if (part_ml[p][n][c].y != 0.0f) m = fmaxf(m, part_ml[p][n][c].x);
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const float2 ml = part_ml[p][n][c];
-                wgt[p] = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((ml.x - m) * kLog2e);  // a piece without keys: 0
-                l += wgt[p] * ml.y;
-            }
-#pragma unroll
-            for (int e = 0; e < PER * C; ++e) {
-                y[e] = 0.0f;
-#pragma unroll
-                for (int p = 0; p < 4; ++p) y[e] += wgt[p] * part[p][(n * 4 + i0 + e / C) * C + e % C][lane];
-            }
-            const int r = r0 + 16 * n + c;
-            if (r < nrows) put(r / a.group - tok0, kvh * a.group + r % a.group, (4 * g + i0) * C, y, m, l);
+        for (int p = 0; p < 4; ++p) {
+            const float2 ml = part_ml[p][n][c];
+            wgt[p] = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((ml.x - m) * kLog2e);  // a piece without keys: 0
+            l += wgt[p] * ml.y;
         }
+#pragma unroll
+        for (int e = 0; e < 4 * C; ++e) {
+            y[e] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) y[e] += wgt[p] * part[p][(n * 4 + e / C) * C + e % C][lane];
+        }
+        finish(n, y, m, l);
     }
 }
 
@@ -760,7 +742,8 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
     if (cell >= cells) return;
     const int64_t row = cell / a.heads;
     const int head = static_cast<int>(cell - row * a.heads);
-    if (sequence_of_row(a.q_starts, a.sequences, row) < 0) return;
+    const int64_t s = sequence_of_row(a.q_starts, a.sequences, row);
+    if (s < 0) return;
     float m = neg_inf();
     for (int p = 0; p < a.splits; ++p) {
         const float2 ml = a.part_ml[p * cells + cell];
@@ -775,6 +758,10 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
             if (lane + 64 * e < D) o[e] += w * a.part_o[(p * cells + cell) * D + lane + 64 * e];
+    }
+    if (__any((l + o[0] + o[1]) * 0.0f != 0.0f)) {  // not finite: see the tiles
+        attend_row<T, D>(a, row, head, sequence_span(a.q_starts, s, a.total_q), sequence_span(a.k_starts, s, a.total_k));
+        return;
     }
     const float r = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll

@@ -126,7 +126,7 @@ def attend(q, k, v, ql, kl, block, selected, scale, causal, bf16):
             for h in range(heads):
                 keys = np.arange(lk)
                 if selected is not None:
-                    mine = [b for b in selected[q0 + i, h // g] if 0 <= b < -(-lk // block)]
+                    mine = sorted({int(b) for b in selected[q0 + i, h // g] if 0 <= b < -(-lk // block)})
                     keys = np.concatenate([np.arange(b * block, min(lk, (b + 1) * block)) for b in mine] or [np.zeros(0, int)])
                 if causal:
                     keys = keys[keys <= i + lk - lq]

@@ -258,7 +258,7 @@ def test_block_attention(s3dx, dtype, case):
 
 @pytest.mark.parametrize("dtype", [0, 1])
 def test_lists_in_any_order(s3dx, dtype):
-    # unsorted, with blocks twice (they count twice) and entries that name no block
+    # unsorted, with blocks twice (they count once) and entries that name no block
     rng = np.random.default_rng(7)
     q, k, v = rows(rng, 70, 2, 64), rows(rng, 300, 2, 64), rows(rng, 300, 2, 64)
     sel = rng.integers(-3, 14, (70, 2, 9)).astype(np.int32)   # 10 blocks of 32
