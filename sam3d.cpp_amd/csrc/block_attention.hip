@@ -357,12 +357,15 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr int VW = C * static_cast<int>(sizeof(T)) / 4;
     constexpr int E = static_cast<int>(sizeof(T));
     static_assert(WAVES == 1 || WAVES == 4);
-    // The table of blocks, TABLE of them at a time for each tile of the workgroup; after the last, its waves' results:
-    // element (set n, i, t) of every lane, maxima and sums.
-    constexpr int TABLE = WAVES == 4 ? 4096 : 1024, TILES = 4 / WAVES;
+    // LDS: each wave's K rows of a step; the table of blocks, TABLE of them at a time for each tile of the
+    // workgroup; after the last step over both, the waves' results: element (set n, i, t) of every lane.
+    constexpr int TABLE = 1024, TILES = 4 / WAVES;
+    constexpr int CH = D * E / 16;                 // 16-byte pieces of a K row
+    constexpr int NP = KC * CH / 64;               // ... of a step, for each lane
+    constexpr int KEYS = KC * D * E, TABLES = LISTED ? TABLE * TILES * 8 : 0;
     constexpr int PART = WAVES == 4 ? 4 * NS * 4 * C * 64 * 4 : 0;
-    constexpr int LDS = LISTED && TABLE * TILES * 8 > PART ? TABLE * TILES * 8 : PART;
-    __shared__ alignas(16) char lds[LDS > 0 ? LDS : 16];
+    constexpr int LDS = 4 * KEYS + TABLES > PART ? 4 * KEYS + TABLES : PART;
+    __shared__ alignas(16) char lds[LDS];
     __shared__ float2 part_ml[WAVES == 4 ? 4 : 1][NS][16];
     auto part = reinterpret_cast<float (*)[NS * 4 * C][64]>(lds);
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -405,7 +408,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     const int least = a.causal ? max(0, min(ks.rows, tok0 + lag + 1)) : ks.rows;          // ... that all rows see
 
     // ---- the tile's steps of KC keys
-    uint64_t *table = reinterpret_cast<uint64_t *>(lds) + (WAVES == 4 ? 0 : wave * TABLE);
+    uint64_t *table = reinterpret_cast<uint64_t *>(lds + 4 * KEYS) + (WAVES == 4 ? 0 : wave * TABLE);
     const int blocks = (most + a.block - 1) >> a.block_log2;  // in reach of the tile
     int w0 = 0, chunk = 0, rank = 0;  // the table's first block, the next 64 of it, chosen blocks before them
     uint64_t todo = 0, mine = 0;      // this wave's blocks among the last 64; this lane's table entry of them
@@ -475,26 +478,37 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         for (int t = 0; t < C; ++t) acc[n][t] = f32x4{0, 0, 0, 0};
     }
     const float cs = a.scale * kLog2e;
-    // Byte offsets of this lane's rows in a step: held where registers allow, else the first and the steps between.
+    // Byte offsets of this lane's rows of V in a step: held where registers allow, else the first and the steps between.
     constexpr bool HELD = D < 128;
     const int kstep = static_cast<int>(a.k_stride) * E, vstep = static_cast<int>(a.v_stride) * E;
-    const int kat = c * kstep + 16 * g, vat = 4 * g * vstep + c * (C * E);
-    int koff[HELD ? KT : 1], voff[HELD ? KT : 1][4];
+    const int vat = 4 * g * vstep + c * (C * E);
+    int voff[HELD ? KT : 1][4];
     if constexpr (HELD) {
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
-            koff[t] = kat + 16 * t * kstep;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) voff[t][i] = vat + (16 * t + i) * vstep;
-        }
-    }
-    uint32_t kf[KT][QV][4];
-    const auto load_k = [&]() __attribute__((always_inline)) {
-        const auto r = rows_buffer<T, D>(a.k, ks.begin + first, a.k_stride, kvh, min(KC, ks.rows - first));
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int j = 0; j < QV; ++j) buffer_dwords<4>(r, (HELD ? koff[HELD ? t : 0] : kat + 16 * t * kstep) + 64 * j, kf[t][j]);
+            for (int i = 0; i < 4; ++i) voff[t][i] = vat + (16 * t + i) * vstep;
+    }
+    // K: lane l fetches pieces l, l + 64, ... of the step's rows, which lie in LDS row by row, a row's pieces xor-ed by its
+    // number so that eight neighbouring rows' pieces of one number lie in different banks.
+    const auto turned = [](int row, int piece) __attribute__((always_inline)) {
+        return piece ^ (CH % 8 == 0 ? row & 7 : (row >> 1) & 3);
+    };
+    char *kt = lds + wave * KEYS;
+    int koff[NP], kput[NP], kget[QV];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        const int row = (p * 64 + lane) / CH, piece = (p * 64 + lane) % CH;
+        koff[p] = row * kstep + piece * 16;
+        kput[p] = (row * CH + turned(row, piece)) * 16;
+    }
+#pragma unroll
+    for (int j = 0; j < QV; ++j) kget[j] = (c * CH + turned(c, 4 * j + g)) * 16;
+    uint32_t kn[NP][4];
+    const auto load_k = [&]() __attribute__((always_inline)) {
+        const auto r = rows_buffer<T, D>(a.k, ks.begin + first, a.k_stride, kvh, min(KC, ks.rows - first));
+#pragma unroll
+        for (int p = 0; p < NP; ++p) buffer_dwords<4>(r, koff[p], kn[p]);
     };
 
     if constexpr (LISTED) first = end = 0;
@@ -528,6 +542,21 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) buffer_dwords<VW>(r, HELD ? voff[HELD ? t : 0][i] : vat + (16 * t + i) * vstep, vf[t][i]);
         }
+        // ---- K of this step to its operand's lanes, the next step's on its way
+        uint32_t kf[KT][QV][4];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) *reinterpret_cast<u32x4 *>(kt + kput[p]) = u32x4{kn[p][0], kn[p][1], kn[p][2], kn[p][3]};
+        more = next();
+        if (more) load_k();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int j = 0; j < QV; ++j) {
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(kt + kget[j] + t * (16 * CH * 16));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kf[t][j][i] = x[i];
+            }
         // ---- sets of 16 rows: S^T, weights
         f32x4 w[NS][KT];
         u32x4 pw[NS][KT / 2 > 0 ? KT / 2 : 1];
@@ -608,8 +637,6 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                 }
             }
         }
-        more = next();
-        if (more) load_k();
         // ---- O^T
         if constexpr (BF) {
             const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
@@ -702,7 +729,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             finish(n, y, top[n] * a.scale, sum[n][0]);
         }
     } else {
-        if constexpr (LISTED) __syncthreads();  // the table is through
+        __syncthreads();  // the steps' LDS is through
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
