@@ -362,10 +362,10 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr int TABLE = 1024, TILES = 4 / WAVES;
     constexpr int CH = D * E / 16;                 // 16-byte pieces of a K row
     constexpr int NP = KC * CH / 64;               // ... of a step, for each lane
-    constexpr int KEYS = KC * D * E, TABLES = LISTED ? TABLE * TILES * 8 : 0;
+    constexpr int KEYS = BF ? KC * D * E : 0, TABLES = LISTED ? TABLE * TILES * 8 : 0;
     constexpr int PART = WAVES == 4 ? 4 * NS * 4 * C * 64 * 4 : 0;
     constexpr int LDS = 4 * KEYS + TABLES > PART ? 4 * KEYS + TABLES : PART;
-    __shared__ alignas(16) char lds[LDS];
+    __shared__ alignas(16) char lds[LDS > 0 ? LDS : 16];
     __shared__ float2 part_ml[WAVES == 4 ? 4 : 1][NS][16];
     auto part = reinterpret_cast<float (*)[NS * 4 * C][64]>(lds);
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -375,7 +375,9 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     const int id = xcd_tile(blockIdx.x, gridDim.x);
     const int split = id / a.tile_groups % a.splits, kvh = id / a.tile_groups / a.splits;
     int tg = id % a.tile_groups;
-    if (a.causal) tg = a.tile_groups - 1 - tg;  // longest rows first
+    // Causal rows see more keys the later they stand: every eighth group in a row, so that the XCDs' runs cost alike,
+    // and the longest first.
+    if (a.causal) tg = a.tile_groups - 1 - (tg % (a.tile_groups >> 3) * 8 + tg / (a.tile_groups >> 3));
     const int64_t tile = WAVES == 4 ? tg : static_cast<int64_t>(tg) * 4 + wave;
     const int64_t s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, a.group, ROWS, tile);
     const Span qs = sequence_span(a.q_starts, s, a.total_q), ks = sequence_span(a.k_starts, s, a.total_k);
@@ -495,20 +497,32 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         return piece ^ (CH % 8 == 0 ? row & 7 : (row >> 1) & 3);
     };
     char *kt = lds + wave * KEYS;
-    int koff[NP], kput[NP], kget[QV];
+    int koff[BF ? NP : KT], kput[BF ? NP : 1], kget[BF ? QV : 1];
+    if constexpr (BF) {
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-        const int row = (p * 64 + lane) / CH, piece = (p * 64 + lane) % CH;
-        koff[p] = row * kstep + piece * 16;
-        kput[p] = (row * CH + turned(row, piece)) * 16;
+        for (int p = 0; p < NP; ++p) {
+            const int row = (p * 64 + lane) / CH, piece = (p * 64 + lane) % CH;
+            koff[p] = row * kstep + piece * 16;
+            kput[p] = (row * CH + turned(row, piece)) * 16;
+        }
+#pragma unroll
+        for (int j = 0; j < QV; ++j) kget[j] = (c * CH + turned(c, 4 * j + g)) * 16;
+    } else {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) koff[t] = (16 * t + c) * kstep + 16 * g;
     }
-#pragma unroll
-    for (int j = 0; j < QV; ++j) kget[j] = (c * CH + turned(c, 4 * j + g)) * 16;
-    uint32_t kn[NP][4];
+    uint32_t kn[BF ? NP : 1][4], kf[KT][QV][4];
     const auto load_k = [&]() __attribute__((always_inline)) {
         const auto r = rows_buffer<T, D>(a.k, ks.begin + first, a.k_stride, kvh, min(KC, ks.rows - first));
+        if constexpr (BF) {
 #pragma unroll
-        for (int p = 0; p < NP; ++p) buffer_dwords<4>(r, koff[p], kn[p]);
+            for (int p = 0; p < NP; ++p) buffer_dwords<4>(r, koff[p], kn[p]);
+        } else {
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int j = 0; j < QV; ++j) buffer_dwords<4>(r, koff[t] + 64 * j, kf[t][j]);
+        }
     };
 
     if constexpr (LISTED) first = end = 0;
@@ -543,20 +557,21 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                 for (int i = 0; i < 4; ++i) buffer_dwords<VW>(r, HELD ? voff[HELD ? t : 0][i] : vat + (16 * t + i) * vstep, vf[t][i]);
         }
         // ---- K of this step to its operand's lanes, the next step's on its way
-        uint32_t kf[KT][QV][4];
+        if constexpr (BF) {
 #pragma unroll
-        for (int p = 0; p < NP; ++p) *reinterpret_cast<u32x4 *>(kt + kput[p]) = u32x4{kn[p][0], kn[p][1], kn[p][2], kn[p][3]};
-        more = next();
-        if (more) load_k();
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int p = 0; p < NP; ++p) *reinterpret_cast<u32x4 *>(kt + kput[p]) = u32x4{kn[p][0], kn[p][1], kn[p][2], kn[p][3]};
+            more = next();
+            if (more) load_k();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+            for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int j = 0; j < QV; ++j) {
-                const u32x4 x = *reinterpret_cast<const u32x4 *>(kt + kget[j] + t * (16 * CH * 16));
+                for (int j = 0; j < QV; ++j) {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(kt + kget[j] + t * (16 * CH * 16));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) kf[t][j][i] = x[i];
-            }
+                    for (int i = 0; i < 4; ++i) kf[t][j][i] = x[i];
+                }
+        }
         // ---- sets of 16 rows: S^T, weights
         f32x4 w[NS][KT];
         u32x4 pw[NS][KT / 2 > 0 ? KT / 2 : 1];
@@ -636,6 +651,10 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                                      pack_bf16x2(hi[2], hi[3])};
                 }
             }
+        }
+        if constexpr (!BF) {
+            more = next();
+            if (more) load_k();
         }
         // ---- O^T
         if constexpr (BF) {
@@ -999,7 +1018,8 @@ S3DX_API s3dx_status s3dx_block_attention(const void *q, const void *k, const vo
         require(!selected || aligned(selected, 4), "selected is not aligned");
         require(!lse || aligned(lse, 4), "lse is not aligned");
         require(total_q * heads <= std::numeric_limits<int32_t>::max(), "total_q * heads is out of range");
-        const AttendCut cut = attend_cut(dtype == S3DX_BF16, total_q, heads, kv_heads, head_dim, sequences, block, top, max_k);
+        AttendCut cut = attend_cut(dtype == S3DX_BF16, total_q, heads, kv_heads, head_dim, sequences, block, top, max_k);
+        if (flags & S3DX_BLOCK_CAUSAL) cut.tile_groups = (cut.tile_groups + 7) / 8 * 8;  // see the kernel's order of tiles
         AttendArgs a = {q, k, v, o, lse, q_starts, k_starts, selected, total_q, total_k, q_stride, k_stride, v_stride, o_stride,
                         sequences, heads, heads / kv_heads, kv_heads, block, block == 32 ? 5 : block == 64 ? 6 : 7, top,
                         flags & S3DX_BLOCK_CAUSAL, cut.splits, static_cast<int32_t>(cut.tile_groups), softmax_scale, nullptr,
