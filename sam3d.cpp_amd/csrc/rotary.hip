@@ -44,9 +44,10 @@ struct TurnArgs {
     HeadRows part[2];  // queries, keys
     const int32_t *positions;
     int64_t position_stride, n;
-    int32_t d, pairs, halves, inverse, norm, gain_stride;
+    int32_t d, pairs, halves, inverse, norm, gain_stride, rows, lanes_log2;
     float eps;
 };
+constexpr int kMaxRows = 4;  // of a workgroup
 
 // cos and sin of a 0.64 fixed-point part of a turn.  The quarter turn is split
 // off in integers, so that the float holds at most an eighth of a turn.
@@ -68,70 +69,184 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
-// One wave per head row, any head_dim up to 256, any stride and alignment: lane
-// l holds pairs l and l + 64 and, of the channels that are not turned, every
-// 64th.  A lane reads what it writes and nothing else, so y may be x.
-template <class TI, class TO>
+// 8 elements at p (16-byte aligned) as floats, and back, rounded to nearest even.
+template <class T>
+__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+    constexpr int N = 8 * static_cast<int>(sizeof(T)) / 16;
+    uint4 t[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = reinterpret_cast<const uint4 *>(p)[i];
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        v[e] = sizeof(T) == 4 ? __builtin_bit_cast(float, w[e])
+                              : __builtin_bit_cast(float, e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+}
+template <class T>
+__device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                                                   pack_bf16x2(v[6], v[7]));
+    } else {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+}
+
+// A workgroup takes `rows` rows: it makes their angles' cosines and sines once, in LDS, for all heads;
+// then its waves take the rows' heads.  The work is the memory's: every head is read
+// and written once (28,265 rows x 16 heads x 64 BF16, 116 MB: 25 us at a copy's rate).
+//
+// VEC: a lane owns 16 channels, two pieces of 8 (bf16: 16 bytes): neighbours where
+// neighbours are paired, else the piece of the first channels and that of the second; lane groups of
+// a power of two take a head, so a wave takes several side by side.  For head_dim a
+// multiple of 16, aligned rows, and pairs of halves in whole pieces.  Else one wave takes a head,
+// a pair (or a channel that does not turn) at a time in each lane, at any width and alignment.
+// In both a lane reads what it writes and nothing else, so y may be x.
+template <class TI, class TO, bool VEC>
 __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
-    const int lane = threadIdx.x & 63;
-    const int64_t heads = a.part[0].heads + a.part[1].heads;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (item >= a.n * heads) return;
-    const int64_t row = item / heads;
-    int32_t head = static_cast<int32_t>(item - row * heads);
-    const HeadRows &p = head < a.part[0].heads ? a.part[0] : a.part[1];
-    if (head >= a.part[0].heads) head -= a.part[0].heads;
-    const TI *x = static_cast<const TI *>(p.x) + row * p.x_stride + static_cast<int64_t>(head) * a.d;
-    TO *y = static_cast<TO *>(p.y) + row * p.y_stride + static_cast<int64_t>(head) * a.d;
-    const float *gain = p.gain ? p.gain + static_cast<int64_t>(head) * a.gain_stride : nullptr;
-    const int step = a.halves ? 1 : 2, apart = a.halves ? a.pairs : 1;
-    float first[2], second[2], rest[4];
-    float sum = 0.0f;
+    __shared__ float2 turns[kMaxRows][kMaxPairs];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.rows;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(a.rows), a.n - row0));
+    for (int e = threadIdx.x; e < rows * a.pairs; e += 256) {
+        const int r = e / a.pairs, j = e - r * a.pairs;
+        const int64_t pos = a.positions[(row0 + r) * a.position_stride + t.axis[j]];
+        float c, s;
+        turn_cos_sin(static_cast<uint64_t>(pos) * t.turns[j], &c, &s);
+        turns[r][j] = make_float2(c, a.inverse ? -s : s);
+    }
+    __syncthreads();
+    const int heads = a.part[0].heads + a.part[1].heads;
+    const int lanes = VEC ? 1 << a.lanes_log2 : 64, side = 64 / lanes;  // lanes of a head, heads of a wave
+    const int sets = (heads + side - 1) / side;
+    for (int item = wave; item < rows * sets; item += 4) {
+        const int r = item / sets;
+        int head = (item - r * sets) * side + lane / lanes;
+        const bool k = head >= a.part[0].heads;
+        const HeadRows &p = a.part[k ? 1 : 0];
+        const bool here = head < heads;
+        if (k) head -= a.part[0].heads;
+        const TI *x = static_cast<const TI *>(p.x) + (row0 + r) * p.x_stride + static_cast<int64_t>(head) * a.d;
+        TO *y = static_cast<TO *>(p.y) + (row0 + r) * p.y_stride + static_cast<int64_t>(head) * a.d;
+        const float *gain = p.gain ? p.gain + static_cast<int64_t>(head) * a.gain_stride : nullptr;
+        if constexpr (VEC) {
+            const int l = lane & (lanes - 1), turning = a.pairs / 8;
+            const bool active = here && l < a.d / 16;
+            // this lane's two pieces of 8 channels
+            const int c0 = a.halves ? (l < turning ? 8 * l : 16 * l) : 16 * l;
+            const int c1 = a.halves && l < turning ? c0 + a.pairs : c0 + 8;
+            float u[8], v[8], gu[8], gv[8];
+            if (active) {
+                load8(x + c0, u);
+                load8(x + c1, v);
+                if (gain) {
+                    load8(gain + c0, gu);
+                    load8(gain + c1, gv);
+                }
+            }
+            float scale = 1.0f;
+            if (a.norm) {
+                float sum = 0.0f;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int j = lane + 64 * q, c = j * step;
-        first[q] = second[q] = 0.0f;
-        if (j >= a.pairs) continue;
-        first[q] = load_as_f32<TI>(x + c);
-        second[q] = load_as_f32<TI>(x + c + apart);
-        sum += first[q] * first[q] + second[q] * second[q];
-        if (gain) {
-            first[q] *= gain[c];
-            second[q] *= gain[c + apart];
+                for (int e = 0; e < 8; ++e) sum += active ? u[e] * u[e] + v[e] * v[e] : 0.0f;
+                for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
+                scale = rsqrtf(sum / static_cast<float>(a.d) + a.eps);
+            }
+            if (!active) continue;
+            if (a.norm) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    u[e] *= gain ? gu[e] * scale : scale;
+                    v[e] *= gain ? gv[e] * scale : scale;
+                }
+            }
+            // pairs 8l..8l+7, in the table's order
+            const float2 *cs = &turns[r][8 * l];
+            if (a.halves) {
+                if (l < turning) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 q = cs[e];
+                        const float first = u[e] * q.x - v[e] * q.y;
+                        v[e] = u[e] * q.y + v[e] * q.x;
+                        u[e] = first;
+                    }
+                }
+            } else {
+                // channels behind the last pair stay as they are (an infinity among them too)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (8 * l + e < a.pairs) {
+                        const float2 q = cs[e];
+                        const float first = u[2 * e] * q.x - u[2 * e + 1] * q.y;
+                        u[2 * e + 1] = u[2 * e] * q.y + u[2 * e + 1] * q.x;
+                        u[2 * e] = first;
+                    }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (8 * l + 4 + e < a.pairs) {
+                        const float2 q = cs[4 + e];
+                        const float first = v[2 * e] * q.x - v[2 * e + 1] * q.y;
+                        v[2 * e + 1] = v[2 * e] * q.y + v[2 * e + 1] * q.x;
+                        v[2 * e] = first;
+                    }
+            }
+            store8(y + c0, u);
+            store8(y + c1, v);
+        } else {
+            const int step = a.halves ? 1 : 2, apart = a.halves ? a.pairs : 1;
+            float first[2], second[2], rest[4], sum = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int j = lane + 64 * q, c = j * step;
+                first[q] = second[q] = 0.0f;
+                if (j >= a.pairs) continue;
+                first[q] = load_as_f32<TI>(x + c);
+                second[q] = load_as_f32<TI>(x + c + apart);
+                sum += first[q] * first[q] + second[q] * second[q];
+                if (gain) {
+                    first[q] *= gain[c];
+                    second[q] *= gain[c + apart];
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int c = 2 * a.pairs + lane + 64 * q;
+                rest[q] = 0.0f;
+                if (c >= a.d) continue;
+                rest[q] = load_as_f32<TI>(x + c);
+                sum += rest[q] * rest[q];
+                if (gain) rest[q] *= gain[c];
+            }
+            const float scale = a.norm ? rsqrtf(wave_sum(sum) / static_cast<float>(a.d) + a.eps) : 1.0f;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int j = lane + 64 * q, c = j * step;
+                if (j >= a.pairs) continue;
+                const float2 cs = turns[r][j];
+                store_from_f32<TO>(y + c, (first[q] * cs.x - second[q] * cs.y) * scale);
+                store_from_f32<TO>(y + c + apart, (first[q] * cs.y + second[q] * cs.x) * scale);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int c = 2 * a.pairs + lane + 64 * q;
+                if (c < a.d) store_from_f32<TO>(y + c, rest[q] * scale);
+            }
         }
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int c = 2 * a.pairs + lane + 64 * q;
-        rest[q] = 0.0f;
-        if (c >= a.d) continue;
-        rest[q] = load_as_f32<TI>(x + c);
-        sum += rest[q] * rest[q];
-        if (gain) rest[q] *= gain[c];
-    }
-    const float r = a.norm ? rsqrtf(wave_sum(sum) / static_cast<float>(a.d) + a.eps) : 1.0f;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int j = lane + 64 * q, c = j * step;
-        if (j >= a.pairs) continue;
-        const int64_t pos = a.positions[row * a.position_stride + t.axis[j]];
-        float cs, sn;
-        turn_cos_sin(static_cast<uint64_t>(pos) * t.turns[j], &cs, &sn);
-        if (a.inverse) sn = -sn;
-        store_from_f32<TO>(y + c, (first[q] * cs - second[q] * sn) * r);
-        store_from_f32<TO>(y + c + apart, (first[q] * sn + second[q] * cs) * r);
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int c = 2 * a.pairs + lane + 64 * q;
-        if (c < a.d) store_from_f32<TO>(y + c, rest[q] * r);
     }
 }
 
 using TurnFn = void (*)(TurnArgs, TurnTable);
+template <bool VEC>
 TurnFn pick_turn(int32_t in, int32_t out) {
-    if (in == S3DX_BF16) return out == S3DX_BF16 ? turn_kernel<uint16_t, uint16_t> : turn_kernel<uint16_t, float>;
-    return out == S3DX_BF16 ? turn_kernel<float, uint16_t> : turn_kernel<float, float>;
+    if (in == S3DX_BF16) return out == S3DX_BF16 ? turn_kernel<uint16_t, uint16_t, VEC> : turn_kernel<uint16_t, float, VEC>;
+    return out == S3DX_BF16 ? turn_kernel<float, uint16_t, VEC> : turn_kernel<float, float, VEC>;
+}
+
+bool whole_pieces(const HeadRows &p, int32_t in, int32_t out) {
+    return p.heads == 0 || (aligned(p.x, 16) && aligned(p.y, 16) && aligned(p.gain, 16) &&
+                            p.x_stride * dtype_size(in) % 16 == 0 && p.y_stride * dtype_size(out) % 16 == 0);
 }
 
 void check_rows(const HeadRows &p, int32_t d, int64_t n, int32_t in, int32_t out) {
@@ -147,15 +262,20 @@ void check_rows(const HeadRows &p, int32_t d, int64_t n, int32_t in, int32_t out
             "in place needs the same dtype and stride for x and y");
 }
 
-void launch_turn(const TurnArgs &a, const s3dx_rotary *rotary, int32_t in, int32_t out, hipStream_t stream) {
+void launch_turn(TurnArgs a, const s3dx_rotary *rotary, int32_t in, int32_t out, hipStream_t stream) {
     if (a.n == 0) return;
     TurnTable t = {};
     if (rotary) {
         std::memcpy(t.turns, rotary->turns, sizeof t.turns);
         std::memcpy(t.axis, rotary->axis, sizeof t.axis);
     }
-    const int64_t items = a.n * (a.part[0].heads + a.part[1].heads);
-    pick_turn(in, out)<<<dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream>>>(a, t);
+    const bool vec = a.d % 16 == 0 && (!a.halves || a.pairs % 8 == 0) && whole_pieces(a.part[0], in, out) &&
+                     whole_pieces(a.part[1], in, out);
+    while ((16 << a.lanes_log2) < a.d) ++a.lanes_log2;
+    // Four rows to a workgroup, unless that leaves compute units without one.
+    a.rows = a.n >= 4 * 256 ? kMaxRows : 1;
+    (vec ? pick_turn<true>(in, out) : pick_turn<false>(in, out))<<<
+        dim3(static_cast<unsigned>((a.n + a.rows - 1) / a.rows)), dim3(256), 0, stream>>>(a, t);
     launch_check("rotary");
 }
 

@@ -180,6 +180,22 @@ def test_a_row_with_nan_or_infinity_stays_alone(s3dx):
     assert np.isnan(e[4, 1]).all() and np.isnan(e[9, 2, 0])
 
 
+@pytest.mark.parametrize("adjacent", [True, False])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_channels_that_do_not_turn_are_copied(s3dx, adjacent, pad):
+    # NaN and infinities among them reach no other channel
+    rng = np.random.default_rng(11)
+    n, h, d = 9, 2, 64
+    x = rng.standard_normal((n, h * d + pad)).astype(np.float32)
+    x[:, 48: 64: 3] = np.inf
+    x[2, 49] = np.nan
+    rot = s3dx.Rotary.per_axis(d, [8, 8, 8], pairing=s3dx.ROTARY_ADJACENT if adjacent else s3dx.ROTARY_HALVES)
+    y = s3dx.DeviceArray((n, h, d), np.float32)
+    rot.apply(R.dev(s3dx, x), s3dx.F32, n, h, R.dev(s3dx, rng.integers(0, 64, (n, 3)).astype(np.int32)), y, x_stride=h * d + pad)
+    got, want = y.download(), x[:, : h * d].reshape(n, h, d)
+    assert np.array_equal(got[..., 48:], want[..., 48:], equal_nan=True) and np.isfinite(got[..., :48]).all()
+
+
 def test_rotary_captured_and_replayed(s3dx):
     rng = np.random.default_rng(10)
     n, h, d = 300, 16, 64
