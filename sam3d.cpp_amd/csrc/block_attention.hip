@@ -4,6 +4,7 @@
 // slat_flow_graph.cpp:304-434, and the decoders' windows,
 // gs_decoder_graph.cpp:93-121, which the reference runs as dense attention).
 #include <cmath>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -76,41 +77,59 @@ struct IndexArgs {
     float *scale;
 };
 
-// One wave per (index row, key head); lane l sums channels l and l + 64 in 64
-// bits, so that the order of the rows does not show.
+// One workgroup per index row and up to 256 channels (whole heads): 32 lanes read a
+// row's channels, 8 each, eight rows at a time; sums in 64 bits, so that their order does
+// not show in a code.  The work is reading the keys once.
 template <class T>
 __global__ void __launch_bounds__(256) index_kernel(IndexArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (item >= a.rows * a.kv_heads) return;
-    const int64_t row = item / a.kv_heads;
-    const int head = static_cast<int>(item - row * a.kv_heads);
+    __shared__ double sums[8][256];
+    __shared__ uint64_t most[8];
+    const int tid = threadIdx.x, lane = tid & 31, part = tid >> 5;
+    const int per = 256 / a.d;  // heads of a workgroup
+    const int64_t row = blockIdx.x;
+    const int head0 = static_cast<int>(blockIdx.y) * per, channels = min(per, a.kv_heads - head0) * a.d;
     const int64_t s = sequence_of_unit(a.k_starts, a.sequences, a.total_k, 1, a.block, row);
     const Span k = sequence_span(a.k_starts, s, a.total_k);
     const int64_t first = (row - (k.begin / a.block + s)) * a.block;
     const int count = static_cast<int>(min(static_cast<int64_t>(a.block), k.rows - first));
-    if (first < 0 || count <= 0) return;
-    const T *x = static_cast<const T *>(a.k) + (k.begin + first) * a.k_stride + static_cast<int64_t>(head) * a.d;
-    double m[2] = {0.0, 0.0};
-    for (int r = 0; r < count; ++r)
-        for (int q = 0; q < 2; ++q)
-            if (lane + 64 * q < a.d) m[q] += static_cast<double>(load_as_f32<T>(x + r * a.k_stride + lane + 64 * q));
-    double most = 0.0;
-    bool fine = true;
-    for (int q = 0; q < 2; ++q) {
-        m[q] /= count;
-        fine = fine && fabs(m[q]) < __builtin_inf();
-        most = fmax(most, fabs(m[q]));
+    if (first < 0 || count <= 0) return;  // the whole workgroup
+    if (tid < 8) most[tid] = 0;
+    double m[8] = {};
+    if (8 * lane < channels) {
+        const T *x = static_cast<const T *>(a.k) + (k.begin + first) * a.k_stride + static_cast<int64_t>(head0) * a.d + 8 * lane;
+#pragma unroll 4
+        for (int r = part; r < count; r += 8) {
+            constexpr int N = 8 * static_cast<int>(sizeof(T)) / 16;
+            uint4 t[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) t[i] = reinterpret_cast<const uint4 *>(x + r * a.k_stride)[i];
+            const uint32_t *w = reinterpret_cast<const uint32_t *>(t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                m[e] += static_cast<double>(__builtin_bit_cast(
+                    float, sizeof(T) == 4 ? w[e] : e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16));
+        }
     }
-    for (int o = 1; o < 64; o <<= 1) most = fmax(most, __shfl_xor(most, o, 64));
-    fine = __all(fine) && codes_fine(most);
-    const int e = exponent_of(most);
-    const double up = two_to(6 - e);
-    int8_t *c = a.codes + (static_cast<int64_t>(head) * a.rows + row) * a.d;
-    for (int q = 0; q < 2; ++q)
-        if (lane + 64 * q < a.d) c[lane + 64 * q] = static_cast<int8_t>(fine ? code_of(m[q], up) : 0);
-    if (lane == 0)
-        a.scale[static_cast<int64_t>(head) * a.rows + row] = fine ? static_cast<float>(two_to(e - 6)) : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[part][8 * lane + e] = m[e];
+    __syncthreads();
+    double mean = 0.0;
+    if (tid < channels) {
+        for (int p = 0; p < 8; ++p) mean += sums[p][tid];
+        mean /= count;
+        // bits of magnitudes rise with them; infinities and NaN stand above all
+        atomicMax(reinterpret_cast<unsigned long long *>(&most[tid / a.d]),
+                  __builtin_bit_cast(unsigned long long, fabs(mean)));
+    }
+    __syncthreads();
+    if (tid >= channels) return;
+    const int head = head0 + tid / a.d, c = tid % a.d;
+    const double big = __builtin_bit_cast(double, most[tid / a.d]);
+    const bool fine = codes_fine(big);
+    const int e = exponent_of(big);
+    a.codes[(static_cast<int64_t>(head) * a.rows + row) * a.d + c] =
+        static_cast<int8_t>(fine ? code_of(mean, two_to(6 - e)) : 0);
+    if (c == 0) a.scale[static_cast<int64_t>(head) * a.rows + row] = fine ? static_cast<float>(two_to(e - 6)) : 0.0f;
 }
 
 // ---------------------------------------------------------------------------
@@ -123,86 +142,236 @@ struct SelectArgs {
     const float *scale;
     int32_t *selected;
     int64_t total_q, total_k, q_stride, sequences, rows;
-    int32_t kv_heads, group, d, block, top, most_blocks, flags;
+    int32_t kv_heads, group, d, block, top, most_blocks, flags, run;
 };
 
-// A float's order as an unsigned whole number (-0 does not occur: scores are
-// whole numbers times powers of two).
+// A float's order as an unsigned whole number: 0x007fffff (-inf) to 0xff800000 (inf).  -0 does not
+// occur: scores are whole numbers times powers of two.
 __device__ __forceinline__ uint32_t order_key(float f) {
     const uint32_t u = __builtin_bit_cast(uint32_t, f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+constexpr uint32_t kNearKey = 0xff800001u;  // above every score
 
-// One wave per (query row, key head): scores into LDS, then `top` times the
-// largest that is left.
-template <class T>
-__global__ void __launch_bounds__(64) select_kernel(SelectArgs a) {
-    extern __shared__ uint32_t keys[];
-    __shared__ int8_t qc[128];
-    const int lane = threadIdx.x;
-    const int64_t row = blockIdx.x / a.kv_heads;
-    const int head = static_cast<int>(blockIdx.x - row * a.kv_heads);
-    const int64_t s = sequence_of_row(a.q_starts, a.sequences, row);
-    if (s < 0) return;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// Sum over a team of 16, 64 or 256 threads, in each of them; `box` is for 256.
+template <int TEAM>
+__device__ __forceinline__ int team_sum(int v, int *box) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);  // row_ror:8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x124, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x122, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x121, 0xf, 0xf, false);
+    if constexpr (TEAM >= 64) {
+        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = static_cast<int>(a[0] + a[1]);
+        const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = static_cast<int>(b[0] + b[1]);
+    }
+    if constexpr (TEAM == 256) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = box[0] + box[1] + box[2] + box[3];
+    }
+    return v;
+}
+// Sum over the team's threads before this one.
+template <int TEAM>
+__device__ __forceinline__ int team_before(int v, int *box) {
+    constexpr int W = TEAM < 64 ? TEAM : 64;
+    const int at = threadIdx.x & (W - 1);
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < W; o <<= 1) {
+        const int y = __shfl_up(x, o, W);
+        if (at >= o) x += y;
+    }
+    if constexpr (TEAM == 256) {
+        const int wave = threadIdx.x >> 6;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 63) box[wave] = x;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) x += box[w];
+    }
+    return x - v;
+}
+
+// A tile of QT queries of one key head.  Scores by integer products (16x16x64: blocks by
+// queries), their order keys in LDS; then a team of 256 / QT threads for each query, each with a run
+// of blocks side by side, finds the `top`-th largest key by halving the range
+// of keys (a count of the keys above the middle each time; it stops as soon as the count is
+// right) and writes its run's chosen blocks behind those of the threads before it, equal
+// keys first come, first served.  HELD: a thread's keys (at most 16) stay in registers.
+// QT 16 fills the products; 4 and 1 are for few rows, and for more blocks than LDS
+// holds of 16 queries.
+template <class T, int QT, bool HELD>
+__global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
+    constexpr int TEAM = 256 / QT;
+    extern __shared__ uint32_t keys[];  // [QT][TEAM * run]
+    __shared__ alignas(16) int8_t qc[16][128];
+    __shared__ int box[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int64_t tile = blockIdx.x / a.kv_heads;
+    const int head = static_cast<int>(blockIdx.x - tile * a.kv_heads);
+    const int64_t s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, 1, QT, tile);
     const Span qs = sequence_span(a.q_starts, s, a.total_q), ks = sequence_span(a.k_starts, s, a.total_k);
-    int32_t *out = a.selected + (row * a.kv_heads + head) * a.top;
-    const T *q = static_cast<const T *>(a.q) + row * a.q_stride + static_cast<int64_t>(head) * a.group * a.d;
-    double m[2] = {0.0, 0.0}, most = 0.0;
-    bool fine = true;
-    for (int w = 0; w < 2; ++w) {
-        if (lane + 64 * w < a.d)
-            for (int g = 0; g < a.group; ++g)
-                m[w] += static_cast<double>(load_as_f32<T>(q + static_cast<int64_t>(g) * a.d + lane + 64 * w));
-        fine = fine && fabs(m[w]) < __builtin_inf();
-        most = fmax(most, fabs(m[w]));
+    const int64_t first = (tile - (qs.begin / QT + s)) * QT;
+    if (first < 0 || first >= qs.rows) return;  // the whole workgroup
+    const int row0 = static_cast<int>(first), queries = min(QT, qs.rows - row0);
+
+    // ---- the queries' codes, 16 threads each
+    {
+        const int q = tid >> 4, l = tid & 15, per = a.d / 16;
+        double m[8] = {}, most = 0.0;
+        bool fine = true;
+        if (q < queries) {
+            const T *x = static_cast<const T *>(a.q) + (qs.begin + row0 + q) * a.q_stride +
+                         static_cast<int64_t>(head) * a.group * a.d + l * per;
+            for (int h = 0; h < a.group; ++h)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < per) m[e] += static_cast<double>(load_as_f32<T>(x + static_cast<int64_t>(h) * a.d + e));
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            fine = fine && fabs(m[e]) < __builtin_inf();
+            most = fmax(most, fabs(m[e]));
+        }
+        int all = fine ? 1 : 0;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            most = fmax(most, __shfl_xor(most, o, 16));
+            all &= __shfl_xor(all, o, 16);
+        }
+        fine = all && codes_fine(most);
+        const double up = two_to(6 - exponent_of(most));
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < per) qc[q][l * per + e] = static_cast<int8_t>(fine ? code_of(m[e], up) : 0);
     }
-    for (int o = 1; o < 64; o <<= 1) most = fmax(most, __shfl_xor(most, o, 64));
-    fine = __all(fine) && codes_fine(most);
-    const double up = two_to(6 - exponent_of(most));
-    for (int w = 0; w < 2; ++w)
-        if (lane + 64 * w < a.d) qc[lane + 64 * w] = static_cast<int8_t>(fine ? code_of(m[w], up) : 0);
     __syncthreads();
-    const int32_t place = static_cast<int32_t>(row - qs.begin) + ks.rows - qs.rows;
-    int32_t nb = min((ks.rows + a.block - 1) / a.block, a.most_blocks);
-    if (a.flags & S3DX_BLOCK_CAUSAL) nb = place < 0 ? 0 : min(nb, place / a.block + 1);
+
+    // ---- scores
+    const int nb = min((ks.rows + a.block - 1) / a.block, a.most_blocks), lag = ks.rows - qs.rows;
+    const int run = a.run;  // blocks of a thread, a multiple of 4
     const int64_t base = static_cast<int64_t>(head) * a.rows + ks.begin / a.block + s;
-    for (int b = lane; b < nb; b += 64) {
-        const int8_t *c = a.codes + (base + b) * a.d;
-        int dot = 0;
-        for (int i = 0; i < a.d; ++i) dot += static_cast<int>(qc[i]) * static_cast<int>(c[i]);
-        uint32_t key = order_key(static_cast<float>(dot) * a.scale[base + b]);
-        if ((a.flags & S3DX_BLOCK_NEAR) && place >= 0 && b == place / a.block) key = 0xffffffffu;
-        keys[b] = key;
+    const auto candidates = [&](int q) __attribute__((always_inline)) {  // blocks that query q may choose
+        const int place = row0 + q + lag;
+        return !(a.flags & S3DX_BLOCK_CAUSAL) ? nb : place < 0 ? 0 : min(nb, place / a.block + 1);
+    };
+    i32x4 qf[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+        qf[t] = 64 * t + 16 * g < a.d ? *reinterpret_cast<const i32x4 *>(&qc[c][64 * t + 16 * g]) : i32x4{0, 0, 0, 0};
+    const int place = row0 + c + lag, near = a.flags & S3DX_BLOCK_NEAR && place >= 0 ? place / a.block : -1;
+    const int seen = candidates(c);
+    for (int j = wave; j < TEAM * run / 16; j += 4) {
+        const int b = 16 * j + c;
+        const int8_t *code = a.codes + (base + min(b, nb - 1)) * a.d;
+        i32x4 dot = {0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            i32x4 x = {0, 0, 0, 0};
+            if (b < nb && 64 * t + 16 * g < a.d) x = *reinterpret_cast<const i32x4 *>(code + 64 * t + 16 * g);
+            if (t == 0 || a.d > 64) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, qf[t], dot, 0, 0, 0);
+        }
+        uint32_t key[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = 16 * j + 4 * g + i;
+            // |dot| < 2^21: the product with a power of two is exact
+            key[i] = at < seen ? order_key(static_cast<float>(dot[i]) * a.scale[base + at]) : 0u;
+            if (at == near && at < seen) key[i] = kNearKey;
+        }
+        if (c < QT)
+            *reinterpret_cast<uint4 *>(&keys[c * (TEAM * run) + 16 * j + 4 * g]) = make_uint4(key[0], key[1], key[2], key[3]);
     }
-    // The wave's lanes read one another's keys only through shuffles; a chosen
-    // block's key becomes 0, which no score has.
-    const int take = min(nb, a.top);
-    for (int t = 0; t < take; ++t) {
-        uint32_t best = 0;
-        int at = 0x7fffffff;
-        for (int b = lane; b < nb; b += 64)
-            if (keys[b] > best) {
-                best = keys[b];
-                at = b;
-            }
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t k2 = __shfl_xor(best, o, 64);
-            const int a2 = __shfl_xor(at, o, 64);
-            if (k2 > best || (k2 == best && a2 < at)) {
-                best = k2;
-                at = a2;
+    __syncthreads();
+
+    // ---- the `top` largest, a team for each query
+    const int q = tid / TEAM, t = tid & (TEAM - 1);
+    const uint32_t *mine = keys + q * (TEAM * run) + t * run;
+    uint32_t held[HELD ? 16 : 1];
+    if constexpr (HELD) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (i < run) x = *reinterpret_cast<const uint4 *>(mine + i);
+            held[i] = x.x, held[i + 1] = x.y, held[i + 2] = x.z, held[i + 3] = x.w;
+        }
+    }
+    const auto each = [&](auto &&f) __attribute__((always_inline)) {  // f(key, index in the run)
+        if constexpr (HELD) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i < run) f(held[i], i);
+        } else {
+            for (int i = 0; i < run; i += 4) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(mine + i);
+                f(x.x, i), f(x.y, i + 1), f(x.z, i + 2), f(x.w, i + 3);
             }
         }
-        if ((at & 63) == lane) keys[at] = 0;
+    };
+    const int may = q < queries ? candidates(q) : 0, take = min(may, a.top);
+    uint32_t low = 0xffffffffu, high = 0;
+    each([&](uint32_t k, int) {
+        if (k) low = min(low, k);
+        high = max(high, k);
+    });
+    {
+        constexpr int W = TEAM < 64 ? TEAM : 64;
+#pragma unroll
+        for (int o = 1; o < W; o <<= 1) {
+            low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), o, W)));
+            high = max(high, static_cast<uint32_t>(__shfl_xor(static_cast<int>(high), o, W)));
+        }
+        if constexpr (TEAM == 256) {
+            __shared__ uint32_t ends[2][4];
+            if (lane == 0) ends[0][wave] = low, ends[1][wave] = high;
+            __syncthreads();
+            for (int w = 0; w < 4; ++w) low = min(low, ends[0][w]), high = max(high, ends[1][w]);
+        }
     }
-    int done = 0;
-    for (int b0 = 0; b0 < nb; b0 += 64) {
-        const bool is = b0 + lane < nb && keys[b0 + lane] == 0;
-        const uint64_t mask = __ballot(is);
-        if (is) out[done + __popcll(mask & ((UINT64_C(1) << lane) - 1))] = b0 + lane;
-        done += __popcll(mask);
+    // at least `take` keys are >= low (count of them: n_low), fewer than that are >= high
+    high += 1;
+    int n_low = may;
+    if (take == 0) low = high = 1, n_low = 0;
+    while (true) {
+        const bool going = n_low != take && high - low > 1;
+        if constexpr (TEAM == 256) {
+            if (!going) break;  // the same for all
+        } else {
+            if (!__any(going)) break;
+        }
+        const uint32_t mid = low + (high - low) / 2;
+        int n = 0;
+        each([&](uint32_t k, int) { n += k >= mid ? 1 : 0; });
+        n = team_sum<TEAM>(n, box);
+        if (going) {
+            if (n >= take) low = mid, n_low = n;
+            else high = mid;
+        }
     }
-    for (int t = done + lane; t < a.top; t += 64) out[t] = -1;
+    // Chosen: keys above low, and of those that equal it the first ones (all, where the count came out right).
+    int above = 0, equal = 0;
+    each([&](uint32_t k, int) {
+        above += k > low ? 1 : 0;
+        equal += k == low ? 1 : 0;
+    });
+    if (take == 0) above = equal = 0;
+    int spare = take - team_sum<TEAM>(above, box);  // equal keys to choose
+    const int equal_before = team_before<TEAM>(equal, box);
+    int left = max(0, min(equal, spare - equal_before));  // ... of this thread's
+    int at = team_before<TEAM>(above + left, box);
+    if (q >= queries) return;
+    int32_t *out = a.selected + ((qs.begin + row0 + q) * a.kv_heads + head) * a.top;
+    each([&](uint32_t k, int i) {
+        const bool same = k == low && left > 0;
+        if (take && (k > low || same)) out[at++] = t * run + i;
+        if (same) --left;
+    });
+    for (int i = take + t; i < a.top; i += TEAM) out[i] = -1;
 }
 
 // ---------------------------------------------------------------------------
@@ -928,10 +1097,11 @@ S3DX_API s3dx_status s3dx_block_index(const void *k, int32_t dtype, int64_t tota
         require(codes && aligned(codes, 16) && scale && aligned(scale, 4), "codes or scale is NULL or not aligned");
         const IndexArgs a = {k, k_starts, total_k, k_stride, sequences, index_rows(total_k, sequences, block),
                              kv_heads, head_dim, block, codes, scale};
-        const int64_t items = a.rows * kv_heads;
-        require(items <= (INT64_C(1) << 32), "too many blocks");
+        const int per = 256 / head_dim;
+        require((kv_heads + per - 1) / per <= 65535, "too many heads");
         (dtype == S3DX_BF16 ? index_kernel<uint16_t> : index_kernel<float>)<<<
-            dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, as_stream(stream)>>>(a);
+            dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>((kv_heads + per - 1) / per)), dim3(256), 0,
+            as_stream(stream)>>>(a);
         launch_check("block index");
     });
 }
@@ -957,15 +1127,29 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
                 "codes or scale is NULL or not aligned");
         SelectArgs a = {q, q_starts, k_starts, codes, scale, selected, total_q, total_k, q_stride, sequences,
                         index_rows(total_k, sequences, block), kv_heads, heads / kv_heads, head_dim, block, top,
-                        static_cast<int32_t>((std::min(max_k, total_k) + block - 1) / block), flags};
-        require(total_q * kv_heads <= std::numeric_limits<int32_t>::max(), "total_q * kv_heads is out of range");
-        const auto kernel = dtype == S3DX_BF16 ? select_kernel<uint16_t> : select_kernel<float>;
-        const size_t lds = static_cast<size_t>(a.most_blocks) * 4;
-        if (lds > 65536)
+                        static_cast<int32_t>((std::min(max_k, total_k) + block - 1) / block), flags, 0};
+        // Queries of a workgroup: 16, unless those leave most compute units without one or their keys take more than
+        // 64 KiB of LDS (1,024 blocks; 4,096 of four queries).
+        const int64_t rows = total_q * kv_heads;
+        const int qt = rows >= 16 * 512 && a.most_blocks <= 1024 ? 16 : rows >= 4 * 256 && a.most_blocks <= 4096 ? 4 : 1;
+        const int team = 256 / qt;
+        a.run = std::max((a.most_blocks + team - 1) / team + 3, 4) / 4 * 4;
+        const bool bf = dtype == S3DX_BF16;
+        const auto pick = [&](auto held) {
+            constexpr bool H = decltype(held)::value;
+            if (qt == 16) return bf ? select_kernel<uint16_t, 16, H> : select_kernel<float, 16, H>;
+            if (qt == 4) return bf ? select_kernel<uint16_t, 4, H> : select_kernel<float, 4, H>;
+            return bf ? select_kernel<uint16_t, 1, H> : select_kernel<float, 1, H>;
+        };
+        const auto kernel = a.run <= 16 ? pick(std::true_type{}) : pick(std::false_type{});
+        const size_t lds = static_cast<size_t>(256) * a.run * 4;
+        if (lds > 65536 - 4096)
             hip_check(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                           hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)),
                       "hipFuncSetAttribute");
-        kernel<<<dim3(static_cast<unsigned>(total_q * kv_heads)), dim3(64), lds, as_stream(stream)>>>(a);
+        const int64_t grid = (total_q / qt + sequences) * kv_heads;
+        require(grid <= std::numeric_limits<int32_t>::max(), "too many rows and sequences");
+        kernel<<<dim3(static_cast<unsigned>(grid)), dim3(256), lds, as_stream(stream)>>>(a);
         launch_check("block select");
     });
 }
