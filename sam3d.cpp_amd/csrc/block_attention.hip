@@ -26,15 +26,16 @@ __device__ __forceinline__ Span sequence_span(const int32_t *starts, int64_t s, 
 }
 
 // The last sequence whose first unit is not behind `unit`, where sequence s
-// begins at unit floor(starts[s] * mul / div) + s: every sequence has room for its
+// begins at unit (starts[s] * mul >> shift) + s: every sequence has room for its
 // last, partial unit, and the units rise with s, empty sequences or not.
 __device__ __forceinline__ int64_t sequence_of_unit(const int32_t *starts, int64_t sequences, int64_t total,
-                                                    int64_t mul, int64_t div, int64_t unit) {
+                                                    int64_t mul, int shift, int64_t unit) {
     int64_t lo = 0, hi = sequences;  // begin(lo) <= unit < begin(hi)
     while (hi - lo > 1) {
         const int64_t mid = (lo + hi) >> 1;
-        const int64_t at = min(max(static_cast<int64_t>(starts[mid]), INT64_C(0)), total) * mul / div + mid;
-        if (at <= unit) lo = mid;
+        const int64_t at = min(max(static_cast<int64_t>(starts[mid]), INT64_C(0)), total) * mul;
+        const int64_t begin = (at >> shift) + mid;
+        if (begin <= unit) lo = mid;
         else hi = mid;
     }
     return lo;
@@ -72,7 +73,7 @@ struct IndexArgs {
     const void *k;
     const int32_t *k_starts;
     int64_t total_k, k_stride, sequences, rows;
-    int32_t kv_heads, d, block;
+    int32_t kv_heads, d, block, block_log2;
     int8_t *codes;
     float *scale;
 };
@@ -88,9 +89,9 @@ __global__ void __launch_bounds__(256) index_kernel(IndexArgs a) {
     const int per = 256 / a.d;  // heads of a workgroup
     const int64_t row = blockIdx.x;
     const int head0 = static_cast<int>(blockIdx.y) * per, channels = min(per, a.kv_heads - head0) * a.d;
-    const int64_t s = sequence_of_unit(a.k_starts, a.sequences, a.total_k, 1, a.block, row);
+    const int64_t s = sequence_of_unit(a.k_starts, a.sequences, a.total_k, 1, a.block_log2, row);
     const Span k = sequence_span(a.k_starts, s, a.total_k);
-    const int64_t first = (row - (k.begin / a.block + s)) * a.block;
+    const int64_t first = (row - ((k.begin >> a.block_log2) + s)) << a.block_log2;
     const int count = static_cast<int>(min(static_cast<int64_t>(a.block), k.rows - first));
     if (first < 0 || count <= 0) return;  // the whole workgroup
     if (tid < 8) most[tid] = 0;
@@ -142,7 +143,7 @@ struct SelectArgs {
     const float *scale;
     int32_t *selected;
     int64_t total_q, total_k, q_stride, sequences, rows;
-    int32_t kv_heads, group, d, block, top, most_blocks, flags, run;
+    int32_t kv_heads, group, d, block, block_log2, top, most_blocks, flags, run;
 };
 
 // A float's order as an unsigned whole number: 0x007fffff (-inf) to 0xff800000 (inf).  -0 does not
@@ -151,7 +152,9 @@ __device__ __forceinline__ uint32_t order_key(float f) {
     const uint32_t u = __builtin_bit_cast(uint32_t, f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-constexpr uint32_t kNearKey = 0xff800001u;  // above every score
+__device__ __forceinline__ float of_key(uint32_t k) {
+    return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -199,13 +202,14 @@ __device__ __forceinline__ int team_before(int v, int *box) {
 
 // A tile of QT queries of one key head.  Scores by integer products (16x16x64: blocks by
 // queries), their order keys in LDS; then a team of 256 / QT threads for each query, each with a run
-// of blocks side by side, finds the `top`-th largest key by halving the range
-// of keys (a count of the keys above the middle each time; it stops as soon as the count is
-// right) and writes its run's chosen blocks behind those of the threads before it, equal
-// keys first come, first served.  HELD: a thread's keys (at most 16) stay in registers.
+// of blocks side by side, finds the `top`-th largest key by cutting the range of keys (by the
+// counts at its ends, then by half, in turn; it stops as soon as the count of the keys
+// from the cut on is right: about five cuts for 80 blocks) and writes its run's chosen
+// blocks behind those of the threads before it, equal keys first come, first served.  RUN: a
+// thread's blocks, whose keys stay in registers; 0: any number, from LDS each time.
 // QT 16 fills the products; 4 and 1 are for few rows, and for more blocks than LDS
 // holds of 16 queries.
-template <class T, int QT, bool HELD>
+template <class T, int QT, int RUN>
 __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
     constexpr int TEAM = 256 / QT;
     extern __shared__ uint32_t keys[];  // [QT][TEAM * run]
@@ -214,7 +218,7 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const int64_t tile = blockIdx.x / a.kv_heads;
     const int head = static_cast<int>(blockIdx.x - tile * a.kv_heads);
-    const int64_t s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, 1, QT, tile);
+    const int64_t s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, 1, QT == 16 ? 4 : QT == 4 ? 2 : 0, tile);
     const Span qs = sequence_span(a.q_starts, s, a.total_q), ks = sequence_span(a.k_starts, s, a.total_k);
     const int64_t first = (tile - (qs.begin / QT + s)) * QT;
     if (first < 0 || first >= qs.rows) return;  // the whole workgroup
@@ -223,89 +227,146 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
     // ---- the queries' codes, 16 threads each
     {
         const int q = tid >> 4, l = tid & 15, per = a.d / 16;
-        double m[8] = {}, most = 0.0;
-        bool fine = true;
-        if (q < queries) {
-            const T *x = static_cast<const T *>(a.q) + (qs.begin + row0 + q) * a.q_stride +
-                         static_cast<int64_t>(head) * a.group * a.d + l * per;
-            for (int h = 0; h < a.group; ++h)
+        // this thread's channels of all heads, pairs (per is even), on their way before the first is used
+        const T *x = static_cast<const T *>(a.q) + (qs.begin + row0 + min(q, queries - 1)) * a.q_stride +
+                     static_cast<int64_t>(head) * a.group * a.d + l * per;
+        const auto channels = [&](float (&v)[8]) __attribute__((always_inline)) {
+            uint32_t w[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (e < per) m[e] += static_cast<double>(load_as_f32<T>(x + static_cast<int64_t>(h) * a.d + e));
+            for (int e = 0; e < 4; ++e) {
+                w[2 * e] = w[2 * e + 1] = 0;
+                if (2 * e >= per) continue;
+                if constexpr (sizeof(T) == 4) {
+                    const uint2 t = reinterpret_cast<const uint2 *>(x)[e];
+                    w[2 * e] = t.x, w[2 * e + 1] = t.y;
+                } else {
+                    w[2 * e] = reinterpret_cast<const uint32_t *>(x)[e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[2 * e] = __builtin_bit_cast(float, sizeof(T) == 4 ? w[2 * e] : w[2 * e] << 16);
+                v[2 * e + 1] = __builtin_bit_cast(float, sizeof(T) == 4 ? w[2 * e + 1] : w[2 * e] & 0xffff0000u);
+            }
+        };
+        float v[8];
+        channels(v);
+        if (a.group == 1) {
+            // nothing is added up: the same codes in 32 bits (magnitudes' bits rise with them, NaN's above all)
+            uint32_t most = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1)
+                most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o, 16)));
+            const bool fine = most >= (127u - 100u) << 23 && most < 0x7f800000u;
+            const int up = fine ? 6 - (static_cast<int>(most >> 23) - 127) : 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < per)
+                    qc[q][l * per + e] =
+                        static_cast<int8_t>(fine ? min(127, max(-127, static_cast<int>(rintf(ldexpf(v[e], up))))) : 0);
+        } else {
+            double m[8], most = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m[e] = static_cast<double>(v[e]);
+            for (int h = 1; h < a.group; ++h) {
+                x += a.d;
+                channels(v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m[e] += static_cast<double>(v[e]);
+            }
+            bool fine = true;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                fine = fine && fabs(m[e]) < __builtin_inf();
+                most = fmax(most, fabs(m[e]));
+            }
+            int all = fine ? 1 : 0;
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) {
+                most = fmax(most, __shfl_xor(most, o, 16));
+                all &= __shfl_xor(all, o, 16);
+            }
+            fine = all && codes_fine(most);
+            const double up = two_to(6 - exponent_of(most));
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < per) qc[q][l * per + e] = static_cast<int8_t>(fine ? code_of(m[e], up) : 0);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            fine = fine && fabs(m[e]) < __builtin_inf();
-            most = fmax(most, fabs(m[e]));
-        }
-        int all = fine ? 1 : 0;
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            most = fmax(most, __shfl_xor(most, o, 16));
-            all &= __shfl_xor(all, o, 16);
-        }
-        fine = all && codes_fine(most);
-        const double up = two_to(6 - exponent_of(most));
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < per) qc[q][l * per + e] = static_cast<int8_t>(fine ? code_of(m[e], up) : 0);
     }
     __syncthreads();
 
     // ---- scores
-    const int nb = min((ks.rows + a.block - 1) / a.block, a.most_blocks), lag = ks.rows - qs.rows;
-    const int run = a.run;  // blocks of a thread, a multiple of 4
-    const int64_t base = static_cast<int64_t>(head) * a.rows + ks.begin / a.block + s;
+    const int nb = min((ks.rows + a.block - 1) >> a.block_log2, a.most_blocks), lag = ks.rows - qs.rows;
+    const int run = RUN ? RUN : a.run;  // blocks of a thread, a multiple of 4
+    const int64_t base = static_cast<int64_t>(head) * a.rows + (ks.begin >> a.block_log2) + s;
     const auto candidates = [&](int q) __attribute__((always_inline)) {  // blocks that query q may choose
         const int place = row0 + q + lag;
-        return !(a.flags & S3DX_BLOCK_CAUSAL) ? nb : place < 0 ? 0 : min(nb, place / a.block + 1);
+        return !(a.flags & S3DX_BLOCK_CAUSAL) ? nb : place < 0 ? 0 : min(nb, (place >> a.block_log2) + 1);
     };
     i32x4 qf[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
         qf[t] = 64 * t + 16 * g < a.d ? *reinterpret_cast<const i32x4 *>(&qc[c][64 * t + 16 * g]) : i32x4{0, 0, 0, 0};
-    const int place = row0 + c + lag, near = a.flags & S3DX_BLOCK_NEAR && place >= 0 ? place / a.block : -1;
-    const int seen = candidates(c);
-    for (int j = wave; j < TEAM * run / 16; j += 4) {
-        const int b = 16 * j + c;
-        const int8_t *code = a.codes + (base + min(b, nb - 1)) * a.d;
-        i32x4 dot = {0, 0, 0, 0};
+    const auto near_of = [&](int q) __attribute__((always_inline)) {  // its own block, or -1
+        const int place = row0 + q + lag, b = place >> a.block_log2;
+        return a.flags & S3DX_BLOCK_NEAR && place >= 0 && b < nb ? b : -1;
+    };
+    const int seen = candidates(c), own = near_of(c);
+    // Chunks of 16 blocks, U at a time, all their codes and scales on the way before the first is used; what is behind
+    // the last block, or behind a code's end (there the query's codes are 0), is read where something is.
+    const int chunks = TEAM * run / 16;
+    constexpr int U = QT == 16 && RUN == 4 ? 1 : QT == 16 && RUN == 8 ? 2 : 4;
+    const int8_t *code0 = a.codes + base * a.d;
+    const float *scale0 = a.scale + base;
+    for (int j0 = wave; nb > 0 && j0 < chunks; j0 += 4 * U) {
+        i32x4 x[U][2];
+        float scale[U][4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            i32x4 x = {0, 0, 0, 0};
-            if (b < nb && 64 * t + 16 * g < a.d) x = *reinterpret_cast<const i32x4 *>(code + 64 * t + 16 * g);
-            if (t == 0 || a.d > 64) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, qf[t], dot, 0, 0, 0);
-        }
-        uint32_t key[4];
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + 4 * u;
+            const uint32_t code = static_cast<uint32_t>(__mul24(min(16 * j + c, nb - 1), a.d));
+            x[u][0] = *reinterpret_cast<const i32x4 *>(code0 + (code + (16 * g < a.d ? 16 * g : 0)));
+            if (a.d > 64) x[u][1] = *reinterpret_cast<const i32x4 *>(code0 + (code + (64 + 16 * g < a.d ? 64 + 16 * g : 0)));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = 16 * j + 4 * g + i;
-            // |dot| < 2^21: the product with a power of two is exact
-            key[i] = at < seen ? order_key(static_cast<float>(dot[i]) * a.scale[base + at]) : 0u;
-            if (at == near && at < seen) key[i] = kNearKey;
+            for (int i = 0; i < 4; ++i) scale[u][i] = scale0[static_cast<uint32_t>(min(16 * j + 4 * g + i, nb - 1))];
         }
-        if (c < QT)
-            *reinterpret_cast<uint4 *>(&keys[c * (TEAM * run) + 16 * j + 4 * g]) = make_uint4(key[0], key[1], key[2], key[3]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + 4 * u;
+            if (j >= chunks) break;
+            i32x4 dot = {0, 0, 0, 0};
+            dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[u][0], qf[0], dot, 0, 0, 0);
+            if (a.d > 64) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[u][1], qf[1], dot, 0, 0, 0);
+            uint32_t key[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = 16 * j + 4 * g + i;
+                // |dot| < 2^21: the product with a power of two is exact.  The own block is chosen without a key.
+                key[i] = at < seen && at != own ? order_key(static_cast<float>(dot[i]) * scale[u][i]) : 0u;
+            }
+            if (c < QT)
+                *reinterpret_cast<uint4 *>(&keys[c * (TEAM * run) + 16 * j + 4 * g]) = make_uint4(key[0], key[1], key[2], key[3]);
+        }
     }
     __syncthreads();
 
     // ---- the `top` largest, a team for each query
     const int q = tid / TEAM, t = tid & (TEAM - 1);
     const uint32_t *mine = keys + q * (TEAM * run) + t * run;
-    uint32_t held[HELD ? 16 : 1];
-    if constexpr (HELD) {
+    uint32_t held[RUN ? RUN : 1];
+    if constexpr (RUN > 0) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (i < run) x = *reinterpret_cast<const uint4 *>(mine + i);
+        for (int i = 0; i < RUN; i += 4) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(mine + i);
             held[i] = x.x, held[i + 1] = x.y, held[i + 2] = x.z, held[i + 3] = x.w;
         }
     }
     const auto each = [&](auto &&f) __attribute__((always_inline)) {  // f(key, index in the run)
-        if constexpr (HELD) {
+        if constexpr (RUN > 0) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < run) f(held[i], i);
+            for (int i = 0; i < RUN; ++i) f(held[i], i);
         } else {
             for (int i = 0; i < run; i += 4) {
                 const uint4 x = *reinterpret_cast<const uint4 *>(mine + i);
@@ -313,7 +374,9 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
             }
         }
     };
-    const int may = q < queries ? candidates(q) : 0, take = min(may, a.top);
+    const int near = q < queries ? near_of(q) : -1, all = q < queries ? candidates(q) : 0;
+    // the own block apart (its place is in reach: it is a candidate): `take` of `may` others
+    const int may = all - (near >= 0 ? 1 : 0), take = min(all, a.top) - (near >= 0 ? 1 : 0);
     uint32_t low = 0xffffffffu, high = 0;
     each([&](uint32_t k, int) {
         if (k) low = min(low, k);
@@ -335,43 +398,52 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
     }
     // at least `take` keys are >= low (count of them: n_low), fewer than that are >= high
     high += 1;
-    int n_low = may;
+    int n_low = may, n_high = 0;
     if (take == 0) low = high = 1, n_low = 0;
-    while (true) {
+    for (int cut = 0;; ++cut) {
         const bool going = n_low != take && high - low > 1;
         if constexpr (TEAM == 256) {
             if (!going) break;  // the same for all
         } else {
-            if (!__any(going)) break;
+            if (__builtin_amdgcn_ballot_w64(going) == 0) break;
         }
-        const uint32_t mid = low + (high - low) / 2;
+        // Where the cut is made decides only how soon it ends: in the values, by the counts and by half in turn;
+        // in the keys by half from the 16th on (at most 32 more), and where the values leave nothing between.
+        uint32_t mid = low + (high - low) / 2;
+        const float f0 = of_key(low), f1 = of_key(high);
+        const float part = cut & 1 ? 0.5f
+                                   : (static_cast<float>(n_low - take) + 0.5f) *
+                                         __builtin_amdgcn_rcpf(static_cast<float>(max(n_low - n_high, 1)));
+        const uint32_t by_value = order_key(f0 + (f1 - f0) * part);
+        if (cut < 16 && by_value > low && by_value < high) mid = by_value;
         int n = 0;
         each([&](uint32_t k, int) { n += k >= mid ? 1 : 0; });
         n = team_sum<TEAM>(n, box);
         if (going) {
             if (n >= take) low = mid, n_low = n;
-            else high = mid;
+            else high = mid, n_high = n;
         }
     }
     // Chosen: keys above low, and of those that equal it the first ones (all, where the count came out right).
     int above = 0, equal = 0;
-    each([&](uint32_t k, int) {
-        above += k > low ? 1 : 0;
-        equal += k == low ? 1 : 0;
-    });
-    if (take == 0) above = equal = 0;
-    int spare = take - team_sum<TEAM>(above, box);  // equal keys to choose
+    if (take > 0)
+        each([&](uint32_t k, int) {
+            above += k > low ? 1 : 0;
+            equal += k == low ? 1 : 0;
+        });
+    const int spare = take - team_sum<TEAM>(above, box);  // equal keys to choose
     const int equal_before = team_before<TEAM>(equal, box);
     int left = max(0, min(equal, spare - equal_before));  // ... of this thread's
-    int at = team_before<TEAM>(above + left, box);
+    const int own_i = near >= t * run && near < t * run + run ? near - t * run : -1;
+    int at = team_before<TEAM>(above + left + (own_i >= 0 ? 1 : 0), box);
     if (q >= queries) return;
     int32_t *out = a.selected + ((qs.begin + row0 + q) * a.kv_heads + head) * a.top;
     each([&](uint32_t k, int i) {
-        const bool same = k == low && left > 0;
-        if (take && (k > low || same)) out[at++] = t * run + i;
+        const bool same = take > 0 && k == low && left > 0;
+        if ((take > 0 && k > low) || same || i == own_i) out[at++] = t * run + i;
         if (same) --left;
     });
-    for (int i = take + t; i < a.top; i += TEAM) out[i] = -1;
+    for (int i = min(all, a.top) + t; i < a.top; i += TEAM) out[i] = -1;
 }
 
 // ---------------------------------------------------------------------------
@@ -548,7 +620,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     // and the longest first.
     if (a.causal) tg = a.tile_groups - 1 - (tg % (a.tile_groups >> 3) * 8 + tg / (a.tile_groups >> 3));
     const int64_t tile = WAVES == 4 ? tg : static_cast<int64_t>(tg) * 4 + wave;
-    const int64_t s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, a.group, ROWS, tile);
+    const int64_t s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, a.group, NS == 4 ? 6 : 5, tile);
     const Span qs = sequence_span(a.q_starts, s, a.total_q), ks = sequence_span(a.k_starts, s, a.total_k);
     const int64_t first_row = (tile - (qs.begin * a.group / ROWS + s)) * ROWS;
     const int nrows = qs.rows * a.group;  // total_q * heads < 2^31
@@ -1013,6 +1085,7 @@ void check_rows(const void *p, int64_t stride, int32_t heads, int32_t head_dim, 
             "a row stride must be whole 16-byte pieces, below 2^22 elements");
 }
 void check_starts(const int32_t *p) { require(p && aligned(p, 4), "starts is NULL or not aligned"); }
+int32_t log2_of(int32_t block) { return block == 32 ? 5 : block == 64 ? 6 : 7; }
 int64_t index_rows(int64_t total_k, int64_t sequences, int32_t block) { return total_k / block + sequences; }
 
 // How an attention call is cut: tiles of rows (an upper bound, as the lengths are on the
@@ -1096,7 +1169,7 @@ S3DX_API s3dx_status s3dx_block_index(const void *k, int32_t dtype, int64_t tota
         check_starts(k_starts);
         require(codes && aligned(codes, 16) && scale && aligned(scale, 4), "codes or scale is NULL or not aligned");
         const IndexArgs a = {k, k_starts, total_k, k_stride, sequences, index_rows(total_k, sequences, block),
-                             kv_heads, head_dim, block, codes, scale};
+                             kv_heads, head_dim, block, log2_of(block), codes, scale};
         const int per = 256 / head_dim;
         require((kv_heads + per - 1) / per <= 65535, "too many heads");
         (dtype == S3DX_BF16 ? index_kernel<uint16_t> : index_kernel<float>)<<<
@@ -1126,7 +1199,7 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
         require(total_k == 0 || (codes && aligned(codes, 16) && scale && aligned(scale, 4)),
                 "codes or scale is NULL or not aligned");
         SelectArgs a = {q, q_starts, k_starts, codes, scale, selected, total_q, total_k, q_stride, sequences,
-                        index_rows(total_k, sequences, block), kv_heads, heads / kv_heads, head_dim, block, top,
+                        index_rows(total_k, sequences, block), kv_heads, heads / kv_heads, head_dim, block, log2_of(block), top,
                         static_cast<int32_t>((std::min(max_k, total_k) + block - 1) / block), flags, 0};
         // Queries of a workgroup: 16, unless those leave most compute units without one or their keys take more than
         // 64 KiB of LDS (1,024 blocks; 4,096 of four queries).
@@ -1135,13 +1208,17 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
         const int team = 256 / qt;
         a.run = std::max((a.most_blocks + team - 1) / team + 3, 4) / 4 * 4;
         const bool bf = dtype == S3DX_BF16;
-        const auto pick = [&](auto held) {
-            constexpr bool H = decltype(held)::value;
-            if (qt == 16) return bf ? select_kernel<uint16_t, 16, H> : select_kernel<float, 16, H>;
-            if (qt == 4) return bf ? select_kernel<uint16_t, 4, H> : select_kernel<float, 4, H>;
-            return bf ? select_kernel<uint16_t, 1, H> : select_kernel<float, 1, H>;
+        a.run = a.run <= 4 ? 4 : a.run <= 8 ? 8 : a.run <= 16 ? 16 : a.run;
+        const auto pick = [&](auto run) {
+            constexpr int R = decltype(run)::value;
+            if (qt == 16) return bf ? select_kernel<uint16_t, 16, R> : select_kernel<float, 16, R>;
+            if (qt == 4) return bf ? select_kernel<uint16_t, 4, R> : select_kernel<float, 4, R>;
+            return bf ? select_kernel<uint16_t, 1, R> : select_kernel<float, 1, R>;
         };
-        const auto kernel = a.run <= 16 ? pick(std::true_type{}) : pick(std::false_type{});
+        const auto kernel = a.run == 4    ? pick(std::integral_constant<int, 4>{})
+                            : a.run == 8  ? pick(std::integral_constant<int, 8>{})
+                            : a.run == 16 ? pick(std::integral_constant<int, 16>{})
+                                          : pick(std::integral_constant<int, 0>{});
         const size_t lds = static_cast<size_t>(256) * a.run * 4;
         if (lds > 65536 - 4096)
             hip_check(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
@@ -1205,7 +1282,7 @@ S3DX_API s3dx_status s3dx_block_attention(const void *q, const void *k, const vo
         AttendCut cut = attend_cut(dtype == S3DX_BF16, total_q, heads, kv_heads, head_dim, sequences, block, top, max_k);
         if (flags & S3DX_BLOCK_CAUSAL) cut.tile_groups = (cut.tile_groups + 7) / 8 * 8;  // see the kernel's order of tiles
         AttendArgs a = {q, k, v, o, lse, q_starts, k_starts, selected, total_q, total_k, q_stride, k_stride, v_stride, o_stride,
-                        sequences, heads, heads / kv_heads, kv_heads, block, block == 32 ? 5 : block == 64 ? 6 : 7, top,
+                        sequences, heads, heads / kv_heads, kv_heads, block, log2_of(block), top,
                         flags & S3DX_BLOCK_CAUSAL, cut.splits, static_cast<int32_t>(cut.tile_groups), softmax_scale, nullptr,
                         nullptr};
         if (cut.splits > 1) {
