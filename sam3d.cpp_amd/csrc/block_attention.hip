@@ -25,31 +25,33 @@ __device__ __forceinline__ Span sequence_span(const int32_t *starts, int64_t s, 
     return {lo, static_cast<int32_t>(hi - lo)};
 }
 
-// The last sequence whose first unit is not behind `unit`, where sequence s
-// begins at unit (starts[s] * mul >> shift) + s: every sequence has room for its
-// last, partial unit, and the units rise with s, empty sequences or not.
-__device__ __forceinline__ int64_t sequence_of_unit(const int32_t *starts, int64_t sequences, int64_t total,
-                                                    int64_t mul, int shift, int64_t unit) {
+// The last sequence that begins at or before `unit`, by the whole wave: 64 beginnings at a
+// time, so one trip to memory for up to 64 sequences and two for 4,096.
+template <class F>
+__device__ __forceinline__ int64_t last_sequence(int64_t sequences, int64_t unit, F &&begin) {
+    const int lane = threadIdx.x & 63;
     int64_t lo = 0, hi = sequences;  // begin(lo) <= unit < begin(hi)
     while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        const int64_t at = min(max(static_cast<int64_t>(starts[mid]), INT64_C(0)), total) * mul;
-        const int64_t begin = (at >> shift) + mid;
-        if (begin <= unit) lo = mid;
-        else hi = mid;
+        const int64_t step = (hi - lo + 63) >> 6, at = lo + lane * step;
+        const bool before = lane == 0 || (at < hi && begin(at) <= unit);
+        lo += (__popcll(__builtin_amdgcn_ballot_w64(before)) - 1) * step;
+        hi = min(hi, lo + step);
     }
     return lo;
 }
-
+// The sequence of a tile, where sequence s begins at tile (starts[s] * mul >> shift) + s: every
+// sequence has room for its last, partial tile, and the beginnings rise with s, empty
+// sequences or not.
+__device__ __forceinline__ int64_t sequence_of_unit(const int32_t *starts, int64_t sequences, int64_t total,
+                                                    int64_t mul, int shift, int64_t unit) {
+    return last_sequence(sequences, unit, [&](int64_t s) {
+        return (min(max(static_cast<int64_t>(starts[s]), INT64_C(0)), total) * mul >> shift) + s;
+    });
+}
 // The sequence that holds row `row`, or -1.
 __device__ __forceinline__ int64_t sequence_of_row(const int32_t *starts, int64_t sequences, int64_t row) {
-    int64_t lo = 0, hi = sequences;
-    while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (starts[mid] <= row) lo = mid;
-        else hi = mid;
-    }
-    return starts[lo] <= row && row < starts[lo + 1] ? lo : -1;
+    const int64_t s = last_sequence(sequences, row, [&](int64_t at) { return static_cast<int64_t>(starts[at]); });
+    return starts[s] <= row && row < starts[s + 1] ? s : -1;
 }
 
 // ---------------------------------------------------------------------------
@@ -158,9 +160,14 @@ __device__ __forceinline__ float of_key(uint32_t k) {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// Sum over a team of 16, 64 or 256 threads, in each of them; `box` is for 256.
+// Threads of a workgroup, and of the team that searches a query's keys.  Sixteen waves fetch the scores of a query by
+// itself, and one of them searches: sums over more took longer than what they saved (30 us instead of 20 for 1,024 blocks).
+constexpr int select_threads(int qt) { return qt == 1 ? 1024 : 256; }
+constexpr int select_team(int qt) { return qt == 16 ? 16 : 64; }
+
+// Sum over a team of 16 or 64 threads, in each of them.
 template <int TEAM>
-__device__ __forceinline__ int team_sum(int v, int *box) {
+__device__ __forceinline__ int team_sum(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);  // row_ror:8
     v += __builtin_amdgcn_update_dpp(0, v, 0x124, 0xf, 0xf, false);
     v += __builtin_amdgcn_update_dpp(0, v, 0x122, 0xf, 0xf, false);
@@ -171,37 +178,23 @@ __device__ __forceinline__ int team_sum(int v, int *box) {
         const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
         v = static_cast<int>(b[0] + b[1]);
     }
-    if constexpr (TEAM == 256) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = box[0] + box[1] + box[2] + box[3];
-    }
     return v;
 }
 // Sum over the team's threads before this one.
 template <int TEAM>
-__device__ __forceinline__ int team_before(int v, int *box) {
-    constexpr int W = TEAM < 64 ? TEAM : 64;
-    const int at = threadIdx.x & (W - 1);
+__device__ __forceinline__ int team_before(int v) {
+    const int at = threadIdx.x & (TEAM - 1);
     int x = v;
 #pragma unroll
-    for (int o = 1; o < W; o <<= 1) {
-        const int y = __shfl_up(x, o, W);
+    for (int o = 1; o < TEAM; o <<= 1) {
+        const int y = __shfl_up(x, o, TEAM);
         if (at >= o) x += y;
-    }
-    if constexpr (TEAM == 256) {
-        const int wave = threadIdx.x >> 6;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 63) box[wave] = x;
-        __syncthreads();
-        for (int w = 0; w < wave; ++w) x += box[w];
     }
     return x - v;
 }
 
 // A tile of QT queries of one key head.  Scores by integer products (16x16x64: blocks by
-// queries), their order keys in LDS; then a team of 256 / QT threads for each query, each with a run
+// queries), their order keys in LDS; then a team of 16 or 64 threads for each query, each with a run
 // of blocks side by side, finds the `top`-th largest key by cutting the range of keys (by the
 // counts at its ends, then by half, in turn; it stops as soon as the count of the keys
 // from the cut on is right: about five cuts for 80 blocks) and writes its run's chosen
@@ -210,11 +203,10 @@ __device__ __forceinline__ int team_before(int v, int *box) {
 // QT 16 fills the products; 4 and 1 are for few rows, and for more blocks than LDS
 // holds of 16 queries.
 template <class T, int QT, int RUN>
-__global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
-    constexpr int TEAM = 256 / QT;
+__global__ void __launch_bounds__(select_threads(QT)) select_kernel(SelectArgs a) {
+    constexpr int TEAM = select_team(QT), WAVES = select_threads(QT) / 64;
     extern __shared__ uint32_t keys[];  // [QT][TEAM * run]
     __shared__ alignas(16) int8_t qc[16][128];
-    __shared__ int box[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const int64_t tile = blockIdx.x / a.kv_heads;
     const int head = static_cast<int>(blockIdx.x - tile * a.kv_heads);
@@ -226,7 +218,7 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
 
     // ---- the queries' codes, 16 threads each
     {
-        const int q = tid >> 4, l = tid & 15, per = a.d / 16;
+        const int q = (tid >> 4) & 15, l = tid & 15, per = a.d / 16;
         // this thread's channels of all heads, pairs (per is even), on their way before the first is used
         const T *x = static_cast<const T *>(a.q) + (qs.begin + row0 + min(q, queries - 1)) * a.q_stride +
                      static_cast<int64_t>(head) * a.group * a.d + l * per;
@@ -270,7 +262,20 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
             double m[8], most = 0.0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) m[e] = static_cast<double>(v[e]);
-            for (int h = 1; h < a.group; ++h) {
+            int h = 1;
+            for (; h + 3 <= a.group; h += 3) {
+                float w[3][8];
+#pragma unroll
+                for (int u = 0; u < 3; ++u) {
+                    x += a.d;
+                    channels(w[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < 3; ++u)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) m[e] += static_cast<double>(w[u][e]);
+            }
+            for (; h < a.group; ++h) {
                 x += a.d;
                 channels(v);
 #pragma unroll
@@ -317,15 +322,15 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
     // Chunks of 16 blocks, U at a time, all their codes and scales on the way before the first is used; what is behind
     // the last block, or behind a code's end (there the query's codes are 0), is read where something is.
     const int chunks = TEAM * run / 16;
-    constexpr int U = QT == 16 && RUN == 4 ? 1 : QT == 16 && RUN == 8 ? 2 : 4;
+    constexpr int U = QT == 16 ? (RUN == 4 ? 1 : RUN == 8 ? 2 : 4) : 4;
     const int8_t *code0 = a.codes + base * a.d;
     const float *scale0 = a.scale + base;
-    for (int j0 = wave; nb > 0 && j0 < chunks; j0 += 4 * U) {
+    for (int j0 = wave; nb > 0 && j0 < chunks; j0 += WAVES * U) {
         i32x4 x[U][2];
         float scale[U][4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + 4 * u;
+            const int j = j0 + WAVES * u;
             const uint32_t code = static_cast<uint32_t>(__mul24(min(16 * j + c, nb - 1), a.d));
             x[u][0] = *reinterpret_cast<const i32x4 *>(code0 + (code + (16 * g < a.d ? 16 * g : 0)));
             if (a.d > 64) x[u][1] = *reinterpret_cast<const i32x4 *>(code0 + (code + (64 + 16 * g < a.d ? 64 + 16 * g : 0)));
@@ -334,7 +339,7 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + 4 * u;
+            const int j = j0 + WAVES * u;
             if (j >= chunks) break;
             i32x4 dot = {0, 0, 0, 0};
             dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[u][0], qf[0], dot, 0, 0, 0);
@@ -353,6 +358,7 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
     __syncthreads();
 
     // ---- the `top` largest, a team for each query
+    if (tid >= QT * TEAM) return;
     const int q = tid / TEAM, t = tid & (TEAM - 1);
     const uint32_t *mine = keys + q * (TEAM * run) + t * run;
     uint32_t held[RUN ? RUN : 1];
@@ -383,17 +389,10 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
         high = max(high, k);
     });
     {
-        constexpr int W = TEAM < 64 ? TEAM : 64;
 #pragma unroll
-        for (int o = 1; o < W; o <<= 1) {
-            low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), o, W)));
-            high = max(high, static_cast<uint32_t>(__shfl_xor(static_cast<int>(high), o, W)));
-        }
-        if constexpr (TEAM == 256) {
-            __shared__ uint32_t ends[2][4];
-            if (lane == 0) ends[0][wave] = low, ends[1][wave] = high;
-            __syncthreads();
-            for (int w = 0; w < 4; ++w) low = min(low, ends[0][w]), high = max(high, ends[1][w]);
+        for (int o = 1; o < TEAM; o <<= 1) {
+            low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), o, TEAM)));
+            high = max(high, static_cast<uint32_t>(__shfl_xor(static_cast<int>(high), o, TEAM)));
         }
     }
     // at least `take` keys are >= low (count of them: n_low), fewer than that are >= high
@@ -402,11 +401,7 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
     if (take == 0) low = high = 1, n_low = 0;
     for (int cut = 0;; ++cut) {
         const bool going = n_low != take && high - low > 1;
-        if constexpr (TEAM == 256) {
-            if (!going) break;  // the same for all
-        } else {
-            if (__builtin_amdgcn_ballot_w64(going) == 0) break;
-        }
+        if (__builtin_amdgcn_ballot_w64(going) == 0) break;
         // Where the cut is made decides only how soon it ends: in the values, by the counts and by half in turn;
         // in the keys by half from the 16th on (at most 32 more), and where the values leave nothing between.
         uint32_t mid = low + (high - low) / 2;
@@ -418,7 +413,7 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
         if (cut < 16 && by_value > low && by_value < high) mid = by_value;
         int n = 0;
         each([&](uint32_t k, int) { n += k >= mid ? 1 : 0; });
-        n = team_sum<TEAM>(n, box);
+        n = team_sum<TEAM>(n);
         if (going) {
             if (n >= take) low = mid, n_low = n;
             else high = mid, n_high = n;
@@ -431,11 +426,11 @@ __global__ void __launch_bounds__(256) select_kernel(SelectArgs a) {
             above += k > low ? 1 : 0;
             equal += k == low ? 1 : 0;
         });
-    const int spare = take - team_sum<TEAM>(above, box);  // equal keys to choose
-    const int equal_before = team_before<TEAM>(equal, box);
+    const int spare = take - team_sum<TEAM>(above);  // equal keys to choose
+    const int equal_before = team_before<TEAM>(equal);
     int left = max(0, min(equal, spare - equal_before));  // ... of this thread's
     const int own_i = near >= t * run && near < t * run + run ? near - t * run : -1;
-    int at = team_before<TEAM>(above + left + (own_i >= 0 ? 1 : 0), box);
+    int at = team_before<TEAM>(above + left + (own_i >= 0 ? 1 : 0));
     if (q >= queries) return;
     int32_t *out = a.selected + ((qs.begin + row0 + q) * a.kv_heads + head) * a.top;
     each([&](uint32_t k, int i) {
@@ -1025,7 +1020,8 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 template <class T, int D>
 __global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
     const int lane = threadIdx.x & 63;
-    const int64_t cell = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6), cells = a.total_q * a.heads;
+    const int64_t cell = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t cells = a.total_q * a.heads;
     if (cell >= cells) return;
     const int64_t row = cell / a.heads;
     const int head = static_cast<int>(cell - row * a.heads);
@@ -1205,7 +1201,7 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
         // 64 KiB of LDS (1,024 blocks; 4,096 of four queries).
         const int64_t rows = total_q * kv_heads;
         const int qt = rows >= 16 * 512 && a.most_blocks <= 1024 ? 16 : rows >= 4 * 256 && a.most_blocks <= 4096 ? 4 : 1;
-        const int team = 256 / qt;
+        const int team = select_team(qt);
         a.run = std::max((a.most_blocks + team - 1) / team + 3, 4) / 4 * 4;
         const bool bf = dtype == S3DX_BF16;
         a.run = a.run <= 4 ? 4 : a.run <= 8 ? 8 : a.run <= 16 ? 16 : a.run;
@@ -1219,14 +1215,14 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
                             : a.run == 8  ? pick(std::integral_constant<int, 8>{})
                             : a.run == 16 ? pick(std::integral_constant<int, 16>{})
                                           : pick(std::integral_constant<int, 0>{});
-        const size_t lds = static_cast<size_t>(256) * a.run * 4;
+        const size_t lds = static_cast<size_t>(qt) * team * a.run * 4;
         if (lds > 65536 - 4096)
             hip_check(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                           hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)),
                       "hipFuncSetAttribute");
         const int64_t grid = (total_q / qt + sequences) * kv_heads;
         require(grid <= std::numeric_limits<int32_t>::max(), "too many rows and sequences");
-        kernel<<<dim3(static_cast<unsigned>(grid)), dim3(256), lds, as_stream(stream)>>>(a);
+        kernel<<<dim3(static_cast<unsigned>(grid)), dim3(select_threads(qt)), lds, as_stream(stream)>>>(a);
         launch_check("block select");
     });
 }
