@@ -467,14 +467,18 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
+// (A vector's element goes through a variable of its own: a bit cast of the element as it stands
+// reads the first one.)
+__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
+
 // Largest over the lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float max_over_groups(float v) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v);
     const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const float m = fmaxf(__builtin_bit_cast(float, a[0]), __builtin_bit_cast(float, a[1]));
+    const float m = fmaxf(as_float(a[0]), as_float(a[1]));
     const uint32_t w = __builtin_bit_cast(uint32_t, m);
     const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return fmaxf(__builtin_bit_cast(float, b[0]), __builtin_bit_cast(float, b[1]));
+    return fmaxf(as_float(b[0]), as_float(b[1]));
 }
 
 // One row by the whole wave, key by key: scores with a key per lane, the running maximum
@@ -565,6 +569,36 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void *x, int
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(p), static_cast<short>(0), bytes, 0x00020000);
 }
 
+// x as the sum of three bfloat16 terms, each cut off from what the ones before left: 8 significant bits a
+// term, 24 together, so nothing is lost (of magnitudes from 2^-102 on, whose last terms are normal
+// numbers).  Pairs of values give pairs of terms.
+__device__ __forceinline__ void three_terms(float x, float y, uint32_t (&out)[3]) {
+    constexpr uint32_t kHigh = 0x07060302u;  // the high halves of both
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x), v = __builtin_bit_cast(uint32_t, y);
+        out[p] = __builtin_amdgcn_perm(v, u, kHigh);
+        if (p == 2) break;
+        x -= __builtin_bit_cast(float, u & 0xffff0000u);
+        y -= __builtin_bit_cast(float, v & 0xffff0000u);
+    }
+}
+
+// d += A B over 32 values: one product of bfloat16 operands, or, of operands in three terms, the six
+// of at least 2^-16 of the whole, the smallest first (what is left out is 2^-24 of it and less).
+template <int P>
+__device__ __forceinline__ f32x4 product(const u32x4 (&x)[P], const u32x4 (&y)[P], f32x4 d) {
+    const auto one = [&](int i, int j) __attribute__((always_inline)) {
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[i]), __builtin_bit_cast(bf16x8, y[j]), d, 0, 0, 0);
+    };
+    if constexpr (P == 3) {
+        one(2, 0), one(1, 1), one(0, 2);
+        one(1, 0), one(0, 1);
+    }
+    one(0, 0);
+    return d;
+}
+
 // Attention of a tile of 16 NS rows (query rows times the heads that share a key head)
 // on matrix units.  A wave computes S^T = K Q^T and O^T = V^T P^T, so that what one
 // product leaves in a lane is what the next one wants there and nothing goes through
@@ -580,6 +614,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void *x, int
 // block, a bit for each row that chose it; rows that did not take weights 0.
 // Neighbouring rows choose alike, which is what makes tiles of them pay.
 //
+// FP32 heads up to 64 wide: the same products on three bfloat16 terms of every value, six for one, each 16 times as
+// fast as FP32's own (5,086 rows x 16 heads x 64, all keys: 880 us with those).  Wider
+// heads' terms do not fit a lane's registers: they take FP32's products.
+//
 // WAVES 4: the workgroup's waves take a tile together, every fourth step (of lists,
 // block) each, and join them through LDS: a quarter of the tiles' length, so that the last
 // ones to run leave fewer units idle.  WAVES 1: a tile each, for rows of few keys.
@@ -588,7 +626,8 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr bool BF = sizeof(T) == 2;
     constexpr int ROWS = 16 * NS;
     constexpr int KT = KC / 16;              // 16-key groups of a step
-    constexpr int QV = BF ? D / 32 : D / 16; // 16-byte pieces of a lane's K or Q row
+    constexpr int P = BF ? 1 : D <= 64 ? 3 : 0; // bfloat16 terms of a value; 0: FP32's products
+    constexpr int QV = P ? D / 32 : D / 16;  // products over a row's channels
     constexpr int C = D / 16;                // channels of a lane's V row
     constexpr int VW = C * static_cast<int>(sizeof(T)) / 4;
     constexpr int E = static_cast<int>(sizeof(T));
@@ -598,7 +637,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr int TABLE = 1024, TILES = 4 / WAVES;
     constexpr int CH = D * E / 16;                 // 16-byte pieces of a K row
     constexpr int NP = KC * CH / 64;               // ... of a step, for each lane
-    constexpr int KEYS = BF ? KC * D * E : 0, TABLES = LISTED ? TABLE * TILES * 8 : 0;
+    constexpr int KEYS = P * KC * D * 2, TABLES = LISTED ? TABLE * TILES * 8 : 0;
     constexpr int PART = WAVES == 4 ? 4 * NS * 4 * C * 64 * 4 : 0;
     constexpr int LDS = 4 * KEYS + TABLES > PART ? 4 * KEYS + TABLES : PART;
     __shared__ alignas(16) char lds[LDS > 0 ? LDS : 16];
@@ -628,7 +667,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 
     // this lane's query of each set of 16, and the keys that it sees: [0, lim)
     int lim[NS];
-    uint32_t qf[NS][QV][4];
+    u32x4 qf[NS][QV][P ? P : 1];
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         const int r = min(r0 + 16 * n + c, nrows - 1), tok = r / a.group;
@@ -637,9 +676,18 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                      static_cast<int64_t>(kvh * a.group + r % a.group) * D;
 #pragma unroll
         for (int j = 0; j < QV; ++j) {
-            const u32x4 t = *reinterpret_cast<const u32x4 *>(q + (BF ? 32 * j + 8 * g : 16 * j + 4 * g));
+            if constexpr (P == 3) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) qf[n][j][i] = t[i];
+                for (int i = 0; i < 4; ++i) {
+                    const float2 t = *reinterpret_cast<const float2 *>(q + 32 * j + 8 * g + 2 * i);
+                    uint32_t terms[3];
+                    three_terms(t.x, t.y, terms);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) qf[n][j][p][i] = terms[p];
+                }
+            } else {
+                qf[n][j][0] = *reinterpret_cast<const u32x4 *>(q + (BF ? 32 * j + 8 * g : 16 * j + 4 * g));
+            }
         }
     }
     const int most = a.causal ? max(0, min(ks.rows, tok0 + ntok + lag)) : ks.rows;  // keys that some row sees
@@ -727,37 +775,43 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) voff[t][i] = vat + (16 * t + i) * vstep;
     }
-    // K: lane l fetches pieces l, l + 64, ... of the step's rows, which lie in LDS row by row, a row's pieces xor-ed by its
-    // number so that eight neighbouring rows' pieces of one number lie in different banks.
+    // K: lane l fetches pieces l, l + 64, ... of the step's rows, which lie in LDS row by row (a plane for each term), a
+    // row's pieces xor-ed by its number so that eight neighbouring rows' pieces of one number lie in different banks.
+    constexpr int ROW = D / 8;  // 16-byte pieces of a row in LDS
     const auto turned = [](int row, int piece) __attribute__((always_inline)) {
-        return piece ^ (CH % 8 == 0 ? row & 7 : (row >> 1) & 3);
+        return piece ^ (ROW % 8 == 0 ? row & 7 : (row >> 1) & 3);
     };
     char *kt = lds + wave * KEYS;
-    int koff[BF ? NP : KT], kput[BF ? NP : 1], kget[BF ? QV : 1];
-    if constexpr (BF) {
+    int koff[P ? NP : KT], kput[P ? NP : 1], kget[P ? QV : 1];
+    if constexpr (P > 0) {
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
             const int row = (p * 64 + lane) / CH, piece = (p * 64 + lane) % CH;
             koff[p] = row * kstep + piece * 16;
-            kput[p] = (row * CH + turned(row, piece)) * 16;
+            kput[p] = BF ? (row * ROW + turned(row, piece)) * 16 : (row * ROW + turned(row, piece >> 1)) * 16 + (piece & 1) * 8;
         }
 #pragma unroll
-        for (int j = 0; j < QV; ++j) kget[j] = (c * CH + turned(c, 4 * j + g)) * 16;
+        for (int j = 0; j < QV; ++j) kget[j] = (c * ROW + turned(c, 4 * j + g)) * 16;
     } else {
 #pragma unroll
         for (int t = 0; t < KT; ++t) koff[t] = (16 * t + c) * kstep + 16 * g;
     }
-    uint32_t kn[BF ? NP : 1][4], kf[KT][QV][4];
+    uint32_t kn[P ? NP : 1][4];
+    u32x4 kf[KT][QV][P ? P : 1];
     const auto load_k = [&]() __attribute__((always_inline)) {
         const auto r = rows_buffer<T, D>(a.k, ks.begin + first, a.k_stride, kvh, min(KC, ks.rows - first));
-        if constexpr (BF) {
+        if constexpr (P > 0) {
 #pragma unroll
             for (int p = 0; p < NP; ++p) buffer_dwords<4>(r, koff[p], kn[p]);
         } else {
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int j = 0; j < QV; ++j) buffer_dwords<4>(r, koff[t] + 64 * j, kf[t][j]);
+                for (int j = 0; j < QV; ++j) {
+                    uint32_t x[4];
+                    buffer_dwords<4>(r, koff[t] + 64 * j, x);
+                    kf[t][j][0] = u32x4{x[0], x[1], x[2], x[3]};
+                }
         }
     };
 
@@ -793,24 +847,33 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                 for (int i = 0; i < 4; ++i) buffer_dwords<VW>(r, HELD ? voff[HELD ? t : 0][i] : vat + (16 * t + i) * vstep, vf[t][i]);
         }
         // ---- K of this step to its operand's lanes, the next step's on its way
-        if constexpr (BF) {
+        if constexpr (P > 0) {
 #pragma unroll
-            for (int p = 0; p < NP; ++p) *reinterpret_cast<u32x4 *>(kt + kput[p]) = u32x4{kn[p][0], kn[p][1], kn[p][2], kn[p][3]};
+            for (int p = 0; p < NP; ++p) {
+                if constexpr (BF) {
+                    *reinterpret_cast<u32x4 *>(kt + kput[p]) = u32x4{kn[p][0], kn[p][1], kn[p][2], kn[p][3]};
+                } else {
+                    uint32_t lo[3], hi[3];
+                    three_terms(__builtin_bit_cast(float, kn[p][0]), __builtin_bit_cast(float, kn[p][1]), lo);
+                    three_terms(__builtin_bit_cast(float, kn[p][2]), __builtin_bit_cast(float, kn[p][3]), hi);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x2 *>(kt + i * (KC * D * 2) + kput[p]) = u32x2{lo[i], hi[i]};
+                }
+            }
             more = next();
             if (more) load_k();
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int j = 0; j < QV; ++j) {
-                    const u32x4 x = *reinterpret_cast<const u32x4 *>(kt + kget[j] + t * (16 * CH * 16));
+                for (int j = 0; j < QV; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) kf[t][j][i] = x[i];
-                }
+                    for (int p = 0; p < P; ++p)
+                        kf[t][j][p] = *reinterpret_cast<const u32x4 *>(kt + p * (KC * D * 2) + kget[j] + t * (16 * ROW * 16));
         }
         // ---- sets of 16 rows: S^T, weights
         f32x4 w[NS][KT];
-        u32x4 pw[NS][KT / 2 > 0 ? KT / 2 : 1];
+        u32x4 pw[NS][KT / 2 > 0 ? KT / 2 : 1][P ? P : 1];
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
             // the set's rows, a bit each (all keys: all of them), and the same for the four lanes of each
@@ -819,7 +882,9 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int t = 0; t < KT; ++t) w[n][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int u = 0; u < KT / 2; ++u) pw[n][u] = u32x4{0, 0, 0, 0};
+                for (int u = 0; u < KT / 2; ++u)
+#pragma unroll
+                    for (int p = 0; p < P; ++p) pw[n][u][p] = u32x4{0, 0, 0, 0};
                 continue;
             }
             const uint32_t twice = rows | rows << 16;
@@ -829,16 +894,12 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                 f32x4 d = {0, 0, 0, 0};
 #pragma unroll
                 for (int j = 0; j < QV; ++j) {
-                    if constexpr (BF) {
-                        const u32x4 x = {kf[t][j][0], kf[t][j][1], kf[t][j][2], kf[t][j][3]};
-                        const u32x4 y = {qf[n][j][0], qf[n][j][1], qf[n][j][2], qf[n][j][3]};
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x),
-                                                                    __builtin_bit_cast(bf16x8, y), d, 0, 0, 0);
+                    if constexpr (P > 0) {
+                        d = product<P ? P : 1>(kf[t][j], qf[n][j], d);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            d = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kf[t][j][i]),
-                                                                     __builtin_bit_cast(float, qf[n][j][i]), d, 0, 0, 0);
+                            d = __builtin_amdgcn_mfma_f32_16x16x4f32(as_float(kf[t][j][0][i]), as_float(qf[n][j][0][i]), d, 0, 0, 0);
                     }
                 }
                 w[n][t] = d;
@@ -877,42 +938,61 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             for (int t = 0; t < KT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[n][t][i] = __builtin_amdgcn_exp2f(fmaf(w[n][t][i], cs, off));
-            if constexpr (BF) {
-                // Weights are rounded to bfloat16 for the product (2^-8 of each at most, of either sign); the sum is taken
-                // of the same rounded weights, by a product with ones.
+            if constexpr (P > 0) {
+                // BF16: weights are rounded to bfloat16 for the product (2^-8 of each at most, of either sign); the sum is
+                // taken of the same rounded weights, by a product with ones.
 #pragma unroll
                 for (int u = 0; u < KT / 2; ++u) {
                     const f32x4 lo = w[n][2 * u], hi = w[n][2 * u + 1];
-                    pw[n][u] = u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
-                                     pack_bf16x2(hi[2], hi[3])};
+                    if constexpr (BF) {
+                        pw[n][u][0] = u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
+                                            pack_bf16x2(hi[2], hi[3])};
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const f32x4 &h = i < 2 ? lo : hi;
+                            uint32_t terms[3];
+                            three_terms(h[2 * (i & 1)], h[2 * (i & 1) + 1], terms);
+#pragma unroll
+                            for (int p = 0; p < P; ++p) pw[n][u][p][i] = terms[p];
+                        }
+                    }
                 }
             }
         }
-        if constexpr (!BF) {
+        if constexpr (P == 0) {
             more = next();
             if (more) load_k();
         }
         // ---- O^T
-        if constexpr (BF) {
-            const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        if constexpr (P > 0) {
+            const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
             for (int u = 0; u < KT / 2; ++u) {
 #pragma unroll
                 for (int n = 0; n < NS; ++n)
-                    sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, one),
-                                                                     __builtin_bit_cast(bf16x8, pw[n][u]), sum[n], 0, 0, 0);
+#pragma unroll
+                    for (int p = P - 1; p >= 0; --p)
+                        sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones),
+                                                                         __builtin_bit_cast(bf16x8, pw[n][u][p]), sum[n], 0, 0, 0);
 #pragma unroll
                 for (int t = 0; t < C; ++t) {
-                    const uint32_t pick = t & 1 ? 0x07060302u : 0x05040100u;
-                    const u32x4 x = {__builtin_amdgcn_perm(vf[2 * u][1][t / 2], vf[2 * u][0][t / 2], pick),
-                                     __builtin_amdgcn_perm(vf[2 * u][3][t / 2], vf[2 * u][2][t / 2], pick),
-                                     __builtin_amdgcn_perm(vf[2 * u + 1][1][t / 2], vf[2 * u + 1][0][t / 2], pick),
-                                     __builtin_amdgcn_perm(vf[2 * u + 1][3][t / 2], vf[2 * u + 1][2][t / 2], pick)};
+                    u32x4 x[P ? P : 1];
 #pragma unroll
-                    for (int n = 0; n < NS; ++n)
-                        acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x),
-                                                                            __builtin_bit_cast(bf16x8, pw[n][u]), acc[n][t],
-                                                                            0, 0, 0);
+                    for (int i = 0; i < 4; ++i) {  // a pair of keys: rows 2i, 2i + 1 of the lane's eight
+                        const uint32_t(&r0v)[VW] = vf[2 * u + (i >> 1)][2 * (i & 1)];
+                        const uint32_t(&r1v)[VW] = vf[2 * u + (i >> 1)][2 * (i & 1) + 1];
+                        if constexpr (BF) {
+                            x[0][i] = __builtin_amdgcn_perm(r1v[t / 2], r0v[t / 2], t & 1 ? 0x07060302u : 0x05040100u);
+                        } else {
+                            uint32_t terms[3];
+                            three_terms(__builtin_bit_cast(float, r0v[t]), __builtin_bit_cast(float, r1v[t]), terms);
+#pragma unroll
+                            for (int p = 0; p < P; ++p) x[p][i] = terms[p];
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NS; ++n) acc[n][t] = product<P ? P : 1>(x, pw[n][u], acc[n][t]);
                 }
             }
         } else {
@@ -930,7 +1010,6 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                     }
         }
     }
-
     } while (again());
 
     // ---- out
