@@ -621,17 +621,21 @@ __device__ __forceinline__ f32x4 product(const u32x4 (&x)[P], const u32x4 (&y)[P
 // WAVES 4: the workgroup's waves take a tile together, every fourth step (of lists,
 // block) each, and join them through LDS: a quarter of the tiles' length, so that the last
 // ones to run leave fewer units idle.  WAVES 1: a tile each, for rows of few keys.
-template <class T, int D, int KC, int NS, bool LISTED, int WAVES>
+// HALVES 2: a tile of 32 NS rows, half of them for each pair of the waves; a pair's waves take every
+// second step.  For heads whose 64 rows one wave's registers do not hold: the pairs run
+// the same steps at about the same time, so the vector cache has the second reading.
+template <class T, int D, int KC, int NS, bool LISTED, int WAVES, int HALVES>
 __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr bool BF = sizeof(T) == 2;
-    constexpr int ROWS = 16 * NS;
+    constexpr int ROWS = 16 * NS * HALVES, SETS = NS * HALVES;
     constexpr int KT = KC / 16;              // 16-key groups of a step
     constexpr int P = BF ? 1 : D <= 64 ? 3 : 0; // bfloat16 terms of a value; 0: FP32's products
     constexpr int QV = P ? D / 32 : D / 16;  // products over a row's channels
     constexpr int C = D / 16;                // channels of a lane's V row
     constexpr int VW = C * static_cast<int>(sizeof(T)) / 4;
     constexpr int E = static_cast<int>(sizeof(T));
-    static_assert(WAVES == 1 || WAVES == 4);
+    static_assert(WAVES == 4 || (WAVES == 1 && HALVES == 1));
+    static_assert(ROWS == 32 || ROWS == 64);
     // LDS: each wave's K rows of a step; the table of blocks, TABLE of them at a time for each tile of the
     // workgroup; after the last step over both, the waves' results: element (set n, i, t) of every lane.
     constexpr int TABLE = 1024, TILES = 4 / WAVES;
@@ -654,7 +658,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     // and the longest first.
     if (a.causal) tg = a.tile_groups - 1 - (tg % (a.tile_groups >> 3) * 8 + tg / (a.tile_groups >> 3));
     const int64_t tile = WAVES == 4 ? tg : static_cast<int64_t>(tg) * 4 + wave;
-    const int64_t s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, a.group, NS == 4 ? 6 : 5, tile);
+    const int64_t s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, a.group, ROWS == 64 ? 6 : 5, tile);
     const Span qs = sequence_span(a.q_starts, s, a.total_q), ks = sequence_span(a.k_starts, s, a.total_k);
     const int64_t first_row = (tile - (qs.begin * a.group / ROWS + s)) * ROWS;
     const int nrows = qs.rows * a.group;  // total_q * heads < 2^31
@@ -663,14 +667,17 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     const int tok0 = r0 / a.group, ntok = (min(r0 + ROWS, nrows) - 1) / a.group - tok0 + 1;
     const int lag = ks.rows - qs.rows;
     // this wave's share of the tile: every `pieces`-th step or chosen block, a power of two
-    const int piece = WAVES == 4 ? split * 4 + wave : split, pieces = WAVES == 4 ? a.splits * 4 : a.splits;
+    constexpr int SHARES = WAVES / HALVES;
+    const int half = HALVES == 2 ? wave >> 1 : 0;
+    const int piece = split * SHARES + (SHARES > 1 ? wave & (SHARES - 1) : 0), pieces = a.splits * SHARES;
+    const int r0w = r0 + half * 16 * NS;  // this wave's first row
 
     // this lane's query of each set of 16, and the keys that it sees: [0, lim)
     int lim[NS];
     u32x4 qf[NS][QV][P ? P : 1];
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-        const int r = min(r0 + 16 * n + c, nrows - 1), tok = r / a.group;
+        const int r = min(r0w + 16 * n + c, nrows - 1), tok = r / a.group;
         lim[n] = a.causal ? max(0, min(ks.rows, tok + lag + 1)) : ks.rows;
         const T *q = static_cast<const T *>(a.q) + (qs.begin + tok) * a.q_stride +
                      static_cast<int64_t>(kvh * a.group + r % a.group) * D;
@@ -710,7 +717,8 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                 mine = chunk + lane < count ? table[chunk + lane] : 0;
                 const uint64_t chosen = __ballot(mine != 0);
                 const int r = rank + __popcll(chosen & ((UINT64_C(1) << lane) - 1));
-                todo = __ballot(mine != 0 && (r & (pieces - 1)) == piece);
+                const uint64_t own = HALVES == 2 ? (mine >> (32 * half)) & 0xffffffffu : mine;
+                todo = __ballot(own != 0 && (r & (pieces - 1)) == piece);
                 rank += __popcll(chosen);
                 chunk += 64;
             }
@@ -877,7 +885,8 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
             // the set's rows, a bit each (all keys: all of them), and the same for the four lanes of each
-            const uint32_t rows = LISTED ? static_cast<uint32_t>(mem >> (16 * n)) & 0xffffu : r0 + 16 * n < nrows ? 0xffffu : 0u;
+            const uint32_t rows = LISTED ? static_cast<uint32_t>(mem >> (32 * half + 16 * n)) & 0xffffu
+                                         : r0w + 16 * n < nrows ? 0xffffu : 0u;
             if (rows == 0) {  // none sees the block: weights 0
 #pragma unroll
                 for (int t = 0; t < KT; ++t) w[n][t] = f32x4{0, 0, 0, 0};
@@ -1073,15 +1082,17 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             if (g == 0) part_ml[wave][n][c] = make_float2(top[n] * a.scale, sum[n][0]);
         }
         __syncthreads();
-        if (wave >= NS) return;
-        const int n = wave;  // a set for each wave
-        float m = neg_inf(), l = 0.0f, wgt[4], y[4 * C];
+        if (wave >= SETS) return;
+        // a set for each wave, from the pieces of its half
+        constexpr int J = 4 / HALVES;
+        const int n = wave % NS, p0 = wave / NS * J;
+        float m = neg_inf(), l = 0.0f, wgt[J], y[4 * C];
 #pragma unroll
-        for (int p = 0; p < 4; ++p)
-            if (part_ml[p][n][c].y != 0.0f) m = fmaxf(m, part_ml[p][n][c].x);
+        for (int p = 0; p < J; ++p)
+            if (part_ml[p0 + p][n][c].y != 0.0f) m = fmaxf(m, part_ml[p0 + p][n][c].x);
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const float2 ml = part_ml[p][n][c];
+        for (int p = 0; p < J; ++p) {
+            const float2 ml = part_ml[p0 + p][n][c];
             wgt[p] = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((ml.x - m) * kLog2e);  // a piece without keys: 0
             l += wgt[p] * ml.y;
         }
@@ -1089,9 +1100,9 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         for (int e = 0; e < 4 * C; ++e) {
             y[e] = 0.0f;
 #pragma unroll
-            for (int p = 0; p < 4; ++p) y[e] += wgt[p] * part[p][(n * 4 + e / C) * C + e % C][lane];
+            for (int p = 0; p < J; ++p) y[e] += wgt[p] * part[p0 + p][(n * 4 + e / C) * C + e % C][lane];
         }
-        finish(n, y, m, l);
+        finish(wave, y, m, l);
     }
 }
 
@@ -1181,9 +1192,9 @@ AttendCut attend_cut(bool bf, int64_t total_q, int32_t heads, int32_t kv_heads, 
     const int64_t waves = std::max<int64_t>((rows / 32 + sequences) * kv_heads * per_tile, 1);
     int32_t splits = 1;
     while (splits < 64 && waves * splits * 2 <= kWaves && keys >= 256 * splits * per_tile) splits *= 2;
-    // Tiles of 64 rows read each key half as often, where a lane's registers hold them (wider heads with one wave a SIMD
-    // for them: 874 us instead of 596, 12,001 causal rows of 128); shorter sequences would leave half of the tile empty.
-    const int32_t sets = bf && per_tile == 4 && head_dim <= 64 && rows >= 48 * sequences ? 4 : 2;
+    // Tiles of 64 rows read each key half as often; shorter sequences would leave half of the tile empty, and FP32's
+    // products take longer than its reads.
+    const int32_t sets = bf && per_tile == 4 && rows >= 48 * sequences ? 4 : 2;
     const int64_t tiles = rows / (16 * sets) + sequences;
     return {per_tile == 4 ? tiles : (tiles + 3) / 4, splits, per_tile, sets};
 }
@@ -1191,22 +1202,24 @@ AttendCut attend_cut(bool bf, int64_t total_q, int32_t heads, int32_t kv_heads, 
 using AttendFn = void (*)(AttendArgs);
 // Steps of keys as registers allow: of 64 for narrow heads and two sets of rows, of 32,
 // FP32's widest heads of 16.
-template <class T, int D, int NS, int WAVES>
+template <class T, int D, int SETS, int WAVES>
 AttendFn pick_step(bool listed, int32_t block) {
     constexpr bool BF = sizeof(T) == 2;
+    constexpr int NS = SETS == 4 && D <= 64 ? 4 : 2, HALVES = SETS / NS;
     if constexpr (BF && D <= 64 && NS == 2)
-        if (block >= 64 || !listed) return listed ? attend_kernel<T, D, 64, NS, true, WAVES> : attend_kernel<T, D, 64, NS, false, WAVES>;
+        if (block >= 64 || !listed)
+            return listed ? attend_kernel<T, D, 64, NS, true, WAVES, HALVES> : attend_kernel<T, D, 64, NS, false, WAVES, HALVES>;
     constexpr int KC = !BF && D > 64 ? 16 : 32;
-    return listed ? attend_kernel<T, D, KC, NS, true, WAVES> : attend_kernel<T, D, KC, NS, false, WAVES>;
+    return listed ? attend_kernel<T, D, KC, NS, true, WAVES, HALVES> : attend_kernel<T, D, KC, NS, false, WAVES, HALVES>;
 }
-template <class T, int NS, int WAVES>
+template <class T, int SETS, int WAVES>
 AttendFn pick_dim(int32_t d, bool listed, int32_t block) {
-    if (d == 32) return pick_step<T, 32, NS, WAVES>(listed, block);
-    if constexpr (NS == 2) {
-        if (d == 96) return pick_step<T, 96, NS, WAVES>(listed, block);
-        if (d == 128) return pick_step<T, 128, NS, WAVES>(listed, block);
+    switch (d) {
+        case 32: return pick_step<T, 32, SETS, WAVES>(listed, block);
+        case 64: return pick_step<T, 64, SETS, WAVES>(listed, block);
+        case 96: return pick_step<T, 96, SETS, WAVES>(listed, block);
+        default: return pick_step<T, 128, SETS, WAVES>(listed, block);
     }
-    return pick_step<T, 64, NS, WAVES>(listed, block);
 }
 template <class T>
 AttendFn pick_attend(int32_t d, bool listed, int32_t block, const AttendCut &cut) {
