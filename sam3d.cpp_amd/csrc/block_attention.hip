@@ -787,7 +787,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     // row's pieces xor-ed by its number so that eight neighbouring rows' pieces of one number lie in different banks.
     constexpr int ROW = D / 8;  // 16-byte pieces of a row in LDS
     const auto turned = [](int row, int piece) __attribute__((always_inline)) {
-        return piece ^ (ROW % 8 == 0 ? row & 7 : (row >> 1) & 3);
+        return piece ^ (ROW % 16 == 0 ? row & 15 : ROW % 8 == 0 ? row & 7 : (row >> 1) & 3);
     };
     char *kt = lds + wave * KEYS;
     int koff[P ? NP : KT], kput[P ? NP : 1], kget[P ? QV : 1];
