@@ -17,6 +17,7 @@ fallback: if the HIP library cannot be loaded, import fails loudly.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from pathlib import Path
 
 import numpy as np
@@ -137,10 +138,16 @@ def lib() -> C.CDLL:
     return _lib
 
 
+_errors = threading.local()  # a thread's error buffer: success clears it, failure is read at once
+
+
 def call(name: str, *args):
     """Call an error-buffer entry point; raise S3dxError on a non-OK status."""
-    buf = C.create_string_buffer(512)
-    status = getattr(lib(), name)(*args, buf, len(buf))
+    try:
+        buf = _errors.buf
+    except AttributeError:
+        buf = _errors.buf = C.create_string_buffer(512)
+    status = getattr(_lib or lib(), name)(*args, buf, 512)
     if status != OK:
         raise S3dxError(status, buf.value.decode(errors="replace"))
     return status
@@ -646,6 +653,15 @@ def convert(x, x_dtype, count, y, y_dtype, stream=None):
 # ---------------------------------------------------------------------------
 # Attention over voxel rows
 # ---------------------------------------------------------------------------
+def _addr(a):
+    """A device pointer as the argument types take it (their calls are short: no object for each pointer)."""
+    return a.ptr if isinstance(a, DeviceArray) else a
+
+
+def _handle(stream):
+    return stream.handle if isinstance(stream, Stream) else stream
+
+
 class Rotary:
     """Rotary positions with several axes (s3dx_rotary): pair j turns by
     position[axis[j]] * frequency[j] radians."""
@@ -675,9 +691,9 @@ class Rotary:
         row = heads * self.head_dim
         xs = row if x_stride is None else x_stride
         ys = y_stride if y_stride is not None else (xs if y is None else row)
-        call("s3dx_rotary_apply", self.handle, int(inverse), _dptr(x), dtype, n, heads, xs, _dptr(positions),
-             self.axes if position_stride is None else position_stride, _dptr(x if y is None else y),
-             dtype if y_dtype is None else y_dtype, ys, _sptr(stream))
+        call("s3dx_rotary_apply", self.handle, int(inverse), _addr(x), dtype, n, heads, xs, _addr(positions),
+             self.axes if position_stride is None else position_stride, _addr(x if y is None else y),
+             dtype if y_dtype is None else y_dtype, ys, _handle(stream))
 
     def __del__(self):
         try:
@@ -696,10 +712,10 @@ def qk_norm_rotary(q, k, dtype, n, q_heads, k_heads, head_dim, eps, q_out=None, 
     qo = q_out_stride if q_out_stride is not None else (qs if q_out is None else q_heads * head_dim)
     ko = k_out_stride if k_out_stride is not None else (ks if k_out is None else k_heads * head_dim)
     ps = position_stride if position_stride is not None else (rotary.axes if rotary is not None else 0)
-    call("s3dx_qk_norm_rotary", rotary.handle if rotary is not None else None, _dptr(positions), ps, _dptr(q), q_heads,
-         qs, _dptr(q_gain), _dptr(k), k_heads, ks, _dptr(k_gain), int(gain_per_head), dtype, n, head_dim, eps,
-         _dptr(q if q_out is None else q_out), qo, _dptr(k if k_out is None else k_out), ko,
-         dtype if out_dtype is None else out_dtype, _sptr(stream))
+    call("s3dx_qk_norm_rotary", rotary.handle if rotary is not None else None, _addr(positions), ps, _addr(q), q_heads,
+         qs, _addr(q_gain), _addr(k), k_heads, ks, _addr(k_gain), int(gain_per_head), dtype, n, head_dim, eps,
+         _addr(q if q_out is None else q_out), qo, _addr(k if k_out is None else k_out), ko,
+         dtype if out_dtype is None else out_dtype, _handle(stream))
 
 
 def block_index_rows(total_k: int, sequences: int, block: int) -> int:
@@ -711,18 +727,18 @@ def block_index_rows(total_k: int, sequences: int, block: int) -> int:
 def block_index(k, dtype, total_k, kv_heads, head_dim, k_starts, sequences, block, codes, scale, k_stride=None,
                 stream=None):
     """The 8-bit index of the key blocks' means (s3dx_block_index)."""
-    call("s3dx_block_index", _dptr(k), dtype, total_k, kv_heads, head_dim,
-         kv_heads * head_dim if k_stride is None else k_stride, _dptr(k_starts), sequences, block, _dptr(codes),
-         _dptr(scale), _sptr(stream))
+    call("s3dx_block_index", _addr(k), dtype, total_k, kv_heads, head_dim,
+         kv_heads * head_dim if k_stride is None else k_stride, _addr(k_starts), sequences, block, _addr(codes),
+         _addr(scale), _handle(stream))
 
 
 def block_select(q, dtype, total_q, total_k, heads, kv_heads, head_dim, q_starts, k_starts, sequences, block, top, max_k,
                  codes, scale, selected, q_stride=None, causal=False, near=False, stream=None):
     """The `top` best key blocks of each query row and key head (s3dx_block_select)."""
-    call("s3dx_block_select", _dptr(q), dtype, total_q, total_k, heads, kv_heads, head_dim,
-         heads * head_dim if q_stride is None else q_stride, _dptr(q_starts), _dptr(k_starts), sequences, block, top,
-         max_k, _dptr(codes), _dptr(scale), (BLOCK_CAUSAL if causal else 0) | (BLOCK_NEAR if near else 0),
-         _dptr(selected), _sptr(stream))
+    call("s3dx_block_select", _addr(q), dtype, total_q, total_k, heads, kv_heads, head_dim,
+         heads * head_dim if q_stride is None else q_stride, _addr(q_starts), _addr(k_starts), sequences, block, top,
+         max_k, _addr(codes), _addr(scale), (BLOCK_CAUSAL if causal else 0) | (BLOCK_NEAR if near else 0),
+         _addr(selected), _handle(stream))
 
 
 def block_attention_workspace_size(total_q, heads, kv_heads, head_dim, sequences, block, top, max_k) -> int:
@@ -739,12 +755,12 @@ def block_attention(q, k, v, dtype, total_q, total_k, heads, kv_heads, head_dim,
     scale: head_dim^-0.5 unless given."""
     if workspace_bytes is None:
         workspace_bytes = workspace.nbytes if isinstance(workspace, DeviceArray) else 0
-    call("s3dx_block_attention", _dptr(q), _dptr(k), _dptr(v), dtype, total_q, total_k, heads, kv_heads, head_dim,
+    call("s3dx_block_attention", _addr(q), _addr(k), _addr(v), dtype, total_q, total_k, heads, kv_heads, head_dim,
          heads * head_dim if q_stride is None else q_stride, kv_heads * head_dim if k_stride is None else k_stride,
-         kv_heads * head_dim if v_stride is None else v_stride, _dptr(q_starts), _dptr(k_starts), sequences, block, max_k,
-         _dptr(selected), top, head_dim ** -0.5 if scale is None else scale, BLOCK_CAUSAL if causal else 0, _dptr(o),
-         heads * head_dim if o_stride is None else o_stride, _dptr(lse), _dptr(workspace), workspace_bytes,
-         _sptr(stream))
+         kv_heads * head_dim if v_stride is None else v_stride, _addr(q_starts), _addr(k_starts), sequences, block, max_k,
+         _addr(selected), top, head_dim ** -0.5 if scale is None else scale, BLOCK_CAUSAL if causal else 0, _addr(o),
+         heads * head_dim if o_stride is None else o_stride, _addr(lse), _addr(workspace), workspace_bytes,
+         _handle(stream))
 
 
 def synchronize(stream=None):

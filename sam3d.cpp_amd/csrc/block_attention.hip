@@ -1296,6 +1296,7 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
         // Queries of a workgroup: 16, unless those leave most compute units without one or their keys take more than
         // 64 KiB of LDS (1,024 blocks; 4,096 of four queries).
         const int64_t rows = total_q * kv_heads;
+        require(rows <= std::numeric_limits<int32_t>::max(), "total_q * kv_heads is out of range");
         const int qt = rows >= 16 * 512 && a.most_blocks <= 1024 ? 16 : rows >= 4 * 256 && a.most_blocks <= 4096 ? 4 : 1;
         const int team = select_team(qt);
         a.run = std::max((a.most_blocks + team - 1) / team + 3, 4) / 4 * 4;
