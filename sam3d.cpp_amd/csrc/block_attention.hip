@@ -195,9 +195,8 @@ __device__ __forceinline__ int team_before(int v) {
 
 // A tile of QT queries of one key head.  Scores by integer products (16x16x64: blocks by
 // queries), their order keys in LDS; then a team of 16 or 64 threads for each query, each with a run
-// of blocks side by side, finds the `top`-th largest key by cutting the range of keys (by the
-// counts at its ends, then by half, in turn; it stops as soon as the count of the keys
-// from the cut on is right: about five cuts for 80 blocks) and writes its run's chosen
+// of blocks side by side, finds the `top`-th largest key by cutting the range of keys (it stops
+// as soon as the count of the keys from the cut on is right) and writes its run's chosen
 // blocks behind those of the threads before it, equal keys first come, first served.  RUN: a
 // thread's blocks, whose keys stay in registers; 0: any number, from LDS each time.
 // QT 16 fills the products; 4 and 1 are for few rows, and for more blocks than LDS
@@ -397,26 +396,24 @@ __global__ void __launch_bounds__(select_threads(QT)) select_kernel(SelectArgs a
     }
     // at least `take` keys are >= low (count of them: n_low), fewer than that are >= high
     high += 1;
-    int n_low = may, n_high = 0;
+    int n_low = may;
     if (take == 0) low = high = 1, n_low = 0;
+    float f_low = of_key(low), f_high = of_key(high);
     for (int cut = 0;; ++cut) {
         const bool going = n_low != take && high - low > 1;
         if (__builtin_amdgcn_ballot_w64(going) == 0) break;
-        // Where the cut is made decides only how soon it ends: in the values, by the counts and by half in turn;
-        // in the keys by half from the 16th on (at most 32 more), and where the values leave nothing between.
-        uint32_t mid = low + (high - low) / 2;
-        const float f0 = of_key(low), f1 = of_key(high);
-        const float part = cut & 1 ? 0.5f
-                                   : (static_cast<float>(n_low - take) + 0.5f) *
-                                         __builtin_amdgcn_rcpf(static_cast<float>(max(n_low - n_high, 1)));
-        const uint32_t by_value = order_key(f0 + (f1 - f0) * part);
-        if (cut < 16 && by_value > low && by_value < high) mid = by_value;
+        // Cut halfway between the values (about eight cuts for 80 blocks; where it is made decides only how soon
+        // it ends); from the 16th on, and where the values leave nothing between, halfway between the keys (at most 32 more).
+        uint32_t mid = order_key(0.5f * f_low + 0.5f * f_high);
+        if (__builtin_amdgcn_ballot_w64(going && (mid <= low || mid >= high || cut >= 16)) != 0 &&
+            (mid <= low || mid >= high || cut >= 16))
+            mid = low + (high - low) / 2;
         int n = 0;
         each([&](uint32_t k, int) { n += k >= mid ? 1 : 0; });
         n = team_sum<TEAM>(n);
         if (going) {
-            if (n >= take) low = mid, n_low = n;
-            else high = mid, n_high = n;
+            if (n >= take) low = mid, f_low = of_key(mid), n_low = n;
+            else high = mid, f_high = of_key(mid);
         }
     }
     // Chosen: keys above low, and of those that equal it the first ones (all, where the count came out right).
