@@ -581,6 +581,14 @@ __device__ __forceinline__ void three_terms(float x, float y, uint32_t (&out)[3]
     }
 }
 
+// Of 16 lanes, lane 4i + a gives the address of four 16-bit values (row i, columns 4a..) and
+// gets column 4i + a of the four rows.
+__device__ __forceinline__ u32x2 transposed(const char *p) {
+    typedef short i16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) i16x4 *)(const_cast<char *>(p))));
+}
+
 // d += A B over 32 values: one product of bfloat16 operands, or, of operands in three terms, the six
 // of at least 2^-16 of the whole, the smallest first (what is left out is 2^-24 of it and less).
 template <int P>
@@ -618,13 +626,15 @@ __device__ __forceinline__ f32x4 product(const u32x4 (&x)[P], const u32x4 (&y)[P
 // WAVES 4: the workgroup's waves take a tile together, every fourth step (of lists,
 // block) each, and join them through LDS: a quarter of the tiles' length, so that the last
 // ones to run leave fewer units idle.  WAVES 1: a tile each, for rows of few keys.
-// HALVES 2: a tile of 32 NS rows, half of them for each pair of the waves; a pair's waves take every
-// second step.  For heads whose 64 rows one wave's registers do not hold: the pairs run
-// the same steps at about the same time, so the vector cache has the second reading.
+// HALVES 2: a tile of 32 NS rows, half of them for each pair of the waves, a pair's waves every second step.
+// For heads whose 64 rows one wave's registers do not hold: the two waves of a step
+// fetch half of its K and V rows each, into LDS that they share (two buffers, one barrier a step);
+// V^T is read from there by the transposing reads of 16-bit data.
 template <class T, int D, int KC, int NS, bool LISTED, int WAVES, int HALVES>
 __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr bool BF = sizeof(T) == 2;
     constexpr int ROWS = 16 * NS * HALVES, SETS = NS * HALVES;
+    constexpr bool SHARED = HALVES == 2;
     constexpr int KT = KC / 16;              // 16-key groups of a step
     constexpr int P = BF ? 1 : D <= 64 ? 3 : 0; // bfloat16 terms of a value; 0: FP32's products
     constexpr int QV = P ? D / 32 : D / 16;  // products over a row's channels
@@ -632,13 +642,16 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr int VW = C * static_cast<int>(sizeof(T)) / 4;
     constexpr int E = static_cast<int>(sizeof(T));
     static_assert(WAVES == 4 || (WAVES == 1 && HALVES == 1));
+    static_assert(HALVES == 1 || (HALVES == 2 && BF));
     static_assert(ROWS == 32 || ROWS == 64);
-    // LDS: each wave's K rows of a step; the table of blocks, TABLE of them at a time for each tile of the
+    // LDS: each wave's K rows of a step (or the shared buffers); the table of blocks, TABLE of them at a time for each tile of the
     // workgroup; after the last step over both, the waves' results: element (set n, i, t) of every lane.
     constexpr int TABLE = 1024, TILES = 4 / WAVES;
     constexpr int CH = D * E / 16;                 // 16-byte pieces of a K row
-    constexpr int NP = KC * CH / 64;               // ... of a step, for each lane
-    constexpr int KEYS = P * KC * D * 2, TABLES = LISTED ? TABLE * TILES * 8 : 0;
+    constexpr int NP = KC * CH / 64 / (SHARED ? 2 : 1);  // ... of a step, for each lane
+    static_assert(KC * CH % (SHARED ? 128 : 64) == 0);
+    constexpr int PLANE = KC * D * 2;              // a step's rows in bfloat16
+    constexpr int KEYS = SHARED ? 2 * PLANE : P * PLANE, TABLES = LISTED ? TABLE * TILES * 8 : 0;
     constexpr int PART = WAVES == 4 ? 4 * NS * 4 * C * 64 * 4 : 0;
     constexpr int LDS = 4 * KEYS + TABLES > PART ? 4 * KEYS + TABLES : PART;
     __shared__ alignas(16) char lds[LDS > 0 ? LDS : 16];
@@ -704,18 +717,22 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     uint64_t todo = 0, mine = 0;      // this wave's blocks among the last 64; this lane's table entry of them
     uint64_t members = ~UINT64_C(0);
     int first, end;                   // the step's first key, the end of its block
+    int whole = 0;                    // ... were it a whole one
     const auto next = [&]() __attribute__((always_inline)) {  // false: no step left in the table
         if constexpr (LISTED) {
             first += KC;
-            if (first < end) return true;
+            // SHARED: every block takes all of its steps, also those behind the last key, so that the waves stay together
+            if (SHARED ? first < whole : first < end) return !SHARED || first < end;
             while (todo == 0) {
                 const int count = min(TABLE, blocks - w0);
-                if (chunk >= count) return false;
+                if (chunk >= count) {
+                    first = 1 << 30;
+                    return false;
+                }
                 mine = chunk + lane < count ? table[chunk + lane] : 0;
                 const uint64_t chosen = __ballot(mine != 0);
                 const int r = rank + __popcll(chosen & ((UINT64_C(1) << lane) - 1));
-                const uint64_t own = HALVES == 2 ? (mine >> (32 * half)) & 0xffffffffu : mine;
-                todo = __ballot(own != 0 && (r & (pieces - 1)) == piece);
+                todo = __ballot(mine != 0 && (r & (pieces - 1)) == piece);
                 rank += __popcll(chosen);
                 chunk += 64;
             }
@@ -724,7 +741,8 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             members = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), bit))) << 32 |
                       static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), bit));
             first = (w0 + chunk - 64 + bit) << a.block_log2;
-            end = min(first + a.block, most);
+            whole = first + a.block;
+            end = min(whole, most);
             return true;
         } else {
             first += pieces * KC;
@@ -770,7 +788,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     }
     const float cs = a.scale * kLog2e;
     // Byte offsets of this lane's rows of V in a step: held where registers allow, else the first and the steps between.
-    constexpr bool HELD = D < 128;
+    constexpr bool HELD = D < 128 && !SHARED;
     const int kstep = static_cast<int>(a.k_stride) * E, vstep = static_cast<int>(a.v_stride) * E;
     const int vat = 4 * g * vstep + c * (C * E);
     int voff[HELD ? KT : 1][4];
@@ -786,13 +804,14 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     const auto turned = [](int row, int piece) __attribute__((always_inline)) {
         return piece ^ (ROW % 16 == 0 ? row & 15 : ROW % 8 == 0 ? row & 7 : (row >> 1) & 3);
     };
-    char *kt = lds + wave * KEYS;
-    int koff[P ? NP : KT], kput[P ? NP : 1], kget[P ? QV : 1];
+    char *kt = SHARED ? lds + (wave & 1) * (4 * PLANE) : lds + wave * KEYS;
+    int koff[P ? NP : KT], kput[P ? NP : 1], kget[P ? QV : 1], vsrc[SHARED ? NP : 1], vget[SHARED ? C : 1];
     if constexpr (P > 0) {
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-            const int row = (p * 64 + lane) / CH, piece = (p * 64 + lane) % CH;
+            const int at = ((SHARED ? half * NP : 0) + p) * 64 + lane, row = at / CH, piece = at % CH;
             koff[p] = row * kstep + piece * 16;
+            if constexpr (SHARED) vsrc[p] = row * vstep + piece * 16;
             kput[p] = BF ? (row * ROW + turned(row, piece)) * 16 : (row * ROW + turned(row, piece >> 1)) * 16 + (piece & 1) * 8;
         }
 #pragma unroll
@@ -801,13 +820,24 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int t = 0; t < KT; ++t) koff[t] = (16 * t + c) * kstep + 16 * g;
     }
-    uint32_t kn[P ? NP : 1][4];
+    if constexpr (SHARED) {
+        // of each 16 lanes, lane 4i + a gives channels 16t + 4a.. of key 4g + i and gets channel 16t + 4i + a of the four keys
+        const int row = 4 * g + (c >> 2);
+#pragma unroll
+        for (int t = 0; t < C; ++t) vget[t] = PLANE + (row * ROW + turned(row, 2 * t + ((c & 3) >> 1))) * 16 + (c & 1) * 8;
+    }
+    uint32_t kn[P ? NP : 1][4], vn[SHARED ? NP : 1][4];
     u32x4 kf[KT][QV][P ? P : 1];
     const auto load_k = [&]() __attribute__((always_inline)) {
         const auto r = rows_buffer<T, D>(a.k, ks.begin + first, a.k_stride, kvh, min(KC, ks.rows - first));
         if constexpr (P > 0) {
 #pragma unroll
             for (int p = 0; p < NP; ++p) buffer_dwords<4>(r, koff[p], kn[p]);
+            if constexpr (SHARED) {
+                const auto rv = rows_buffer<T, D>(a.v, ks.begin + first, a.v_stride, kvh, min(KC, ks.rows - first));
+#pragma unroll
+                for (int p = 0; p < NP; ++p) buffer_dwords<4>(rv, vsrc[p], vn[p]);
+            }
         } else {
 #pragma unroll
             for (int t = 0; t < KT; ++t)
@@ -823,6 +853,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     if constexpr (LISTED) first = end = 0;
     else first = (piece - pieces) * KC, end = most;
     bool more;
+    int buffer = 0, rank0 = 0;  // SHARED: the step's buffer; chosen blocks before the table
     const auto begin = [&]() __attribute__((always_inline)) {
         if constexpr (LISTED) fill_table();
         more = next();
@@ -837,45 +868,9 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         together();
         return true;
     };
-    do {
-    begin();
-    while (more) {
-        const int at = first;
-        const uint64_t mem = members;
-        // ---- V of this step
-        uint32_t vf[KT][4][VW];  // rows 16t + 4g + i
-        {
-            const auto r = rows_buffer<T, D>(a.v, ks.begin + at, a.v_stride, kvh, min(KC, ks.rows - at));
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) buffer_dwords<VW>(r, HELD ? voff[HELD ? t : 0][i] : vat + (16 * t + i) * vstep, vf[t][i]);
-        }
-        // ---- K of this step to its operand's lanes, the next step's on its way
-        if constexpr (P > 0) {
-#pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                if constexpr (BF) {
-                    *reinterpret_cast<u32x4 *>(kt + kput[p]) = u32x4{kn[p][0], kn[p][1], kn[p][2], kn[p][3]};
-                } else {
-                    uint32_t lo[3], hi[3];
-                    three_terms(__builtin_bit_cast(float, kn[p][0]), __builtin_bit_cast(float, kn[p][1]), lo);
-                    three_terms(__builtin_bit_cast(float, kn[p][2]), __builtin_bit_cast(float, kn[p][3]), hi);
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x2 *>(kt + i * (KC * D * 2) + kput[p]) = u32x2{lo[i], hi[i]};
-                }
-            }
-            more = next();
-            if (more) load_k();
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int j = 0; j < QV; ++j)
-#pragma unroll
-                    for (int p = 0; p < P; ++p)
-                        kf[t][j][p] = *reinterpret_cast<const u32x4 *>(kt + p * (KC * D * 2) + kget[j] + t * (16 * ROW * 16));
-        }
+    // A step: the keys from `at` on for the rows of `mem`, of the operands in kf and (vf or LDS).
+    uint32_t vf[SHARED ? 1 : KT][4][VW];  // rows 16t + 4g + i
+    const auto step = [&](int at, uint64_t mem) __attribute__((always_inline)) {
         // ---- sets of 16 rows: S^T, weights
         f32x4 w[NS][KT];
         u32x4 pw[NS][KT / 2 > 0 ? KT / 2 : 1][P ? P : 1];
@@ -984,17 +979,23 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int t = 0; t < C; ++t) {
                     u32x4 x[P ? P : 1];
+                    if constexpr (SHARED) {
+                        const char *from = kt + buffer + vget[t] + u * (32 * ROW * 16);
+                        const u32x2 lo = transposed(from), hi = transposed(from + 16 * ROW * 16);
+                        x[0] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {  // a pair of keys: rows 2i, 2i + 1 of the lane's eight
-                        const uint32_t(&r0v)[VW] = vf[2 * u + (i >> 1)][2 * (i & 1)];
-                        const uint32_t(&r1v)[VW] = vf[2 * u + (i >> 1)][2 * (i & 1) + 1];
-                        if constexpr (BF) {
-                            x[0][i] = __builtin_amdgcn_perm(r1v[t / 2], r0v[t / 2], t & 1 ? 0x07060302u : 0x05040100u);
-                        } else {
-                            uint32_t terms[3];
-                            three_terms(__builtin_bit_cast(float, r0v[t]), __builtin_bit_cast(float, r1v[t]), terms);
+                        for (int i = 0; i < 4; ++i) {  // a pair of keys: rows 2i, 2i + 1 of the lane's eight
+                            const uint32_t(&r0v)[VW] = vf[2 * u + (i >> 1)][2 * (i & 1)];
+                            const uint32_t(&r1v)[VW] = vf[2 * u + (i >> 1)][2 * (i & 1) + 1];
+                            if constexpr (BF) {
+                                x[0][i] = __builtin_amdgcn_perm(r1v[t / 2], r0v[t / 2], t & 1 ? 0x07060302u : 0x05040100u);
+                            } else {
+                                uint32_t terms[3];
+                                three_terms(__builtin_bit_cast(float, r0v[t]), __builtin_bit_cast(float, r1v[t]), terms);
 #pragma unroll
-                            for (int p = 0; p < P; ++p) x[p][i] = terms[p];
+                                for (int p = 0; p < P; ++p) x[p][i] = terms[p];
+                            }
                         }
                     }
 #pragma unroll
@@ -1015,7 +1016,90 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                                                                              acc[n][x], 0, 0, 0);
                     }
         }
-    }
+    };
+    const auto read_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int j = 0; j < QV; ++j)
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+                    kf[t][j][p] = *reinterpret_cast<const u32x4 *>(kt + (SHARED ? buffer : 0) + p * PLANE + kget[j] + t * (16 * ROW * 16));
+    };
+    do {
+        begin();
+        if constexpr (SHARED) {
+            // The workgroup's steps: those of its piece that has most.
+            const int p0 = split * 2;
+            int steps = 0;
+            if constexpr (LISTED) {
+                int chosen = 0;
+                for (int e = 0; e < min(TABLE, blocks - w0); e += 64)
+                    chosen += __popcll(__ballot(e + lane < min(TABLE, blocks - w0) && table[e + lane] != 0));
+                const auto before = [&](int r, int p) { return r > p ? (r - p + pieces - 1) / pieces : 0; };
+                for (int p = p0; p < p0 + 2; ++p)
+                    steps = max(steps, (before(rank0 + chosen, p) - before(rank0, p)) * (a.block / KC));
+                rank0 += chosen;
+            } else {
+                steps = max(0, ((most + KC - 1) / KC - p0 + pieces - 1) / pieces);
+            }
+            for (int it = 0; it < steps; ++it) {
+                const int at = first;
+                const uint64_t mem = members;
+                const bool now = more;
+                char *to = kt + (it & 1) * (2 * PLANE);
+                if (now) {
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) {
+                        *reinterpret_cast<u32x4 *>(to + kput[p]) = u32x4{kn[p][0], kn[p][1], kn[p][2], kn[p][3]};
+                        *reinterpret_cast<u32x4 *>(to + PLANE + kput[p]) = u32x4{vn[p][0], vn[p][1], vn[p][2], vn[p][3]};
+                    }
+                }
+                more = it + 1 < steps && next();
+                if (more) load_k();
+                // this step's rows are in LDS (the next ones' fetches go on), and all have read the step before the last
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (now && (!LISTED || ((mem >> (32 * half)) & 0xffffffffu) != 0)) {
+                    buffer = (it & 1) * (2 * PLANE);
+                    read_k();
+                    step(at, mem);
+                }
+            }
+        } else {
+            while (more) {
+                const int at = first;
+                const uint64_t mem = members;
+                // ---- V of this step
+                {
+                    const auto r = rows_buffer<T, D>(a.v, ks.begin + at, a.v_stride, kvh, min(KC, ks.rows - at));
+#pragma unroll
+                    for (int t = 0; t < KT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            buffer_dwords<VW>(r, HELD ? voff[HELD ? t : 0][i] : vat + (16 * t + i) * vstep, vf[t][i]);
+                }
+                // ---- K of this step to its operand's lanes, the next step's on its way
+                if constexpr (P > 0) {
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) {
+                        if constexpr (BF) {
+                            *reinterpret_cast<u32x4 *>(kt + kput[p]) = u32x4{kn[p][0], kn[p][1], kn[p][2], kn[p][3]};
+                        } else {
+                            uint32_t lo[3], hi[3];
+                            three_terms(__builtin_bit_cast(float, kn[p][0]), __builtin_bit_cast(float, kn[p][1]), lo);
+                            three_terms(__builtin_bit_cast(float, kn[p][2]), __builtin_bit_cast(float, kn[p][3]), hi);
+#pragma unroll
+                            for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x2 *>(kt + i * PLANE + kput[p]) = u32x2{lo[i], hi[i]};
+                        }
+                    }
+                    more = next();
+                    if (more) load_k();
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    read_k();
+                }
+                step(at, mem);
+            }
+        }
     } while (again());
 
     // ---- out
@@ -1053,7 +1137,18 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         for (int e = 0; e < 4 * C; ++e) odd += y[e] * 0.0f;
         uint64_t bad = parts ? 0 : __ballot(r < nrows && odd != 0.0f);  // pieces: the join looks
         bad = (bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffffu;
-        if (r < nrows && !((bad >> c) & 1u)) put(r / a.group - tok0, kvh * a.group + r % a.group, 4 * g * C, y, m, l);
+        if (r < nrows && !((bad >> c) & 1u)) {
+            const int t0 = r / a.group - tok0, h = kvh * a.group + r % a.group;
+            if constexpr (SHARED) {  // element i*C + t is channel 16t + 4g + i
+#pragma unroll
+                for (int t = 0; t < C; ++t) {
+                    const float four[4] = {y[t], y[C + t], y[2 * C + t], y[3 * C + t]};
+                    put(t0, h, 16 * t + 4 * g, four, m, l);
+                }
+            } else {  // ... channel (4g + i)*C + t
+                put(t0, h, 4 * g * C, y, m, l);
+            }
+        }
         while (bad) {
             const int w = r0 + 16 * n + __builtin_ctzll(bad);
             bad &= bad - 1;

@@ -242,6 +242,19 @@ ATTEND = [
     ([1, 1], [2500, 64], 12, 12, 64, 64, 0, True),           # ... over everything
     ([2], [4000], 4, 4, 64, 128, 0, False),
     ([3], [2000], 4, 1, 64, 32, 30, True),
+    # tiles that several waves take together, whole ones and the last
+    ([150], [700], 4, 2, 128, 64, 0, True),
+    ([120], [900], 2, 2, 96, 32, 17, False),
+    ([130], [700], 6, 3, 128, 128, 5, True),
+    ([70, 0, 100], [600, 0, 650], 2, 2, 96, 64, 9, False),
+    ([65], [1300], 2, 1, 128, 64, 0, False),
+    ([97], [1100], 3, 3, 64, 64, 10, True),
+    ([100], [600], 2, 2, 64, 64, 0, True),
+    ([64, 64], [520, 1], 2, 2, 32, 32, 0, False),
+    # more blocks than a tile's table holds at a time
+    ([50], [40000], 2, 1, 32, 32, 20, False),
+    ([50], [40000], 2, 1, 128, 32, 20, True),
+    ([20, 3], [35000, 20000], 2, 2, 64, 32, 4, True),
 ]
 
 
@@ -271,13 +284,14 @@ def test_lists_in_any_order(s3dx, dtype):
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
-@pytest.mark.parametrize("n,lk,top,late", [(90, 200, 2, 0), (1, 1500, 9, 0), (70, 200, 0, 0), (70, 200, 0, 130)])
-def test_what_a_row_does_not_see_does_not_reach_it(s3dx, dtype, n, lk, top, late):
+@pytest.mark.parametrize("n,lk,top,late,d", [(90, 200, 2, 0, 64), (1, 1500, 9, 0, 64), (70, 200, 0, 0, 64), (70, 200, 0, 130, 64),
+                                             (90, 700, 17, 0, 64), (90, 700, 17, 0, 128), (200, 900, 0, 790, 96), (3, 4000, 0, 3900, 32)])
+def test_what_a_row_does_not_see_does_not_reach_it(s3dx, dtype, n, lk, top, late, d):
     rng = np.random.default_rng(n)
-    q, k, v = rows(rng, n, 4, 64), rows(rng, lk, 2, 64), rows(rng, lk, 2, 64)
+    q, k, v = rows(rng, n, 4, d), rows(rng, lk, 2, d), rows(rng, lk, 2, d)
     sel = choose(rng, [n], [lk], 2, 32, top) if top else None
     # with all keys and without `late` every row sees the first of them
-    bad = [late + 1, late + 40, lk - n + 1 + late // 6, lk - 2] if n > 1 else [33, 700, 1400]
+    bad = [late + 1, late + 40, lk - n + 1 + late // 6, lk - 2] if n > 3 else [33, 700, 1400] if n == 1 else [lk - 2, lk - 1]
     if n == 1:
         sel[sel == 1] = 2
         sel[(sel == 700 // 32) | (sel == 1400 // 32)] = 5
