@@ -251,10 +251,17 @@ ATTEND = [
     ([97], [1100], 3, 3, 64, 64, 10, True),
     ([100], [600], 2, 2, 64, 64, 0, True),
     ([64, 64], [520, 1], 2, 2, 32, 32, 0, False),
+    # many tiles of a wave each, of several steps
+    ([300] + [5] * 40, [300] + [5] * 40, 20, 20, 64, 64, 0, False),
+    ([4] * 40 + [290], [4] * 40 + [290], 20, 20, 128, 32, 3, True),
+    ([3] * 40 + [200], [9] * 40 + [310], 40, 20, 32, 64, 0, True),
+    ([250] + [6] * 40, [250] + [6] * 40, 20, 20, 96, 128, 1, False),
+    ([200, 1] + [0] * 60, [270, 1] + [0] * 60, 20, 20, 64, 32, 5, False),
     # more blocks than a tile's table holds at a time
     ([50], [40000], 2, 1, 32, 32, 20, False),
     ([50], [40000], 2, 1, 128, 32, 20, True),
     ([20, 3], [35000, 20000], 2, 2, 64, 32, 4, True),
+    ([9] + [1] * 60, [20000] + [3] * 60, 20, 20, 64, 32, 3, False),
 ]
 
 
