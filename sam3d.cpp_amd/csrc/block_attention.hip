@@ -1209,20 +1209,32 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
     const int head = static_cast<int>(cell - row * a.heads);
     const int64_t s = sequence_of_row(a.q_starts, a.sequences, row);
     if (s < 0) return;
-    float m = neg_inf();
-    for (int p = 0; p < a.splits; ++p) {
-        const float2 ml = a.part_ml[p * cells + cell];
-        if (ml.y != 0.0f) m = fmaxf(m, ml.x);
-    }
-    float l = 0.0f, o[2] = {0.0f, 0.0f};
-    for (int p = 0; p < a.splits; ++p) {
-        const float2 ml = a.part_ml[p * cells + cell];
-        if (ml.y == 0.0f) continue;  // a piece without keys (a NaN is not 0 and stays)
-        const float w = exp2f((ml.x - m) * kLog2e);
-        l += w * ml.y;
+    // a lane for each piece (there are at most 64): its weight, 0 for one without keys (a sum that is a NaN is not 0 and stays)
+    const float2 ml = lane < a.splits ? a.part_ml[lane * cells + cell] : make_float2(neg_inf(), 0.0f);
+    float m = ml.y != 0.0f ? ml.x : neg_inf();
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    const float w = ml.y != 0.0f ? exp2f((ml.x - m) * kLog2e) : 0.0f;
+    float l = w == 0.0f ? 0.0f : w * ml.y, o[2] = {0.0f, 0.0f};
+    for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
+    // four pieces' values on their way at a time
+    for (uint64_t left = __ballot(ml.y != 0.0f); left;) {
+        float wp[4], x[4][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-            if (lane + 64 * e < D) o[e] += w * a.part_o[(p * cells + cell) * D + lane + 64 * e];
+        for (int u = 0; u < 4; ++u) {
+            const int p = left ? __builtin_ctzll(left) : -1;
+            left &= left - 1;
+            wp[u] = 0.0f;
+            x[u][0] = x[u][1] = 0.0f;
+            if (p < 0) continue;
+            wp[u] = __shfl(w, p, 64);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (lane + 64 * e < D) x[u][e] = a.part_o[(p * cells + cell) * D + lane + 64 * e];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) o[e] += wp[u] * x[u][e];
     }
     if (__any((l + o[0] + o[1]) * 0.0f != 0.0f)) {  // not finite: see the tiles
         attend_row<T, D>(a, row, head, sequence_span(a.q_starts, s, a.total_q), sequence_span(a.k_starts, s, a.total_k));
