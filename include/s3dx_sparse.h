@@ -576,7 +576,8 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
  * logarithm of the row's sum of exp(score).  A row that sees no key, or only
  * scores of -inf, gets zeros and lse -inf; keys and values that a row does not
  * see do not reach it, whatever they hold.  BF16 weights are rounded to bfloat16
- * before they meet the values, FP32 ones are not.  Rows whose result is not
+ * before they meet the values (their sum and lse are of the weights before that),
+ * FP32 ones are not.  Rows whose result is not
  * finite are computed a second time key by key, more slowly.
  * The workspace holds partial results where there are too few rows to fill the GPU
  * (s3dx_block_attention_workspace_size, 0 bytes where none are needed); the

@@ -478,6 +478,16 @@ __device__ __forceinline__ float max_over_groups(float v) {
     return fmaxf(as_float(b[0]), as_float(b[1]));
 }
 
+// Sum over the same lanes.
+__device__ __forceinline__ float sum_over_groups(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const float m = as_float(a[0]) + as_float(a[1]);
+    const uint32_t w = __builtin_bit_cast(uint32_t, m);
+    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return as_float(b[0]) + as_float(b[1]);
+}
+
 // One row by the whole wave, key by key: scores with a key per lane, the running maximum
 // and sum, values with a channel pair per lane.  Only keys that the row sees are
 // multiplied, so nothing else reaches it: for rows whose tile gave no finite result.
@@ -939,9 +949,19 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             for (int t = 0; t < KT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[n][t][i] = __builtin_amdgcn_exp2f(fmaf(w[n][t][i], cs, off));
+            // The sum: in 32 bits, lane by lane; of weights in three terms, which are exact, by products with ones below.
+            if constexpr (P != 3) {
+                float add = 0.0f;
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    const float four = (w[n][t][0] + w[n][t][1]) + (w[n][t][2] + w[n][t][3]);
+                    add = t ? add + four : four;
+                }
+                sum[n][0] += add;
+            }
             if constexpr (P > 0) {
-                // BF16: weights are rounded to bfloat16 for the product (2^-8 of each at most, of either sign); the sum is
-                // taken of the same rounded weights, by a product with ones.
+                // BF16: weights are rounded to bfloat16 for the product (2^-8 of each at most, of either sign); their sum is
+                // of the weights before that.
 #pragma unroll
                 for (int u = 0; u < KT / 2; ++u) {
                     const f32x4 lo = w[n][2 * u], hi = w[n][2 * u + 1];
@@ -967,15 +987,17 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         }
         // ---- O^T
         if constexpr (P > 0) {
-            const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
             for (int u = 0; u < KT / 2; ++u) {
+                if constexpr (P == 3) {
+                    const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
-                for (int n = 0; n < NS; ++n)
+                    for (int n = 0; n < NS; ++n)
 #pragma unroll
-                    for (int p = P - 1; p >= 0; --p)
-                        sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones),
-                                                                         __builtin_bit_cast(bf16x8, pw[n][u][p]), sum[n], 0, 0, 0);
+                        for (int p = P - 1; p >= 0; --p)
+                            sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones),
+                                                                             __builtin_bit_cast(bf16x8, pw[n][u][p]), sum[n], 0, 0, 0);
+                }
 #pragma unroll
                 for (int t = 0; t < C; ++t) {
                     u32x4 x[P ? P : 1];
@@ -1009,7 +1031,6 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int n = 0; n < NS; ++n) {
-                        sum[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, w[n][t][i], sum[n], 0, 0, 0);
 #pragma unroll
                         for (int x = 0; x < C; ++x)
                             acc[n][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vf[t][i][x]), w[n][t][i],
@@ -1161,7 +1182,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             float y[4 * C];
 #pragma unroll
             for (int e = 0; e < 4 * C; ++e) y[e] = acc[n][e % C][e / C];
-            finish(n, y, top[n] * a.scale, sum[n][0]);
+            finish(n, y, top[n] * a.scale, P == 3 ? sum[n][0] : sum_over_groups(sum[n][0]));
         }
     } else {
         __syncthreads();  // the steps' LDS is through
@@ -1171,7 +1192,8 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             for (int t = 0; t < C; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[wave][(n * 4 + i) * C + t][lane] = acc[n][t][i];
-            if (g == 0) part_ml[wave][n][c] = make_float2(top[n] * a.scale, sum[n][0]);
+            const float l = P == 3 ? sum[n][0] : sum_over_groups(sum[n][0]);
+            if (g == 0) part_ml[wave][n][c] = make_float2(top[n] * a.scale, l);
         }
         __syncthreads();
         if (wave >= SETS) return;

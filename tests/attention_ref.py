@@ -114,8 +114,9 @@ def attend(q, k, v, ql, kl, block, selected, scale, causal, bf16):
 
     With u = 2^-24: a score is off by at most (d + 4) u scale sum|q k| (d products and sums, the scale), and an
     exponential by that, its argument's rounding (|score| u, twice) and 4 u of its own: `w`, relative to each weight.
-    Numerator and denominator are both off by at most w and one u for each of their sums, the weights rounded to bfloat16
-    by 2^-8 in the numerator and perhaps in the denominator.  The output's own rounding is the caller's."""
+    Numerator and denominator are both off by at most w and one u for each of their sums, the numerator by 2^-8 more where
+    its weights are rounded to bfloat16 (and as much again where the denominator's were); lse is in 32 bits throughout.
+    The output's own rounding is the caller's."""
     n, heads, d = q.shape
     g = heads // k.shape[1]
     o, lse = np.zeros((n, heads, d)), np.full((n, heads), -np.inf)
@@ -147,7 +148,7 @@ def attend(q, k, v, ql, kl, block, selected, scale, causal, bf16):
                                + 2 * np.abs(s[fine]).max(initial=0))
                     most = 2 * w + 2 * U32 * (keys.size + 8) + (2 * UBF if bf16 else 0.0)
                     off[q0 + i, h] = most * (p @ np.abs(vv)) / total
-                    lse_off[q0 + i, h] = w + U32 * (keys.size + 8 + abs(lse[q0 + i, h])) + (UBF if bf16 else 0.0)
+                    lse_off[q0 + i, h] = w + U32 * (keys.size + 8 + abs(lse[q0 + i, h]))
         q0, k0 = q0 + lq, k0 + lk
     return o, lse, off, lse_off
 
