@@ -47,7 +47,8 @@ struct TurnArgs {
     int32_t d, pairs, halves, inverse, norm, gain_stride, rows, lanes_log2;
     float eps;
 };
-constexpr int kMaxRows = 4;  // of a workgroup
+constexpr int kMaxRows = 32;    // of a workgroup
+constexpr int kMaxTurns = 512;  // pairs of those rows
 
 // cos and sin of a 0.64 fixed-point part of a turn.  The quarter turn is split
 // off in integers, so that the float holds at most an eighth of a turn.
@@ -97,15 +98,21 @@ __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
 // then its waves take the rows' heads.  The work is the memory's: every head is read
 // and written once (28,265 rows x 16 heads x 64 BF16, 116 MB: 25 us at a copy's rate).
 //
-// VEC: a lane owns 16 channels, two pieces of 8 (bf16: 16 bytes): neighbours where
+// WHOLE: a lane owns 16 channels, two pieces of 8 (bf16: 16 bytes): neighbours where
 // neighbours are paired, else the piece of the first channels and that of the second; lane groups of
-// a power of two take a head, so a wave takes several side by side.  For head_dim a
-// multiple of 16, aligned rows, and pairs of halves in whole pieces.  Else one wave takes a head,
-// a pair (or a channel that does not turn) at a time in each lane, at any width and alignment.
-// In both a lane reads what it writes and nothing else, so y may be x.
-template <class TI, class TO, bool VEC>
+// a power of two take a head, so a wave takes several side by side.  For head_dim a multiple of 16 and
+// aligned rows.  MEET: the same for halves that are not whole pieces: a lane keeps neighbouring
+// channels and reads their partners in LDS (a form of its own, as its LDS costs the others a
+// quarter of their rate).  Else, SINGLE, one wave takes a head, a pair (or a channel that does
+// not turn) at a time in each lane, at any width and alignment (39,729 rows of 9 heads of 32
+// in halves of 6 pairs: 190 us that way).  In all of them a wave reads the heads that it
+// writes before it writes any, so y may be x.
+enum Form { SINGLE, WHOLE, MEET };
+template <class TI, class TO, int FORM>
 __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
-    __shared__ float2 turns[kMaxRows][kMaxPairs];
+    __shared__ float2 turns[kMaxTurns];
+    constexpr int STAGE = 17;  // floats of a lane, one more than its channels: neighbours in other banks
+    __shared__ float stage[FORM == MEET ? 4 : 1][FORM == MEET ? 64 * STAGE : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.rows;
     const int rows = static_cast<int>(min(static_cast<int64_t>(a.rows), a.n - row0));
@@ -114,11 +121,11 @@ __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
         const int64_t pos = a.positions[(row0 + r) * a.position_stride + t.axis[j]];
         float c, s;
         turn_cos_sin(static_cast<uint64_t>(pos) * t.turns[j], &c, &s);
-        turns[r][j] = make_float2(c, a.inverse ? -s : s);
+        turns[e] = make_float2(c, a.inverse ? -s : s);
     }
     __syncthreads();
     const int heads = a.part[0].heads + a.part[1].heads;
-    const int lanes = VEC ? 1 << a.lanes_log2 : 64, side = 64 / lanes;  // lanes of a head, heads of a wave
+    const int lanes = FORM != SINGLE ? 1 << a.lanes_log2 : 64, side = 64 / lanes;  // lanes of a head, heads of a wave
     const int sets = (heads + side - 1) / side;
     for (int item = wave; item < rows * sets; item += 4) {
         const int r = item / sets;
@@ -130,12 +137,13 @@ __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
         const TI *x = static_cast<const TI *>(p.x) + (row0 + r) * p.x_stride + static_cast<int64_t>(head) * a.d;
         TO *y = static_cast<TO *>(p.y) + (row0 + r) * p.y_stride + static_cast<int64_t>(head) * a.d;
         const float *gain = p.gain ? p.gain + static_cast<int64_t>(head) * a.gain_stride : nullptr;
-        if constexpr (VEC) {
+        if constexpr (FORM != SINGLE) {
             const int l = lane & (lanes - 1), turning = a.pairs / 8;
             const bool active = here && l < a.d / 16;
             // this lane's two pieces of 8 channels
-            const int c0 = a.halves ? (l < turning ? 8 * l : 16 * l) : 16 * l;
-            const int c1 = a.halves && l < turning ? c0 + a.pairs : c0 + 8;
+            const bool halves = a.halves && FORM == WHOLE;
+            const int c0 = halves && l < turning ? 8 * l : 16 * l;
+            const int c1 = halves && l < turning ? c0 + a.pairs : c0 + 8;
             float u[8], v[8], gu[8], gv[8];
             if (active) {
                 load8(x + c0, u);
@@ -153,7 +161,7 @@ __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
                 for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
                 scale = rsqrtf(sum / static_cast<float>(a.d) + a.eps);
             }
-            if (!active) continue;
+            if (FORM == WHOLE && !active) continue;
             if (a.norm) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -162,8 +170,30 @@ __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
                 }
             }
             // pairs 8l..8l+7, in the table's order
-            const float2 *cs = &turns[r][8 * l];
-            if (a.halves) {
+            const float2 *cs = &turns[r * a.pairs + 8 * l];
+            if constexpr (FORM == MEET) {
+                float *own = &stage[wave][lane * STAGE];
+                if (active) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) own[e] = u[e], own[8 + e] = v[e];
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the head's lanes are this wave's
+                if (active) {
+                    const float *first = &stage[wave][(lane - l) * STAGE];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int c = 16 * l + e;
+                        if (c >= 2 * a.pairs) continue;
+                        const int j = c < a.pairs ? c : c - a.pairs, other = c < a.pairs ? c + a.pairs : j;
+                        const float2 q = turns[r * a.pairs + j];
+                        const float x1 = first[(other >> 4) * STAGE + (other & 15)];
+                        float &x0 = e < 8 ? u[e & 7] : v[e & 7];
+                        x0 = c < a.pairs ? x0 * q.x - x1 * q.y : x1 * q.y + x0 * q.x;
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // read before the next heads take the place
+                if (!active) continue;
+            } else if (halves) {
                 if (l < turning) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -224,7 +254,7 @@ __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
             for (int q = 0; q < 2; ++q) {
                 const int j = lane + 64 * q, c = j * step;
                 if (j >= a.pairs) continue;
-                const float2 cs = turns[r][j];
+                const float2 cs = turns[r * a.pairs + j];
                 store_from_f32<TO>(y + c, (first[q] * cs.x - second[q] * cs.y) * scale);
                 store_from_f32<TO>(y + c + apart, (first[q] * cs.y + second[q] * cs.x) * scale);
             }
@@ -238,10 +268,10 @@ __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
 }
 
 using TurnFn = void (*)(TurnArgs, TurnTable);
-template <bool VEC>
+template <int FORM>
 TurnFn pick_turn(int32_t in, int32_t out) {
-    if (in == S3DX_BF16) return out == S3DX_BF16 ? turn_kernel<uint16_t, uint16_t, VEC> : turn_kernel<uint16_t, float, VEC>;
-    return out == S3DX_BF16 ? turn_kernel<float, uint16_t, VEC> : turn_kernel<float, float, VEC>;
+    if (in == S3DX_BF16) return out == S3DX_BF16 ? turn_kernel<uint16_t, uint16_t, FORM> : turn_kernel<uint16_t, float, FORM>;
+    return out == S3DX_BF16 ? turn_kernel<float, uint16_t, FORM> : turn_kernel<float, float, FORM>;
 }
 
 bool whole_pieces(const HeadRows &p, int32_t in, int32_t out) {
@@ -269,13 +299,20 @@ void launch_turn(TurnArgs a, const s3dx_rotary *rotary, int32_t in, int32_t out,
         std::memcpy(t.turns, rotary->turns, sizeof t.turns);
         std::memcpy(t.axis, rotary->axis, sizeof t.axis);
     }
-    const bool vec = a.d % 16 == 0 && (!a.halves || a.pairs % 8 == 0) && whole_pieces(a.part[0], in, out) &&
-                     whole_pieces(a.part[1], in, out);
+    const bool vec = a.d % 16 == 0 && whole_pieces(a.part[0], in, out) && whole_pieces(a.part[1], in, out);
     while ((16 << a.lanes_log2) < a.d) ++a.lanes_log2;
-    // Four rows to a workgroup, unless that leaves compute units without one.
-    a.rows = a.n >= 4 * 256 ? kMaxRows : 1;
-    (vec ? pick_turn<true>(in, out) : pick_turn<false>(in, out))<<<
-        dim3(static_cast<unsigned>((a.n + a.rows - 1) / a.rows)), dim3(256), 0, stream>>>(a, t);
+    // Four rows to a workgroup, unless that leaves compute units without one; more of narrow rows, up to
+    // 4,608 channels, as a workgroup's launch and first loads take longer than the rest of four of them
+    // (39,729 rows of 288 channels: 33 us with 4 rows, 23 us with 16; 2,048 channels: no difference).
+    const int64_t channels = static_cast<int64_t>(a.part[0].heads + a.part[1].heads) * a.d;
+    a.rows = a.n >= 4 * 256 ? 4 : 1;
+    while (a.rows > 1 && a.rows < kMaxRows && 2 * a.rows * channels <= 4608 && 2 * a.rows * a.pairs <= kMaxTurns &&
+           a.n >= 2 * a.rows * 1024)
+        a.rows *= 2;
+    const TurnFn fn = !vec                            ? pick_turn<SINGLE>(in, out)
+                      : a.halves && a.pairs % 8 != 0 ? pick_turn<MEET>(in, out)
+                                                     : pick_turn<WHOLE>(in, out);
+    fn<<<dim3(static_cast<unsigned>((a.n + a.rows - 1) / a.rows)), dim3(256), 0, stream>>>(a, t);
     launch_check("rotary");
 }
 

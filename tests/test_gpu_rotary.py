@@ -7,7 +7,8 @@ import attention_ref as R
 
 pytestmark = pytest.mark.gpu
 
-PER_AXIS = {"xyz": [10, 10, 10], "one": [16], "two": [3, 8], "four": [1, 2, 3, 4]}
+PER_AXIS = {"xyz": [10, 10, 10], "one": [16], "two": [3, 8], "four": [1, 2, 3, 4], "few": [1], "most": [31],
+            "odd": [3, 4, 6]}
 
 
 def inputs(rng, n, heads, stride, d):
@@ -36,6 +37,16 @@ def compare(got, want, size, rel, out_step, what):
     (40, 2, 32, "one", True, 0, 4096),       # every channel turns
     (31, 3, 23, "four", False, 5, 64),       # odd width and stride
     (9, 2, 256, "two", True, 3, 64),
+    # halves that are not whole pieces of 8 channels, many and few rows
+    (40, 5, 64, "odd", False, 0, 64),
+    (1500, 3, 64, "most", False, 0, 4096),
+    (7, 4, 256, "odd", False, 64, 64),
+    (3, 9, 32, "few", False, 0, 64),
+    (11, 3, 96, "most", False, 32, 64),
+    # many narrow rows
+    (16500, 2, 64, "most", True, 5, 4096),
+    (33001, 1, 32, "odd", False, 0, 64),
+    (8300, 3, 24, "few", False, 2, 64),
 ])
 def test_rotary(s3dx, x_dtype, y_dtype, n, heads, d, axes, adjacent, pad, span):
     rng = np.random.default_rng(n + d)
@@ -108,6 +119,8 @@ def norm_rel(d):
     (20, 4, 0, 32, "one", False, None, 1e-6),        # queries alone
     (13, 5, 3, 20, "one10", True, "head", 1e-6),     # odd width
     (65, 7, 7, 256, "two", True, "head", 1e-6),
+    (1030, 6, 2, 64, "odd", False, "head", 1e-6),
+    (9, 5, 5, 128, "most", False, "all", 1e-6),
 ])
 def test_qk_norm_rotary(s3dx, dtype, out_dtype, n, h, kv, d, axes, adjacent, gain, eps):
     rng = np.random.default_rng(n + h + d)
