@@ -43,7 +43,7 @@ struct HeadRows {
 struct TurnArgs {
     HeadRows part[2];  // queries, keys
     const int32_t *positions;
-    int64_t position_stride, n;
+    int64_t position_stride, first, n;  // rows [first, n)
     int32_t d, pairs, halves, inverse, norm, gain_stride, rows, lanes_log2;
     float eps;
 };
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
     constexpr int STAGE = 17;  // floats of a lane, one more than its channels: neighbours in other banks
     __shared__ float stage[FORM == MEET ? 4 : 1][FORM == MEET ? 64 * STAGE : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.rows;
+    const int64_t row0 = a.first + static_cast<int64_t>(blockIdx.x) * a.rows;
     const int rows = static_cast<int>(min(static_cast<int64_t>(a.rows), a.n - row0));
     for (int e = threadIdx.x; e < rows * a.pairs; e += 256) {
         const int r = e / a.pairs, j = e - r * a.pairs;
@@ -312,7 +312,12 @@ void launch_turn(TurnArgs a, const s3dx_rotary *rotary, int32_t in, int32_t out,
     const TurnFn fn = !vec                            ? pick_turn<SINGLE>(in, out)
                       : a.halves && a.pairs % 8 != 0 ? pick_turn<MEET>(in, out)
                                                      : pick_turn<WHOLE>(in, out);
-    fn<<<dim3(static_cast<unsigned>((a.n + a.rows - 1) / a.rows)), dim3(256), 0, stream>>>(a, t);
+    // A launch's threads stay below 2^32: 2^20 workgroups at a time.
+    const int64_t n = a.n, most = a.rows * (INT64_C(1) << 20);
+    for (; a.first < n; a.first += most) {
+        a.n = std::min(n, a.first + most);
+        fn<<<dim3(static_cast<unsigned>((a.n - a.first + a.rows - 1) / a.rows)), dim3(256), 0, stream>>>(a, t);
+    }
     launch_check("rotary");
 }
 

@@ -225,3 +225,17 @@ def test_rotary_captured_and_replayed(s3dx):
         s3dx.qk_norm_rotary(x, None, s3dx.F32, n, h, 0, d, 1e-6, z, rotary=rot, positions=pos)
         assert np.array_equal(y.download(), z.download())
     g.close()
+
+
+def test_rotary_of_more_rows_than_a_launch_takes(s3dx):
+    rng = np.random.default_rng(12)
+    n = 2 ** 25 + 5
+    x = np.tile(rng.standard_normal((64, 2)).astype(np.float32), (n // 64 + 1, 1))[:n]
+    pos = np.arange(n, dtype=np.int32)
+    y = R.filled(s3dx, (n + 1, 2), np.float32, 0x5A)
+    s3dx.Rotary(2, [0], [0.3]).apply(R.dev(s3dx, x), s3dx.F32, n, 1, R.dev(s3dx, pos[:, None]), y)
+    got = y.download()
+    assert np.all(got[n].view(np.uint8) == 0x5A)
+    at = np.r_[0:2000, rng.integers(0, n, 20000), 2 ** 25 - 2000: n]
+    want, size = R.turn(x[at, None].astype(np.float64), pos[at, None], [0], [0.3], True)
+    compare(got[at, None].astype(np.float64), want, size, TURN, R.half_step(s3dx, s3dx.F32), "rows")
