@@ -485,7 +485,8 @@ S3DX_API s3dx_status s3dx_convert(const void *x, int32_t x_dtype, int64_t count,
  * sequence s holds rows [starts[s], starts[s+1]); sequences may be empty, and
  * rows behind the last one are neither read nor written.  Query i of a
  * sequence of lq queries and lk keys stands at key place i + lk - lq (the
- * last query at the last key).  Starts outside [0, total] are cut to it.
+ * last query at the last key).  Starts outside [0, total] are cut to it.  The
+ * block calls take up to 2^29 rows.
  *
  * Nothing here allocates device memory or synchronizes: the calls can be
  * captured into a graph, and the buffers belong to the current device.  Zero
@@ -559,7 +560,7 @@ S3DX_API s3dx_status s3dx_block_index(const void *k, int32_t dtype, int64_t tota
  * selected int32 [total_q][kv_heads][top], ascending, -1 behind the last.  A
  * block's score is the integer product of its codes with the codes of the
  * query (the sum of the heads that share the key head, in 64 bits, coded in the
- * same way), times its scale: exact, so the choice depends on no order of
+ * same way), times its scale: exact below 2^128, so the choice depends on no order of
  * sums; equal scores go to the lower block.  With S3DX_BLOCK_CAUSAL blocks
  * that begin behind the query's place are not chosen.  max_k: at least the keys of
  * the longest sequence, at most 32768 * block; blocks behind it are not looked at. */
@@ -577,10 +578,13 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
  * scores of -inf, gets zeros and lse -inf; keys and values that a row does not
  * see do not reach it, whatever they hold.  BF16 weights are rounded to bfloat16
  * before they meet the values (their sum and lse are of the weights before that),
- * FP32 ones are not.  Rows whose result is not
+ * FP32 ones are not (heads up to 64 wide: products of 24 significant bits, of values
+ * below 2^-102 down to 2^-126).  o overlaps no input.  max_k, the keys of the longest sequence,
+ * decides how the work is cut and not what is computed.  Rows whose result is not
  * finite are computed a second time key by key, more slowly.
  * The workspace holds partial results where there are too few rows to fill the GPU
- * (s3dx_block_attention_workspace_size, 0 bytes where none are needed); the
+ * (s3dx_block_attention_workspace_size of the same arguments, 0 bytes where none are
+ * needed); calls that may run at the same time need one each.  The
  * pieces are joined in a fixed order: results are deterministic. */
 S3DX_API s3dx_status s3dx_block_attention_workspace_size(int64_t total_q, int32_t heads, int32_t kv_heads,
                                                          int32_t head_dim, int64_t sequences, int32_t block,

@@ -1279,7 +1279,12 @@ constexpr int32_t kMaxTop = 4096;
 constexpr int64_t kMaxBlocks = 32768;
 
 void check_total(int64_t total) {
-    require(total >= 0 && total <= std::numeric_limits<int32_t>::max(), "a row count is out of range");
+    // places of keys plus a tile's steps stay below 2^31, and 2^30 ends a list of blocks
+    require(total >= 0 && total <= (INT64_C(1) << 29), "a row count is out of range (0 to 2^29)");
+}
+// Threads of a launch along x stay below 2^32.
+void check_grid(int64_t groups, int threads) {
+    require(groups <= 0xffffffffll / threads, "too many rows and sequences");
 }
 void check_shape(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t sequences, int32_t block) {
     require_dtype(dtype);
@@ -1391,6 +1396,7 @@ S3DX_API s3dx_status s3dx_block_index(const void *k, int32_t dtype, int64_t tota
                              kv_heads, head_dim, block, log2_of(block), codes, scale};
         const int per = 256 / head_dim;
         require((kv_heads + per - 1) / per <= 65535, "too many heads");
+        check_grid(a.rows, 256);
         (dtype == S3DX_BF16 ? index_kernel<uint16_t> : index_kernel<float>)<<<
             dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>((kv_heads + per - 1) / per)), dim3(256), 0,
             as_stream(stream)>>>(a);
@@ -1445,7 +1451,7 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
                                           hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)),
                       "hipFuncSetAttribute");
         const int64_t grid = (total_q / qt + sequences) * kv_heads;
-        require(grid <= std::numeric_limits<int32_t>::max(), "too many rows and sequences");
+        check_grid(grid, select_threads(qt));
         kernel<<<dim3(static_cast<unsigned>(grid)), dim3(select_threads(qt)), lds, as_stream(stream)>>>(a);
         launch_check("block select");
     });
@@ -1512,7 +1518,7 @@ S3DX_API s3dx_status s3dx_block_attention(const void *q, const void *k, const vo
             a.part_ml = w.take<float2>(static_cast<uint64_t>(cut.splits) * total_q * heads);
         }
         const int64_t grid = cut.tile_groups * kv_heads * cut.splits;
-        require(grid <= std::numeric_limits<int32_t>::max(), "too many rows and sequences");
+        check_grid(grid, 256);
         const bool bf = dtype == S3DX_BF16;
         (bf ? pick_attend<uint16_t>(head_dim, selected, block, cut) : pick_attend<float>(head_dim, selected, block, cut))<<<
             dim3(static_cast<unsigned>(grid)), dim3(256), 0, as_stream(stream)>>>(a);

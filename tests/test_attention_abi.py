@@ -84,13 +84,14 @@ ATTEND = dict(q=P, k=P, v=P, dtype=1, total_q=10, total_k=100, heads=4, kv_heads
               flags=0, o=P, o_stride=256, lse=None, workspace=P, workspace_bytes=2 ** 40, stream=None)
 SHAPES = [(dict(dtype=2), "dtype"), (dict(head_dim=80), "head_dim"), (dict(head_dim=256), "head_dim"),
           (dict(block=16), "block"), (dict(block=0), "block"), (dict(sequences=-1), "sequences"), (dict(kv_heads=0), "heads"),
-          (dict(total_k=-1), "row count"), (dict(total_k=2 ** 31), "row count"), (dict(k_starts=None), "starts"),
+          (dict(total_k=-1), "row count"), (dict(total_k=2 ** 31), "row count"),
+          (dict(total_k=2 ** 29 + 1), "row count"), (dict(k_starts=None), "starts"),
           (dict(k_starts=P + 1), "starts")]
 
 
 @pytest.mark.parametrize("change,word", SHAPES + [
     (dict(k=None), "NULL"), (dict(k=P + 8), "aligned"), (dict(k_stride=127), "stride"), (dict(k_stride=132), "16-byte pieces"),
-    (dict(k_stride=2 ** 22), "2^22"), (dict(codes=P + 8), "codes"), (dict(scale=None), "scale")])
+    (dict(total_k=2 ** 29, block=32), "too many"), (dict(k_stride=2 ** 22), "2^22"), (dict(codes=P + 8), "codes"), (dict(scale=None), "scale")])
 def test_block_index_refuses(s3dx, change, word):
     refused(s3dx, "s3dx_block_index", {**INDEX, **change}.values(), word)
 
@@ -100,6 +101,7 @@ def test_block_index_refuses(s3dx, change, word):
     (dict(max_k=-1), "max_k"), (dict(max_k=32768 * 64 + 1), "max_k"), (dict(q=None), "NULL"), (dict(q_stride=255), "stride"),
     (dict(q_starts=None), "starts"), (dict(selected=None), "selected"), (dict(selected=P + 2), "selected"),
     (dict(codes=None), "codes"), (dict(total_q=-1), "row count"),
+    (dict(total_q=2 ** 29), "too many"), (dict(total_q=2 ** 29, heads=8, kv_heads=8, q_stride=512), "out of range"),
     (dict(total_q=2 ** 31 - 1, heads=8, kv_heads=8, q_stride=512), "out of range")])
 def test_block_select_refuses(s3dx, change, word):
     refused(s3dx, "s3dx_block_select", {**SELECT, **change}.values(), word)
@@ -111,7 +113,7 @@ def test_block_select_refuses(s3dx, change, word):
     (dict(softmax_scale=float("inf")), "softmax_scale"), (dict(softmax_scale=-1.0), "softmax_scale"), (dict(v=None), "NULL"),
     (dict(o=None), "NULL"), (dict(o=P + 2), "aligned"), (dict(o_stride=128), "stride"), (dict(v_stride=64), "stride"),
     (dict(lse=P + 2), "lse"), (dict(selected=P + 1), "selected"), (dict(max_k=-1), "row count"), (dict(q_starts=P + 2), "starts"),
-    (dict(total_q=2 ** 31 - 1), "out of range")])
+    (dict(total_q=2 ** 29, heads=2, sequences=2 ** 24), "too many"), (dict(total_q=2 ** 31 - 1), "out of range")])
 def test_block_attention_refuses(s3dx, change, word):
     refused(s3dx, "s3dx_block_attention", {**ATTEND, **change}.values(), word)
 
