@@ -504,7 +504,10 @@ __device__ void attend_row(const AttendArgs &a, int64_t row, int head, Span qs, 
 #pragma unroll
     for (int w = 0; w < 2; ++w) qv[w] = lane + 64 * w < D ? load_as_f32<T>(q + lane + 64 * w) * a.scale : 0.0f;
     float m = neg_inf(), l = 0.0f, o[2] = {0.0f, 0.0f};
-    for (int t = 0; t < (list ? a.top : blocks); ++t) {
+    // A weight that is a NaN makes the whole row one: the rest need not be read (5,086 rows x 16 heads x 64
+    // bf16 with a NaN among the keys: 0.9 ms; 30 ms key by key to the end, as for one among the values).
+    bool lost = false;
+    for (int t = 0; t < (list ? a.top : blocks) && !lost; ++t) {
         const int b = list ? list[t] : t;
         if (b < 0 || b >= blocks) continue;
         if (list) {  // a block counts once
@@ -512,7 +515,7 @@ __device__ void attend_row(const AttendArgs &a, int64_t row, int head, Span qs, 
             for (int e = lane; e < t; e += 64) before = before || list[e] == b;
             if (__any(before)) continue;
         }
-        for (int k0 = b << a.block_log2; k0 < min((b + 1) << a.block_log2, seen); k0 += 64) {
+        for (int k0 = b << a.block_log2; k0 < min((b + 1) << a.block_log2, seen) && !lost; k0 += 64) {
             const int count = min(64, min((b + 1) << a.block_log2, seen) - k0);
             const T *kr = k + static_cast<int64_t>(k0 + min(lane, count - 1)) * a.k_stride;
             const T *vr = v + static_cast<int64_t>(k0) * a.v_stride;
@@ -528,6 +531,7 @@ __device__ void attend_row(const AttendArgs &a, int64_t row, int head, Span qs, 
             o[0] *= alpha;
             o[1] *= alpha;
             m = mn;
+            lost = __any(lane < count && p != p);
             for (int j = 0; j < count; ++j) {
                 const float pj = __shfl(p, j, 64);
 #pragma unroll
