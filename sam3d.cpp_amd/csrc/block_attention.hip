@@ -620,21 +620,27 @@ __device__ __forceinline__ f32x4 product(const u32x4 (&x)[P], const u32x4 (&y)[P
 
 // Attention of a tile of 16 NS rows (query rows times the heads that share a key head)
 // on matrix units.  A wave computes S^T = K Q^T and O^T = V^T P^T, so that what one
-// product leaves in a lane is what the next one wants there and nothing goes through
-// LDS.  A 16x16 product leaves lane (c, g) = (lane & 15, lane >> 4) with rows
+// product leaves in a lane is what the next one wants there: the weights stay in
+// registers.  A 16x16 product leaves lane (c, g) = (lane & 15, lane >> 4) with rows
 // 4g..4g+3 of column c: of S^T four keys of query c, and two such (keys 4g.. of one
 // 16-key group and of the next) are the eight k-values that lane (c, g) holds of the
 // operand P^T.  V^T's operand wants the same eight keys of one channel: the lane
 // reads D/16 channels of eight rows and pairs them up by byte permutes; channel
 // c*(D/16) + t goes with product t, so O^T leaves each lane D/4 channels that lie
-// side by side.  Statistics, scales and masks are per query, hence per lane.
+// side by side.  K's rows are read whole, 16 bytes a lane one after the other, and turned in LDS, as
+// K's operand read from memory takes 16 bytes from each of 16 rows (5,086 rows x 16 heads x 64 bf16,
+// all keys: 157 us so, 138 us turned); V through LDS as well took 144 us.  Statistics, scales and
+// masks are per query, hence per lane.
+//
+// What bounds it, at 137 us (774 TFLOP/s) for that call: issue.  A step of 64 rows and 32 keys is 32
+// products and about 400 vector instructions (exponentials, maxima, rounding), which share the SIMD's slots.
 //
 // The keys of a tile are those of any of its rows' blocks: a table in LDS gets, for each
 // block, a bit for each row that chose it; rows that did not take weights 0.
 // Neighbouring rows choose alike, which is what makes tiles of them pay.
 //
 // FP32 heads up to 64 wide: the same products on three bfloat16 terms of every value, six for one, each 16 times as
-// fast as FP32's own (5,086 rows x 16 heads x 64, all keys: 880 us with those).  Wider
+// fast as FP32's own (5,086 rows x 16 heads x 64, all keys: 615 us, 880 with FP32's).  Wider
 // heads' terms do not fit a lane's registers: they take FP32's products.
 //
 // WAVES 4: the workgroup's waves take a tile together, every fourth step (of lists,
@@ -643,7 +649,8 @@ __device__ __forceinline__ f32x4 product(const u32x4 (&x)[P], const u32x4 (&y)[P
 // HALVES 2: a tile of 32 NS rows, half of them for each pair of the waves, a pair's waves every second step.
 // For heads whose 64 rows one wave's registers do not hold: the two waves of a step
 // fetch half of its K and V rows each, into LDS that they share (two buffers, one barrier a step);
-// V^T is read from there by the transposing reads of 16-bit data.
+// V^T is read from there by the transposing reads of 16-bit data (12,001 ragged rows x 16 / 4 heads
+// x 128, top 32: 596 us with a wave's 32 rows by itself, 546 us so).
 template <class T, int D, int KC, int NS, bool LISTED, int WAVES, int HALVES>
 __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr bool BF = sizeof(T) == 2;
@@ -1129,8 +1136,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 
     // ---- out
     const bool parts = a.splits > 1;
-    // Channels [ch, ch + N) of a row.  A weight of 0 times a value that is not finite is a NaN: with `bad`, a set's rows
-    // that got one are left out, and computed again below from the keys that they see alone.  The test costs nothing in the loop.
+    // Channels [ch, ch + N) of a row.
     const auto put = [&]<int N>(int t, int h, int ch, const float (&y)[N], float m, float l) __attribute__((always_inline)) {
         static_assert(N % 4 == 0);
         const int64_t token = qs.begin + tok0 + t;
@@ -1155,6 +1161,8 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         }
         if (a.lse && ch == 0) a.lse[token * a.heads + h] = l == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l) * kLn2;
     };
+    // A weight of 0 times a value that is not finite is a NaN: a set's rows that got one are left out, and computed
+    // again from the keys that they see alone.  The test costs nothing in the loop.
     const auto finish = [&](int n, const float (&y)[4 * C], float m, float l) __attribute__((always_inline)) {
         const int r = r0 + 16 * n + c;
         float odd = l * 0.0f;
