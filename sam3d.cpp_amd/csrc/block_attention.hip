@@ -629,11 +629,12 @@ __device__ __forceinline__ f32x4 product(const u32x4 (&x)[P], const u32x4 (&y)[P
 // c*(D/16) + t goes with product t, so O^T leaves each lane D/4 channels that lie
 // side by side.  K's rows are read whole, 16 bytes a lane one after the other, and turned in LDS, as
 // K's operand read from memory takes 16 bytes from each of 16 rows (5,086 rows x 16 heads x 64 bf16,
-// all keys: 157 us so, 138 us turned); V through LDS as well took 144 us.  Statistics, scales and
+// all keys: 157 us so, 138 us turned; 144 us with V through LDS as well).  Statistics, scales and
 // masks are per query, hence per lane.
 //
-// What bounds it, at 137 us (774 TFLOP/s) for that call: issue.  A step of 64 rows and 32 keys is 32
-// products and about 400 vector instructions (exponentials, maxima, rounding), which share the SIMD's slots.
+// What bounds it, at 134 us (791 TFLOP/s) for that call: a step of 64 rows and 32 keys is 32 products
+// of 16 cycles and about 150 vector instructions, among them 32 exponentials of 16, which take longer
+// than the products and cover them in part.
 //
 // The keys of a tile are those of any of its rows' blocks: a table in LDS gets, for each
 // block, a bit for each row that chose it; rows that did not take weights 0.
@@ -656,6 +657,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     constexpr bool BF = sizeof(T) == 2;
     constexpr int ROWS = 16 * NS * HALVES, SETS = NS * HALVES;
     constexpr bool SHARED = HALVES == 2;
+    constexpr bool FLAT = BF && !LISTED && WAVES == 4;
     constexpr int KT = KC / 16;              // 16-key groups of a step
     constexpr int P = BF ? 1 : D <= 64 ? 3 : 0; // bfloat16 terms of a value; 0: FP32's products
     constexpr int QV = P ? D / 32 : D / 16;  // products over a row's channels
@@ -892,25 +894,10 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
     // A step: the keys from `at` on for the rows of `mem`, of the operands in kf and (vf or LDS).
     uint32_t vf[SHARED ? 1 : KT][4][VW];  // rows 16t + 4g + i
     const auto step = [&](int at, uint64_t mem) __attribute__((always_inline)) {
-        // ---- sets of 16 rows: S^T, weights
         f32x4 w[NS][KT];
         u32x4 pw[NS][KT / 2 > 0 ? KT / 2 : 1][P ? P : 1];
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            // the set's rows, a bit each (all keys: all of them), and the same for the four lanes of each
-            const uint32_t rows = LISTED ? static_cast<uint32_t>(mem >> (32 * half + 16 * n)) & 0xffffu
-                                         : r0w + 16 * n < nrows ? 0xffffu : 0u;
-            if (rows == 0) {  // none sees the block: weights 0
-#pragma unroll
-                for (int t = 0; t < KT; ++t) w[n][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int u = 0; u < KT / 2; ++u)
-#pragma unroll
-                    for (int p = 0; p < P; ++p) pw[n][u][p] = u32x4{0, 0, 0, 0};
-                continue;
-            }
-            const uint32_t twice = rows | rows << 16;
-            const uint64_t lanes = static_cast<uint64_t>(twice) << 32 | twice;
+        // ---- of a set of 16 rows: S^T
+        const auto scores = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < KT; ++t) {
                 f32x4 d = {0, 0, 0, 0};
@@ -926,36 +913,38 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                 }
                 w[n][t] = d;
             }
-            if (at + KC > least) {
+        };
+        const auto mask = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-                for (int t = 0; t < KT; ++t)
+            for (int t = 0; t < KT; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (at + 16 * t + 4 * g + i >= lim[n]) w[n][t][i] = neg_inf();
-            }
+                for (int i = 0; i < 4; ++i)
+                    if (at + 16 * t + 4 * g + i >= lim[n]) w[n][t][i] = neg_inf();
+        };
+        const auto largest = [&](int n) __attribute__((always_inline)) {
             float mx = neg_inf();
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, w[n][t][i]);
-            // What weights are relative to moves only where a weight would pass 2^8: far less often than the
-            // maximum, and floating point loses nothing by it.
-            if ((__builtin_amdgcn_ballot_w64(mx > above[n]) & lanes) != 0) {
-                const bool in = !LISTED || __builtin_amdgcn_inverse_ballot_w64(lanes);
-                mx = max_over_groups(mx);
-                const float now = in ? fmaxf(top[n], mx) : top[n];
-                // nothing seen yet: any finite base leaves weights of 0
-                const float to = now == neg_inf() ? 0.0f : now * cs;
-                const float alpha = __builtin_amdgcn_exp2f(top[n] * cs - to);
-                sum[n] *= alpha;
+            return mx;
+        };
+        // What weights are relative to moves only where a weight would pass 2^8: far less often than the
+        // maximum, and floating point loses nothing by it.
+        const auto move = [&](int n, float mx, bool in) __attribute__((always_inline)) {
+            mx = max_over_groups(mx);
+            const float now = in ? fmaxf(top[n], mx) : top[n];
+            // nothing seen yet: any finite base leaves weights of 0
+            const float to = now == neg_inf() ? 0.0f : now * cs;
+            const float alpha = __builtin_amdgcn_exp2f(top[n] * cs - to);
+            sum[n] *= alpha;
 #pragma unroll
-                for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
-                top[n] = now;
-                base[n] = to;
-                above[n] = now + 8.0f / cs;
-            }
-            // rows that do not see the block: weights 2^-inf
-            const float off = !LISTED || __builtin_amdgcn_inverse_ballot_w64(lanes) ? -base[n] : neg_inf();
+            for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
+            top[n] = now;
+            base[n] = to;
+            above[n] = now + 8.0f / cs;
+        };
+        const auto weights = [&](int n, float off) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -991,6 +980,89 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
                     }
                 }
             }
+        };
+        // V^T's operand of product t, 32 keys from 32u on
+        const auto values = [&](int u, int t, u32x4 (&x)[P ? P : 1]) __attribute__((always_inline)) {
+            if constexpr (SHARED) {
+                const char *from = kt + buffer + vget[t] + u * (32 * ROW * 16);
+                const u32x2 lo = transposed(from), hi = transposed(from + 16 * ROW * 16);
+                x[0] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+            } else if constexpr (P > 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // a pair of keys: rows 2i, 2i + 1 of the lane's eight
+                    const uint32_t(&r0v)[VW] = vf[2 * u + (i >> 1)][2 * (i & 1)];
+                    const uint32_t(&r1v)[VW] = vf[2 * u + (i >> 1)][2 * (i & 1) + 1];
+                    if constexpr (BF) {
+                        x[0][i] = __builtin_amdgcn_perm(r1v[t / 2], r0v[t / 2], t & 1 ? 0x07060302u : 0x05040100u);
+                    } else {
+                        uint32_t terms[3];
+                        three_terms(__builtin_bit_cast(float, r0v[t]), __builtin_bit_cast(float, r1v[t]), terms);
+#pragma unroll
+                        for (int p = 0; p < P; ++p) x[p][i] = terms[p];
+                    }
+                }
+            }
+        };
+        if constexpr (FLAT) {
+            // All keys: the sets in one run without branches, so that one set's products go on under the next one's weights
+            // (5,086 rows x 16 heads x 64 bf16: 142 us set by set, 137 us so, on one card in turns).
+            float mx[NS];
+            bool over = false;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) scores(n);
+            if (at + KC > least) {
+#pragma unroll
+                for (int n = 0; n < NS; ++n) mask(n);
+            }
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                mx[n] = largest(n);
+                over = over || mx[n] > above[n];
+            }
+            if (__builtin_amdgcn_ballot_w64(over) != 0) {
+#pragma unroll
+                for (int n = 0; n < NS; ++n) move(n, mx[n], true);
+            }
+            u32x4 x[KT / 2][C][P ? P : 1];
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                weights(n, -base[n]);
+                if (n == 0) {
+#pragma unroll
+                    for (int u = 0; u < KT / 2; ++u)
+#pragma unroll
+                        for (int t = 0; t < C; ++t) values(u, t, x[u][t]);
+                }
+#pragma unroll
+                for (int u = 0; u < KT / 2; ++u)
+#pragma unroll
+                    for (int t = 0; t < C; ++t) acc[n][t] = product<P ? P : 1>(x[u][t], pw[n][u], acc[n][t]);
+            }
+            return;
+        }
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            // the set's rows, a bit each (all keys: all of them), and the same for the four lanes of each
+            const uint32_t rows = LISTED ? static_cast<uint32_t>(mem >> (32 * half + 16 * n)) & 0xffffu
+                                         : r0w + 16 * n < nrows ? 0xffffu : 0u;
+            if (rows == 0) {  // none sees the block: weights 0
+#pragma unroll
+                for (int t = 0; t < KT; ++t) w[n][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < KT / 2; ++u)
+#pragma unroll
+                    for (int p = 0; p < P; ++p) pw[n][u][p] = u32x4{0, 0, 0, 0};
+                continue;
+            }
+            const uint32_t twice = rows | rows << 16;
+            const uint64_t lanes = static_cast<uint64_t>(twice) << 32 | twice;
+            scores(n);
+            if (at + KC > least) mask(n);
+            const float mx = largest(n);
+            const auto in = [&]() __attribute__((always_inline)) { return !LISTED || __builtin_amdgcn_inverse_ballot_w64(lanes); };
+            if ((__builtin_amdgcn_ballot_w64(mx > above[n]) & lanes) != 0) move(n, mx, in());
+            // rows that do not see the block: weights 2^-inf
+            weights(n, in() ? -base[n] : neg_inf());
         }
         if constexpr (P == 0) {
             more = next();
@@ -1012,25 +1084,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int t = 0; t < C; ++t) {
                     u32x4 x[P ? P : 1];
-                    if constexpr (SHARED) {
-                        const char *from = kt + buffer + vget[t] + u * (32 * ROW * 16);
-                        const u32x2 lo = transposed(from), hi = transposed(from + 16 * ROW * 16);
-                        x[0] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {  // a pair of keys: rows 2i, 2i + 1 of the lane's eight
-                            const uint32_t(&r0v)[VW] = vf[2 * u + (i >> 1)][2 * (i & 1)];
-                            const uint32_t(&r1v)[VW] = vf[2 * u + (i >> 1)][2 * (i & 1) + 1];
-                            if constexpr (BF) {
-                                x[0][i] = __builtin_amdgcn_perm(r1v[t / 2], r0v[t / 2], t & 1 ? 0x07060302u : 0x05040100u);
-                            } else {
-                                uint32_t terms[3];
-                                three_terms(__builtin_bit_cast(float, r0v[t]), __builtin_bit_cast(float, r1v[t]), terms);
-#pragma unroll
-                                for (int p = 0; p < P; ++p) x[p][i] = terms[p];
-                            }
-                        }
-                    }
+                    values(u, t, x);
 #pragma unroll
                     for (int n = 0; n < NS; ++n) acc[n][t] = product<P ? P : 1>(x, pw[n][u], acc[n][t]);
                 }
