@@ -104,6 +104,9 @@ SELECT = [
     ([33], [500], 5, 1, 64, 32, 40, False, False),                  # more than there are
     ([260], [260], 2, 2, 64, 128, 1, False, True),
     ([17], [6000], 3, 3, 64, 32, 20, False, False),                 # 188 blocks
+    # rows and blocks in plenty: 625 blocks, and 282 and 1,000 in one batch
+    ([2101], [20000], 4, 4, 32, 32, 7, True, True),
+    ([4100, 13], [9000, 32000], 4, 2, 64, 32, 33, False, True),
 ]
 
 
