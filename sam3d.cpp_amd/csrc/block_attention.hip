@@ -488,6 +488,15 @@ __device__ __forceinline__ float sum_over_groups(float v) {
     return as_float(b[0]) + as_float(b[1]);
 }
 
+// Whether a row's sums (l: the weights', y: anything made of its values') have to be made again: 0 times what is not
+// finite is a NaN, also for a key that the row does not see.  Where every row sees every key the NaN or infinity is the
+// result's own, unless the weights are not finite themselves (in three terms an infinity is not one) or nothing is seen.
+template <class T>
+__device__ __forceinline__ bool again_of(const AttendArgs &a, float l, float y) {
+    const bool own = sizeof(T) == 2 && !a.selected && !a.causal && l != 0.0f;
+    return (own ? l : l + y) * 0.0f != 0.0f;
+}
+
 // One row by the whole wave, key by key: scores with a key per lane, the running maximum
 // and sum, values with a channel pair per lane.  Only keys that the row sees are
 // multiplied, so nothing else reaches it: for rows whose tile gave no finite result.
@@ -505,7 +514,7 @@ __device__ void attend_row(const AttendArgs &a, int64_t row, int head, Span qs, 
     for (int w = 0; w < 2; ++w) qv[w] = lane + 64 * w < D ? load_as_f32<T>(q + lane + 64 * w) * a.scale : 0.0f;
     float m = neg_inf(), l = 0.0f, o[2] = {0.0f, 0.0f};
     // A weight that is a NaN makes the whole row one: the rest need not be read (5,086 rows x 16 heads x 64
-    // bf16 with a NaN among the keys: 0.9 ms; 30 ms key by key to the end, as for one among the values).
+    // bf16 with a NaN among the keys: 0.9 ms; 30 ms key by key to the end).
     bool lost = false;
     for (int t = 0; t < (list ? a.top : blocks) && !lost; ++t) {
         const int b = list ? list[t] : t;
@@ -1215,14 +1224,13 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         }
         if (a.lse && ch == 0) a.lse[token * a.heads + h] = l == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l) * kLn2;
     };
-    // A weight of 0 times a value that is not finite is a NaN: a set's rows that got one are left out, and computed
-    // again from the keys that they see alone.  The test costs nothing in the loop.
+    // A set's rows whose sums are not finite are left out, and computed again from the keys that they see alone.  The test costs nothing in the loop.
     const auto finish = [&](int n, const float (&y)[4 * C], float m, float l) __attribute__((always_inline)) {
         const int r = r0 + 16 * n + c;
-        float odd = l * 0.0f;
+        float odd = 0.0f;
 #pragma unroll
         for (int e = 0; e < 4 * C; ++e) odd += y[e] * 0.0f;
-        uint64_t bad = parts ? 0 : __ballot(r < nrows && odd != 0.0f);  // pieces: the join looks
+        uint64_t bad = parts ? 0 : __ballot(r < nrows && again_of<T>(a, l, odd));  // pieces: the join looks
         bad = (bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffffu;
         if (r < nrows && !((bad >> c) & 1u)) {
             const int t0 = r / a.group - tok0, h = kvh * a.group + r % a.group;
@@ -1324,7 +1332,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) o[e] += wp[u] * x[u][e];
     }
-    if (__any((l + o[0] + o[1]) * 0.0f != 0.0f)) {  // not finite: see the tiles
+    if (__any(again_of<T>(a, l, o[0] * 0.0f + o[1] * 0.0f))) {
         attend_row<T, D>(a, row, head, sequence_span(a.q_starts, s, a.total_q), sequence_span(a.k_starts, s, a.total_k));
         return;
     }

@@ -314,6 +314,23 @@ def test_what_a_row_does_not_see_does_not_reach_it(s3dx, dtype, n, lk, top, late
     check(s3dx, dtype, got, lse, want)
 
 
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n,lk,d", [(40, 100, 64), (70, 700, 64), (65, 1300, 128), (90, 600, 96), (3, 4000, 64), (1, 300, 32)])
+def test_values_that_are_not_finite_stay_in_their_channels(s3dx, dtype, n, lk, d):
+    rng = np.random.default_rng(n + d)
+    q, k, v = rows(rng, n, 4, d), rows(rng, lk, 2, d), rows(rng, lk, 2, d)
+    v[7, :, 3], v[60, :, 4], v[lk - 1, :, 5] = np.inf, np.nan, -np.inf
+    v[2, 0, 9], v[lk - 3, 0, 9] = np.inf, -np.inf
+    with np.errstate(invalid="ignore"):
+        got, lse, want = run_attend(s3dx, q, k, v, dtype, [n], [lk], 64)
+        check(s3dx, dtype, got, lse, want)
+        assert np.all(got[:, :, 3] == np.inf) and np.all(np.isnan(got[:, :, 4])) and np.all(np.isnan(got[:, :2, 9]))
+        k[:, 1] = np.where(np.arange(d) == 0, -np.inf, 0.0)  # ... of rows that see scores of -inf alone
+        q[:, :, 0] = 1.0
+        got, lse, want = run_attend(s3dx, q, k, v, dtype, [n], [lk], 64)
+        assert np.all(got[:, 2:] == 0) and np.all(lse[:, 2:] == -np.inf)
+
+
 def test_scores_of_any_size(s3dx):
     # scores of thousands (one key takes all), of the type's lowest value, and infinities
     rng = np.random.default_rng(12)
