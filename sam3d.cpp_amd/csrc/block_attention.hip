@@ -897,6 +897,9 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         if (w0 + TABLE >= blocks) return false;
         w0 += TABLE;
         chunk = 0;
+        // SHARED waves take as many steps as the longest of them and may leave a table before its last chunk, where their
+        // own count ends: whose turn a block is goes by the whole table's count
+        if constexpr (SHARED) rank = rank0;
         together();
         return true;
     };
