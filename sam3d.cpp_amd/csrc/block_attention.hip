@@ -450,7 +450,7 @@ struct AttendArgs {
     int32_t heads, group, kv_heads, block, block_log2, top, causal, splits, tile_groups;
     float scale;
     float *part_o;   // [splits][total_q][heads][d]: not yet divided by the sum
-    float2 *part_ml; // [splits][total_q][heads]: maximum (natural units), sum
+    float2 *part_ml; // [splits][total_q][heads]: the power of two that weights are relative to, their sum
 };
 
 constexpr float kLn2 = 0.693147180559945309f;
@@ -486,6 +486,11 @@ __device__ __forceinline__ float sum_over_groups(float v) {
     const uint32_t w = __builtin_bit_cast(uint32_t, m);
     const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
     return as_float(b[0]) + as_float(b[1]);
+}
+
+// The logarithm of a sum of weights l relative to 2^m; of nothing seen -inf.
+__device__ __forceinline__ float log_of(float m, float l) {
+    return l == 0.0f ? neg_inf() : fmaf(m, kLn2, __builtin_amdgcn_logf(l) * kLn2);
 }
 
 // Whether a row's sums (l: the weights', y: anything made of its values') have to be made again: 0 times what is not
@@ -948,7 +953,9 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             const float now = in ? fmaxf(top[n], mx) : top[n];
             // nothing seen yet: any finite base leaves weights of 0
             const float to = now == neg_inf() ? 0.0f : now * cs;
-            const float alpha = __builtin_amdgcn_exp2f(top[n] * cs - to);
+            // From base to base, as they are: the products they were rounded from differ by up to 2^-24 of them, and a row
+            // would carry that on with every move, its neighbours' too.
+            const float alpha = __builtin_amdgcn_exp2f(top[n] == neg_inf() ? neg_inf() : base[n] - to);
             sum[n] *= alpha;
 #pragma unroll
             for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
@@ -1225,7 +1232,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             for (int w = 0; w < N; w += 4)
                 *reinterpret_cast<f32x4 *>(to + w) = f32x4{y[w] * r, y[w + 1] * r, y[w + 2] * r, y[w + 3] * r};
         }
-        if (a.lse && ch == 0) a.lse[token * a.heads + h] = l == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l) * kLn2;
+        if (a.lse && ch == 0) a.lse[token * a.heads + h] = log_of(m, l);
     };
     // A set's rows whose sums are not finite are left out, and computed again from the keys that they see alone.  The test costs nothing in the loop.
     const auto finish = [&](int n, const float (&y)[4 * C], float m, float l) __attribute__((always_inline)) {
@@ -1259,7 +1266,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             float y[4 * C];
 #pragma unroll
             for (int e = 0; e < 4 * C; ++e) y[e] = acc[n][e % C][e / C];
-            finish(n, y, top[n] * a.scale, P == 3 ? sum[n][0] : sum_over_groups(sum[n][0]));
+            finish(n, y, base[n], P == 3 ? sum[n][0] : sum_over_groups(sum[n][0]));
         }
     } else {
         __syncthreads();  // the steps' LDS is through
@@ -1270,7 +1277,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[wave][(n * 4 + i) * C + t][lane] = acc[n][t][i];
             const float l = P == 3 ? sum[n][0] : sum_over_groups(sum[n][0]);
-            if (g == 0) part_ml[wave][n][c] = make_float2(top[n] * a.scale, l);
+            if (g == 0) part_ml[wave][n][c] = make_float2(base[n], l);
         }
         __syncthreads();
         if (wave >= SETS) return;
@@ -1284,7 +1291,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int p = 0; p < J; ++p) {
             const float2 ml = part_ml[p0 + p][n][c];
-            wgt[p] = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((ml.x - m) * kLog2e);  // a piece without keys: 0
+            wgt[p] = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);  // a piece without keys: 0
             l += wgt[p] * ml.y;
         }
 #pragma unroll
@@ -1312,7 +1319,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
     const float2 ml = lane < a.splits ? a.part_ml[lane * cells + cell] : make_float2(neg_inf(), 0.0f);
     float m = ml.y != 0.0f ? ml.x : neg_inf();
     for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    const float w = ml.y != 0.0f ? exp2f((ml.x - m) * kLog2e) : 0.0f;
+    const float w = ml.y != 0.0f ? exp2f(ml.x - m) : 0.0f;
     float l = w == 0.0f ? 0.0f : w * ml.y, o[2] = {0.0f, 0.0f};
     for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
     // four pieces' values on their way at a time
@@ -1345,7 +1352,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
         if (lane + 64 * e < D)
             store_from_f32<T>(static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(head) * D + lane + 64 * e,
                               l == 0.0f ? 0.0f : o[e] * r);
-    if (a.lse && lane == 0) a.lse[cell] = l == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l) * kLn2;
+    if (a.lse && lane == 0) a.lse[cell] = log_of(m, l);
 }
 
 // ---------------------------------------------------------------------------

@@ -55,3 +55,32 @@ def test_neighbours_lists_across_tables(s3dx, seed, n, lk, heads, kv, d, block, 
     sel = alike(rng, n, kv, block, lk, top, seed % 3)
     got, lse, want = B.run_attend(s3dx, q, k, v, s3dx.BF16, [n], [lk], block, sel, causal)
     B.check(s3dx, s3dx.BF16, got, lse, want)
+
+
+# ---------------------------------------------------------------------------
+# What weights are relative to
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("d,lk", [(64, 5000), (128, 5000), (32, 5000)])
+def test_a_row_keeps_its_weights_while_its_neighbours_maxima_rise(s3dx, dtype, d, lk):
+    # Even rows: one score for all keys, hence the mean of the values.  Odd rows: scores that rise by more than 8 binary
+    # orders at every step, so that the tile's bases move all the time.  All raw products are exact.  399 sequences
+    # without rows keep the tile in one piece.
+    n, scale = 32, 0.71
+    q, k = np.zeros((n, 1, d), np.float32), np.zeros((lk, 1, d), np.float32)
+    q[::2, 0, 0] = 2.0 ** 11 * np.arange(65, 81)
+    q[1::2, 0, 1] = 1.0
+    k[:, 0, 0], k[:, 0, 1] = 1.0, 16.0 * (np.arange(lk) // 32)
+    v = np.where(np.arange(lk) < lk // 2, 1.0, -1.0).astype(np.float32)[:, None, None] * np.ones((1, 1, d), np.float32)
+    dq, dk, dv = (R.dev(s3dx, R.stored(s3dx, a, dtype)[0]) for a in (q, k, v))
+    o, lse = s3dx.DeviceArray((n, 1, d), R.store_type(s3dx, dtype)), s3dx.DeviceArray((n, 1), np.float32)
+    qs, ks = B.starts(s3dx, [n] + [0] * 399), B.starts(s3dx, [lk] + [0] * 399)
+    size = s3dx.block_attention_workspace_size(n, 1, 1, d, 400, 64, 0, lk)
+    s3dx.block_attention(dq, dk, dv, dtype, n, lk, 1, 1, d, qs, ks, 400, 64, lk, o, lse, scale=scale,
+                         workspace=s3dx.DeviceArray(max(1, size), np.uint8))
+    got, l = R.values(s3dx, o, dtype)[::2], lse.download()[::2, 0].astype(np.float64)
+    print("  off by", np.abs(got).max(), flush=True)
+    # equal weights (rounded alike), a sum of lk terms above and below
+    assert np.all(np.abs(got) <= 2 * (lk + 8) * R.U32)
+    want = q[::2, 0, 0].astype(np.float64) * np.float64(np.float32(scale)) + np.log(lk)
+    assert np.all(np.abs(l - want) <= 8 * R.U32 * want)
