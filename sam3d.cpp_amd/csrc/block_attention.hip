@@ -1320,7 +1320,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
     float m = ml.y != 0.0f ? ml.x : neg_inf();
     for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
     const float w = ml.y != 0.0f ? exp2f(ml.x - m) : 0.0f;
-    float l = w == 0.0f ? 0.0f : w * ml.y, o[2] = {0.0f, 0.0f};
+    float l = ml.y != 0.0f ? w * ml.y : 0.0f, o[2] = {0.0f, 0.0f};
     for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
     // four pieces' values on their way at a time
     for (uint64_t left = __ballot(ml.y != 0.0f); left;) {

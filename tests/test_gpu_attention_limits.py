@@ -84,3 +84,14 @@ def test_a_row_keeps_its_weights_while_its_neighbours_maxima_rise(s3dx, dtype, d
     assert np.all(np.abs(got) <= 2 * (lk + 8) * R.U32)
     want = q[::2, 0, 0].astype(np.float64) * np.float64(np.float32(scale)) + np.log(lk)
     assert np.all(np.abs(l - want) <= 8 * R.U32 * want)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("lk,d,stretch,period", [(2048, 64, 256, 1024), (2048, 64, 128, 512), (2048, 128, 128, 512), (5000, 32, 256, 2048),
+                                                 (5000, 64, 256, 2048), (5000, 128, 128, 1024), (300, 64, 32, 128)])
+def test_nan_keys_that_are_all_of_a_piece(s3dx, dtype, lk, d, stretch, period):
+    rng = np.random.default_rng(lk)
+    q, k, v = B.rows(rng, 1, 1, d), B.rows(rng, lk, 1, d), B.rows(rng, lk, 1, d)
+    k[np.arange(lk) % period < stretch] = np.nan
+    got, lse, _ = B.run_attend(s3dx, q, k, v, dtype, [1], [lk], 64)
+    assert np.isnan(got).all() and np.isnan(lse).all()
