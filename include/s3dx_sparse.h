@@ -582,7 +582,8 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
  * below 2^-102 down to 2^-126).  o overlaps no input.  max_k, the keys of the longest sequence,
  * decides how the work is cut and not what is computed.  Rows whose result is not
  * finite are computed a second time key by key, more slowly (BF16 rows over all
- * keys without S3DX_BLOCK_CAUSAL only where their weights are not).
+ * keys without S3DX_BLOCK_CAUSAL only where their weights are not); so are rows
+ * whose largest score, of any part of their keys, passes 1.1e7 either way.
  * The workspace holds partial results where there are too few rows to fill the GPU
  * (s3dx_block_attention_workspace_size of the same arguments, 0 bytes where none are
  * needed); calls that may run at the same time need one each.  The

@@ -455,6 +455,7 @@ struct AttendArgs {
 
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kMostBase = 0x1p24f;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -504,7 +505,8 @@ __device__ __forceinline__ bool again_of(const AttendArgs &a, float l, float y) 
 
 // One row by the whole wave, key by key: scores with a key per lane, the running maximum
 // and sum, values with a channel pair per lane.  Only keys that the row sees are
-// multiplied, so nothing else reaches it: for rows whose tile gave no finite result.
+// multiplied, so nothing else reaches it: for rows whose tile gave no finite result, or none
+// that its bases hold.
 template <class T, int D>
 __device__ void attend_row(const AttendArgs &a, int64_t row, int head, Span qs, Span ks) {
     const int lane = threadIdx.x & 63, kvh = head / a.group;
@@ -957,6 +959,10 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             // would carry that on with every move, its neighbours' too.
             const float alpha = __builtin_amdgcn_exp2f(top[n] == neg_inf() ? neg_inf() : base[n] - to);
             sum[n] *= alpha;
+            // A base is rounded to 24 bits, and its weights keep what that is off by: up to 2^-0.5 .. 2^0.5 of them below
+            // 2^24, all of them and more far above (scores from 1e9 on).  There the sum is a NaN from now on, and the row
+            // is computed key by key, differences first.
+            if (!(fabsf(to) < kMostBase)) sum[n] = __builtin_nanf("") + sum[n];
 #pragma unroll
             for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
             top[n] = now;

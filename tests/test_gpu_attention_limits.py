@@ -87,6 +87,45 @@ def test_a_row_keeps_its_weights_while_its_neighbours_maxima_rise(s3dx, dtype, d
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("lk", [1, 2, 5, 100, 700, 4000])
+@pytest.mark.parametrize("n,d,listed", [(40, 64, False), (70, 128, False), (3, 96, False), (40, 64, True), (70, 128, True)])
+def test_scores_from_a_million_to_1e30(s3dx, dtype, lk, n, d, listed):
+    # equal scores, of either sign: the mean of the values, whatever their size
+    rng = np.random.default_rng(lk + n)
+    q, k, v = np.zeros((n, 1, d), np.float32), np.zeros((lk, 1, d), np.float32), B.rows(rng, lk, 1, d)
+    q[:, 0, 0] = 10.0 ** rng.uniform(6, 12, n) * rng.choice([-1, 1], n)
+    q[::7, 0, 0] *= 1e18
+    k[:, 0, 0] = 1.0
+    sel = np.tile(np.arange(-(-lk // 32), dtype=np.int32), (n, 1, 1)) if listed else None
+    got, lse, _ = B.run_attend(s3dx, q, k, v, dtype, [n], [lk], 32, sel, scale=1.0)
+    v64, q64 = R.stored(s3dx, v, dtype)[1][:, 0], R.stored(s3dx, q, dtype)[1][:, 0, 0]
+    mean, size = v64.mean(0), np.abs(v64).mean(0)
+    # weights are equal (bfloat16: rounded alike, their sum is not rounded so: 2^-8), sums of lk terms
+    off = np.abs(got[:, 0] - mean) - R.half_step(s3dx, dtype) * np.abs(mean) * 1.01
+    assert np.all(off <= (2 * (lk + 8) * R.U32 + (1.01 * R.UBF if dtype else 0)) * size), (np.abs(got[:, 0] - mean).max())
+    assert np.all(np.abs(lse[:, 0] - (q64 + np.log(lk))) <= 8 * R.U32 * np.abs(q64) + 1e-6)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n,lk,d", [(40, 300, 64), (70, 1300, 128), (3, 4000, 64)])
+def test_one_score_far_above_the_others(s3dx, dtype, n, lk, d):
+    # the key takes all; below: far scores among ordinary ones count for nothing
+    rng = np.random.default_rng(n)
+    for far in (1e9, 3e10, 1e12, 1e30):
+        q, k, v = np.zeros((n, 1, d), np.float32), 0.1 * B.rows(rng, lk, 1, d), B.rows(rng, lk, 1, d)
+        q[:, 0, 0], k[:, 0, 0] = 1.0, 0.0
+        k[lk // 3, 0, 0] = far
+        got, _, _ = B.run_attend(s3dx, q, k, v, dtype, [n], [lk], 32, scale=1.0)
+        assert np.array_equal(got[:, 0], np.tile(R.stored(s3dx, v, dtype)[1][lk // 3, 0], (n, 1)))
+        k[:, 0, 0] = np.where(np.arange(lk) % 5 == 0, np.float32(-far), 0.0)
+        got, lse, _ = B.run_attend(s3dx, q, k, v, dtype, [n], [lk], 32, scale=1.0)
+        v64 = R.stored(s3dx, v, dtype)[1][np.arange(lk) % 5 != 0, 0]
+        off = np.abs(got[:, 0] - v64.mean(0)) - R.half_step(s3dx, dtype) * np.abs(v64.mean(0))
+        assert np.all(off <= (2 * (lk + 8) * R.U32 + (1.01 * R.UBF if dtype else 0)) * np.abs(v64).mean(0))
+        assert np.all(np.abs(lse[:, 0] - np.log(len(v64))) <= (lk + 8) * R.U32)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
 @pytest.mark.parametrize("lk,d,stretch,period", [(2048, 64, 256, 1024), (2048, 64, 128, 512), (2048, 128, 128, 512), (5000, 32, 256, 2048),
                                                  (5000, 64, 256, 2048), (5000, 128, 128, 1024), (300, 64, 32, 128)])
 def test_nan_keys_that_are_all_of_a_piece(s3dx, dtype, lk, d, stretch, period):
