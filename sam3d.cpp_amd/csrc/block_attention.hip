@@ -489,9 +489,19 @@ __device__ __forceinline__ float sum_over_groups(float v) {
     return as_float(b[0]) + as_float(b[1]);
 }
 
-// The logarithm of a sum of weights l relative to 2^m; of nothing seen -inf.
-__device__ __forceinline__ float log_of(float m, float l) {
-    return l == 0.0f ? neg_inf() : fmaf(m, kLn2, __builtin_amdgcn_logf(l) * kLn2);
+// Binary orders by which weights over `keys` keys are kept down, so that sums of finite values stay finite whatever the
+// values: weights pass 1 by 8 orders and a base's rounding before that moves, and there are as many as keys.  Where
+// again_of looks at the weights alone; elsewhere 0, as a sum that is not finite is made again, and small values keep their
+// lowest bits.
+template <class T>
+__device__ __forceinline__ int room_of(const AttendArgs &a, int keys) {
+    return sizeof(T) == 2 && !a.selected && !a.causal ? 9 + 32 - __builtin_clz(keys | 1) : 0;
+}
+
+// The logarithm of a sum of weights l relative to 2^m, `room` of whose orders kept them down; of nothing seen -inf.
+__device__ __forceinline__ float log_of(float m, float l, int room) {
+    return l == 0.0f ? neg_inf()
+                     : fmaf(m - static_cast<float>(room), kLn2, __builtin_amdgcn_logf(ldexpf(l, room)) * kLn2);
 }
 
 // Whether a row's sums (l: the weights', y: anything made of its values') have to be made again: 0 times what is not
@@ -520,6 +530,7 @@ __device__ void attend_row(const AttendArgs &a, int64_t row, int head, Span qs, 
 #pragma unroll
     for (int w = 0; w < 2; ++w) qv[w] = lane + 64 * w < D ? load_as_f32<T>(q + lane + 64 * w) * a.scale : 0.0f;
     float m = neg_inf(), l = 0.0f, o[2] = {0.0f, 0.0f};
+    const int room = 32 - __builtin_clz(seen | 1);  // weights add up to 1 at most, so that sums of finite values stay finite
     // A weight that is a NaN makes the whole row one: the rest need not be read (5,086 rows x 16 heads x 64
     // bf16 with a NaN among the keys: 0.9 ms; 30 ms key by key to the end).
     bool lost = false;
@@ -542,7 +553,7 @@ __device__ void attend_row(const AttendArgs &a, int64_t row, int head, Span qs, 
             for (int w = 1; w < 64; w <<= 1) mx = fmaxf(mx, __shfl_xor(mx, w, 64));
             const float mn = fmaxf(m, mx), base = mn == neg_inf() ? 0.0f : mn;
             // the difference first: scores of the type's lowest value stay finite
-            const float alpha = exp2f((m - base) * kLog2e), p = exp2f((sc - base) * kLog2e);
+            const float alpha = exp2f((m - base) * kLog2e), p = exp2f(fmaf(sc - base, kLog2e, -static_cast<float>(room)));
             l = l * alpha + (lane < count ? p : 0.0f);
             o[0] *= alpha;
             o[1] *= alpha;
@@ -562,7 +573,7 @@ __device__ void attend_row(const AttendArgs &a, int64_t row, int head, Span qs, 
 #pragma unroll
     for (int w = 0; w < 2; ++w)
         if (lane + 64 * w < D) store_from_f32<T>(y + lane + 64 * w, l == 0.0f ? 0.0f : o[w] * r);
-    if (a.lse && lane == 0) a.lse[row * a.heads + head] = l == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(l) * kLn2;
+    if (a.lse && lane == 0) a.lse[row * a.heads + head] = l == 0.0f ? neg_inf() : m + __builtin_amdgcn_logf(ldexpf(l, room)) * kLn2;
 }
 
 // N dwords at byte offset `at` of a buffer; zeros from its end on.
@@ -826,6 +837,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         for (int t = 0; t < C; ++t) acc[n][t] = f32x4{0, 0, 0, 0};
     }
     const float cs = a.scale * kLog2e;
+    const int room = room_of<T>(a, ks.rows);
     // Byte offsets of this lane's rows of V in a step: held where registers allow, else the first and the steps between.
     constexpr bool HELD = D < 128 && !SHARED;
     const int kstep = static_cast<int>(a.k_stride) * E, vstep = static_cast<int>(a.v_stride) * E;
@@ -954,15 +966,15 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             mx = max_over_groups(mx);
             const float now = in ? fmaxf(top[n], mx) : top[n];
             // nothing seen yet: any finite base leaves weights of 0
-            const float to = now == neg_inf() ? 0.0f : now * cs;
+            float to = now == neg_inf() ? 0.0f : fmaf(now, cs, static_cast<float>(room));
+            // A base is rounded to 24 bits, and its weights keep what that is off by: up to 2^-0.5 .. 2^0.5 of them below
+            // 2^24, all of them and more far above (scores from 1e9 on).  There it is a NaN, and so are the row's weights
+            // from now on: it is computed key by key, differences first.
+            to = fabsf(to) < kMostBase ? to : __builtin_nanf("");
             // From base to base, as they are: the products they were rounded from differ by up to 2^-24 of them, and a row
             // would carry that on with every move, its neighbours' too.
             const float alpha = __builtin_amdgcn_exp2f(top[n] == neg_inf() ? neg_inf() : base[n] - to);
             sum[n] *= alpha;
-            // A base is rounded to 24 bits, and its weights keep what that is off by: up to 2^-0.5 .. 2^0.5 of them below
-            // 2^24, all of them and more far above (scores from 1e9 on).  There the sum is a NaN from now on, and the row
-            // is computed key by key, differences first.
-            if (!(fabsf(to) < kMostBase)) sum[n] = __builtin_nanf("") + sum[n];
 #pragma unroll
             for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
             top[n] = now;
@@ -1238,7 +1250,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
             for (int w = 0; w < N; w += 4)
                 *reinterpret_cast<f32x4 *>(to + w) = f32x4{y[w] * r, y[w + 1] * r, y[w + 2] * r, y[w + 3] * r};
         }
-        if (a.lse && ch == 0) a.lse[token * a.heads + h] = log_of(m, l);
+        if (a.lse && ch == 0) a.lse[token * a.heads + h] = log_of(m, l, room);
     };
     // A set's rows whose sums are not finite are left out, and computed again from the keys that they see alone.  The test costs nothing in the loop.
     const auto finish = [&](int n, const float (&y)[4 * C], float m, float l) __attribute__((always_inline)) {
@@ -1321,6 +1333,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
     const int head = static_cast<int>(cell - row * a.heads);
     const int64_t s = sequence_of_row(a.q_starts, a.sequences, row);
     if (s < 0) return;
+    const Span ks = sequence_span(a.k_starts, s, a.total_k);
     // a lane for each piece (there are at most 64): its weight, 0 for one without keys (a sum that is a NaN is not 0 and stays)
     const float2 ml = lane < a.splits ? a.part_ml[lane * cells + cell] : make_float2(neg_inf(), 0.0f);
     float m = ml.y != 0.0f ? ml.x : neg_inf();
@@ -1349,7 +1362,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
             for (int e = 0; e < 2; ++e) o[e] += wp[u] * x[u][e];
     }
     if (__any(again_of<T>(a, l, o[0] * 0.0f + o[1] * 0.0f))) {
-        attend_row<T, D>(a, row, head, sequence_span(a.q_starts, s, a.total_q), sequence_span(a.k_starts, s, a.total_k));
+        attend_row<T, D>(a, row, head, sequence_span(a.q_starts, s, a.total_q), ks);
         return;
     }
     const float r = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1358,7 +1371,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a) {
         if (lane + 64 * e < D)
             store_from_f32<T>(static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(head) * D + lane + 64 * e,
                               l == 0.0f ? 0.0f : o[e] * r);
-    if (a.lse && lane == 0) a.lse[cell] = log_of(m, l);
+    if (a.lse && lane == 0) a.lse[cell] = log_of(m, l, room_of<T>(a, ks.rows));
 }
 
 // ---------------------------------------------------------------------------

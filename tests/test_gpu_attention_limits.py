@@ -126,6 +126,25 @@ def test_one_score_far_above_the_others(s3dx, dtype, n, lk, d):
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("power", [115, 121, 127])
+@pytest.mark.parametrize("n,lk,d,top,causal", [(40, 100, 64, 0, False), (70, 700, 64, 0, False), (65, 1300, 128, 0, False),
+                                               (3, 4000, 64, 0, False), (90, 600, 96, 0, False), (70, 700, 32, 0, True),
+                                               (70, 700, 64, 9, False), (65, 1300, 128, 17, True), (3, 4000, 64, 30, False)])
+def test_values_near_the_types_largest(s3dx, dtype, power, n, lk, d, top, causal):
+    # Scores that rise by 7.9 binary orders from the first key to the last: weights are relative to the first ones' for long.
+    rng = np.random.default_rng(n + lk)
+    q, k, v = np.zeros((n, 2, d), np.float32), np.zeros((lk, 2, d), np.float32), B.rows(rng, lk, 2, d)
+    q[:, :, 0] = 1.0
+    k[:, :, 0] = (7.9 * np.log(2) / lk * np.arange(lk))[:, None]
+    v = np.clip(np.exp(0.2 * v), 0.5, 1.9).astype(np.float32) * np.float32(2.0 ** power)
+    v[:, :, ::2] *= -1
+    sel = B.choose(rng, [n], [lk], 2, 32, top) if top else None
+    got, lse, want = B.run_attend(s3dx, q, k, v, dtype, [n], [lk], 32, sel, causal, scale=1.0)
+    assert np.isfinite(want[0]).all() and np.isfinite(got).all()
+    B.check(s3dx, dtype, got, lse, want)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
 @pytest.mark.parametrize("lk,d,stretch,period", [(2048, 64, 256, 1024), (2048, 64, 128, 512), (2048, 128, 128, 512), (5000, 32, 256, 2048),
                                                  (5000, 64, 256, 2048), (5000, 128, 128, 1024), (300, 64, 32, 128)])
 def test_nan_keys_that_are_all_of_a_piece(s3dx, dtype, lk, d, stretch, period):
