@@ -826,11 +826,12 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
 
     // ---- state
     f32x4 acc[NS][C], sum[NS];
-    // what weights are relative to: a raw product, and the same as a power of two; the product from which on it moves
-    float top[NS], base[NS], above[NS];
+    // what weights are relative to, a power of two; the raw product from which on it moves (-inf: nothing seen yet, when
+    // any finite base leaves weights of 0)
+    float base[NS], above[NS];
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-        top[n] = above[n] = neg_inf();
+        above[n] = neg_inf();
         base[n] = 0.0f;
         sum[n] = f32x4{0, 0, 0, 0};
 #pragma unroll
@@ -964,22 +965,20 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendArgs a) {
         // maximum, and floating point loses nothing by it.
         const auto move = [&](int n, float mx, bool in) __attribute__((always_inline)) {
             mx = max_over_groups(mx);
-            const float now = in ? fmaxf(top[n], mx) : top[n];
-            // nothing seen yet: any finite base leaves weights of 0
-            float to = now == neg_inf() ? 0.0f : fmaf(now, cs, static_cast<float>(room));
+            const bool over = in && mx > above[n];
             // A base is rounded to 24 bits, and its weights keep what that is off by: up to 2^-0.5 .. 2^0.5 of them below
             // 2^24, all of them and more far above (scores from 1e9 on).  There it is a NaN, and so are the row's weights
             // from now on: it is computed key by key, differences first.
-            to = fabsf(to) < kMostBase ? to : __builtin_nanf("");
+            float to = fmaf(mx, cs, static_cast<float>(room));
+            to = !over ? base[n] : fabsf(to) < kMostBase ? to : __builtin_nanf("");
             // From base to base, as they are: the products they were rounded from differ by up to 2^-24 of them, and a row
-            // would carry that on with every move, its neighbours' too.
-            const float alpha = __builtin_amdgcn_exp2f(top[n] == neg_inf() ? neg_inf() : base[n] - to);
+            // would carry that on with every move.  (Before the first there is nothing to keep.)
+            const float alpha = above[n] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(base[n] - to);
             sum[n] *= alpha;
 #pragma unroll
             for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
-            top[n] = now;
             base[n] = to;
-            above[n] = now + 8.0f / cs;
+            above[n] = over ? mx + 8.0f / cs : above[n];
         };
         const auto weights = [&](int n, float off) __attribute__((always_inline)) {
 #pragma unroll
