@@ -49,6 +49,9 @@ struct TurnArgs {
 };
 constexpr int kMaxRows = 32;    // of a workgroup
 constexpr int kMaxTurns = 512;  // pairs of those rows
+// Heads whose squares' sum passes 2^128 (|x| of 2^60 and more) are summed again smaller: 256 squares of at most 2^116,
+// beside which eps is nothing.
+constexpr float kLess = 0x1p-70f;
 
 // cos and sin of a 0.64 fixed-point part of a turn.  The quarter turn is split
 // off in integers, so that the float holds at most an eighth of a turn.
@@ -134,7 +137,7 @@ __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
         const HeadRows &p = a.part[k ? 1 : 0];
         const bool here = head < heads;
         if (k) head -= a.part[0].heads;
-        const TI *x = static_cast<const TI *>(p.x) + (row0 + r) * p.x_stride + static_cast<int64_t>(head) * a.d;
+        const TI *from = static_cast<const TI *>(p.x) + (row0 + r) * p.x_stride + static_cast<int64_t>(head) * a.d;
         TO *y = static_cast<TO *>(p.y) + (row0 + r) * p.y_stride + static_cast<int64_t>(head) * a.d;
         const float *gain = p.gain ? p.gain + static_cast<int64_t>(head) * a.gain_stride : nullptr;
         if constexpr (FORM != SINGLE) {
@@ -146,8 +149,8 @@ __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
             const int c1 = halves && l < turning ? c0 + a.pairs : c0 + 8;
             float u[8], v[8], gu[8], gv[8];
             if (active) {
-                load8(x + c0, u);
-                load8(x + c1, v);
+                load8(from + c0, u);
+                load8(from + c1, v);
                 if (gain) {
                     load8(gain + c0, gu);
                     load8(gain + c1, gv);
@@ -160,6 +163,13 @@ __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
                 for (int e = 0; e < 8; ++e) sum += active ? u[e] * u[e] + v[e] * v[e] : 0.0f;
                 for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
                 scale = rsqrtf(sum / static_cast<float>(a.d) + a.eps);
+                if (!(sum < __builtin_inff())) {  // the same for a head's lanes
+                    sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum += active ? (u[e] * kLess) * (u[e] * kLess) + (v[e] * kLess) * (v[e] * kLess) : 0.0f;
+                    for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
+                    scale = rsqrtf(sum / static_cast<float>(a.d)) * kLess;
+                }
             }
             if (FORM == WHOLE && !active) continue;
             if (a.norm) {
@@ -226,42 +236,44 @@ __global__ void __launch_bounds__(256) turn_kernel(TurnArgs a, TurnTable t) {
             store8(y + c1, v);
         } else {
             const int step = a.halves ? 1 : 2, apart = a.halves ? a.pairs : 1;
-            float first[2], second[2], rest[4], sum = 0.0f;
+            float x[8], g[8];  // the pairs' first and second channels, the rest
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int j = lane + 64 * q, c = j * step;
-                first[q] = second[q] = 0.0f;
-                if (j >= a.pairs) continue;
-                first[q] = load_as_f32<TI>(x + c);
-                second[q] = load_as_f32<TI>(x + c + apart);
-                sum += first[q] * first[q] + second[q] * second[q];
-                if (gain) {
-                    first[q] *= gain[c];
-                    second[q] *= gain[c + apart];
+            for (int q = 0; q < 8; ++q) {
+                const int j = lane + 64 * (q >> 1);
+                const int c = q < 4 ? j * step + (q & 1) * apart : 2 * a.pairs + lane + 64 * (q - 4);
+                const bool any = q < 4 ? j < a.pairs : c < a.d;
+                x[q] = any ? load_as_f32<TI>(from + c) : 0.0f;
+                g[q] = gain && any ? gain[c] : 1.0f;
+            }
+            if (a.norm) {
+                const auto squares = [&]() __attribute__((always_inline)) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) sum += x[q] * x[q];
+                    return wave_sum(sum);
+                };
+                float sum = squares(), eps = a.eps;
+                if (!(sum < __builtin_inff())) {  // the same for the wave
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) x[q] *= kLess;
+                    sum = squares(), eps = 0.0f;
                 }
-            }
+                const float scale = rsqrtf(sum / static_cast<float>(a.d) + eps);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int c = 2 * a.pairs + lane + 64 * q;
-                rest[q] = 0.0f;
-                if (c >= a.d) continue;
-                rest[q] = load_as_f32<TI>(x + c);
-                sum += rest[q] * rest[q];
-                if (gain) rest[q] *= gain[c];
+                for (int q = 0; q < 8; ++q) x[q] *= g[q] * scale;
             }
-            const float scale = a.norm ? rsqrtf(wave_sum(sum) / static_cast<float>(a.d) + a.eps) : 1.0f;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 const int j = lane + 64 * q, c = j * step;
                 if (j >= a.pairs) continue;
                 const float2 cs = turns[r * a.pairs + j];
-                store_from_f32<TO>(y + c, (first[q] * cs.x - second[q] * cs.y) * scale);
-                store_from_f32<TO>(y + c + apart, (first[q] * cs.y + second[q] * cs.x) * scale);
+                store_from_f32<TO>(y + c, x[2 * q] * cs.x - x[2 * q + 1] * cs.y);
+                store_from_f32<TO>(y + c + apart, x[2 * q] * cs.y + x[2 * q + 1] * cs.x);
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int c = 2 * a.pairs + lane + 64 * q;
-                if (c < a.d) store_from_f32<TO>(y + c, rest[q] * scale);
+                if (c < a.d) store_from_f32<TO>(y + c, x[4 + q]);
             }
         }
     }

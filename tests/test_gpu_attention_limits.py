@@ -153,3 +153,32 @@ def test_nan_keys_that_are_all_of_a_piece(s3dx, dtype, lk, d, stretch, period):
     k[np.arange(lk) % period < stretch] = np.nan
     got, lse, _ = B.run_attend(s3dx, q, k, v, dtype, [1], [lk], 64)
     assert np.isnan(got).all() and np.isnan(lse).all()
+
+
+# ---------------------------------------------------------------------------
+# Norms of large rows
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("d,pairs,adjacent,pad", [(64, 30, True, 0), (64, 24, False, 0), (64, 30, False, 0), (20, 10, True, 0), (64, 30, True, 1),
+                                                  (128, 0, True, 0), (33, 0, True, 0)])
+def test_norms_of_rows_of_any_size(s3dx, dtype, d, pairs, adjacent, pad):
+    # x / sqrt(mean(x^2) + eps) is of order one however large x is, also where x^2 passes float32's range
+    rng = np.random.default_rng(d + pairs)
+    n, h = 41, 3
+    x = rng.standard_normal((n, h * d + pad)).astype(np.float32) * np.exp2(np.linspace(-40, 125, n)).astype(np.float32)[:, None]
+    x = np.clip(x, -3e38, 3e38)
+    xs, xv = R.stored(s3dx, x, dtype)
+    gain = (1 + 0.2 * rng.standard_normal((h, d))).astype(np.float32)
+    pos = rng.integers(0, 64, (n, 1)).astype(np.int32)
+    rot = s3dx.Rotary.per_axis(d, [pairs], 1000.0, s3dx.ROTARY_ADJACENT if adjacent else s3dx.ROTARY_HALVES) if pairs else None
+    y = s3dx.DeviceArray((n, h, d), np.float32)
+    s3dx.qk_norm_rotary(R.dev(s3dx, xs), None, dtype, n, h, 0, d, 1e-6, y, rotary=rot, positions=R.dev(s3dx, pos) if pairs else None,
+                        position_stride=1, q_gain=R.dev(s3dx, gain), q_stride=h * d + pad, out_dtype=s3dx.F32)
+    want = R.rms(xv[:, : h * d].reshape(n, h, d), gain, 1e-6)
+    size = np.abs(want)
+    if pairs:
+        want, size = R.turn(want, pos, [0] * pairs, [1000.0 ** (-j / pairs) for j in range(pairs)], adjacent)
+    off = np.abs(y.download() - want)
+    # the sum of squares, its root, gain and scale, the turn (8 u), the output's rounding
+    bound = ((d + 2) / 2 + 8 + 8 + 1) * R.U32 * (size + np.abs(want))
+    assert np.all(off <= bound + 1e-37), np.argwhere(off > bound + 1e-37)[:4]
