@@ -578,12 +578,13 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
  * scores of -inf, gets zeros and lse -inf; keys and values that a row does not
  * see do not reach it, whatever they hold.  BF16 weights are rounded to bfloat16
  * before they meet the values (their sum and lse are of the weights before that),
- * FP32 ones are not (heads up to 64 wide: products of 24 significant bits, of values
- * below 2^-102 down to 2^-126).  o overlaps no input.  max_k, the keys of the longest sequence,
- * decides how the work is cut and not what is computed.  Rows whose result is not
- * finite are computed a second time key by key, more slowly (BF16 rows over all
- * keys without S3DX_BLOCK_CAUSAL only where their weights are not); so are rows
- * whose largest score, of any part of their keys, passes 1.1e7 either way.
+ * FP32 ones are not (heads up to 64 wide: values whole, their products short by up to 2^-21,
+ * 2^-24.5 in the mean; values below 2^-102 lose bits down to 2^-126).  o overlaps no input.  max_k, the keys of the longest
+ * sequence, decides how the work is cut and not what is computed.  Rows whose sums are
+ * not finite (values near float32's largest do that too) are computed a second time key
+ * by key, more slowly (BF16 rows over all keys without S3DX_BLOCK_CAUSAL only where their
+ * weights are not); so are rows whose largest score, of any part of their keys, passes
+ * 1.1e7 either way.
  * The workspace holds partial results where there are too few rows to fill the GPU
  * (s3dx_block_attention_workspace_size of the same arguments, 0 bytes where none are
  * needed); calls that may run at the same time need one each.  The

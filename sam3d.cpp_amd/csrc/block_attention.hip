@@ -631,7 +631,8 @@ __device__ __forceinline__ u32x2 transposed(const char *p) {
 }
 
 // d += A B over 32 values: one product of bfloat16 operands, or, of operands in three terms, the six
-// of at least 2^-16 of the whole, the smallest first (what is left out is 2^-24 of it and less).
+// largest, the smallest of them first.  Terms are cut off, not rounded, so the second reaches 2^-7 of the first and the
+// third 2^-15: what is left out is up to 2^-21 of a product, 2^-24.5 in the mean, and of the product's sign.
 template <int P>
 __device__ __forceinline__ f32x4 product(const u32x4 (&x)[P], const u32x4 (&y)[P], f32x4 d) {
     const auto one = [&](int i, int j) __attribute__((always_inline)) {

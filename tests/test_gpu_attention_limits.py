@@ -156,6 +156,24 @@ def test_nan_keys_that_are_all_of_a_piece(s3dx, dtype, lk, d, stretch, period):
 
 
 # ---------------------------------------------------------------------------
+# FP32: how close to 64 bits over many elements
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n,lk,heads,kv,d,top", [(100, 400, 2, 2, 64, 0), (200, 600, 2, 1, 32, 0), (100, 900, 2, 2, 64, 9), (3, 4000, 16, 4, 64, 30),
+                                                 (60, 500, 2, 2, 128, 0), (60, 500, 2, 2, 96, 5)])
+def test_float32_keeps_its_bits(s3dx, n, lk, heads, kv, d, top):
+    # Three terms a value leave at most 2^-21 of a product, 2^-24.5 in the mean: a score of d products of about
+    # 1.5 / sqrt(d) each is short by sqrt(d) 2^-21 at the very most, the values' products by 2^-21: 4e-6 in all, and less than
+    # 1e-6 with the mean.  Two terms (2^-14 of a product and more) give 3e-5.
+    rng = np.random.default_rng(n + d)
+    q, k, v = B.rows(rng, n, heads, d), B.rows(rng, lk, kv, d), B.rows(rng, lk, kv, d)
+    sel = B.choose(rng, [n], [lk], kv, 32, top) if top else None
+    got, lse, want = B.run_attend(s3dx, q, k, v, s3dx.F32, [n], [lk], 32, sel)
+    rel = np.linalg.norm(got - want[0]) / np.linalg.norm(want[0])
+    print(f"  rel-L2 {rel:.2e} over {got.size}", flush=True)
+    assert got.size > 2000 and rel <= 4e-6
+
+
+# ---------------------------------------------------------------------------
 # Norms of large rows
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [0, 1])
