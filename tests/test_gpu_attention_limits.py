@@ -200,3 +200,43 @@ def test_norms_of_rows_of_any_size(s3dx, dtype, d, pairs, adjacent, pad):
     # the sum of squares, its root, gain and scale, the turn (8 u), the output's rounding
     bound = ((d + 2) / 2 + 8 + 8 + 1) * R.U32 * (size + np.abs(want))
     assert np.all(off <= bound + 1e-37), np.argwhere(off > bound + 1e-37)[:4]
+
+
+# ---------------------------------------------------------------------------
+# Caches with room behind their keys
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("lens,room,heads,kv,d,block,top", [([150, 1, 190], 200, 8, 2, 128, 64, 2), ([3000, 2047, 64, 0], 3010, 4, 4, 64, 32, 20)])
+def test_single_rows_over_caches_that_grow(s3dx, dtype, lens, room, heads, kv, d, block, top):
+    # The room of a cache is a sequence without queries.  What it holds (NaN here) reaches nothing.
+    rng = np.random.default_rng(room)
+    b, lens = len(lens), list(lens)
+    k, v = np.full((b * room, kv, d), np.nan, np.float32), np.full((b * room, kv, d), np.nan, np.float32)
+    for s, n in enumerate(lens):
+        k[s * room: s * room + n], v[s * room: s * room + n] = B.rows(rng, n, kv, d), B.rows(rng, n, kv, d)
+    rows = s3dx.block_index_rows(b * room, 2 * b, block)
+    codes, scale = s3dx.DeviceArray((kv, rows, d), np.int8), s3dx.DeviceArray((kv, rows), np.float32)
+    qs = B.starts(s3dx, [1, 0] * b)
+    for step in range(3):
+        for s in range(b):   # a new key each
+            k[s * room + lens[s]], v[s * room + lens[s]] = B.rows(rng, 1, kv, d)[0], B.rows(rng, 1, kv, d)[0]
+            lens[s] += 1
+        q = B.rows(rng, b, heads, d)
+        (dq, q64), (dk, k64), (dv, v64) = ((R.dev(s3dx, st), val) for st, val in (R.stored(s3dx, a, dtype) for a in (q, k, v)))
+        ks = B.starts(s3dx, [n for s in range(b) for n in (lens[s], room - lens[s])])
+        s3dx.block_index(dk, dtype, b * room, kv, d, ks, 2 * b, block, codes, scale)
+        sel = R.filled(s3dx, (b, kv, top), np.int32, 0x5A)
+        s3dx.block_select(dq, dtype, b, b * room, heads, kv, d, qs, ks, 2 * b, block, top, max(lens), codes, scale, sel, causal=True, near=True)
+        real = np.concatenate([np.arange(s * room, s * room + n) for s, n in enumerate(lens)])
+        packed_k, packed_v = k64[real], v64[real]
+        c, power, _ = R.index_of(packed_k, lens, block)
+        want = R.select(q64, c, power, [1] * b, lens, block, top, True, True)
+        assert np.array_equal(sel.download(), want)
+        for chosen in (want, None):
+            n = 0 if chosen is None else top
+            o, lse = s3dx.DeviceArray((b, heads, d), R.store_type(s3dx, dtype)), s3dx.DeviceArray((b, heads), np.float32)
+            ws = s3dx.DeviceArray(max(1, s3dx.block_attention_workspace_size(b, heads, kv, d, 2 * b, block, n, max(lens))), np.uint8)
+            s3dx.block_attention(dq, dk, dv, dtype, b, b * room, heads, kv, d, qs, ks, 2 * b, block, max(lens), o, lse,
+                                 None if chosen is None else sel, n, causal=True, workspace=ws)
+            B.check(s3dx, dtype, R.values(s3dx, o, dtype), lse.download().astype(np.float64),
+                    R.attend(q64, packed_k, packed_v, [1] * b, lens, block, chosen, d ** -0.5, True, dtype == s3dx.BF16))
