@@ -660,9 +660,10 @@ __device__ __forceinline__ f32x4 product(const u32x4 (&x)[P], const u32x4 (&y)[P
 // all keys: 157 us so, 138 us turned; 144 us with V through LDS as well).  Statistics, scales and
 // masks are per query, hence per lane.
 //
-// What bounds it, at 134 us (791 TFLOP/s) for that call: a step of 64 rows and 32 keys is 32 products
-// of 16 cycles and about 150 vector instructions, among them 32 exponentials of 16, which take longer
-// than the products and cover them in part.
+// What bounds it, at 130-136 us (780-815 TFLOP/s) for that call: a step of 64 rows and 32 keys is 32 products of 16 cycles
+// and 166 vector instructions of about 800 cycles, 32 exponentials among them, and the two waves of a SIMD hardly cover
+// one's products with the other's weights: by the counters both together are 84% of all cycles.  A tile's start, join
+// and end cost about 11 us beside (16,384 rows: 865 TFLOP/s).
 //
 // The keys of a tile are those of any of its rows' blocks: a table in LDS gets, for each
 // block, a bit for each row that chose it; rows that did not take weights 0.

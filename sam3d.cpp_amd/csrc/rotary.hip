@@ -3,9 +3,10 @@
 //
 // Per head row x[0, d): y = x * rsqrt(mean(x^2) + eps) * gain, then each pair
 // (a, b) of channels turns by the angle p * f, p the row's position on the
-// pair's axis: (a cos - b sin, a sin + b cos).  The transformer blocks of the
-// SLat flow norm and turn their heads this way between the sparse blocks
-// (slat_flow_graph.cpp:304-434); the reference's graph has an op for each step.
+// pair's axis: (a cos - b sin, a sin + b cos).  For attention between the sparse
+// blocks (the SLat flow's place for it is slat_flow_graph.cpp:304-434) in models
+// whose heads carry their rows' places; the reference's own flow adds an absolute
+// embedding to its coarse rows instead (sparse_ops.cpp:49-173).
 #include <cmath>
 #include <vector>
 

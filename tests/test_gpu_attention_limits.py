@@ -1,5 +1,6 @@
 """GPU: attention and norms at the ends of their ranges: lists across the tables
-of a tile, values near the type's largest, scores of any size, NaN in one piece."""
+of a tile, values near the type's largest, scores of any size, NaN in one piece,
+caches with room behind their keys."""
 import numpy as np
 import pytest
 
