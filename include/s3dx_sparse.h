@@ -575,7 +575,8 @@ S3DX_API s3dx_status s3dx_block_select(const void *q, int32_t dtype, int64_t tot
  * its sequence where selected is NULL and top 0.  o [total_q][heads][head_dim] in
  * dtype by o_stride; lse (may be NULL): float32 [total_q][heads], the natural
  * logarithm of the row's sum of exp(score).  A row that sees no key, or only
- * scores of -inf, gets zeros and lse -inf; keys and values that a row does not
+ * scores of -inf (q k^T is in float32 before the scale, and counts as that below
+ * its range), gets zeros and lse -inf; keys and values that a row does not
  * see do not reach it, whatever they hold.  BF16 weights are rounded to bfloat16
  * before they meet the values (their sum and lse are of the weights before that),
  * FP32 ones are not (heads up to 64 wide: values whole, their products short by up to 2^-21,
