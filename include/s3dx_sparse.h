@@ -603,6 +603,105 @@ S3DX_API s3dx_status s3dx_block_attention(const void *q, const void *k, const vo
                                           void *workspace, uint64_t workspace_bytes, s3dx_stream stream, char *error,
                                           uint64_t error_capacity);
 
+/* ------------------------------------------------------------------------
+ * Rows over a cache in 8 bits.  For models that answer row by row, or chunk by
+ * chunk: what earlier rows left as keys and values stays in pages, and new
+ * rows are written behind it and attend to it.  The reference keeps no such state
+ * (its blocks attend within one forward, slat_flow_graph.cpp:304-434); the calls
+ * stand beside the attention over packed rows above and share its conventions.
+ *
+ * A cache is one caller-owned device buffer of s3dx_cache_size bytes (16-byte aligned): a
+ * page holds `block` (64 or 128) rows of all key heads.  In it
+ *   codes  uint8 [pages][kv_heads][2][block * head_dim]: of each head first the keys'
+ *          ([block][head_dim]), then the values' ([head_dim][block])
+ *   steps  float32 [pages][kv_heads][2] (keys', values'), behind the codes
+ * and a code u stands for (u - 128) * step.  head_dim is 32, 64, 96 or 128.  The object is
+ * host memory alone and may be used by any number of calls at once.
+ *
+ * Which pages a sequence has is the caller's: table is a DEVICE int32 [sequences][table_stride],
+ * block j of sequence s lies in page table[s*table_stride + j], and lengths, a DEVICE int32
+ * [sequences], is how many rows it has, new ones among them (cut to 0 .. table_stride * block, at
+ * most 2^29).  The new rows are packed (starts, as above): of a sequence's n rows and length l
+ * row i stands at place i + l - n, the last row at the last place.  Pages of two sequences may be
+ * the same for reading.
+ *
+ * Nothing here allocates device memory or synchronizes; lengths and table are read when the
+ * work runs, so a captured call goes on with what stands in them. */
+typedef struct s3dx_cache s3dx_cache;
+S3DX_API s3dx_status s3dx_cache_size(int32_t pages, int32_t kv_heads, int32_t head_dim, int32_t block, uint64_t *bytes,
+                                     char *error, uint64_t error_capacity);
+S3DX_API s3dx_status s3dx_cache_create(void *buffer, int32_t pages, int32_t kv_heads, int32_t head_dim, int32_t block,
+                                       s3dx_cache **out, char *error, uint64_t error_capacity);
+S3DX_API void s3dx_cache_free(s3dx_cache *cache);
+/* Quantises the rows k, v [total][kv_heads][head_dim] (F32 or BF16, strides in elements, whole
+ * 16-byte pieces) into their places.  For each block and head, keys and values apart: with 2^e <=
+ * most < 2^(e+1), most the largest finite magnitude of the rows written to it, the step is 2^(e-6)
+ * (0 for most below 2^-100), and a value's code 128 + round(x / step), halves to even, cut to 1 .. 255; NaN is
+ * written as 0 and infinities as the ends.  A block that holds earlier rows keeps its step, or, where
+ * the new rows need a larger one, has its codes rounded to that.  A block whose first place is
+ * among the new rows' begins afresh: what its page held does not count.  Places behind a sequence's last
+ * row hold nothing of use.  Rows before place 0, or whose page is not one of the cache's, are not written.
+ * Pages that one call writes to must be distinct. */
+S3DX_API s3dx_status s3dx_cache_write(const s3dx_cache *cache, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                                      int32_t dtype, int64_t total, const int32_t *starts, const int32_t *table,
+                                      int32_t table_stride, const int32_t *lengths, int64_t sequences, s3dx_stream stream,
+                                      char *error, uint64_t error_capacity);
+/* The values that the cache holds for the same rows, into k and v: each sequence's last n
+ * places (exact in either type, but below float32's and bfloat16's normal range).  Rows that it does not
+ * hold are zeros. */
+S3DX_API s3dx_status s3dx_cache_read(const s3dx_cache *cache, void *k, int64_t k_stride, void *v, int64_t v_stride, int32_t dtype,
+                                     int64_t total, const int32_t *starts, const int32_t *table, int32_t table_stride,
+                                     const int32_t *lengths, int64_t sequences, s3dx_stream stream, char *error,
+                                     uint64_t error_capacity);
+/* o = softmax(softmax_scale * q k^T) v over the cached rows of each query row's sequence, query head h
+ * reading key head h / (heads / kv_heads).  With S3DX_BLOCK_CAUSAL a row at place p sees places up to p; with
+ * window > 0 (causal only) those from p - window + 1 on, and of the ones before them the first `sinks`.  Keys on pages that are not the
+ * cache's count for nothing.  o [total_q][heads][head_dim] in dtype by o_stride, overlapping no input;
+ * lse (may be NULL): float32 [total_q][heads], the natural logarithm of the row's sum of exp(score).  A row that sees no
+ * key, or only scores of -inf, gets zeros and lse -inf; one with a query that is not finite, or with a score past float32's
+ * range, NaN.
+ * Keys and values enter the products as they are held.  A query's channels do so in units of 2^-38 of its row's largest
+ * power of two, BF16 ones exactly from 2^-31 of it on, FP32 ones to 22 bits (2^-22 off at most).  Weights meet the values
+ * rounded to 11 bits (2^-11 off at most, of either sign), with FP32 queries to 22, and in steps of 2^-31 of the row's largest
+ * at most; their sum and lse are of the weights before that.
+ * max_k, the keys of the longest sequence, decides how the work is cut and not what is computed.  The
+ * workspace holds partial results where there are too few rows to fill the GPU
+ * (s3dx_cache_attention_workspace_size of the same arguments, 0 bytes where none are needed); calls that may run at
+ * the same time need one each.  Deterministic. */
+S3DX_API s3dx_status s3dx_cache_attention_workspace_size(const s3dx_cache *cache, int64_t total_q, int32_t heads, int64_t sequences,
+                                                         int64_t max_k, int32_t window, int32_t sinks, uint64_t *bytes,
+                                                         char *error, uint64_t error_capacity);
+S3DX_API s3dx_status s3dx_cache_attention(const s3dx_cache *cache, const void *q, int32_t dtype, int64_t total_q, int32_t heads,
+                                          int64_t q_stride, const int32_t *q_starts, const int32_t *table, int32_t table_stride,
+                                          const int32_t *lengths, int64_t sequences, int64_t max_k, int32_t window,
+                                          int32_t sinks, float softmax_scale, int32_t flags, void *o, int64_t o_stride,
+                                          float *lse, void *workspace, uint64_t workspace_bytes, s3dx_stream stream, char *error,
+                                          uint64_t error_capacity);
+
+/* The step between two branches of a block, in one pass (slat_flow_graph.cpp:304-434 has it as
+ * separate ops: gate, sum, norm, modulate):
+ *   y = x + residual_scale * gate . post(branch)
+ *   h = pre(y) . (1 + mod_scale) + mod_shift
+ * post and pre: S3DX_NORM_NONE, S3DX_NORM_LAYER ((v - mean) / sqrt(var + eps)) or S3DX_NORM_RMS
+ * (v / sqrt(mean(v^2) + eps)), times w, plus b (device float32 [c], each may be NULL).  gate (NULL: 1),
+ * mod_scale and mod_shift (NULL: 0): device float32, channel j of set i at i*mod_stride + j, so
+ * that they may lie side by side in one projection's output; a row's set is
+ * sets[row*set_stride] (int32; the batch of voxel coordinates: coords, stride 4), or 0 for all
+ * rows where sets is NULL.  Rows with a set outside [0, set_count) take gate, scale and shift as 0 (those that
+ * are given).  x and y are in x_dtype, 1 <= c <= 16384; strides in elements, any.  h is
+ * of y before its rounding; h NULL: the sum alone, without pre.  All in float32, each output rounded once.  y and h may
+ * be x or branch (same dtype and stride) and overlap nothing otherwise. */
+#define S3DX_NORM_NONE 0
+#define S3DX_NORM_LAYER 1
+#define S3DX_NORM_RMS 2
+S3DX_API s3dx_status s3dx_gated_norm_rows(const void *x, int32_t x_dtype, int64_t x_stride, const void *branch, int32_t branch_dtype,
+                                          int64_t branch_stride, int64_t n, int32_t c, int32_t post, const float *post_w,
+                                          const float *post_b, float residual_scale, const float *gate, int32_t pre,
+                                          const float *pre_w, const float *pre_b, const float *mod_scale, const float *mod_shift,
+                                          int64_t mod_stride, const int32_t *sets, int64_t set_stride, int32_t set_count, float eps,
+                                          void *y, int64_t y_stride, void *h, int32_t h_dtype, int64_t h_stride, s3dx_stream stream,
+                                          char *error, uint64_t error_capacity);
+
 #ifdef __cplusplus
 }
 #endif

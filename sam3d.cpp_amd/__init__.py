@@ -10,6 +10,8 @@ operator interface for this path:
                                        mesh_decoder_graph.cpp:81-103 convolution
   Rotary, qk_norm_rotary, block_*      the attention over voxel rows between
                                        the sparse blocks (slat_flow_graph.cpp:304-434)
+  KvCache, gated_norm_rows             rows over a cache in 8 bits, and the step
+                                       between two branches of such a block
 
 Device memory is plain device pointers owned by DeviceArray.  There is no
 fallback: if the HIP library cannot be loaded, import fails loudly.
@@ -36,6 +38,9 @@ ROTARY_ADJACENT = 0
 ROTARY_HALVES = 1
 BLOCK_CAUSAL = 1
 BLOCK_NEAR = 2
+NORM_NONE = 0
+NORM_LAYER = 1
+NORM_RMS = 2
 
 OK, INVALID_ARGUMENT, OUT_OF_MEMORY, INTERNAL_ERROR = 0, 1, 2, 3
 
@@ -118,6 +123,16 @@ SIGNATURES = {
                                             True),
     "s3dx_block_attention": (_u32, [_vp, _vp, _vp, _i32, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _vp, _vp, _i64,
                                     _i32, _i64, _vp, _i32, _f32, _i32, _vp, _i64, _vp, _vp, _u64, _vp], True),
+    "s3dx_cache_size": (_u32, [_i32, _i32, _i32, _i32, C.POINTER(_u64)], True),
+    "s3dx_cache_create": (_u32, [_vp, _i32, _i32, _i32, _i32, C.POINTER(_vp)], True),
+    "s3dx_cache_free": (None, [_vp], False),
+    "s3dx_cache_write": (_u32, [_vp, _vp, _i64, _vp, _i64, _i32, _i64, _vp, _vp, _i32, _vp, _i64, _vp], True),
+    "s3dx_cache_read": (_u32, [_vp, _vp, _i64, _vp, _i64, _i32, _i64, _vp, _vp, _i32, _vp, _i64, _vp], True),
+    "s3dx_cache_attention_workspace_size": (_u32, [_vp, _i64, _i32, _i64, _i64, _i32, _i32, C.POINTER(_u64)], True),
+    "s3dx_cache_attention": (_u32, [_vp, _vp, _i32, _i64, _i32, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i32, _i32, _f32, _i32,
+                                    _vp, _i64, _vp, _vp, _u64, _vp], True),
+    "s3dx_gated_norm_rows": (_u32, [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i32, _i32, _vp, _vp, _f32, _vp, _i32, _vp, _vp, _vp,
+                                    _vp, _i64, _vp, _i64, _i32, _f32, _vp, _i64, _vp, _i32, _i64, _vp], True),
 }
 
 _lib = None
@@ -761,6 +776,80 @@ def block_attention(q, k, v, dtype, total_q, total_k, heads, kv_heads, head_dim,
          _addr(selected), top, head_dim ** -0.5 if scale is None else scale, BLOCK_CAUSAL if causal else 0, _addr(o),
          heads * head_dim if o_stride is None else o_stride, _addr(lse), _addr(workspace), workspace_bytes,
          _handle(stream))
+
+
+# ---------------------------------------------------------------------------
+# Rows over a cache in 8 bits
+# ---------------------------------------------------------------------------
+class KvCache:
+    """Keys and values in pages of 8-bit codes with a step for each block of rows and head (s3dx_cache).  `buffer` is device
+    memory of KvCache.size bytes; table int32 [sequences][table_stride] says which pages a sequence has, lengths
+    int32 [sequences] how many rows, new ones among them."""
+
+    def __init__(self, buffer, pages: int, kv_heads: int, head_dim: int, block: int = 64):
+        self.handle = None
+        p = _vp()
+        call("s3dx_cache_create", _addr(buffer), pages, kv_heads, head_dim, block, C.byref(p))
+        self.handle = p.value
+        self.buffer, self.pages, self.kv_heads, self.head_dim, self.block = buffer, pages, kv_heads, head_dim, block
+
+    @staticmethod
+    def size(pages: int, kv_heads: int, head_dim: int, block: int = 64) -> int:
+        b = _u64(0)
+        call("s3dx_cache_size", pages, kv_heads, head_dim, block, C.byref(b))
+        return int(b.value)
+
+    def write(self, k, v, dtype, total, starts, table, table_stride, lengths, sequences, k_stride=None, v_stride=None, stream=None):
+        """Quantises new rows into their sequences' last places (s3dx_cache_write)."""
+        row = self.kv_heads * self.head_dim
+        call("s3dx_cache_write", self.handle, _addr(k), row if k_stride is None else k_stride, _addr(v),
+             row if v_stride is None else v_stride, dtype, total, _addr(starts), _addr(table), table_stride, _addr(lengths),
+             sequences, _handle(stream))
+
+    def read(self, k, v, dtype, total, starts, table, table_stride, lengths, sequences, k_stride=None, v_stride=None, stream=None):
+        """The values of each sequence's last rows, into k and v (s3dx_cache_read)."""
+        row = self.kv_heads * self.head_dim
+        call("s3dx_cache_read", self.handle, _addr(k), row if k_stride is None else k_stride, _addr(v),
+             row if v_stride is None else v_stride, dtype, total, _addr(starts), _addr(table), table_stride, _addr(lengths),
+             sequences, _handle(stream))
+
+    def attention_workspace_size(self, total_q, heads, sequences, max_k, window=0, sinks=0) -> int:
+        b = _u64(0)
+        call("s3dx_cache_attention_workspace_size", self.handle, total_q, heads, sequences, max_k, window, sinks, C.byref(b))
+        return int(b.value)
+
+    def attention(self, q, dtype, total_q, heads, q_starts, table, table_stride, lengths, sequences, max_k, o, lse=None,
+                  q_stride=None, o_stride=None, scale=None, causal=False, window=0, sinks=0, workspace=None, workspace_bytes=None,
+                  stream=None):
+        """softmax(scale q k^T) v over the cached rows (s3dx_cache_attention); scale: head_dim^-0.5 unless given."""
+        if workspace_bytes is None:
+            workspace_bytes = workspace.nbytes if isinstance(workspace, DeviceArray) else 0
+        row = heads * self.head_dim
+        call("s3dx_cache_attention", self.handle, _addr(q), dtype, total_q, heads, row if q_stride is None else q_stride,
+             _addr(q_starts), _addr(table), table_stride, _addr(lengths), sequences, max_k, window, sinks,
+             self.head_dim ** -0.5 if scale is None else scale, BLOCK_CAUSAL if causal else 0, _addr(o),
+             row if o_stride is None else o_stride, _addr(lse), _addr(workspace), workspace_bytes, _handle(stream))
+
+    def __del__(self):
+        try:
+            if self.handle:
+                lib().s3dx_cache_free(_vp(self.handle))
+        except Exception:
+            pass
+
+
+def gated_norm_rows(x, x_dtype, branch, branch_dtype, n, c, eps, y=None, h=None, h_dtype=None, post=NORM_NONE, pre=NORM_NONE,
+                    post_w=None, post_b=None, pre_w=None, pre_b=None, residual_scale=1.0, gate=None, mod_scale=None, mod_shift=None,
+                    mod_stride=None, sets=None, set_stride=1, set_count=1, x_stride=None, branch_stride=None, y_stride=None,
+                    h_stride=None, stream=None):
+    """y (default: x itself) = x + residual_scale * gate * post(branch), h = pre(y) * (1 + mod_scale) + mod_shift
+    (s3dx_gated_norm_rows)."""
+    xs = c if x_stride is None else x_stride
+    call("s3dx_gated_norm_rows", _addr(x), x_dtype, xs, _addr(branch), branch_dtype, c if branch_stride is None else branch_stride,
+         n, c, post, _addr(post_w), _addr(post_b), residual_scale, _addr(gate), pre, _addr(pre_w), _addr(pre_b), _addr(mod_scale),
+         _addr(mod_shift), c if mod_stride is None else mod_stride, _addr(sets), set_stride, set_count, eps,
+         _addr(x if y is None else y), y_stride if y_stride is not None else (xs if y is None else c), _addr(h),
+         branch_dtype if h_dtype is None else h_dtype, c if h_stride is None else h_stride, _handle(stream))
 
 
 def synchronize(stream=None):

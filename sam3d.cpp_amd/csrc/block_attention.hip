@@ -6,53 +6,10 @@
 #include <cmath>
 #include <type_traits>
 
-#include "common.hpp"
+#include "packed_rows.hpp"
 
 namespace s3dx {
 namespace {
-
-// ---------------------------------------------------------------------------
-// Packed sequences
-// ---------------------------------------------------------------------------
-struct Span {
-    int64_t begin;
-    int32_t rows;
-};
-// Rows [begin, begin + rows) of sequence s, cut to [0, total].
-__device__ __forceinline__ Span sequence_span(const int32_t *starts, int64_t s, int64_t total) {
-    const int64_t lo = min(max(static_cast<int64_t>(starts[s]), INT64_C(0)), total);
-    const int64_t hi = min(max(static_cast<int64_t>(starts[s + 1]), lo), total);
-    return {lo, static_cast<int32_t>(hi - lo)};
-}
-
-// The last sequence that begins at or before `unit`, by the whole wave: 64 beginnings at a
-// time, so one trip to memory for up to 64 sequences and two for 4,096.
-template <class F>
-__device__ __forceinline__ int64_t last_sequence(int64_t sequences, int64_t unit, F &&begin) {
-    const int lane = threadIdx.x & 63;
-    int64_t lo = 0, hi = sequences;  // begin(lo) <= unit < begin(hi)
-    while (hi - lo > 1) {
-        const int64_t step = (hi - lo + 63) >> 6, at = lo + lane * step;
-        const bool before = lane == 0 || (at < hi && begin(at) <= unit);
-        lo += (__popcll(__builtin_amdgcn_ballot_w64(before)) - 1) * step;
-        hi = min(hi, lo + step);
-    }
-    return lo;
-}
-// The sequence of a tile, where sequence s begins at tile (starts[s] * mul >> shift) + s: every
-// sequence has room for its last, partial tile, and the beginnings rise with s, empty
-// sequences or not.
-__device__ __forceinline__ int64_t sequence_of_unit(const int32_t *starts, int64_t sequences, int64_t total,
-                                                    int64_t mul, int shift, int64_t unit) {
-    return last_sequence(sequences, unit, [&](int64_t s) {
-        return (min(max(static_cast<int64_t>(starts[s]), INT64_C(0)), total) * mul >> shift) + s;
-    });
-}
-// The sequence that holds row `row`, or -1.
-__device__ __forceinline__ int64_t sequence_of_row(const int32_t *starts, int64_t sequences, int64_t row) {
-    const int64_t s = last_sequence(sequences, row, [&](int64_t at) { return static_cast<int64_t>(starts[at]); });
-    return starts[s] <= row && row < starts[s + 1] ? s : -1;
-}
 
 // ---------------------------------------------------------------------------
 // 8-bit codes.  2^e <= most < 2^(e+1): x * 2^(6-e) is exact, the rounding to a
@@ -453,8 +410,6 @@ struct AttendArgs {
     float2 *part_ml; // [splits][total_q][heads]: the power of two that weights are relative to, their sum
 };
 
-constexpr float kLn2 = 0.693147180559945309f;
-constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kMostBase = 0x1p24f;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -462,32 +417,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
-
-// (A vector's element goes through a variable of its own: a bit cast of the element as it stands
-// reads the first one.)
-__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
-
-// Largest over the lanes l, l ^ 16, l ^ 32, l ^ 48.
-__device__ __forceinline__ float max_over_groups(float v) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const float m = fmaxf(as_float(a[0]), as_float(a[1]));
-    const uint32_t w = __builtin_bit_cast(uint32_t, m);
-    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return fmaxf(as_float(b[0]), as_float(b[1]));
-}
-
-// Sum over the same lanes.
-__device__ __forceinline__ float sum_over_groups(float v) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const float m = as_float(a[0]) + as_float(a[1]);
-    const uint32_t w = __builtin_bit_cast(uint32_t, m);
-    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return as_float(b[0]) + as_float(b[1]);
-}
 
 // Binary orders by which weights over `keys` keys are kept down, so that sums of finite values stay finite whatever the
 // values: weights pass 1 by 8 orders and a base's rounding before that moves, and there are as many as keys.  Where

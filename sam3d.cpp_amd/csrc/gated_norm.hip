@@ -1,0 +1,261 @@
+// The step between two branches of a transformer block, in one pass: the
+// branch's own norm, its gate and the sum with the stream, and the norm and
+// modulation that the next branch begins with (slat_flow_graph.cpp:304-434 runs
+// them one by one).
+//
+//   y = x + residual_scale gate . post(branch),   h = pre(y) . (1 + scale) + shift
+//
+// What bounds it: memory.  A row is held in registers between its parts, so that x and
+// branch are read once and y and h written once.
+#include "common.hpp"
+
+namespace s3dx {
+namespace {
+
+struct NormArgs {
+    const void *x, *branch;
+    void *y, *h;  // h NULL: the sum alone
+    const float *post_w, *post_b, *pre_w, *pre_b, *gate, *scale, *shift;
+    const int32_t *sets;
+    int64_t first, n, x_stride, branch_stride, y_stride, h_stride, mod_stride, set_stride;
+    int32_t c, set_count, post, pre, x_bf, branch_bf, h_bf, lanes_log2;
+    float eps, residual_scale;
+};
+
+// Rows whose squares' sum passes 2^128 are summed again smaller; eps is nothing beside them.
+constexpr float kLess = 0x1p-70f;
+
+// Sum over a row's threads: 2^lanes_log2 lanes of a wave, or all of a workgroup.
+template <bool WIDE>
+__device__ __forceinline__ float row_sum(float v, int lanes_log2, float *across) {
+    for (int o = 1; o < (WIDE ? 64 : 1 << lanes_log2); o <<= 1) v += __shfl_xor(v, o, 64);
+    if constexpr (WIDE) {
+        __syncthreads();  // the last sum's is read
+        if ((threadIdx.x & 63) == 0) across[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = (across[0] + across[1]) + (across[2] + across[3]);
+    }
+    return v;
+}
+
+// Piece p of a thread's: 8 channels side by side where rows are whole 16-byte pieces; else the p-th run of 8
+// times the threads, a thread's channels as far apart as there are threads.
+template <int PPL, bool WIDE, bool VEC>
+__global__ void __launch_bounds__(256) gated_norm_kernel(NormArgs a) {
+    __shared__ float across[4];
+    const int threads = WIDE ? 256 : 1 << a.lanes_log2;
+    const int t = threadIdx.x & (threads - 1), rows = 256 / threads;
+    const int64_t row = a.first + static_cast<int64_t>(blockIdx.x) * rows + (WIDE ? 0 : threadIdx.x >> a.lanes_log2);
+    if (row >= a.n) return;  // WIDE: the whole workgroup
+    const auto channel = [&](int p, int e) { return VEC ? (p * threads + t) * 8 + e : (p * 8 + e) * threads + t; };
+    const auto load = [&](const void *base, int64_t at, bool bf, float (&v)[PPL][8]) __attribute__((always_inline)) {
+        if (VEC) {
+#pragma unroll
+            for (int p = 0; p < PPL; ++p) {
+                const int c = channel(p, 0);
+                if (c >= a.c) continue;
+                if (bf) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + at + c);
+                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[p][e] = __builtin_bit_cast(float, e & 1 ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16);
+                } else {
+                    const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at + c);
+                    const float4 lo = f[0], hi = f[1];
+                    v[p][0] = lo.x, v[p][1] = lo.y, v[p][2] = lo.z, v[p][3] = lo.w;
+                    v[p][4] = hi.x, v[p][5] = hi.y, v[p][6] = hi.z, v[p][7] = hi.w;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int p = 0; p < PPL; ++p)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int c = channel(p, e);
+                    if (c < a.c) v[p][e] = bf ? bf16_to_f32(static_cast<const uint16_t *>(base)[at + c]) : static_cast<const float *>(base)[at + c];
+                }
+        }
+    };
+    const auto store = [&](void *base, int64_t at, bool bf, const float (&v)[PPL][8]) __attribute__((always_inline)) {
+        if (VEC) {
+#pragma unroll
+            for (int p = 0; p < PPL; ++p) {
+                const int c = channel(p, 0);
+                if (c >= a.c) continue;
+                if (bf) {
+                    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(base) + at + c) =
+                        make_uint4(pack_bf16x2(v[p][0], v[p][1]), pack_bf16x2(v[p][2], v[p][3]), pack_bf16x2(v[p][4], v[p][5]),
+                                   pack_bf16x2(v[p][6], v[p][7]));
+                } else {
+                    float4 *f = reinterpret_cast<float4 *>(static_cast<float *>(base) + at + c);
+                    f[0] = make_float4(v[p][0], v[p][1], v[p][2], v[p][3]);
+                    f[1] = make_float4(v[p][4], v[p][5], v[p][6], v[p][7]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int p = 0; p < PPL; ++p)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int c = channel(p, e);
+                    if (c >= a.c) continue;
+                    if (bf) static_cast<uint16_t *>(base)[at + c] = f32_to_bf16(v[p][e]);
+                    else static_cast<float *>(base)[at + c] = v[p][e];
+                }
+        }
+    };
+    const auto each = [&](auto &&f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < PPL; ++p)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (channel(p, e) < a.c) f(p, e);
+    };
+    const auto norm = [&](float (&v)[PPL][8], int kind, const float *w, const float *b) __attribute__((always_inline)) {
+        if (kind == S3DX_NORM_NONE) return;
+        float less = 1.0f, mean, rstd;
+        for (;;) {
+            mean = 0.0f;
+            if (kind == S3DX_NORM_LAYER) {
+                each([&](int p, int e) { mean += v[p][e] * less; });
+                mean = row_sum<WIDE>(mean, a.lanes_log2, across) / static_cast<float>(a.c);
+            }
+            float q = 0.0f;
+            each([&](int p, int e) {
+                const float d = v[p][e] * less - mean;
+                q += d * d;
+            });
+            q = row_sum<WIDE>(q, a.lanes_log2, across);
+            // the same for the row's threads (a wave may hold several rows: those that are through wait)
+            if (q < __builtin_inff() || less != 1.0f) {
+                rstd = rsqrtf(q / static_cast<float>(a.c) + (less == 1.0f ? a.eps : 0.0f));
+                break;
+            }
+            less = kLess;
+        }
+        float g[PPL][8];
+        each([&](int p, int e) { v[p][e] = (v[p][e] * less - mean) * rstd; });
+        if (w) {
+            load(w, 0, false, g);
+            each([&](int p, int e) { v[p][e] *= g[p][e]; });
+        }
+        if (b) {
+            load(b, 0, false, g);
+            each([&](int p, int e) { v[p][e] += g[p][e]; });
+        }
+    };
+
+    const int32_t set = a.sets ? a.sets[row * a.set_stride] : 0;
+    const bool in = set >= 0 && set < a.set_count;  // rows of no set: gate, scale and shift 0
+    const int64_t mods = in ? set * a.mod_stride : 0;
+    float v[PPL][8], y[PPL][8], g[PPL][8];
+    load(a.branch, row * a.branch_stride, a.branch_bf, v);
+    load(a.x, row * a.x_stride, a.x_bf, y);
+    norm(v, a.post, a.post_w, a.post_b);
+    if (a.gate) {
+        load(a.gate, mods, false, g);
+        each([&](int p, int e) { v[p][e] *= in ? g[p][e] : 0.0f; });
+    }
+    each([&](int p, int e) { y[p][e] = fmaf(v[p][e], a.residual_scale, y[p][e]); });
+    store(a.y, row * a.y_stride, a.x_bf, y);
+    if (!a.h) return;
+    norm(y, a.pre, a.pre_w, a.pre_b);
+    if (in && a.scale) {
+        load(a.scale, mods, false, g);
+        each([&](int p, int e) { y[p][e] = fmaf(y[p][e], g[p][e], y[p][e]); });
+    }
+    if (in && a.shift) {
+        load(a.shift, mods, false, g);
+        each([&](int p, int e) { y[p][e] += g[p][e]; });
+    }
+    store(a.h, row * a.h_stride, a.h_bf, y);
+}
+
+constexpr int32_t kMostChannels = 16384;
+
+using NormFn = void (*)(NormArgs);
+template <bool WIDE, bool VEC>
+NormFn pick_pieces(int per) {
+    if (per <= 1) return gated_norm_kernel<1, WIDE, VEC>;
+    if (per <= 2) return gated_norm_kernel<2, WIDE, VEC>;
+    if (per <= 4) return gated_norm_kernel<4, WIDE, VEC>;
+    return gated_norm_kernel<8, WIDE, VEC>;
+}
+
+void check_rows(const void *p, int64_t stride, int64_t n, int32_t c, int32_t dtype, const char *what) {
+    const std::string name(what);
+    require_dtype(dtype);
+    require(stride >= c && stride <= (INT64_C(1) << 40), (name + ": the row stride is out of range (channels to 2^40)").c_str());
+    require(n == 0 || (p && aligned(p, dtype_size(dtype))), (name + " is NULL or not aligned to its elements").c_str());
+}
+bool whole_pieces(const void *p, int64_t stride, int32_t dtype) { return aligned(p, 16) && stride * dtype_size(dtype) % 16 == 0; }
+
+}  // namespace
+}  // namespace s3dx
+
+using namespace s3dx;
+
+extern "C" {
+
+S3DX_API s3dx_status s3dx_gated_norm_rows(const void *x, int32_t x_dtype, int64_t x_stride, const void *branch, int32_t branch_dtype,
+                                          int64_t branch_stride, int64_t n, int32_t c, int32_t post, const float *post_w,
+                                          const float *post_b, float residual_scale, const float *gate, int32_t pre,
+                                          const float *pre_w, const float *pre_b, const float *mod_scale, const float *mod_shift,
+                                          int64_t mod_stride, const int32_t *sets, int64_t set_stride, int32_t set_count, float eps,
+                                          void *y, int64_t y_stride, void *h, int32_t h_dtype, int64_t h_stride, s3dx_stream stream,
+                                          char *error, uint64_t error_capacity) {
+    return boundary(error, error_capacity, [&] {
+        require(n >= 0 && n <= std::numeric_limits<int32_t>::max(), "n is out of range");
+        require(c >= 1 && c <= kMostChannels, "c must be 1 to 16384");
+        for (int32_t kind : {post, pre})
+            require(kind == S3DX_NORM_NONE || kind == S3DX_NORM_LAYER || kind == S3DX_NORM_RMS, "unknown norm");
+        require(post != S3DX_NORM_NONE || (!post_w && !post_b), "post_w or post_b without a norm");
+        require(pre != S3DX_NORM_NONE || (!pre_w && !pre_b), "pre_w or pre_b without a norm");
+        require(h || (pre == S3DX_NORM_NONE && !mod_scale && !mod_shift), "h is NULL beside a norm or modulation of it");
+        require(eps > 0.0f && eps <= 1.0f, "eps must be above 0 and at most 1");
+        require(std::abs(residual_scale) < std::numeric_limits<float>::infinity(), "residual_scale is not finite");
+        check_rows(x, x_stride, n, c, x_dtype, "x");
+        check_rows(branch, branch_stride, n, c, branch_dtype, "branch");
+        check_rows(y, y_stride, n, c, x_dtype, "y");
+        if (h) check_rows(h, h_stride, n, c, h_dtype, "h");
+        const bool mods = gate || mod_scale || mod_shift;
+        if (sets) {
+            require(aligned(sets, 4) && set_stride >= 1 && set_stride <= (INT64_C(1) << 31), "sets is not aligned, or set_stride out of range");
+            require(set_count >= 0, "set_count is out of range");
+        }
+        require(!mods || !sets || set_count == 0 || (mod_stride >= c && mod_stride <= (INT64_C(1) << 40)), "mod_stride is shorter than c, or above 2^40");
+        for (const float *p : {post_w, post_b, pre_w, pre_b, gate, mod_scale, mod_shift}) require(aligned(p, 4), "a vector is not aligned");
+        if (n == 0) return;
+        // y and h may lie where x or branch does, row by row
+        const auto beside = [&](const void *out, int64_t out_stride, int32_t out_dtype, const void *in, int64_t in_stride, int32_t in_dtype) {
+            require(out != in || (out_dtype == in_dtype && (n == 1 || out_stride == in_stride)), "in place needs the same dtype and stride");
+        };
+        beside(y, y_stride, x_dtype, x, x_stride, x_dtype);
+        beside(y, y_stride, x_dtype, branch, branch_stride, branch_dtype);
+        if (h) {
+            beside(h, h_stride, h_dtype, x, x_stride, x_dtype);
+            beside(h, h_stride, h_dtype, branch, branch_stride, branch_dtype);
+            require(h != y, "h and y are the same");
+        }
+        NormArgs a = {x, branch, y, h, post_w, post_b, pre_w, pre_b, gate, mod_scale, mod_shift, sets, 0, n, x_stride, branch_stride,
+                      y_stride, h_stride, sets ? mod_stride : 0, set_stride, c, sets ? set_count : 1, post, pre, x_dtype == S3DX_BF16,
+                      branch_dtype == S3DX_BF16, h_dtype == S3DX_BF16, 0, eps, residual_scale};
+        bool vec = c % 8 == 0 && whole_pieces(x, x_stride, x_dtype) && whole_pieces(branch, branch_stride, branch_dtype) &&
+                   whole_pieces(y, y_stride, x_dtype) && (!h || whole_pieces(h, h_stride, h_dtype)) && a.mod_stride % 4 == 0;
+        for (const float *p : {post_w, post_b, pre_w, pre_b, gate, mod_scale, mod_shift}) vec = vec && aligned(p, 16);
+        const bool wide = c > 64 * 8 * 4;
+        while (!wide && a.lanes_log2 < 6 && (8 << a.lanes_log2) < c) ++a.lanes_log2;
+        const int threads = wide ? 256 : 1 << a.lanes_log2, per = (c + 8 * threads - 1) / (8 * threads), rows = 256 / threads;
+        const NormFn fn = wide ? (vec ? pick_pieces<true, true>(per) : pick_pieces<true, false>(per))
+                               : (vec ? pick_pieces<false, true>(per) : pick_pieces<false, false>(per));
+        // a launch's threads stay below 2^32
+        const int64_t most = rows * (INT64_C(1) << 23);
+        for (; a.first < n; a.first += most) {
+            a.n = std::min(n, a.first + most);
+            fn<<<dim3(static_cast<unsigned>((a.n - a.first + rows - 1) / rows)), dim3(256), 0, as_stream(stream)>>>(a);
+        }
+        launch_check("gated norm");
+    });
+}
+
+}  // extern "C"
