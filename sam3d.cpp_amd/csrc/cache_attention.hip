@@ -26,7 +26,7 @@ struct AttendArgs {
     int32_t heads, group, causal, window, sinks, splits, tile_groups;
     float scale;
     float *part_o;    // [splits][total_q][heads][d], divided by their sums
-    float4 *part_ml;  // [splits][total_q][heads]: see Sum
+    float4 *part_ml;  // [splits][total_q][heads]: see sum_of
 };
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -82,364 +82,511 @@ __device__ __forceinline__ f32x4 product(const u32x4 &a, const u32x4 &b, f32x4 d
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), d, 0, 0, 0);
 }
 
-// Attention of a tile of 16 NS rows (query rows times the heads that share a key head).  A
-// wave computes S^T = K Q^T and O^T = V^T P^T, so that what one product leaves in a
-// lane is what the next one wants there.  A 16x16 product leaves lane (c, g) = (lane & 15, lane >> 4) with rows 4g..4g+3 of
-// column c; product t of a step takes key 16 (c >> 2) + 4t + (c & 3) as its row c, so that lane
-// (c, g) gets keys 16g + 4t + i of query c: the lane's 16 weights are of keys 16g..16g+15, and the
-// values' operand wants the same keys of a channel: one 16-byte piece of the cache, as it lies.
-// The keys' operand wants channels of a row, in any order that the queries share: 16 side by side for two products.
-// So codes go from memory to a product's registers through two instructions for every four, without LDS.
-//
-// SHARES 4: the workgroup's waves take every fourth step of a tile each, and join through LDS; 1: a tile each.
-template <class T, int D, int NS, int SHARES>
-__global__ void __launch_bounds__(256, 2) cache_attend_kernel(AttendArgs a) {
-    constexpr bool BF = sizeof(T) == 2;
-    constexpr int P = BF ? 1 : 2;      // half-precision terms of a query's channel and of a weight
-    constexpr int ROWS = 16 * NS, KT = kStep / 16;
-    constexpr int QV = D / 32, C = D / 16;
-    constexpr int KD = D / 16;         // dwords of a key row that a lane reads
-    __shared__ float part[SHARES == 4 ? 4 : 1][SHARES == 4 ? NS * 4 * C : 1][64];
-    __shared__ float4 part_ml[SHARES == 4 ? 4 : 1][NS][16];
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // consecutive workgroups of one XCD run neighbouring tiles of a head: its L2 holds their keys
-    const int id = xcd_tile(blockIdx.x, gridDim.x);
-    const int split = id / a.tile_groups % a.splits, kvh = id / a.tile_groups / a.splits;
-    const int64_t tg = id % a.tile_groups, tile = SHARES == 4 ? tg : tg * 4 + wave;
-    const int64_t s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, a.group, ROWS == 64 ? 6 : ROWS == 32 ? 5 : 4, tile);
-    const Span qs = sequence_span(a.q_starts, s, a.total_q);
-    const int64_t first_row = (tile - (qs.begin * a.group / ROWS + s)) * ROWS;
-    const int nrows = qs.rows * a.group;  // total_q * heads < 2^31
-    if (first_row < 0 || first_row >= nrows) return;  // SHARES 4: the whole workgroup
-    const int r0 = static_cast<int>(first_row);
-    const int tok0 = r0 / a.group, last = (min(r0 + ROWS, nrows) - 1) / a.group;
-    const int keys = cached_rows(a.cache, s), lag = keys - qs.rows;
-    const int piece = split * SHARES + (SHARES == 4 ? wave : 0), pieces = a.splits * SHARES;
+// What a tile of a sequence's rows (query rows times the heads that share a key head) sees, and how its keys are cut into
+// steps: those of the first keys that stay visible, then from the window's beginning on.
+struct Tile {
+    Span qs;
+    int64_t s;
+    int r0, nrows, keys, lag;            // its first row, the sequence's rows, keys, their difference
+    int least, low_all, sinks;           // keys that all rows see: below `least`, and from `low_all` on or below `sinks`
+    int steps, sink_steps, skip;
+    __device__ __forceinline__ int key_of(int step) const { return (step < sink_steps ? step : step + skip) * kStep; }
+    // Whether some row of the tile does not see all keys of the step at key `at`.
+    __device__ __forceinline__ bool cut(int at) const { return at + kStep > least || (at < low_all && at + kStep > sinks); }
+};
+// Keys [from, lim) and those below the tile's sinks: what a row sees.
+struct Sight {
+    int lim, from;
+};
+__device__ __forceinline__ Sight sight_of(const AttendArgs &a, const Tile &t, int tok) {
+    return {a.causal ? max(0, min(t.keys, tok + t.lag + 1)) : t.keys, a.window ? tok + t.lag - a.window + 1 : 0};
+}
+// Rows [r0, r0 + rows) of sequence s; rows == 0: none.
+__device__ __forceinline__ Tile tile_of(const AttendArgs &a, int64_t tile, int rows, int rows_log2) {
+    Tile t = {};
+    t.s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, a.group, rows_log2, tile);
+    t.qs = sequence_span(a.q_starts, t.s, a.total_q);
+    const int64_t first = (tile - ((t.qs.begin * a.group >> rows_log2) + t.s)) << rows_log2;
+    t.nrows = t.qs.rows * a.group;  // total_q * heads < 2^31
+    if (first < 0 || first >= t.nrows) {
+        t.nrows = 0;
+        return t;
+    }
+    t.r0 = static_cast<int>(first);
+    t.keys = cached_rows(a.cache, t.s);
+    t.lag = t.keys - t.qs.rows;
+    const Sight head = sight_of(a, t, t.r0 / a.group), tail = sight_of(a, t, (min(t.r0 + rows, t.nrows) - 1) / a.group);
+    t.least = head.lim;
+    t.low_all = max(0, tail.from);
+    t.sinks = a.sinks;
+    const int end = (tail.lim + kStep - 1) / kStep;
+    t.sink_steps = min(end, (a.sinks + kStep - 1) / kStep);
+    t.skip = max(0, max(0, head.from) / kStep - t.sink_steps);
+    t.steps = t.sink_steps + max(0, end - t.sink_steps - t.skip);
+    return t;
+}
 
-    // keys below `most` are seen by some row, below `least` by all as far as the causal end goes; from `low` on by some, from
-    // `low_all` on by all as far as the window's beginning goes
-    const int most = a.causal ? max(0, min(keys, last + lag + 1)) : keys;
-    const int least = a.causal ? max(0, min(keys, tok0 + lag + 1)) : keys;
-    const int low = a.window ? max(0, tok0 + lag - a.window + 1) : 0, low_all = a.window ? max(0, last + lag - a.window + 1) : 0;
-    // steps: those of the first keys that stay visible, then from the window's beginning on
-    const int end = (most + kStep - 1) / kStep, sink_steps = min(end, (a.sinks + kStep - 1) / kStep);
-    const int skip = max(0, low / kStep - sink_steps), steps = sink_steps + max(0, end - sink_steps - skip);
+// A lane's queries: of each set of 16 rows that of its column, in units of a power of two, in P half-precision terms.
+template <class T, int D, int NS>
+struct Queries {
+    static constexpr int P = sizeof(T) == 2 ? 1 : 2, QV = D / 32;
+    u32x4 f[NS][QV][P];
+    float unit[NS];  // binary orders of a score for each unit of its product, before the keys' step
+    Sight sight[NS];
 
-    // ---- this lane's query of each set of 16
-    int lim[NS], from[NS];  // it sees keys [from, lim) and those before a.sinks
-    u32x4 qf[NS][QV][P];
-    float fq[NS];           // binary orders of a score for each unit of its product, before the keys' step
+    __device__ __forceinline__ void load(const AttendArgs &a, const Tile &t, int r0, int kvh) {
+        constexpr bool BF = sizeof(T) == 2;
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-        const int r = min(r0 + 16 * n + c, nrows - 1), tok = r / a.group;
-        lim[n] = a.causal ? max(0, min(keys, tok + lag + 1)) : keys;
-        from[n] = a.window ? tok + lag - a.window + 1 : 0;
-        const T *q = static_cast<const T *>(a.q) + (qs.begin + tok) * a.q_stride + static_cast<int64_t>(kvh * a.group + r % a.group) * D;
-        float x[QV][8];
-        uint32_t big = 0;
+        for (int n = 0; n < NS; ++n) {
+            const int r = min(r0 + 16 * n + c, t.nrows - 1), tok = r / a.group;
+            sight[n] = sight_of(a, t, tok);
+            const T *q = static_cast<const T *>(a.q) + (t.qs.begin + tok) * a.q_stride + static_cast<int64_t>(kvh * a.group + r % a.group) * D;
+            float x[QV][8];
+            uint32_t big = 0;
 #pragma unroll
-        for (int j = 0; j < QV; ++j) {
-            // products 2h and 2h + 1: channels 64h + 16g.., 64h + 16g + 8..; a last one by itself: 8g.. of the last 32
-            const T *qj = q + (j == QV - 1 && QV % 2 ? 32 * j + 8 * g : 64 * (j / 2) + 16 * g + 8 * (j & 1));
-            constexpr int N = 8 * static_cast<int>(sizeof(T)) / 16;
-            uint4 t[N];
+            for (int j = 0; j < QV; ++j) {
+                // products 2h and 2h + 1: channels 64h + 16g.., 64h + 16g + 8..; a last one by itself: 8g.. of the last 32
+                const T *qj = q + (j == QV - 1 && QV % 2 ? 32 * j + 8 * g : 64 * (j / 2) + 16 * g + 8 * (j & 1));
+                constexpr int N = 8 * static_cast<int>(sizeof(T)) / 16;
+                uint4 v[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) t[i] = reinterpret_cast<const uint4 *>(qj)[i];
-            const uint32_t *w = reinterpret_cast<const uint32_t *>(t);
+                for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const uint4 *>(qj)[i];
+                const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t u = BF ? (e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16) : w[e];
-                x[j][e] = as_float(u);
-                big = max(big, u & 0x7fffffffu);
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t u = BF ? (e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16) : w[e];
+                    x[j][e] = as_float(u);
+                    big = max(big, u & 0x7fffffffu);
+                }
             }
-        }
-        // the row's power: its largest magnitude to [2^14, 2^15).  Magnitudes' bits rise with them, infinities and NaN above all;
-        // their rows keep them, and give NaN.
-        big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 16, 64)));
-        big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 32, 64)));
-        const int e = min(max(static_cast<int>(big >> 23) - 127, -100), 127);
-        fq[n] = ldexpf(a.scale * kLog2e, e - 14);
+            // the row's power: its largest magnitude to [2^14, 2^15).  Magnitudes' bits rise with them, infinities and NaN above
+            // all; their rows keep them, and give NaN.
+            big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 16, 64)));
+            big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 32, 64)));
+            const int e = min(max(static_cast<int>(big >> 23) - 127, -100), 127);
+            unit[n] = ldexpf(a.scale * kLog2e, e - 14);
 #pragma unroll
-        for (int j = 0; j < QV; ++j)
+            for (int j = 0; j < QV; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float u = ldexpf(x[j][2 * i], 14 - e), v = ldexpf(x[j][2 * i + 1], 14 - e);
+                    f[n][j][0][i] = pack_f16x2(u, v);
+                    if constexpr (P == 2) {
+                        const f32x2 h = unpack_f16x2(f[n][j][0][i]);
+                        f[n][j][1][i] = pack_f16x2(u - h[0], v - h[1]);
+                    }
+                }
+        }
+    }
+};
+
+// A lane's running results of NS sets of 16 rows.
+template <int D, int NS, int P>
+struct Sums {
+    static constexpr int KT = kStep / 16, C = D / 16;
+    f32x4 acc[NS][C];  // in units of `unit`, the largest step of values met
+    float sum[NS], hi[NS], lo[NS], above[NS];  // above: the score from which on the base moves (-inf: nothing seen yet)
+    float unit;
+    bool far;  // some base is in two parts
+
+    __device__ __forceinline__ void clear() {
+        unit = 0.0f;
+        far = false;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            sum[n] = hi[n] = lo[n] = 0.0f;
+            above[n] = neg_inf();
+#pragma unroll
+            for (int t = 0; t < C; ++t) acc[n][t] = f32x4{0, 0, 0, 0};
+        }
+    }
+
+    // From a set's products w of a step's keys (the lane's are at + 16g..) to its weights, ready to meet the values.
+    __device__ __forceinline__ void weigh(int n, f32x4 (&w)[KT], float f, int at, bool cut, Sight see, int sinks, u32x4 (&pw)[KT / 2][P]) {
+        const int g = (threadIdx.x & 63) >> 4;
+        if (cut) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = at + 16 * g + 4 * t + i;
+                    if (key >= see.lim || (key < see.from && key >= sinks)) w[t][i] = neg_inf();
+                }
+        }
+        float mx = neg_inf();
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, w[t][i]);
+        if (__builtin_amdgcn_ballot_w64(mx != neg_inf() && mx * f > above[n]) != 0) {
+            mx = max_over_groups(mx);
+            const bool over = mx != neg_inf() && mx * f > above[n];
+            float h = mx * f, l = fmaf(mx, f, -h) - kUnder;
+            if (fabsf(h) < kFar) {
+                h += l;
+                l = 0.0f;
+            }
+            const float alpha = !over ? 1.0f : above[n] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f((hi[n] - h) + (lo[n] - l));
+            sum[n] *= alpha;
+#pragma unroll
+            for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
+            if (over) {
+                hi[n] = h;
+                lo[n] = l;
+                above[n] = h + (l + kReach);
+            }
+            far = far || __builtin_amdgcn_ballot_w64(lo[n] != 0.0f) != 0;
+        }
+        if (cut || far) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[t][i] = w[t][i] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(fmaf(w[t][i], f, -hi[n]) - lo[n]);
+        } else {
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[t][i] = __builtin_amdgcn_exp2f(fmaf(w[t][i], f, -hi[n]));
+        }
+        // their sum in 32 bits, before they are rounded
+#pragma unroll
+        for (int t = 0; t < KT; ++t) sum[n] += (w[t][0] + w[t][1]) + (w[t][2] + w[t][3]);
+        // half precision keeps 11 bits of a weight (2^-11 off at most), two terms 22
+#pragma unroll
+        for (int u = 0; u < KT / 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float u = ldexpf(x[j][2 * i], 14 - e), v = ldexpf(x[j][2 * i + 1], 14 - e);
-                qf[n][j][0][i] = pack_f16x2(u, v);
+                const float x = w[2 * u + (i >> 1)][2 * (i & 1)], y = w[2 * u + (i >> 1)][2 * (i & 1) + 1];
+                pw[u][0][i] = pack_f16x2(x, y);
                 if constexpr (P == 2) {
-                    const f32x2 t = unpack_f16x2(qf[n][j][0][i]);
-                    qf[n][j][1][i] = pack_f16x2(u - t[0], v - t[1]);
+                    const f32x2 t = unpack_f16x2(pw[u][0][i]);
+                    pw[u][1][i] = pack_f16x2(x - t[0], y - t[1]);
                 }
             }
     }
 
-    // ---- this wave's steps: pages and steps of 64 of them at a time, one a lane
-    int it = -1, pages = 0, page = 0, k0 = 0, at = 0;
-    float2 sizes = make_float2(0.0f, 0.0f);
-    float step_k = 0.0f, step_v = 0.0f;
-    const auto key_of = [&](int i) { return (i < sink_steps ? i : i + skip) * kStep; };
-    const auto next = [&]() __attribute__((always_inline)) {  // false: none left
+    // Makes the unit at least a step of values.
+    __device__ __forceinline__ void reach(float step_v) {
+        if (!(step_v > unit)) return;
+        const float ratio = unit / step_v;  // powers of two, or 0
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int t = 0; t < C; ++t) acc[n][t] *= ratio;
+        unit = step_v;
+    }
+};
+// Values count in units of the largest step met; a smaller one's ratio goes into its codes (down to 2^-24 they stay
+// exact), or, smaller still, into their products.
+constexpr float kLeastRatio = 0x1p-24f;
+
+// A row's channels 16t + 4g.. out: divided by the sum before the unit, so that means of finite values are finite.
+template <class T, int D>
+__device__ __forceinline__ void put(const AttendArgs &a, const Tile &t, int split, int r, int kvh, const float (&y)[D / 4], float h, float l,
+                                    float total, float unit) {
+    const int g = (threadIdx.x & 63) >> 4;
+    if (r >= t.nrows) return;
+    const int64_t token = t.qs.begin + r / a.group;
+    const int head = kvh * a.group + r % a.group;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const int64_t cell = token * a.heads + head, part = split * a.total_q * a.heads + cell;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) {
+        const f32x4 z = {y[4 * e] * inv * unit, y[4 * e + 1] * inv * unit, y[4 * e + 2] * inv * unit, y[4 * e + 3] * inv * unit};
+        if (a.splits > 1) {
+            *reinterpret_cast<f32x4 *>(a.part_o + part * D + 16 * e + 4 * g) = z;
+        } else {
+            T *to = static_cast<T *>(a.o) + token * a.o_stride + static_cast<int64_t>(head) * D + 16 * e + 4 * g;
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2 *>(to) = u32x2{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3])};
+            else *reinterpret_cast<f32x4 *>(to) = z;
+        }
+    }
+    if (g != 0) return;
+    if (a.splits > 1) a.part_ml[part] = sum_of(h, l, total, 1.0f);
+    else if (a.lse) a.lse[cell] = log_of(h, l, total);
+}
+
+// A wave's walk over its steps of a tile: pages and steps of 64 of them at a time, one a lane.
+struct Walk {
+    int it, pages, page, k0;
+    float2 sizes;
+    const uint8_t *codes;  // of the page's head
+
+    // Goes to the next step of every `pieces`-th from `piece` on whose page is one; false: none is left.
+    __device__ __forceinline__ bool next(const AttendArgs &a, const Tile &t, int kvh, int piece, int pieces, int head_bytes) {
+        const int lane = threadIdx.x & 63;
         for (;;) {
             ++it;
             const int i = piece + it * pieces;
-            if (i >= steps) return false;
+            if (i >= t.steps) return false;
             if ((it & 63) == 0) {
                 const int mine = i + lane * pieces;
-                pages = mine < steps ? page_of(a.cache, s, key_of(mine) >> a.cache.block_log2) : -1;
+                pages = mine < t.steps ? page_of(a.cache, t.s, t.key_of(mine) >> a.cache.block_log2) : -1;
                 sizes = pages >= 0 ? a.cache.steps[static_cast<int64_t>(pages) * a.cache.kv_heads + kvh] : make_float2(0.0f, 0.0f);
             }
             page = __builtin_amdgcn_readlane(pages, it & 63);
             if (page < 0) continue;  // no such page: its keys count for nothing
-            k0 = key_of(i);
+            k0 = t.key_of(i);
+            codes = a.cache.codes + (static_cast<int64_t>(page) * a.cache.kv_heads + kvh) * head_bytes;
             return true;
         }
-    };
-    const int block = 1 << a.cache.block_log2;
-    uint32_t kr[KT][KD], vr[C][4];
-    const int kat = (16 * (c >> 2) + (c & 3)) * D, vat = (c << a.cache.block_log2) + 16 * g;
-    const uint8_t *codes = nullptr;
-    const auto place = [&]() __attribute__((always_inline)) {
-        codes = a.cache.codes + ((static_cast<int64_t>(page) * a.cache.kv_heads + kvh) << (a.cache.block_log2 + 1)) * D;
-    };
+    }
+    __device__ __forceinline__ float step_k() const { return as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, sizes.x), it & 63)); }
+    __device__ __forceinline__ float step_v() const { return as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, sizes.y), it & 63)); }
+};
+
+// The operands of a step as they lie in a page.  S^T = K Q^T and O^T = V^T P^T, so that what one product leaves in a
+// lane is what the next one wants there.  A 16x16 product leaves lane (c, g) = (lane & 15, lane >> 4) with rows 4g..4g+3 of
+// column c; product t of a step takes key 16 (c >> 2) + 4t + (c & 3) as its row c, so that lane
+// (c, g) gets keys 16g + 4t + i of query c: the lane's 16 weights are of keys 16g..16g+15, and the
+// values' operand wants the same keys of a channel: one 16-byte piece of the cache.
+// The keys' operand wants channels of a row, in any order that the queries share: 16 side by side for two products.
+template <int D>
+__device__ __forceinline__ void fetch_keys(const uint8_t *codes, int place, int t, uint32_t (&w)[D / 16]) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const uint8_t *p = codes + place * D + (16 * (c >> 2) + (c & 3)) * D + 4 * t * D;
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p + 64 * h + 16 * g);
+        w[4 * h] = v.x, w[4 * h + 1] = v.y, w[4 * h + 2] = v.z, w[4 * h + 3] = v.w;
+    }
+    if constexpr (D % 64 != 0) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p + 64 * (D / 64) + 8 * g);
+        w[D / 16 - 2] = v.x, w[D / 16 - 1] = v.y;
+    }
+}
+template <int D>
+__device__ __forceinline__ void fetch_values(const uint8_t *codes, int block_log2, int place, int t, uint32_t (&w)[4]) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const uint4 v = *reinterpret_cast<const uint4 *>(codes + ((D + 16 * t + c) << block_log2) + place + 16 * g);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+}
+
+// Few rows: a tile of 16 of one sequence.  The workgroup's four waves take every fourth step each, and join through LDS.
+// Codes go from memory to a product's registers through two instructions for every four, without LDS; the next step's
+// keys are on their way from the first product on, its values from the last.
+template <class T, int D>
+__global__ void __launch_bounds__(256, 2) cache_rows_kernel(AttendArgs a) {
+    using Q = Queries<T, D, 1>;
+    constexpr int P = Q::P, QV = Q::QV, KT = kStep / 16, C = D / 16;
+    __shared__ float part[4][4 * C][64];
+    __shared__ float4 part_ml[4][16];
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = xcd_tile(blockIdx.x, gridDim.x);
+    const int split = id / a.tile_groups % a.splits, kvh = id / a.tile_groups / a.splits;
+    const Tile t = tile_of(a, id % a.tile_groups, 16, 4);
+    if (t.nrows == 0) return;
+    Q q;
+    q.load(a, t, t.r0, kvh);
+    Sums<D, 1, P> r;
+    r.clear();
+    const int piece = split * 4 + wave, pieces = a.splits * 4, block = 1 << a.cache.block_log2, head_bytes = 2 * block * D;
+    Walk walk = {-1, 0, 0, 0, make_float2(0.0f, 0.0f), nullptr};
+    uint32_t kr[KT][D / 16], vr[C][4];
     const auto load_k = [&]() __attribute__((always_inline)) {
-        const uint8_t *p = codes + (k0 & (block - 1)) * D;
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-#pragma unroll
-            for (int h = 0; h < KD / 4; ++h) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(p + kat + 4 * t * D + 64 * h + 16 * g);
-                kr[t][4 * h] = w.x, kr[t][4 * h + 1] = w.y, kr[t][4 * h + 2] = w.z, kr[t][4 * h + 3] = w.w;
-            }
-            if constexpr (KD % 4 != 0) {
-                const uint2 w = *reinterpret_cast<const uint2 *>(p + kat + 4 * t * D + 64 * (KD / 4) + 8 * g);
-                kr[t][KD - 2] = w.x, kr[t][KD - 1] = w.y;
-            }
-        }
+        for (int i = 0; i < KT; ++i) fetch_keys<D>(walk.codes, walk.k0 & (block - 1), i, kr[i]);
     };
     const auto load_v = [&]() __attribute__((always_inline)) {
-        const uint8_t *p = codes + block * D + (k0 & (block - 1));
 #pragma unroll
-        for (int t = 0; t < C; ++t) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(p + vat + (t << (a.cache.block_log2 + 4)));
-            vr[t][0] = w.x, vr[t][1] = w.y, vr[t][2] = w.z, vr[t][3] = w.w;
-        }
+        for (int i = 0; i < C; ++i) fetch_values<D>(walk.codes, a.cache.block_log2, walk.k0 & (block - 1), i, vr[i]);
     };
-
-    // ---- state
-    f32x4 acc[NS][C];  // in units of `unit`, the largest step of values met
-    float sum[NS], hi[NS], lo[NS], above[NS];  // above: the score from which on the base moves (-inf: nothing seen yet)
-    float unit = 0.0f;
-    bool far = false;
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-        sum[n] = hi[n] = lo[n] = 0.0f;
-        above[n] = neg_inf();
-#pragma unroll
-        for (int t = 0; t < C; ++t) acc[n][t] = f32x4{0, 0, 0, 0};
-    }
-
-    bool more = next();
+    bool more = walk.next(a, t, kvh, piece, pieces, head_bytes);
     if (more) {
-        place();
         load_k();
         load_v();
     }
     while (more) {
-        step_k = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, sizes.x), it & 63));
-        step_v = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, sizes.y), it & 63));
-        at = k0;
-        // ---- S^T
-        f32x4 w[NS][KT];
+        const float step_k = walk.step_k(), step_v = walk.step_v();
+        const int at = walk.k0;
+        f32x4 w[KT];
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int t = 0; t < KT; ++t) w[n][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
+        for (int i = 0; i < KT; ++i) {
+            w[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < QV; ++j) {
-                const u32x4 x = codes_f16(kr[t][2 * j], kr[t][2 * j + 1]);
+                const u32x4 x = codes_f16(kr[i][2 * j], kr[i][2 * j + 1]);
 #pragma unroll
-                for (int n = 0; n < NS; ++n)
-#pragma unroll
-                    for (int p = P - 1; p >= 0; --p) w[n][t] = product(x, qf[n][j][p], w[n][t]);
+                for (int p = P - 1; p >= 0; --p) w[i] = product(x, q.f[0][j][p], w[i]);
             }
-        more = next();
-        if (more) {
-            place();
-            load_k();
         }
-        // ---- weights
-        const bool cut = at + kStep > least || (at < low_all && at + kStep > a.sinks);
-        u32x4 pw[NS][KT / 2][P];
+        more = walk.next(a, t, kvh, piece, pieces, head_bytes);
+        if (more) load_k();
+        u32x4 pw[KT / 2][P];
+        r.weigh(0, w, q.unit[0] * step_k, at, t.cut(at), q.sight[0], t.sinks, pw);
+        r.reach(step_v);
+        const float ratio = r.unit > 0.0f ? step_v / r.unit : 0.0f;
+        if (ratio >= kLeastRatio) {
+            const _Float16 h = static_cast<_Float16>(ratio), b = static_cast<_Float16>(-1152.0f * ratio);
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            if (cut) {
-#pragma unroll
-                for (int t = 0; t < KT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = at + 16 * g + 4 * t + i;
-                        if (key >= lim[n] || (key < from[n] && key >= a.sinks)) w[n][t][i] = neg_inf();
-                    }
-            }
-            const float f = fq[n] * step_k;
-            float mx = neg_inf();
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, w[n][t][i]);
-            if (__builtin_amdgcn_ballot_w64(mx != neg_inf() && mx * f > above[n]) != 0) {
-                mx = max_over_groups(mx);
-                const bool over = mx != neg_inf() && mx * f > above[n];
-                float h = mx * f, l = fmaf(mx, f, -h) - kUnder;
-                if (fabsf(h) < kFar) {
-                    h += l;
-                    l = 0.0f;
-                }
-                const float alpha = !over ? 1.0f : above[n] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f((hi[n] - h) + (lo[n] - l));
-                sum[n] *= alpha;
-#pragma unroll
-                for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
-                if (over) {
-                    hi[n] = h;
-                    lo[n] = l;
-                    above[n] = h + (l + kReach);
-                }
-                far = far || __builtin_amdgcn_ballot_w64(lo[n] != 0.0f) != 0;
-            }
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = fmaf(w[n][t][i], f, -hi[n]);
-                    if (far) x -= lo[n];
-                    if (cut && w[n][t][i] == neg_inf()) x = neg_inf();
-                    w[n][t][i] = __builtin_amdgcn_exp2f(x);
-                }
-            // their sum in 32 bits, before they are rounded
-#pragma unroll
-            for (int t = 0; t < KT; ++t) sum[n] += (w[n][t][0] + w[n][t][1]) + (w[n][t][2] + w[n][t][3]);
-            // half precision keeps 11 bits of a weight (2^-11 off at most), two terms 22
-#pragma unroll
-            for (int u = 0; u < KT / 2; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = w[n][2 * u + (i >> 1)][2 * (i & 1)], y = w[n][2 * u + (i >> 1)][2 * (i & 1) + 1];
-                    pw[n][u][0][i] = pack_f16x2(x, y);
-                    if constexpr (P == 2) {
-                        const f32x2 t = unpack_f16x2(pw[n][u][0][i]);
-                        pw[n][u][1][i] = pack_f16x2(x - t[0], y - t[1]);
-                    }
-                }
-        }
-        // ---- O^T.  Values count in units of the largest step met; a smaller one's ratio goes into its codes (down to 2^-24 they
-        // stay exact), or, smaller still, into their products.
-        if (step_v > unit) {
-            const float ratio = unit / step_v;  // powers of two, or 0
-#pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-                for (int t = 0; t < C; ++t) acc[n][t] *= ratio;
-            unit = step_v;
-        }
-        const float ratio = unit > 0.0f ? step_v / unit : 0.0f;
-        if (ratio >= 0x1p-24f) {
-            const _Float16 r = static_cast<_Float16>(ratio), b = static_cast<_Float16>(-1152.0f * ratio);
-#pragma unroll
-            for (int t = 0; t < C; ++t)
+            for (int i = 0; i < C; ++i)
 #pragma unroll
                 for (int u = 0; u < KT / 2; ++u) {
-                    const u32x4 x = codes_f16(vr[t][2 * u], vr[t][2 * u + 1], f16x2{r, r}, f16x2{b, b});
+                    const u32x4 x = codes_f16(vr[i][2 * u], vr[i][2 * u + 1], f16x2{h, h}, f16x2{b, b});
 #pragma unroll
-                    for (int n = 0; n < NS; ++n)
-#pragma unroll
-                        for (int p = P - 1; p >= 0; --p) acc[n][t] = product(x, pw[n][u][p], acc[n][t]);
+                    for (int p = P - 1; p >= 0; --p) r.acc[0][i] = product(x, pw[u][p], r.acc[0][i]);
                 }
         } else if (ratio > 0.0f) {
 #pragma unroll
-            for (int t = 0; t < C; ++t)
+            for (int i = 0; i < C; ++i) {
+                f32x4 d = {0, 0, 0, 0};
 #pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    f32x4 d = {0, 0, 0, 0};
+                for (int u = 0; u < KT / 2; ++u)
 #pragma unroll
-                    for (int u = 0; u < KT / 2; ++u)
-#pragma unroll
-                        for (int p = P - 1; p >= 0; --p) d = product(codes_f16(vr[t][2 * u], vr[t][2 * u + 1]), pw[n][u][p], d);
-                    acc[n][t] += d * ratio;
-                }
+                    for (int p = P - 1; p >= 0; --p) d = product(codes_f16(vr[i][2 * u], vr[i][2 * u + 1]), pw[u][p], d);
+                r.acc[0][i] += d * ratio;
+            }
         }
         if (more) load_v();
     }
 
-    // ---- out
-    const bool parts = a.splits > 1;
-    const auto finish = [&](int n, const float (&y)[4 * C], float h, float l, float total, float u) __attribute__((always_inline)) {
-        const int r = r0 + 16 * n + c;
-        if (r >= nrows) return;
-        const int64_t token = qs.begin + r / a.group;
-        const int head = kvh * a.group + r % a.group;
-        // divided by the sum before the unit, so that means of finite values are finite
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        const int64_t cell = token * a.heads + head;
-        if (parts) {
-            float *to = a.part_o + (split * a.total_q * a.heads + cell) * D;
+    // ---- the waves' results, joined by the first
 #pragma unroll
-            for (int t = 0; t < C; ++t)
-                *reinterpret_cast<f32x4 *>(to + 16 * t + 4 * g) =
-                    f32x4{y[4 * t] * inv * u, y[4 * t + 1] * inv * u, y[4 * t + 2] * inv * u, y[4 * t + 3] * inv * u};
-            if (g == 0) a.part_ml[split * a.total_q * a.heads + cell] = sum_of(h, l, total, 1.0f);
-            return;
-        }
-        T *to = static_cast<T *>(a.o) + token * a.o_stride + static_cast<int64_t>(head) * D;
+    for (int i = 0; i < C; ++i)
 #pragma unroll
-        for (int t = 0; t < C; ++t) {
-            const f32x4 z = {y[4 * t] * inv * u, y[4 * t + 1] * inv * u, y[4 * t + 2] * inv * u, y[4 * t + 3] * inv * u};
-            if constexpr (BF) *reinterpret_cast<u32x2 *>(to + 16 * t + 4 * g) = u32x2{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3])};
-            else *reinterpret_cast<f32x4 *>(to + 16 * t + 4 * g) = z;
-        }
-        if (a.lse && g == 0) a.lse[cell] = log_of(h, l, total);
+        for (int e = 0; e < 4; ++e) part[wave][4 * i + e][lane] = r.acc[0][i][e];
+    const float l = sum_over_groups(r.sum[0]);
+    if (g == 0) part_ml[wave][c] = sum_of(r.hi[0], r.lo[0], l, r.unit);
+    __syncthreads();
+    if (wave != 0) return;
+    float4 top = sum_of(neg_inf(), 0.0f, 0.0f, 0.0f);
+    float unit = 0.0f, total = 0.0f, y[4 * C];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const float4 m = part_ml[p][c];
+        if (m.z != 0.0f && above_of(m, top)) top = m;
+        unit = fmaxf(unit, m.w);
+    }
+#pragma unroll
+    for (int e = 0; e < 4 * C; ++e) y[e] = 0.0f;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const float4 m = part_ml[p][c];
+        const float wgt = m.z == 0.0f ? 0.0f : weight_of(m, top), scaled = m.w > 0.0f ? wgt * (m.w / unit) : wgt * 0.0f;
+        total += wgt * m.z;
+#pragma unroll
+        for (int e = 0; e < 4 * C; ++e) y[e] += scaled * part[p][e][lane];
+    }
+    put<T, D>(a, t, split, t.r0 + c, kvh, y, top.x, top.y, total, unit);
+}
+
+// Many rows: a tile of 64 NS of one sequence, 16 NS of them for each of the workgroup's four waves.  A step's codes
+// become half precision once, a quarter of them by each wave, and lie in LDS (two buffers, one barrier a step) as the
+// products' operands, lane by lane: reads and writes are whole rows of 1 KiB.
+template <class T, int D, int NS>
+__global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
+    using Q = Queries<T, D, NS>;
+    constexpr int P = Q::P, QV = Q::QV, KT = kStep / 16, C = D / 16, VT = (C + 3) / 4;
+    constexpr int KEYS = KT * QV, VALUES = C * (KT / 2);  // operands of a step, 1 KiB each
+    __shared__ u32x4 operands[2][KEYS + VALUES][64];
+    const int lane = threadIdx.x & 63, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // consecutive workgroups of one XCD run neighbouring tiles of a head: its L2 holds their keys
+    const int id = xcd_tile(blockIdx.x, gridDim.x);
+    const int split = id / a.tile_groups % a.splits, kvh = id / a.tile_groups / a.splits;
+    const Tile t = tile_of(a, id % a.tile_groups, 64 * NS, NS == 1 ? 6 : NS == 2 ? 7 : 8);
+    if (t.nrows == 0) return;
+    const int r0 = t.r0 + 16 * NS * wave;
+    Q q;
+    q.load(a, t, r0, kvh);
+    Sums<D, NS, P> r;
+    r.clear();
+    const int block = 1 << a.cache.block_log2, head_bytes = 2 * block * D;
+    Walk walk = {-1, 0, 0, 0, make_float2(0.0f, 0.0f), nullptr};
+    uint32_t kr[D / 16], vr[VT][4];
+    float unit = 0.0f, ratio = 0.0f, step_k = 0.0f, step_v = 0.0f;  // of the step whose codes are fetched
+    const auto fetch = [&]() __attribute__((always_inline)) {
+        fetch_keys<D>(walk.codes, walk.k0 & (block - 1), wave, kr);
+#pragma unroll
+        for (int i = 0; i < VT; ++i)
+            if (wave + 4 * i < C) fetch_values<D>(walk.codes, a.cache.block_log2, walk.k0 & (block - 1), wave + 4 * i, vr[i]);
+        step_k = walk.step_k();
+        step_v = walk.step_v();
     };
-    if constexpr (SHARES == 1) {
+    // fetched codes to a buffer
+    const auto lay_out = [&](int buffer) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            float y[4 * C];
+        for (int j = 0; j < QV; ++j) operands[buffer][wave * QV + j][lane] = codes_f16(kr[2 * j], kr[2 * j + 1]);
+        unit = fmaxf(unit, step_v);
+        ratio = unit > 0.0f ? step_v / unit : 0.0f;
+        const bool in = ratio >= kLeastRatio;
+        const _Float16 h = static_cast<_Float16>(in ? ratio : 1.0f), b = static_cast<_Float16>(in ? -1152.0f * ratio : -1152.0f);
 #pragma unroll
-            for (int e = 0; e < 4 * C; ++e) y[e] = acc[n][e / 4][e % 4];
-            finish(n, y, hi[n], lo[n], sum_over_groups(sum[n]), unit);
-        }
-    } else {
+        for (int i = 0; i < VT; ++i)
+            if (wave + 4 * i < C) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-#pragma unroll
-            for (int t = 0; t < C; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) part[wave][(n * C + t) * 4 + i][lane] = acc[n][t][i];
-            const float l = sum_over_groups(sum[n]);
-            if (g == 0) part_ml[wave][n][c] = sum_of(hi[n], lo[n], l, unit);
-        }
-        __syncthreads();
-        for (int n = wave; n < NS; n += 4) {
-            float4 top = sum_of(neg_inf(), 0.0f, 0.0f, 0.0f);
-            float u = 0.0f, total = 0.0f, y[4 * C];
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const float4 m = part_ml[p][n][c];
-                if (m.z != 0.0f && above_of(m, top)) top = m;
-                u = fmaxf(u, m.w);
+                for (int u = 0; u < KT / 2; ++u)
+                    operands[buffer][KEYS + (wave + 4 * i) * (KT / 2) + u][lane] = codes_f16(vr[i][2 * u], vr[i][2 * u + 1], f16x2{h, h}, f16x2{b, b});
             }
+    };
+    bool more = walk.next(a, t, kvh, split, a.splits, head_bytes);  // the same for all waves
+    if (more) {
+        fetch();
+        lay_out(0);
+    }
+    for (int buffer = 0; more; buffer ^= 1) {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const int at = walk.k0;
+        const float now_k = step_k, now_v = step_v, now_ratio = ratio;
+        more = walk.next(a, t, kvh, split, a.splits, head_bytes);
+        if (more) fetch();
+        if (r0 < t.nrows) {
+            f32x4 w[NS][KT];
 #pragma unroll
-            for (int e = 0; e < 4 * C; ++e) y[e] = 0.0f;
+            for (int i = 0; i < KT; ++i) {
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const float4 m = part_ml[p][n][c];
-                const float wgt = m.z == 0.0f ? 0.0f : weight_of(m, top), scaled = m.w > 0.0f ? wgt * (m.w / u) : wgt * 0.0f;
-                total += wgt * m.z;
+                for (int n = 0; n < NS; ++n) w[n][i] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int e = 0; e < 4 * C; ++e) y[e] += scaled * part[p][n * 4 * C + e][lane];
+                for (int j = 0; j < QV; ++j) {
+                    const u32x4 x = operands[buffer][i * QV + j][lane];
+#pragma unroll
+                    for (int n = 0; n < NS; ++n)
+#pragma unroll
+                        for (int p = P - 1; p >= 0; --p) w[n][i] = product(x, q.f[n][j][p], w[n][i]);
+                }
             }
-            finish(n, y, top.x, top.y, total, u);
+            const bool cut = t.cut(at);
+            u32x4 pw[NS][KT / 2][P];
+#pragma unroll
+            for (int n = 0; n < NS; ++n) r.weigh(n, w[n], q.unit[n] * now_k, at, cut, q.sight[n], t.sinks, pw[n]);
+            r.reach(now_v);
+            if (now_ratio >= kLeastRatio) {
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+#pragma unroll
+                    for (int u = 0; u < KT / 2; ++u) {
+                        const u32x4 x = operands[buffer][KEYS + i * (KT / 2) + u][lane];
+#pragma unroll
+                        for (int n = 0; n < NS; ++n)
+#pragma unroll
+                            for (int p = P - 1; p >= 0; --p) r.acc[n][i] = product(x, pw[n][u][p], r.acc[n][i]);
+                    }
+            } else if (now_ratio > 0.0f) {
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+#pragma unroll
+                    for (int n = 0; n < NS; ++n) {
+                        f32x4 d = {0, 0, 0, 0};
+#pragma unroll
+                        for (int u = 0; u < KT / 2; ++u)
+#pragma unroll
+                            for (int p = P - 1; p >= 0; --p) d = product(operands[buffer][KEYS + i * (KT / 2) + u][lane], pw[n][u][p], d);
+                        r.acc[n][i] += d * now_ratio;
+                    }
+            }
         }
+        if (more) lay_out(buffer ^ 1);
+    }
+    if (r0 >= t.nrows) return;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+        float y[4 * C];
+#pragma unroll
+        for (int e = 0; e < 4 * C; ++e) y[e] = r.acc[n][e / 4][e % 4];
+        put<T, D>(a, t, split, r0 + 16 * n + c, kvh, y, r.hi[n], r.lo[n], sum_over_groups(r.sum[n]), r.unit);
     }
 }
 
@@ -491,37 +638,28 @@ __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
     if (a.lse && lane == 0) a.lse[cell] = log_of(top.x, top.y, total);
 }
 
-// How a call is cut: tiles of 16, 32 or 64 rows as sequences fill them (an upper bound, as the lengths are on the device); four
-// waves to a tile, and several workgroups, where there would be fewer than two waves for each SIMD, with at least
-// four steps a wave.
+// How a call is cut: by sequences' mean rows into tiles of 16 (four waves share a tile's keys) or of 64 and 128 (four waves share
+// its rows), an upper bound of each, as the lengths are on the device; and, where there would be fewer than two waves for each
+// SIMD, every tile's keys over several workgroups, with at least four steps a wave.
 struct Cut {
     int64_t tile_groups;
-    int32_t splits, sets, shares;
+    int32_t splits, sets;  // 0: tiles of 16 rows
 };
 Cut cut_of(int64_t total_q, int32_t heads, int32_t kv_heads, int32_t d, int64_t sequences, int64_t max_k, int32_t window, int32_t sinks) {
-    constexpr int64_t kWaves = 256 * 4 * 2;
+    constexpr int64_t kGroups = 256 * 2;
     const int64_t rows = total_q * (heads / kv_heads), per = rows / std::max<int64_t>(sequences, 1);
-    const int32_t sets = per <= 16 ? 1 : per <= 32 || d > 64 ? 2 : 4;
-    const int64_t tiles = rows / (16 * sets) + sequences, waves = std::max<int64_t>(tiles * kv_heads, 1);
+    const int32_t sets = per <= 16 ? 0 : per <= 64 ? 1 : 2;
+    const int64_t tiles = rows / (sets == 0 ? 16 : 64 * sets) + sequences, groups = std::max<int64_t>(tiles * kv_heads, 1);
     const int64_t keys = window ? std::min<int64_t>(max_k, static_cast<int64_t>(window) + sinks + per + 2 * kStep) : max_k;
-    const int32_t shares = waves >= kWaves || keys <= kStep ? 1 : 4;
     int32_t splits = 1;
-    if (shares == 4)
-        while (splits < 64 && waves * 4 * splits * 2 <= kWaves && keys >= 4 * kStep * 4 * splits) splits *= 2;
-    return {shares == 4 ? tiles : (tiles + 3) / 4, splits, sets, shares};
+    while (splits < 64 && groups * splits * 2 <= kGroups && keys >= (sets == 0 ? 16 : 4) * kStep * splits) splits *= 2;
+    return {tiles, splits, sets};
 }
 
 using AttendFn = void (*)(AttendArgs);
 template <class T, int D>
 AttendFn pick_tile(const Cut &cut) {
-    // float32's wide heads: two terms of 32 rows do not fit a lane's registers
-    constexpr int MOST = sizeof(T) == 4 ? (D > 64 ? 1 : 2) : D > 64 ? 2 : 4;
-    const bool all = cut.shares == 4;
-    if constexpr (MOST >= 4)
-        if (cut.sets == 4) return all ? cache_attend_kernel<T, D, 4, 4> : cache_attend_kernel<T, D, 4, 1>;
-    if constexpr (MOST >= 2)
-        if (cut.sets == 2) return all ? cache_attend_kernel<T, D, 2, 4> : cache_attend_kernel<T, D, 2, 1>;
-    return all ? cache_attend_kernel<T, D, 1, 4> : cache_attend_kernel<T, D, 1, 1>;
+    return cut.sets == 0 ? cache_rows_kernel<T, D> : cut.sets == 1 ? cache_chunk_kernel<T, D, 1> : cache_chunk_kernel<T, D, 2>;
 }
 template <class T>
 AttendFn pick_attend(int32_t d, const Cut &cut) {
@@ -588,14 +726,7 @@ S3DX_API s3dx_status s3dx_cache_attention(const s3dx_cache *cache, const void *q
         }
         require(q_starts && aligned(q_starts, 4), "starts is NULL or not aligned");
         require(!lse || aligned(lse, 4), "lse is not aligned");
-        Cut cut = cut_of(total_q, heads, cache->kv_heads, cache->head_dim, sequences, max_k, window, sinks);
-        // fewer rows of float32 a tile than of bfloat16: more tiles
-        const int32_t most = dtype == S3DX_BF16 ? 4 : cache->head_dim > 64 ? 1 : 2;
-        if (cut.sets > most) {
-            const int64_t tiles = total_q * (heads / cache->kv_heads) / (16 * most) + sequences;
-            cut.sets = most;
-            cut.tile_groups = cut.shares == 4 ? tiles : (tiles + 3) / 4;
-        }
+        const Cut cut = cut_of(total_q, heads, cache->kv_heads, cache->head_dim, sequences, max_k, window, sinks);
         AttendArgs a = {view_of(cache, table, table_stride, lengths), q, o, lse, q_starts, total_q, q_stride, o_stride, sequences,
                         heads, heads / cache->kv_heads, flags & S3DX_BLOCK_CAUSAL, window, sinks, cut.splits,
                         static_cast<int32_t>(cut.tile_groups), softmax_scale, nullptr, nullptr};
