@@ -41,9 +41,11 @@ constexpr int kStep = 64;  // keys of a step: half or all of a block
 // Weights are 2^(score - base), score in binary orders.  A base stands 2^7 below the largest score when it is set
 // and moves once a weight would pass 2^15: half precision keeps its 11 bits of weights down to 2^-21 of the
 // largest and some down to 2^-31; a base that follows every maximum would scale the sums at every step.
-// From 2^20 on a base is kept in two parts (lo: what hi is rounded by, and the 7), so that scores of any size have weights
-// as exact as their difference.
+// Beyond 2^20 a base's own rounding would show in its weights: such rows are computed again, key by key.
 constexpr float kUnder = 7.0f, kReach = 15.0f, kFar = 0x1p20f;
+// Values count in units of the largest step met, and a smaller one's ratio goes into its codes: down to 2^-24 they
+// stay exact in half precision.  Rows that meet steps further apart are computed again, key by key.
+constexpr float kLeastRatio = 0x1p-24f;
 
 // A row's sum of weights l relative to base hi + lo.
 __device__ __forceinline__ float4 sum_of(float hi, float lo, float l, float unit) { return make_float4(hi, lo, l, unit); }
@@ -185,17 +187,17 @@ struct Queries {
 template <int D, int NS, int P>
 struct Sums {
     static constexpr int KT = kStep / 16, C = D / 16;
-    f32x4 acc[NS][C];  // in units of `unit`, the largest step of values met
-    float sum[NS], hi[NS], lo[NS], above[NS];  // above: the score from which on the base moves (-inf: nothing seen yet)
+    f32x4 acc[NS][C];  // in units of `unit`
+    float sum[NS], base[NS], above[NS];  // above: the score from which on the base moves (-inf: nothing seen yet)
     float unit;
-    bool far;  // some base is in two parts
+    bool again;  // the rows are to be computed key by key
 
     __device__ __forceinline__ void clear() {
         unit = 0.0f;
-        far = false;
+        again = false;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-            sum[n] = hi[n] = lo[n] = 0.0f;
+            sum[n] = base[n] = 0.0f;
             above[n] = neg_inf();
 #pragma unroll
             for (int t = 0; t < C; ++t) acc[n][t] = f32x4{0, 0, 0, 0};
@@ -204,52 +206,41 @@ struct Sums {
 
     // From a set's products w of a step's keys (the lane's are at + 16g..) to its weights, ready to meet the values.
     __device__ __forceinline__ void weigh(int n, f32x4 (&w)[KT], float f, int at, bool cut, Sight see, int sinks, u32x4 (&pw)[KT / 2][P]) {
-        const int g = (threadIdx.x & 63) >> 4;
         if (cut) {
+            // (the first key's place is made here, so that nothing of this is done where no key is hidden)
+            int key = at + 16 * ((threadIdx.x & 63) >> 4);
+            asm volatile("" : "+v"(key));
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int key = at + 16 * g + 4 * t + i;
-                    if (key >= see.lim || (key < see.from && key >= sinks)) w[t][i] = neg_inf();
+                    const int k = key + 4 * t + i;
+                    w[t][i] = (k >= see.lim) | ((k < see.from) & (k >= sinks)) ? neg_inf() : w[t][i];
                 }
         }
+        f = fmaxf(f, 0x1p-126f);  // products of 0 stay 0, hidden ones -inf
         float mx = neg_inf();
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) mx = fmaxf(mx, w[t][i]);
-        if (__builtin_amdgcn_ballot_w64(mx != neg_inf() && mx * f > above[n]) != 0) {
-            mx = max_over_groups(mx);
-            const bool over = mx != neg_inf() && mx * f > above[n];
-            float h = mx * f, l = fmaf(mx, f, -h) - kUnder;
-            if (fabsf(h) < kFar) {
-                h += l;
-                l = 0.0f;
-            }
-            const float alpha = !over ? 1.0f : above[n] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f((hi[n] - h) + (lo[n] - l));
+        if (__builtin_amdgcn_ballot_w64(mx * f > above[n]) != 0) {
+            mx = max_over_groups(mx) * f;
+            const bool over = mx > above[n];
+            const float to = over ? mx - kUnder : base[n];
+            const float alpha = above[n] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(base[n] - to);
             sum[n] *= alpha;
 #pragma unroll
             for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
-            if (over) {
-                hi[n] = h;
-                lo[n] = l;
-                above[n] = h + (l + kReach);
-            }
-            far = far || __builtin_amdgcn_ballot_w64(lo[n] != 0.0f) != 0;
+            base[n] = to;
+            above[n] = over ? to + kReach : above[n];
+            // (past float32's range a row is NaN either way)
+            again = again || __builtin_amdgcn_ballot_w64(fabsf(to) >= kFar && fabsf(to) < __builtin_inff()) != 0;
         }
-        if (cut || far) {
 #pragma unroll
-            for (int t = 0; t < KT; ++t)
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    w[t][i] = w[t][i] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(fmaf(w[t][i], f, -hi[n]) - lo[n]);
-        } else {
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[t][i] = __builtin_amdgcn_exp2f(fmaf(w[t][i], f, -hi[n]));
-        }
+            for (int i = 0; i < 4; ++i) w[t][i] = __builtin_amdgcn_exp2f(fmaf(w[t][i], f, -base[n]));
         // their sum in 32 bits, before they are rounded
 #pragma unroll
         for (int t = 0; t < KT; ++t) sum[n] += (w[t][0] + w[t][1]) + (w[t][2] + w[t][3]);
@@ -267,45 +258,135 @@ struct Sums {
             }
     }
 
-    // Makes the unit at least a step of values.
-    __device__ __forceinline__ void reach(float step_v) {
-        if (!(step_v > unit)) return;
-        const float ratio = unit / step_v;  // powers of two, or 0
+    // Makes the unit at least a step of values; the step's ratio to it.
+    __device__ __forceinline__ float reach(float step_v) {
+        if (step_v > unit) {
+            const float ratio = unit / step_v;  // powers of two, or 0
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
+            for (int n = 0; n < NS; ++n)
 #pragma unroll
-            for (int t = 0; t < C; ++t) acc[n][t] *= ratio;
-        unit = step_v;
+                for (int t = 0; t < C; ++t) acc[n][t] *= ratio;
+            again = again || (ratio < kLeastRatio && unit > 0.0f);
+            unit = step_v;
+        }
+        const float ratio = unit > 0.0f ? step_v / unit : 0.0f;
+        again = again || (ratio < kLeastRatio && step_v > 0.0f);
+        return ratio;
     }
 };
-// Values count in units of the largest step met; a smaller one's ratio goes into its codes (down to 2^-24 they stay
-// exact), or, smaller still, into their products.
-constexpr float kLeastRatio = 0x1p-24f;
+
+// Where a row's results go: the output, or its piece's place in the workspace.
+template <class T, int D>
+struct Place {
+    int64_t cell, part;
+    T *to;
+    __device__ __forceinline__ Place(const AttendArgs &a, const Tile &t, int split, int r, int kvh) {
+        const int64_t token = t.qs.begin + r / a.group;
+        const int head = kvh * a.group + r % a.group;
+        cell = token * a.heads + head;
+        part = split * a.total_q * a.heads + cell;
+        to = static_cast<T *>(a.o) + token * a.o_stride + static_cast<int64_t>(head) * D;
+    }
+    // (base + lo: what weights are relative to)
+    __device__ __forceinline__ void sums(const AttendArgs &a, float base, float lo, float total) const {
+        if (a.splits > 1) a.part_ml[part] = sum_of(base, lo, total, 1.0f);
+        else if (a.lse) a.lse[cell] = log_of(base, lo, total);
+    }
+};
 
 // A row's channels 16t + 4g.. out: divided by the sum before the unit, so that means of finite values are finite.
 template <class T, int D>
-__device__ __forceinline__ void put(const AttendArgs &a, const Tile &t, int split, int r, int kvh, const float (&y)[D / 4], float h, float l,
+__device__ __forceinline__ void put(const AttendArgs &a, const Tile &t, int split, int r, int kvh, const float (&y)[D / 4], float base,
                                     float total, float unit) {
     const int g = (threadIdx.x & 63) >> 4;
     if (r >= t.nrows) return;
-    const int64_t token = t.qs.begin + r / a.group;
-    const int head = kvh * a.group + r % a.group;
+    const Place<T, D> place(a, t, split, r, kvh);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    const int64_t cell = token * a.heads + head, part = split * a.total_q * a.heads + cell;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) {
         const f32x4 z = {y[4 * e] * inv * unit, y[4 * e + 1] * inv * unit, y[4 * e + 2] * inv * unit, y[4 * e + 3] * inv * unit};
-        if (a.splits > 1) {
-            *reinterpret_cast<f32x4 *>(a.part_o + part * D + 16 * e + 4 * g) = z;
-        } else {
-            T *to = static_cast<T *>(a.o) + token * a.o_stride + static_cast<int64_t>(head) * D + 16 * e + 4 * g;
-            if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2 *>(to) = u32x2{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3])};
-            else *reinterpret_cast<f32x4 *>(to) = z;
+        if (a.splits > 1) *reinterpret_cast<f32x4 *>(a.part_o + place.part * D + 16 * e + 4 * g) = z;
+        else if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2 *>(place.to + 16 * e + 4 * g) = u32x2{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3])};
+        else *reinterpret_cast<f32x4 *>(place.to + 16 * e + 4 * g) = z;
+    }
+    if (g == 0) place.sums(a, base, 0.0f, total);
+}
+
+// One row by the whole wave, key by key: of every `splits`-th run of `run` steps, scores with a key per lane, values with a
+// channel per lane, in 32 bits.  A base is kept in two parts, its rounding apart, and weights are of differences: for rows
+// whose scores or values' steps pass what the tiles hold.
+template <class T, int D>
+__device__ void row_by_keys(const AttendArgs &a, const Tile &t, int split, int run, int r, int kvh) {
+    const int lane = threadIdx.x & 63, tok = r / a.group, block = 1 << a.cache.block_log2;
+    const T *q = static_cast<const T *>(a.q) + (t.qs.begin + tok) * a.q_stride + static_cast<int64_t>(kvh * a.group + r % a.group) * D;
+    const Sight see = sight_of(a, t, tok);
+    float x[2], o[2] = {0.0f, 0.0f}, hi = neg_inf(), lo = 0.0f, total = 0.0f;
+    uint32_t big = 0;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        x[w] = lane + 64 * w < D ? load_as_f32<T>(q + lane + 64 * w) : 0.0f;
+        big = max(big, __builtin_bit_cast(uint32_t, x[w]) & 0x7fffffffu);
+    }
+    for (int d = 1; d < 64; d <<= 1) big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), d, 64)));
+    const int e = min(max(static_cast<int>(big >> 23) - 127, -100), 127);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) x[w] = ldexpf(x[w], 14 - e);
+    const int room = 32 - __builtin_clz(t.keys | 1);  // weights add up to 1 at most, so that sums of finite values stay finite
+    for (int i = 0; i < t.steps; ++i) {
+        if (i / run % a.splits != split) continue;
+        const int k0 = t.key_of(i), page = page_of(a.cache, t.s, k0 >> a.cache.block_log2);
+        if (page < 0) continue;
+        const int64_t cell = static_cast<int64_t>(page) * a.cache.kv_heads + kvh;
+        const float2 sizes = a.cache.steps[cell];
+        const uint8_t *codes = a.cache.codes + cell * (2 * block * D);
+        const uint8_t *kc = codes + ((k0 & (block - 1)) + lane) * D;
+        float s = 0.0f;
+        for (int c = 0; c < D; c += 4) {
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(kc + c);
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                s = fmaf(__shfl(c < 64 ? x[0] : x[1], (c + b) & 63, 64), static_cast<float>((w >> (8 * b)) & 0xffu) - 128.0f, s);
+        }
+        const float f = fmaxf(ldexpf(a.scale * kLog2e, e - 14) * sizes.x, 0x1p-126f);
+        const int key = k0 + lane;
+        const bool hidden = key >= see.lim || (key < see.from && key >= t.sinks);
+        if (hidden) s = neg_inf();
+        float mx = s;
+        for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+        const float h = mx * f, l = fmaf(mx, f, -h);
+        if (mx != neg_inf() && (h > hi || (h == hi && l > lo))) {
+            const float alpha = hi == neg_inf() ? 0.0f : exp2f((hi - h) + (lo - l));
+            total *= alpha;
+            o[0] *= alpha;
+            o[1] *= alpha;
+            hi = h;
+            lo = l;
+        }
+        const float p = hidden ? 0.0f : exp2f(hi == neg_inf() ? s : (fmaf(s, f, -hi) - lo) - static_cast<float>(room));
+        float all = p;
+        for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d, 64);
+        total += all;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            if (64 * w >= D) continue;
+            const uint8_t *vc = codes + ((D + min(lane + 64 * w, D - 1)) << a.cache.block_log2) + (k0 & (block - 1));
+            for (int j = 0; j < kStep; j += 4) {
+                const uint32_t v = *reinterpret_cast<const uint32_t *>(vc + j);
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    o[w] = fmaf(__shfl(p, j + b, 64), (static_cast<float>((v >> (8 * b)) & 0xffu) - 128.0f) * sizes.y, o[w]);
+            }
         }
     }
-    if (g != 0) return;
-    if (a.splits > 1) a.part_ml[part] = sum_of(h, l, total, 1.0f);
-    else if (a.lse) a.lse[cell] = log_of(h, l, total);
+    const Place<T, D> place(a, t, split, r, kvh);
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        if (lane + 64 * w >= D) continue;
+        if (a.splits > 1) a.part_o[place.part * D + lane + 64 * w] = o[w] * inv;
+        else store_from_f32<T>(place.to + lane + 64 * w, o[w] * inv);
+    }
+    if (lane == 0) place.sums(a, hi, lo + static_cast<float>(room), total);
 }
 
 // A wave's walk over its steps of a tile: pages and steps of 64 of them at a time, one a lane.
@@ -417,60 +498,54 @@ __global__ void __launch_bounds__(256, 2) cache_rows_kernel(AttendArgs a) {
         if (more) load_k();
         u32x4 pw[KT / 2][P];
         r.weigh(0, w, q.unit[0] * step_k, at, t.cut(at), q.sight[0], t.sinks, pw);
-        r.reach(step_v);
-        const float ratio = r.unit > 0.0f ? step_v / r.unit : 0.0f;
-        if (ratio >= kLeastRatio) {
-            const _Float16 h = static_cast<_Float16>(ratio), b = static_cast<_Float16>(-1152.0f * ratio);
+        const float ratio = r.reach(step_v);
+        const _Float16 h = static_cast<_Float16>(ratio), b = static_cast<_Float16>(-1152.0f * ratio);
 #pragma unroll
-            for (int i = 0; i < C; ++i)
+        for (int i = 0; i < C; ++i)
 #pragma unroll
-                for (int u = 0; u < KT / 2; ++u) {
-                    const u32x4 x = codes_f16(vr[i][2 * u], vr[i][2 * u + 1], f16x2{h, h}, f16x2{b, b});
+            for (int u = 0; u < KT / 2; ++u) {
+                const u32x4 x = codes_f16(vr[i][2 * u], vr[i][2 * u + 1], f16x2{h, h}, f16x2{b, b});
 #pragma unroll
-                    for (int p = P - 1; p >= 0; --p) r.acc[0][i] = product(x, pw[u][p], r.acc[0][i]);
-                }
-        } else if (ratio > 0.0f) {
-#pragma unroll
-            for (int i = 0; i < C; ++i) {
-                f32x4 d = {0, 0, 0, 0};
-#pragma unroll
-                for (int u = 0; u < KT / 2; ++u)
-#pragma unroll
-                    for (int p = P - 1; p >= 0; --p) d = product(codes_f16(vr[i][2 * u], vr[i][2 * u + 1]), pw[u][p], d);
-                r.acc[0][i] += d * ratio;
+                for (int p = P - 1; p >= 0; --p) r.acc[0][i] = product(x, pw[u][p], r.acc[0][i]);
             }
-        }
         if (more) load_v();
     }
 
     // ---- the waves' results, joined by the first
+    const float l = sum_over_groups(r.sum[0]);
+    if (g == 0) part_ml[wave][c] = sum_of(r.base[0], r.again ? 1.0f : 0.0f, l, r.unit);
 #pragma unroll
     for (int i = 0; i < C; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) part[wave][4 * i + e][lane] = r.acc[0][i][e];
-    const float l = sum_over_groups(r.sum[0]);
-    if (g == 0) part_ml[wave][c] = sum_of(r.hi[0], r.lo[0], l, r.unit);
     __syncthreads();
-    if (wave != 0) return;
-    float4 top = sum_of(neg_inf(), 0.0f, 0.0f, 0.0f);
-    float unit = 0.0f, total = 0.0f, y[4 * C];
+    float least = __builtin_inff(), unit = 0.0f, base = neg_inf(), total = 0.0f, y[4 * C];
+    bool again = false;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const float4 m = part_ml[p][c];
-        if (m.z != 0.0f && above_of(m, top)) top = m;
+        again = again || m.y != 0.0f;
+        if (m.z != 0.0f) base = fmaxf(base, m.x);
+        if (m.w > 0.0f) least = fminf(least, m.w);
         unit = fmaxf(unit, m.w);
     }
+    if (again || least < unit * kLeastRatio) {  // the same for the workgroup
+        for (int i = wave; i < min(16, t.nrows - t.r0); i += 4) row_by_keys<T, D>(a, t, split, 4, t.r0 + i, kvh);
+        return;
+    }
+    if (wave != 0) return;
 #pragma unroll
     for (int e = 0; e < 4 * C; ++e) y[e] = 0.0f;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const float4 m = part_ml[p][c];
-        const float wgt = m.z == 0.0f ? 0.0f : weight_of(m, top), scaled = m.w > 0.0f ? wgt * (m.w / unit) : wgt * 0.0f;
+        // (a sum that is a NaN is not 0 and stays)
+        const float wgt = m.z == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m.x - base), scaled = m.w > 0.0f ? wgt * (m.w / unit) : 0.0f;
         total += wgt * m.z;
 #pragma unroll
         for (int e = 0; e < 4 * C; ++e) y[e] += scaled * part[p][e][lane];
     }
-    put<T, D>(a, t, split, t.r0 + c, kvh, y, top.x, top.y, total, unit);
+    put<T, D>(a, t, split, t.r0 + c, kvh, y, base, total, unit);
 }
 
 // Many rows: a tile of 64 NS of one sequence, 16 NS of them for each of the workgroup's four waves.  A step's codes
@@ -497,7 +572,7 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
     const int block = 1 << a.cache.block_log2, head_bytes = 2 * block * D;
     Walk walk = {-1, 0, 0, 0, make_float2(0.0f, 0.0f), nullptr};
     uint32_t kr[D / 16], vr[VT][4];
-    float unit = 0.0f, ratio = 0.0f, step_k = 0.0f, step_v = 0.0f;  // of the step whose codes are fetched
+    float unit = 0.0f, step_k = 0.0f, step_v = 0.0f;  // of the step whose codes are fetched
     const auto fetch = [&]() __attribute__((always_inline)) {
         fetch_keys<D>(walk.codes, walk.k0 & (block - 1), wave, kr);
 #pragma unroll
@@ -511,9 +586,8 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
 #pragma unroll
         for (int j = 0; j < QV; ++j) operands[buffer][wave * QV + j][lane] = codes_f16(kr[2 * j], kr[2 * j + 1]);
         unit = fmaxf(unit, step_v);
-        ratio = unit > 0.0f ? step_v / unit : 0.0f;
-        const bool in = ratio >= kLeastRatio;
-        const _Float16 h = static_cast<_Float16>(in ? ratio : 1.0f), b = static_cast<_Float16>(in ? -1152.0f * ratio : -1152.0f);
+        const float ratio = unit > 0.0f ? step_v / unit : 0.0f;  // as `reach` has it
+        const _Float16 h = static_cast<_Float16>(ratio), b = static_cast<_Float16>(-1152.0f * ratio);
 #pragma unroll
         for (int i = 0; i < VT; ++i)
             if (wave + 4 * i < C) {
@@ -530,63 +604,69 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
     for (int buffer = 0; more; buffer ^= 1) {
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         const int at = walk.k0;
-        const float now_k = step_k, now_v = step_v, now_ratio = ratio;
+        const float now_k = step_k, now_v = step_v;
         more = walk.next(a, t, kvh, split, a.splits, head_bytes);
         if (more) fetch();
         if (r0 < t.nrows) {
+            // operands of the next few products are on their way while these run (the barriers to the compiler's order keep them there)
+            const u32x4 (*from)[64] = operands[buffer];
+            u32x4 x[2][QV], y[2][4];
             f32x4 w[NS][KT];
 #pragma unroll
+            for (int j = 0; j < QV; ++j) x[0][j] = from[j][lane];
+#pragma unroll
             for (int i = 0; i < KT; ++i) {
+                if (i + 1 < KT) {
+#pragma unroll
+                    for (int j = 0; j < QV; ++j) x[(i + 1) & 1][j] = from[(i + 1) * QV + j][lane];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[0][j] = from[KEYS + j][lane];
+                }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int n = 0; n < NS; ++n) w[n][i] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int j = 0; j < QV; ++j) {
-                    const u32x4 x = operands[buffer][i * QV + j][lane];
+                for (int j = 0; j < QV; ++j)
 #pragma unroll
                     for (int n = 0; n < NS; ++n)
 #pragma unroll
-                        for (int p = P - 1; p >= 0; --p) w[n][i] = product(x, q.f[n][j][p], w[n][i]);
-                }
+                        for (int p = P - 1; p >= 0; --p) w[n][i] = product(x[i & 1][j], q.f[n][j][p], w[n][i]);
             }
             const bool cut = t.cut(at);
             u32x4 pw[NS][KT / 2][P];
 #pragma unroll
             for (int n = 0; n < NS; ++n) r.weigh(n, w[n], q.unit[n] * now_k, at, cut, q.sight[n], t.sinks, pw[n]);
             r.reach(now_v);
-            if (now_ratio >= kLeastRatio) {
 #pragma unroll
-                for (int i = 0; i < C; ++i)
+            for (int i = 0; i < C; i += 2) {  // two runs of 16 channels
+                if (i + 2 < C) {
 #pragma unroll
-                    for (int u = 0; u < KT / 2; ++u) {
-                        const u32x4 x = operands[buffer][KEYS + i * (KT / 2) + u][lane];
+                    for (int j = 0; j < 4; ++j) y[(i / 2 + 1) & 1][j] = from[KEYS + (i + 2) * 2 + j][lane];
+                }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int n = 0; n < NS; ++n)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                            for (int p = P - 1; p >= 0; --p) r.acc[n][i] = product(x, pw[n][u][p], r.acc[n][i]);
-                    }
-            } else if (now_ratio > 0.0f) {
+                    for (int n = 0; n < NS; ++n)
 #pragma unroll
-                for (int i = 0; i < C; ++i)
-#pragma unroll
-                    for (int n = 0; n < NS; ++n) {
-                        f32x4 d = {0, 0, 0, 0};
-#pragma unroll
-                        for (int u = 0; u < KT / 2; ++u)
-#pragma unroll
-                            for (int p = P - 1; p >= 0; --p) d = product(operands[buffer][KEYS + i * (KT / 2) + u][lane], pw[n][u][p], d);
-                        r.acc[n][i] += d * now_ratio;
-                    }
+                        for (int p = P - 1; p >= 0; --p)
+                            r.acc[n][i + j / 2] = product(y[(i / 2) & 1][j], pw[n][j & 1][p], r.acc[n][i + j / 2]);
             }
         }
         if (more) lay_out(buffer ^ 1);
     }
     if (r0 >= t.nrows) return;
+    if (r.again) {
+        for (int i = r0; i < min(r0 + 16 * NS, t.nrows); ++i) row_by_keys<T, D>(a, t, split, 1, i, kvh);
+        return;
+    }
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         float y[4 * C];
 #pragma unroll
         for (int e = 0; e < 4 * C; ++e) y[e] = r.acc[n][e / 4][e % 4];
-        put<T, D>(a, t, split, r0 + 16 * n + c, kvh, y, r.hi[n], r.lo[n], sum_over_groups(r.sum[n]), r.unit);
+        put<T, D>(a, t, split, r0 + 16 * n + c, kvh, y, r.base[n], sum_over_groups(r.sum[n]), r.unit);
     }
 }
 
