@@ -33,6 +33,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -46,6 +47,12 @@ constexpr float kUnder = 7.0f, kReach = 15.0f, kFar = 0x1p20f;
 // Values count in units of the largest step met, and a smaller one's ratio goes into its codes: down to 2^-24 they
 // stay exact in half precision.  Rows that meet steps further apart are computed again, key by key.
 constexpr float kLeastRatio = 0x1p-24f;
+
+// step / unit of steps up to the unit, which are powers of two or 0 (below 2^-126: 0).
+__device__ __forceinline__ float ratio_of(float step, float unit) {
+    const int32_t bits = __builtin_bit_cast(int32_t, step) - __builtin_bit_cast(int32_t, unit) + 0x3f800000;
+    return step > 0.0f && bits > 0 ? __builtin_bit_cast(float, bits) : 0.0f;
+}
 
 // A row's sum of weights l relative to base hi + lo.
 __device__ __forceinline__ float4 sum_of(float hi, float lo, float l, float unit) { return make_float4(hi, lo, l, unit); }
@@ -82,6 +89,9 @@ __device__ __forceinline__ u32x4 codes_f16(uint32_t lo, uint32_t hi, f16x2 ratio
 }
 __device__ __forceinline__ f32x4 product(const u32x4 &a, const u32x4 &b, f32x4 d) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), d, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 product(const u32x4 &a, const u32x4 &b, f32x16 d) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), d, 0, 0, 0);
 }
 
 // What a tile of a sequence's rows (query rows times the heads that share a key head) sees, and how its keys are cut into
@@ -128,148 +138,152 @@ __device__ __forceinline__ Tile tile_of(const AttendArgs &a, int64_t tile, int r
     return t;
 }
 
-// A lane's queries: of each set of 16 rows that of its column, in units of a power of two, in P half-precision terms.
-template <class T, int D, int NS>
-struct Queries {
-    static constexpr int P = sizeof(T) == 2 ? 1 : 2, QV = D / 32;
-    u32x4 f[NS][QV][P];
-    float unit[NS];  // binary orders of a score for each unit of its product, before the keys' step
-    Sight sight[NS];
+// A lane's query, that of its column in products of COLUMNS, in units of a power of two, in P half-precision terms.  Lane
+// (c, g) has channels 64 / COLUMNS times 16 apart: 16 side by side from 16g on for two products, and where there is no
+// second one 8 from 8g on.
+template <class T, int D, int COLUMNS>
+struct Query {
+    static constexpr int P = sizeof(T) == 2 ? 1 : 2, G = 64 / COLUMNS, QV = D / (8 * G);
+    u32x4 f[QV][P];
+    float unit;  // binary orders of a score for each unit of its product, before the keys' step
+    Sight sight;
 
     __device__ __forceinline__ void load(const AttendArgs &a, const Tile &t, int r0, int kvh) {
         constexpr bool BF = sizeof(T) == 2;
-        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+        const int lane = threadIdx.x & 63, c = lane % COLUMNS, g = lane / COLUMNS;
+        const int r = min(r0 + c, t.nrows - 1), tok = r / a.group;
+        sight = sight_of(a, t, tok);
+        const T *q = static_cast<const T *>(a.q) + (t.qs.begin + tok) * a.q_stride + static_cast<int64_t>(kvh * a.group + r % a.group) * D;
+        float x[QV][8];
+        uint32_t big = 0;
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            const int r = min(r0 + 16 * n + c, t.nrows - 1), tok = r / a.group;
-            sight[n] = sight_of(a, t, tok);
-            const T *q = static_cast<const T *>(a.q) + (t.qs.begin + tok) * a.q_stride + static_cast<int64_t>(kvh * a.group + r % a.group) * D;
-            float x[QV][8];
-            uint32_t big = 0;
+        for (int j = 0; j < QV; ++j) {
+            const T *qj = q + (j == QV - 1 && QV % 2 ? 8 * G * j + 8 * g : 16 * G * (j / 2) + 16 * g + 8 * (j & 1));
+            constexpr int N = 8 * static_cast<int>(sizeof(T)) / 16;
+            uint4 v[N];
 #pragma unroll
-            for (int j = 0; j < QV; ++j) {
-                // products 2h and 2h + 1: channels 64h + 16g.., 64h + 16g + 8..; a last one by itself: 8g.. of the last 32
-                const T *qj = q + (j == QV - 1 && QV % 2 ? 32 * j + 8 * g : 64 * (j / 2) + 16 * g + 8 * (j & 1));
-                constexpr int N = 8 * static_cast<int>(sizeof(T)) / 16;
-                uint4 v[N];
+            for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const uint4 *>(qj)[i];
+            const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const uint4 *>(qj)[i];
-                const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t u = BF ? (e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16) : w[e];
+                x[j][e] = as_float(u);
+                big = max(big, u & 0x7fffffffu);
+            }
+        }
+        // the row's power: its largest magnitude to [2^14, 2^15).  Magnitudes' bits rise with them, infinities and NaN above
+        // all; their rows keep them, and give NaN.
+        if constexpr (G == 4) big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 16, 64)));
+        big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 32, 64)));
+        const int e = min(max(static_cast<int>(big >> 23) - 127, -100), 127);
+        unit = ldexpf(a.scale * kLog2e, e - 14);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t u = BF ? (e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16) : w[e];
-                    x[j][e] = as_float(u);
-                    big = max(big, u & 0x7fffffffu);
+        for (int j = 0; j < QV; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = ldexpf(x[j][2 * i], 14 - e), v = ldexpf(x[j][2 * i + 1], 14 - e);
+                f[j][0][i] = pack_f16x2(u, v);
+                if constexpr (P == 2) {
+                    const f32x2 h = unpack_f16x2(f[j][0][i]);
+                    f[j][1][i] = pack_f16x2(u - h[0], v - h[1]);
                 }
             }
-            // the row's power: its largest magnitude to [2^14, 2^15).  Magnitudes' bits rise with them, infinities and NaN above
-            // all; their rows keep them, and give NaN.
-            big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 16, 64)));
-            big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 32, 64)));
-            const int e = min(max(static_cast<int>(big >> 23) - 127, -100), 127);
-            unit[n] = ldexpf(a.scale * kLog2e, e - 14);
-#pragma unroll
-            for (int j = 0; j < QV; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float u = ldexpf(x[j][2 * i], 14 - e), v = ldexpf(x[j][2 * i + 1], 14 - e);
-                    f[n][j][0][i] = pack_f16x2(u, v);
-                    if constexpr (P == 2) {
-                        const f32x2 h = unpack_f16x2(f[n][j][0][i]);
-                        f[n][j][1][i] = pack_f16x2(u - h[0], v - h[1]);
-                    }
-                }
-        }
     }
 };
 
-// A lane's running results of NS sets of 16 rows.
-template <int D, int NS, int P>
+// Binary orders of a score for each unit of a product.  Never 0: products of 0 stay 0, hidden ones -inf.
+__device__ __forceinline__ float score_unit(float query, float step_k) { return fmaxf(query * step_k, 0x1p-126f); }
+
+// Largest and sum over the lanes that hold a column.
+template <int COLUMNS>
+__device__ __forceinline__ float column_max(float v) {
+    if constexpr (COLUMNS == 16) return max_over_groups(v);
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(as_float(a[0]), as_float(a[1]));
+}
+template <int COLUMNS>
+__device__ __forceinline__ float column_sum(float v) {
+    if constexpr (COLUMNS == 16) return sum_over_groups(v);
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return as_float(a[0]) + as_float(a[1]);
+}
+
+// A lane's running results of its column's row.  Of a step it holds W products, of keys 16 side by side.
+template <int D, int COLUMNS, int P>
 struct Sums {
-    static constexpr int KT = kStep / 16, C = D / 16;
-    f32x4 acc[NS][C];  // in units of `unit`
-    float sum[NS], base[NS], above[NS];  // above: the score from which on the base moves (-inf: nothing seen yet)
+    static constexpr int W = COLUMNS == 16 ? 16 : 32, G = 64 / COLUMNS, C = D / COLUMNS;
+    typedef float Four __attribute__((ext_vector_type(COLUMNS == 16 ? 4 : 16)));
+    Four acc[C];  // in units of `unit`
+    float sum, base, above;  // above: the score from which on the base moves (-inf: nothing seen yet)
     float unit;
     bool again;  // the rows are to be computed key by key
 
     __device__ __forceinline__ void clear() {
-        unit = 0.0f;
+        unit = sum = base = 0.0f;
+        above = neg_inf();
         again = false;
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            sum[n] = base[n] = 0.0f;
-            above[n] = neg_inf();
-#pragma unroll
-            for (int t = 0; t < C; ++t) acc[n][t] = f32x4{0, 0, 0, 0};
-        }
+        for (int t = 0; t < C; ++t) acc[t] = 0.0f;
     }
 
-    // From a set's products w of a step's keys (the lane's are at + 16g..) to its weights, ready to meet the values.
-    __device__ __forceinline__ void weigh(int n, f32x4 (&w)[KT], float f, int at, bool cut, Sight see, int sinks, u32x4 (&pw)[KT / 2][P]) {
-        if (cut) {
-            // (the first key's place is made here, so that nothing of this is done where no key is hidden)
-            int key = at + 16 * ((threadIdx.x & 63) >> 4);
-            asm volatile("" : "+v"(key));
+    // Hides of a step's products w what the row does not see: the lane's are of keys at + 16g.., and from 16 G on of the next such.
+    __device__ __forceinline__ static void hide(float (&w)[W], int at, Sight see, int sinks) {
+        // (the first key's place is made here, so that nothing of this is done where no key is hidden)
+        int key = at + 16 * ((threadIdx.x & 63) / COLUMNS);
+        asm volatile("" : "+v"(key));
 #pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int k = key + 4 * t + i;
-                    w[t][i] = (k >= see.lim) | ((k < see.from) & (k >= sinks)) ? neg_inf() : w[t][i];
-                }
+        for (int i = 0; i < W; ++i) {
+            const int k = key + (i / 16) * 16 * G + i % 16;
+            w[i] = (k >= see.lim) | ((k < see.from) & (k >= sinks)) ? neg_inf() : w[i];
         }
-        f = fmaxf(f, 0x1p-126f);  // products of 0 stay 0, hidden ones -inf
+    }
+    // Moves the base where a weight would pass its reach; f: binary orders of a score for each unit of a product.
+    __device__ __forceinline__ void settle(const float (&w)[W], float f) {
         float mx = neg_inf();
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+        for (int i = 0; i < W; ++i) mx = fmaxf(mx, w[i]);
+        if (__builtin_amdgcn_ballot_w64(mx * f > above) == 0) return;
+        mx = column_max<COLUMNS>(mx) * f;
+        const bool over = mx > above;
+        const float to = over ? mx - kUnder : base;
+        const float alpha = above == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(base - to);
+        sum *= alpha;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, w[t][i]);
-        if (__builtin_amdgcn_ballot_w64(mx * f > above[n]) != 0) {
-            mx = max_over_groups(mx) * f;
-            const bool over = mx > above[n];
-            const float to = over ? mx - kUnder : base[n];
-            const float alpha = above[n] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(base[n] - to);
-            sum[n] *= alpha;
-#pragma unroll
-            for (int t = 0; t < C; ++t) acc[n][t] *= alpha;
-            base[n] = to;
-            above[n] = over ? to + kReach : above[n];
-            // (past float32's range a row is NaN either way)
-            again = again || __builtin_amdgcn_ballot_w64(fabsf(to) >= kFar && fabsf(to) < __builtin_inff()) != 0;
-        }
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[t][i] = __builtin_amdgcn_exp2f(fmaf(w[t][i], f, -base[n]));
-        // their sum in 32 bits, before they are rounded
-#pragma unroll
-        for (int t = 0; t < KT; ++t) sum[n] += (w[t][0] + w[t][1]) + (w[t][2] + w[t][3]);
-        // half precision keeps 11 bits of a weight (2^-11 off at most), two terms 22
-#pragma unroll
-        for (int u = 0; u < KT / 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = w[2 * u + (i >> 1)][2 * (i & 1)], y = w[2 * u + (i >> 1)][2 * (i & 1) + 1];
-                pw[u][0][i] = pack_f16x2(x, y);
-                if constexpr (P == 2) {
-                    const f32x2 t = unpack_f16x2(pw[u][0][i]);
-                    pw[u][1][i] = pack_f16x2(x - t[0], y - t[1]);
-                }
-            }
+        for (int t = 0; t < C; ++t) acc[t] *= alpha;
+        base = to;
+        above = over ? to + kReach : above;
+        // (past float32's range a row is NaN either way)
+        again = again || __builtin_amdgcn_ballot_w64(fabsf(to) >= kFar && fabsf(to) < __builtin_inff()) != 0;
     }
-
+    // The weights of products 4i..: their sum in 32 bits, before they are rounded; then half precision keeps 11 bits of a weight (2^-11
+    // off at most), two terms 22.
+    __device__ __forceinline__ void weigh(int i, const float (&w)[W], float f, u32x4 (&pw)[W / 8][P]) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(w[4 * i + e], f, -base));
+        sum += (x[0] + x[1]) + (x[2] + x[3]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t high = pack_f16x2(x[2 * e], x[2 * e + 1]);
+            pw[i / 2][0][2 * (i & 1) + e] = high;
+            if constexpr (P == 2) {
+                const f32x2 h = unpack_f16x2(high);
+                pw[i / 2][1][2 * (i & 1) + e] = pack_f16x2(x[2 * e] - h[0], x[2 * e + 1] - h[1]);
+            }
+        }
+    }
     // Makes the unit at least a step of values; the step's ratio to it.
     __device__ __forceinline__ float reach(float step_v) {
         if (step_v > unit) {
-            const float ratio = unit / step_v;  // powers of two, or 0
+            const float ratio = ratio_of(unit, step_v);
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-                for (int t = 0; t < C; ++t) acc[n][t] *= ratio;
+            for (int t = 0; t < C; ++t) acc[t] *= ratio;
             again = again || (ratio < kLeastRatio && unit > 0.0f);
             unit = step_v;
         }
-        const float ratio = unit > 0.0f ? step_v / unit : 0.0f;
+        const float ratio = ratio_of(step_v, unit);
         again = again || (ratio < kLeastRatio && step_v > 0.0f);
         return ratio;
     }
@@ -294,20 +308,22 @@ struct Place {
     }
 };
 
-// A row's channels 16t + 4g.. out: divided by the sum before the unit, so that means of finite values are finite.
-template <class T, int D>
-__device__ __forceinline__ void put(const AttendArgs &a, const Tile &t, int split, int r, int kvh, const float (&y)[D / 4], float base,
-                                    float total, float unit) {
-    const int g = (threadIdx.x & 63) >> 4;
+// A row's channels out, the lane's D / G of them, four side by side 4 G apart: divided by the sum before the unit, so that
+// means of finite values are finite.
+template <class T, int D, int COLUMNS>
+__device__ __forceinline__ void put(const AttendArgs &a, const Tile &t, int split, int r, int kvh, const float (&y)[D * COLUMNS / 64],
+                                    float base, float total, float unit) {
+    const int g = (threadIdx.x & 63) / COLUMNS;
     if (r >= t.nrows) return;
     const Place<T, D> place(a, t, split, r, kvh);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e) {
+    for (int e = 0; e < D * COLUMNS / 256; ++e) {
         const f32x4 z = {y[4 * e] * inv * unit, y[4 * e + 1] * inv * unit, y[4 * e + 2] * inv * unit, y[4 * e + 3] * inv * unit};
-        if (a.splits > 1) *reinterpret_cast<f32x4 *>(a.part_o + place.part * D + 16 * e + 4 * g) = z;
-        else if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2 *>(place.to + 16 * e + 4 * g) = u32x2{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3])};
-        else *reinterpret_cast<f32x4 *>(place.to + 16 * e + 4 * g) = z;
+        const int ch = 256 / COLUMNS * e + 4 * g;
+        if (a.splits > 1) *reinterpret_cast<f32x4 *>(a.part_o + place.part * D + ch) = z;
+        else if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2 *>(place.to + ch) = u32x2{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3])};
+        else *reinterpret_cast<f32x4 *>(place.to + ch) = z;
     }
     if (g == 0) place.sums(a, base, 0.0f, total);
 }
@@ -419,15 +435,17 @@ struct Walk {
 };
 
 // The operands of a step as they lie in a page.  S^T = K Q^T and O^T = V^T P^T, so that what one product leaves in a
-// lane is what the next one wants there.  A 16x16 product leaves lane (c, g) = (lane & 15, lane >> 4) with rows 4g..4g+3 of
-// column c; product t of a step takes key 16 (c >> 2) + 4t + (c & 3) as its row c, so that lane
-// (c, g) gets keys 16g + 4t + i of query c: the lane's 16 weights are of keys 16g..16g+15, and the
-// values' operand wants the same keys of a channel: one 16-byte piece of the cache.
-// The keys' operand wants channels of a row, in any order that the queries share: 16 side by side for two products.
+// lane is what the next one wants there.  A product of 16 (32) columns leaves lane (c, g) = (lane % 16, lane / 16) with
+// four rows of column c, 4g.., (with four such, 8 apart).  Rows take keys so that over a step lane (c, g) gets keys
+// 16g..16g+15 of query c (and 32 + 16g..): then the values' operand wants 16 keys side by side of a channel, one 16-byte
+// piece of the cache.  The keys' operand wants channels of a row, in any order that the queries share: 16 side by
+// side for two products.
+//
+// 16 columns, product t of a step: 16 rows.
 template <int D>
-__device__ __forceinline__ void fetch_keys(const uint8_t *codes, int place, int t, uint32_t (&w)[D / 16]) {
+__device__ __forceinline__ void fetch_keys16(const uint8_t *codes, int place, int t, uint32_t (&w)[D / 16]) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const uint8_t *p = codes + place * D + (16 * (c >> 2) + (c & 3)) * D + 4 * t * D;
+    const uint8_t *p = codes + (place + 16 * (c >> 2) + 4 * t + (c & 3)) * D;
 #pragma unroll
     for (int h = 0; h < D / 64; ++h) {
         const uint4 v = *reinterpret_cast<const uint4 *>(p + 64 * h + 16 * g);
@@ -438,42 +456,76 @@ __device__ __forceinline__ void fetch_keys(const uint8_t *codes, int place, int 
         w[D / 16 - 2] = v.x, w[D / 16 - 1] = v.y;
     }
 }
+// ... 16 channels from 16t on, of 64 keys.
 template <int D>
-__device__ __forceinline__ void fetch_values(const uint8_t *codes, int block_log2, int place, int t, uint32_t (&w)[4]) {
+__device__ __forceinline__ uint4 fetch_values16(const uint8_t *codes, int block_log2, int place, int t) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const uint4 v = *reinterpret_cast<const uint4 *>(codes + ((D + 16 * t + c) << block_log2) + place + 16 * g);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    return *reinterpret_cast<const uint4 *>(codes + ((D + 16 * t + c) << block_log2) + place + 16 * g);
+}
+// 32 columns: 32 keys of the step's half t, 32 channels from 32h on.
+template <int D>
+__device__ __forceinline__ uint4 fetch_keys32(const uint8_t *codes, int place, int t, int h) {
+    const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+    // row 8i + 4g' + j of a product is lane group g's product 4i + j: key 16g' + 4i + j of the half
+    const int key = 32 * t + 16 * ((c >> 2) & 1) + 4 * (c >> 3) + (c & 3);
+    return *reinterpret_cast<const uint4 *>(codes + (place + key) * D + 32 * h + 16 * g);
+}
+// ... the same channels of the same keys.
+template <int D>
+__device__ __forceinline__ uint4 fetch_values32(const uint8_t *codes, int block_log2, int place, int t, int h) {
+    const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
+    return *reinterpret_cast<const uint4 *>(codes + ((D + 32 * h + c) << block_log2) + place + 32 * t + 16 * g);
 }
 
-// Few rows: a tile of 16 of one sequence.  The workgroup's four waves take every fourth step each, and join through LDS.
+// Few rows: a tile of 16 or 32 of one sequence.  The workgroup's four waves take every fourth step each, and join through LDS.
 // Codes go from memory to a product's registers through two instructions for every four, without LDS; the next step's
 // keys are on their way from the first product on, its values from the last.
-template <class T, int D>
+template <class T, int D, int COLUMNS>
 __global__ void __launch_bounds__(256, 2) cache_rows_kernel(AttendArgs a) {
-    using Q = Queries<T, D, 1>;
-    constexpr int P = Q::P, QV = Q::QV, KT = kStep / 16, C = D / 16;
-    __shared__ float part[4][4 * C][64];
-    __shared__ float4 part_ml[4][16];
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    using Q = Query<T, D, COLUMNS>;
+    using S = Sums<D, COLUMNS, Q::P>;
+    constexpr int P = Q::P, QV = Q::QV, W = S::W, KT = kStep / COLUMNS, C = S::C, Y = D * COLUMNS / 64;
+    constexpr int E = COLUMNS * COLUMNS / 64;  // values of a product that a lane holds
+    __shared__ float part[4][Y][64];
+    __shared__ float4 part_ml[4][COLUMNS];
+    const int lane = threadIdx.x & 63, c = lane % COLUMNS, g = lane / COLUMNS;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int id = xcd_tile(blockIdx.x, gridDim.x);
     const int split = id / a.tile_groups % a.splits, kvh = id / a.tile_groups / a.splits;
-    const Tile t = tile_of(a, id % a.tile_groups, 16, 4);
+    const Tile t = tile_of(a, id % a.tile_groups, COLUMNS, COLUMNS == 16 ? 4 : 5);
     if (t.nrows == 0) return;
     Q q;
     q.load(a, t, t.r0, kvh);
-    Sums<D, 1, P> r;
+    S r;
     r.clear();
     const int piece = split * 4 + wave, pieces = a.splits * 4, block = 1 << a.cache.block_log2, head_bytes = 2 * block * D;
     Walk walk = {-1, 0, 0, 0, make_float2(0.0f, 0.0f), nullptr};
-    uint32_t kr[KT][D / 16], vr[C][4];
+    uint32_t kr[KT][2 * QV];  // two dwords a product
+    uint32_t vr[C][W / 4];    // a dword for four keys
     const auto load_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < KT; ++i) fetch_keys<D>(walk.codes, walk.k0 & (block - 1), i, kr[i]);
+        for (int i = 0; i < KT; ++i) {
+            if constexpr (COLUMNS == 16) {
+                fetch_keys16<D>(walk.codes, walk.k0 & (block - 1), i, kr[i]);
+            } else {
+#pragma unroll
+                for (int h = 0; h < C; ++h) {
+                    const uint4 w = fetch_keys32<D>(walk.codes, walk.k0 & (block - 1), i, h);
+                    kr[i][4 * h] = w.x, kr[i][4 * h + 1] = w.y, kr[i][4 * h + 2] = w.z, kr[i][4 * h + 3] = w.w;
+                }
+            }
+        }
     };
     const auto load_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < C; ++i) fetch_values<D>(walk.codes, a.cache.block_log2, walk.k0 & (block - 1), i, vr[i]);
+        for (int i = 0; i < C; ++i)
+#pragma unroll
+            for (int h = 0; h < W / 16; ++h) {
+                uint4 w;
+                if constexpr (COLUMNS == 16) w = fetch_values16<D>(walk.codes, a.cache.block_log2, walk.k0 & (block - 1), i);
+                else w = fetch_values32<D>(walk.codes, a.cache.block_log2, walk.k0 & (block - 1), h, i);
+                vr[i][4 * h] = w.x, vr[i][4 * h + 1] = w.y, vr[i][4 * h + 2] = w.z, vr[i][4 * h + 3] = w.w;
+            }
     };
     bool more = walk.next(a, t, kvh, piece, pieces, head_bytes);
     if (more) {
@@ -483,43 +535,47 @@ __global__ void __launch_bounds__(256, 2) cache_rows_kernel(AttendArgs a) {
     while (more) {
         const float step_k = walk.step_k(), step_v = walk.step_v();
         const int at = walk.k0;
-        f32x4 w[KT];
+        float w[W];
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
-            w[i] = f32x4{0, 0, 0, 0};
+            typename S::Four d = {};
 #pragma unroll
             for (int j = 0; j < QV; ++j) {
                 const u32x4 x = codes_f16(kr[i][2 * j], kr[i][2 * j + 1]);
 #pragma unroll
-                for (int p = P - 1; p >= 0; --p) w[i] = product(x, q.f[0][j][p], w[i]);
+                for (int p = P - 1; p >= 0; --p) d = product(x, q.f[j][p], d);
             }
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[E * i + e] = d[e];
         }
         more = walk.next(a, t, kvh, piece, pieces, head_bytes);
         if (more) load_k();
-        u32x4 pw[KT / 2][P];
-        r.weigh(0, w, q.unit[0] * step_k, at, t.cut(at), q.sight[0], t.sinks, pw);
+        u32x4 pw[W / 8][P];
+        if (t.cut(at)) r.hide(w, at, q.sight, t.sinks);
+        const float f = score_unit(q.unit, step_k);
+        r.settle(w, f);
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) r.weigh(i, w, f, pw);
         const float ratio = r.reach(step_v);
         const _Float16 h = static_cast<_Float16>(ratio), b = static_cast<_Float16>(-1152.0f * ratio);
 #pragma unroll
         for (int i = 0; i < C; ++i)
 #pragma unroll
-            for (int u = 0; u < KT / 2; ++u) {
+            for (int u = 0; u < W / 8; ++u) {
                 const u32x4 x = codes_f16(vr[i][2 * u], vr[i][2 * u + 1], f16x2{h, h}, f16x2{b, b});
 #pragma unroll
-                for (int p = P - 1; p >= 0; --p) r.acc[0][i] = product(x, pw[u][p], r.acc[0][i]);
+                for (int p = P - 1; p >= 0; --p) r.acc[i] = product(x, pw[u][p], r.acc[i]);
             }
         if (more) load_v();
     }
 
     // ---- the waves' results, joined by the first
-    const float l = sum_over_groups(r.sum[0]);
-    if (g == 0) part_ml[wave][c] = sum_of(r.base[0], r.again ? 1.0f : 0.0f, l, r.unit);
+    const float l = column_sum<COLUMNS>(r.sum);
+    if (g == 0) part_ml[wave][c] = sum_of(r.base, r.again ? 1.0f : 0.0f, l, r.unit);
 #pragma unroll
-    for (int i = 0; i < C; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) part[wave][4 * i + e][lane] = r.acc[0][i][e];
+    for (int e = 0; e < Y; ++e) part[wave][e][lane] = r.acc[e / E][e % E];
     __syncthreads();
-    float least = __builtin_inff(), unit = 0.0f, base = neg_inf(), total = 0.0f, y[4 * C];
+    float least = __builtin_inff(), unit = 0.0f, base = neg_inf(), total = 0.0f;
     bool again = false;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
@@ -530,144 +586,200 @@ __global__ void __launch_bounds__(256, 2) cache_rows_kernel(AttendArgs a) {
         unit = fmaxf(unit, m.w);
     }
     if (again || least < unit * kLeastRatio) {  // the same for the workgroup
-        for (int i = wave; i < min(16, t.nrows - t.r0); i += 4) row_by_keys<T, D>(a, t, split, 4, t.r0 + i, kvh);
+        for (int i = wave; i < min(COLUMNS, t.nrows - t.r0); i += 4) row_by_keys<T, D>(a, t, split, 4, t.r0 + i, kvh);
         return;
     }
     if (wave != 0) return;
+    float y[Y];
 #pragma unroll
-    for (int e = 0; e < 4 * C; ++e) y[e] = 0.0f;
+    for (int e = 0; e < Y; ++e) y[e] = 0.0f;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const float4 m = part_ml[p][c];
         // (a sum that is a NaN is not 0 and stays)
-        const float wgt = m.z == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m.x - base), scaled = m.w > 0.0f ? wgt * (m.w / unit) : 0.0f;
+        const float wgt = m.z == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m.x - base), scaled = wgt * ratio_of(m.w, unit);
         total += wgt * m.z;
 #pragma unroll
-        for (int e = 0; e < 4 * C; ++e) y[e] += scaled * part[p][e][lane];
+        for (int e = 0; e < Y; ++e) y[e] += scaled * part[p][e][lane];
     }
-    put<T, D>(a, t, split, t.r0 + c, kvh, y, base, total, unit);
+    put<T, D, COLUMNS>(a, t, split, t.r0 + c, kvh, y, base, total, unit);
 }
 
-// Many rows: a tile of 64 NS of one sequence, 16 NS of them for each of the workgroup's four waves.  A step's codes
+// Many rows: a tile of 128 of one sequence, 32 of them for each of the workgroup's four waves.  A step's codes
 // become half precision once, a quarter of them by each wave, and lie in LDS (two buffers, one barrier a step) as the
 // products' operands, lane by lane: reads and writes are whole rows of 1 KiB.
-template <class T, int D, int NS>
+//
+template <class T, int D>
 __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
-    using Q = Queries<T, D, NS>;
-    constexpr int P = Q::P, QV = Q::QV, KT = kStep / 16, C = D / 16, VT = (C + 3) / 4;
-    constexpr int KEYS = KT * QV, VALUES = C * (KT / 2);  // operands of a step, 1 KiB each
-    __shared__ u32x4 operands[2][KEYS + VALUES][64];
-    const int lane = threadIdx.x & 63, c = lane & 15;
+    using Q = Query<T, D, 32>;
+    constexpr int P = Q::P, QV = Q::QV, C = D / 32;
+    constexpr int PIECES = 2 * C, MINE = (PIECES + 3) / 4;  // of 32 keys and 32 channels: a 16-byte piece a lane, two operands
+    __shared__ u32x4 key_rows[2][2 * PIECES][64], value_rows[2][2 * PIECES][64];
+    const int lane = threadIdx.x & 63, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // consecutive workgroups of one XCD run neighbouring tiles of a head: its L2 holds their keys
     const int id = xcd_tile(blockIdx.x, gridDim.x);
     const int split = id / a.tile_groups % a.splits, kvh = id / a.tile_groups / a.splits;
-    const Tile t = tile_of(a, id % a.tile_groups, 64 * NS, NS == 1 ? 6 : NS == 2 ? 7 : 8);
+    const Tile t = tile_of(a, id % a.tile_groups, 128, 7);
     if (t.nrows == 0) return;
-    const int r0 = t.r0 + 16 * NS * wave;
+    const int r0 = t.r0 + 32 * wave;
     Q q;
     q.load(a, t, r0, kvh);
-    Sums<D, NS, P> r;
+    Sums<D, 32, P> r;
     r.clear();
     const int block = 1 << a.cache.block_log2, head_bytes = 2 * block * D;
     Walk walk = {-1, 0, 0, 0, make_float2(0.0f, 0.0f), nullptr};
-    uint32_t kr[D / 16], vr[VT][4];
-    float unit = 0.0f, step_k = 0.0f, step_v = 0.0f;  // of the step whose codes are fetched
-    const auto fetch = [&]() __attribute__((always_inline)) {
-        fetch_keys<D>(walk.codes, walk.k0 & (block - 1), wave, kr);
-#pragma unroll
-        for (int i = 0; i < VT; ++i)
-            if (wave + 4 * i < C) fetch_values<D>(walk.codes, a.cache.block_log2, walk.k0 & (block - 1), wave + 4 * i, vr[i]);
-        step_k = walk.step_k();
-        step_v = walk.step_v();
+    uint4 kr[MINE], vr[MINE];
+    float unit = 0.0f;  // of the last values laid out
+    // A step on its way: whether it is one, its codes' page, first key and steps.
+    struct Step {
+        bool is;
+        const uint8_t *codes;
+        int at;
+        float step_k, step_v;
     };
-    // fetched codes to a buffer
-    const auto lay_out = [&](int buffer) __attribute__((always_inline)) {
+    const auto next = [&]() __attribute__((always_inline)) {  // the same for all waves
+        Step x = {walk.next(a, t, kvh, split, a.splits, head_bytes), walk.codes, walk.k0, 0.0f, 0.0f};
+        if (x.is) x.step_k = walk.step_k(), x.step_v = walk.step_v();
+        return x;
+    };
+    const auto fetch_k = [&](const Step &x) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < QV; ++j) operands[buffer][wave * QV + j][lane] = codes_f16(kr[2 * j], kr[2 * j + 1]);
-        unit = fmaxf(unit, step_v);
-        const float ratio = unit > 0.0f ? step_v / unit : 0.0f;  // as `reach` has it
+        for (int i = 0; i < MINE; ++i)
+            if (wave + 4 * i < PIECES) kr[i] = fetch_keys32<D>(x.codes, x.at & (block - 1), (wave + 4 * i) / C, (wave + 4 * i) % C);
+    };
+    const auto fetch_v = [&](const Step &x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+            if (wave + 4 * i < PIECES)
+                vr[i] = fetch_values32<D>(x.codes, a.cache.block_log2, x.at & (block - 1), (wave + 4 * i) / C, (wave + 4 * i) % C);
+    };
+    // keys: operand 2h + b of half t; values: operand b of half t and channels 32h..
+    const auto put_k = [&](int buffer) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+            if (wave + 4 * i < PIECES) {
+                key_rows[buffer][2 * (wave + 4 * i)][lane] = codes_f16(kr[i].x, kr[i].y);
+                key_rows[buffer][2 * (wave + 4 * i) + 1][lane] = codes_f16(kr[i].z, kr[i].w);
+            }
+    };
+    const auto put_v = [&](int buffer, const Step &x) __attribute__((always_inline)) {
+        unit = fmaxf(unit, x.step_v);
+        const float ratio = ratio_of(x.step_v, unit);  // as `reach` has it
         const _Float16 h = static_cast<_Float16>(ratio), b = static_cast<_Float16>(-1152.0f * ratio);
 #pragma unroll
-        for (int i = 0; i < VT; ++i)
-            if (wave + 4 * i < C) {
-#pragma unroll
-                for (int u = 0; u < KT / 2; ++u)
-                    operands[buffer][KEYS + (wave + 4 * i) * (KT / 2) + u][lane] = codes_f16(vr[i][2 * u], vr[i][2 * u + 1], f16x2{h, h}, f16x2{b, b});
+        for (int i = 0; i < MINE; ++i)
+            if (wave + 4 * i < PIECES) {
+                value_rows[buffer][2 * (wave + 4 * i)][lane] = codes_f16(vr[i].x, vr[i].y, f16x2{h, h}, f16x2{b, b});
+                value_rows[buffer][2 * (wave + 4 * i) + 1][lane] = codes_f16(vr[i].z, vr[i].w, f16x2{h, h}, f16x2{b, b});
             }
     };
-    bool more = walk.next(a, t, kvh, split, a.splits, head_bytes);  // the same for all waves
-    if (more) {
-        fetch();
-        lay_out(0);
-    }
-    for (int buffer = 0; more; buffer ^= 1) {
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const int at = walk.k0;
-        const float now_k = step_k, now_v = step_v;
-        more = walk.next(a, t, kvh, split, a.splits, head_bytes);
-        if (more) fetch();
-        if (r0 < t.nrows) {
-            // operands of the next few products are on their way while these run (the barriers to the compiler's order keep them there)
-            const u32x4 (*from)[64] = operands[buffer];
-            u32x4 x[2][QV], y[2][4];
-            f32x4 w[NS][KT];
+    const auto together = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    float w[32], f = 0.0f;
+    u32x4 pw[4][P];
+    // S^T; operands of the next products are on their way while some run (the barriers to the compiler's order keep them there)
+    const auto scores = [&](const u32x4 (*keys)[64]) __attribute__((always_inline)) {
+        f32x16 d[2];
+        const f32x16 zeros = {};
+        u32x4 x[3][2];
 #pragma unroll
-            for (int j = 0; j < QV; ++j) x[0][j] = from[j][lane];
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < KT; ++i) {
-                if (i + 1 < KT) {
+            for (int i = 0; i < 2; ++i) x[j][i] = keys[i * QV + j][lane];
 #pragma unroll
-                    for (int j = 0; j < QV; ++j) x[(i + 1) & 1][j] = from[(i + 1) * QV + j][lane];
-                } else {
+        for (int j = 0; j < QV; ++j) {
+            if (j + 2 < QV) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) y[0][j] = from[KEYS + j][lane];
-                }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int n = 0; n < NS; ++n) w[n][i] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int j = 0; j < QV; ++j)
-#pragma unroll
-                    for (int n = 0; n < NS; ++n)
-#pragma unroll
-                        for (int p = P - 1; p >= 0; --p) w[n][i] = product(x[i & 1][j], q.f[n][j][p], w[n][i]);
+                for (int i = 0; i < 2; ++i) x[(j + 2) % 3][i] = keys[i * QV + j + 2][lane];
             }
-            const bool cut = t.cut(at);
-            u32x4 pw[NS][KT / 2][P];
 #pragma unroll
-            for (int n = 0; n < NS; ++n) r.weigh(n, w[n], q.unit[n] * now_k, at, cut, q.sight[n], t.sinks, pw[n]);
-            r.reach(now_v);
+            for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-            for (int i = 0; i < C; i += 2) {  // two runs of 16 channels
-                if (i + 2 < C) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) y[(i / 2 + 1) & 1][j] = from[KEYS + (i + 2) * 2 + j][lane];
-                }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int n = 0; n < NS; ++n)
-#pragma unroll
-                        for (int p = P - 1; p >= 0; --p)
-                            r.acc[n][i + j / 2] = product(y[(i / 2) & 1][j], pw[n][j & 1][p], r.acc[n][i + j / 2]);
-            }
+                for (int i = 0; i < 2; ++i) d[i] = product(x[j % 3][i], q.f[j][p], j == 0 && p == P - 1 ? zeros : d[i]);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (more) lay_out(buffer ^ 1);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w[i] = d[i / 16][i % 16];
+    };
+    // O^T
+    const auto meet = [&](const u32x4 (*values)[64], float step_v) __attribute__((always_inline)) {
+        r.reach(step_v);
+        // operand b of half t and channels 32h.. stands at 2 (C t + h) + b
+        u32x4 y[2][C];
+#pragma unroll
+        for (int h = 0; h < C; ++h) y[0][h] = values[2 * h][lane];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (u < 3) {
+#pragma unroll
+                for (int h = 0; h < C; ++h) y[(u + 1) & 1][h] = values[2 * (C * ((u + 1) / 2) + h) + ((u + 1) & 1)][lane];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+                for (int h = 0; h < C; ++h) r.acc[h] = product(y[u & 1][h], pw[u][p], r.acc[h]);
+        }
+    };
+    // ---- the first step's operands; the second's codes on their way
+    Step now = next(), then = {false, nullptr, 0, 0.0f, 0.0f};
+    if (now.is) {
+        fetch_k(now);
+        fetch_v(now);
+        put_k(0);
+        put_v(0, now);
+        then = next();
+        if (then.is) {
+            fetch_k(then);
+            fetch_v(then);
+        }
     }
-    if (r0 >= t.nrows) return;
-    if (r.again) {
-        for (int i = r0; i < min(r0 + 16 * NS, t.nrows); ++i) row_by_keys<T, D>(a, t, split, 1, i, kvh);
+    Step after;
+    int buffer = 0;
+    // the workgroup's part of a step: the next one's operands to the other buffers, the codes behind them on their way
+    const auto share = [&]() __attribute__((always_inline)) {
+        together();
+        after = {false, nullptr, 0, 0.0f, 0.0f};
+        if (!then.is) return;
+        put_k(buffer ^ 1);
+        put_v(buffer ^ 1, then);
+        after = next();
+        if (after.is) {
+            fetch_k(after);
+            fetch_v(after);
+        }
+    };
+    const auto advance = [&]() __attribute__((always_inline)) {
+        now = then;
+        then = after;
+        buffer ^= 1;
+    };
+    if (r0 >= t.nrows) {  // no rows for this wave
+        for (; now.is; advance()) share();
         return;
     }
+    for (; now.is; advance()) {
+        share();
+        __builtin_amdgcn_s_setprio(1);  // products before the other wave's vector work: 677 -> 667 us
+        scores(key_rows[buffer]);
+        __builtin_amdgcn_s_setprio(0);
+        f = score_unit(q.unit, now.step_k);
+        if (t.cut(now.at)) r.hide(w, now.at, q.sight, t.sinks);
+        r.settle(w, f);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-        float y[4 * C];
-#pragma unroll
-        for (int e = 0; e < 4 * C; ++e) y[e] = r.acc[n][e / 4][e % 4];
-        put<T, D>(a, t, split, r0 + 16 * n + c, kvh, y, r.base[n], sum_over_groups(r.sum[n]), r.unit);
+        for (int i = 0; i < 8; ++i) r.weigh(i, w, f, pw);
+        __builtin_amdgcn_s_setprio(1);
+        meet(value_rows[buffer], now.step_v);
+        __builtin_amdgcn_s_setprio(0);
     }
+    if (r.again) {
+        for (int i = r0; i < min(r0 + 32, t.nrows); ++i) row_by_keys<T, D>(a, t, split, 1, i, kvh);
+        return;
+    }
+    float y[D / 2];
+#pragma unroll
+    for (int e = 0; e < D / 2; ++e) y[e] = r.acc[e / 16][e % 16];
+    put<T, D, 32>(a, t, split, r0 + c, kvh, y, r.base, column_sum<32>(r.sum), r.unit);
 }
 
 // Joins the pieces of each (row, head), in their order; a wave each.
@@ -718,28 +830,29 @@ __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
     if (a.lse && lane == 0) a.lse[cell] = log_of(top.x, top.y, total);
 }
 
-// How a call is cut: by sequences' mean rows into tiles of 16 (four waves share a tile's keys) or of 64 and 128 (four waves share
+// How a call is cut: by sequences' mean rows into tiles of 16 or 32 (four waves share a tile's keys) or of 128 (four waves share
 // its rows), an upper bound of each, as the lengths are on the device; and, where there would be fewer than two waves for each
 // SIMD, every tile's keys over several workgroups, with at least four steps a wave.
 struct Cut {
     int64_t tile_groups;
-    int32_t splits, sets;  // 0: tiles of 16 rows
+    int32_t splits, rows;  // of a tile
 };
-Cut cut_of(int64_t total_q, int32_t heads, int32_t kv_heads, int32_t d, int64_t sequences, int64_t max_k, int32_t window, int32_t sinks) {
+Cut cut_of(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, int64_t max_k, int32_t window, int32_t sinks) {
     constexpr int64_t kGroups = 256 * 2;
-    const int64_t rows = total_q * (heads / kv_heads), per = rows / std::max<int64_t>(sequences, 1);
-    const int32_t sets = per <= 16 ? 0 : per <= 64 ? 1 : 2;
-    const int64_t tiles = rows / (sets == 0 ? 16 : 64 * sets) + sequences, groups = std::max<int64_t>(tiles * kv_heads, 1);
+    const int64_t rows = total_q * (heads / kv_heads), each = std::max<int64_t>(sequences, 1), per = (rows + each - 1) / each;
+    const int32_t tile = per <= 16 ? 16 : per <= 64 ? 32 : 128;
+    // (of sequences of one length, which take fewer than the bound)
+    const int64_t groups = std::max<int64_t>(each * ((per + tile - 1) / tile) * kv_heads, 1);
     const int64_t keys = window ? std::min<int64_t>(max_k, static_cast<int64_t>(window) + sinks + per + 2 * kStep) : max_k;
     int32_t splits = 1;
-    while (splits < 64 && groups * splits * 2 <= kGroups && keys >= (sets == 0 ? 16 : 4) * kStep * splits) splits *= 2;
-    return {tiles, splits, sets};
+    while (splits < 64 && groups * splits * 2 <= kGroups && keys >= (tile == 128 ? 4 : 16) * kStep * splits) splits *= 2;
+    return {rows / tile + sequences, splits, tile};
 }
 
 using AttendFn = void (*)(AttendArgs);
 template <class T, int D>
 AttendFn pick_tile(const Cut &cut) {
-    return cut.sets == 0 ? cache_rows_kernel<T, D> : cut.sets == 1 ? cache_chunk_kernel<T, D, 1> : cache_chunk_kernel<T, D, 2>;
+    return cut.rows == 16 ? cache_rows_kernel<T, D, 16> : cut.rows == 32 ? cache_rows_kernel<T, D, 32> : cache_chunk_kernel<T, D>;
 }
 template <class T>
 AttendFn pick_attend(int32_t d, const Cut &cut) {
@@ -774,7 +887,7 @@ S3DX_API s3dx_status s3dx_cache_attention_workspace_size(const s3dx_cache *cache
     return boundary(error, error_capacity, [&] {
         require(bytes, "bytes is NULL");
         check_call(cache, total_q, heads, sequences, max_k, window, sinks);
-        const Cut cut = cut_of(total_q, heads, cache->kv_heads, cache->head_dim, sequences, max_k, window, sinks);
+        const Cut cut = cut_of(total_q, heads, cache->kv_heads, sequences, max_k, window, sinks);
         *bytes = 0;
         if (cut.splits == 1) return;
         Sizer z;
@@ -806,7 +919,7 @@ S3DX_API s3dx_status s3dx_cache_attention(const s3dx_cache *cache, const void *q
         }
         require(q_starts && aligned(q_starts, 4), "starts is NULL or not aligned");
         require(!lse || aligned(lse, 4), "lse is not aligned");
-        const Cut cut = cut_of(total_q, heads, cache->kv_heads, cache->head_dim, sequences, max_k, window, sinks);
+        const Cut cut = cut_of(total_q, heads, cache->kv_heads, sequences, max_k, window, sinks);
         AttendArgs a = {view_of(cache, table, table_stride, lengths), q, o, lse, q_starts, total_q, q_stride, o_stride, sequences,
                         heads, heads / cache->kv_heads, flags & S3DX_BLOCK_CAUSAL, window, sinks, cut.splits,
                         static_cast<int32_t>(cut.tile_groups), softmax_scale, nullptr, nullptr};
