@@ -116,8 +116,9 @@ __device__ __forceinline__ Sight sight_of(const AttendArgs &a, const Tile &t, in
 // Rows [r0, r0 + rows) of sequence s; rows == 0: none.
 __device__ __forceinline__ Tile tile_of(const AttendArgs &a, int64_t tile, int rows, int rows_log2) {
     Tile t = {};
-    t.s = sequence_of_unit(a.q_starts, a.sequences, a.total_q, a.group, rows_log2, tile);
-    t.qs = sequence_span(a.q_starts, t.s, a.total_q);
+    const Sequence q = sequence_at(a.q_starts, a.cache.lengths, a.sequences, a.total_q, a.group, rows_log2, 1, tile);
+    t.s = q.s;
+    t.qs = q.rows;
     const int64_t first = (tile - ((t.qs.begin * a.group >> rows_log2) + t.s)) << rows_log2;
     t.nrows = t.qs.rows * a.group;  // total_q * heads < 2^31
     if (first < 0 || first >= t.nrows) {
@@ -125,7 +126,7 @@ __device__ __forceinline__ Tile tile_of(const AttendArgs &a, int64_t tile, int r
         return t;
     }
     t.r0 = static_cast<int>(first);
-    t.keys = cached_rows(a.cache, t.s);
+    t.keys = cached_rows(a.cache, q.entry);
     t.lag = t.keys - t.qs.rows;
     const Sight head = sight_of(a, t, t.r0 / a.group), tail = sight_of(a, t, (min(t.r0 + rows, t.nrows) - 1) / a.group);
     t.least = head.lim;
@@ -785,16 +786,27 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
 // Joins the pieces of each (row, head), in their order; a wave each.
 template <class T, int D>
 __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
+    constexpr int N = 8;  // pieces on their way at a time
     const int lane = threadIdx.x & 63;
     const int64_t cell = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t cells = a.total_q * a.heads;
     if (cell >= cells) return;
     const int64_t row = cell / a.heads;
     const int head = static_cast<int>(cell - row * a.heads);
-    if (sequence_of_row(a.q_starts, a.sequences, row) < 0) return;
+    const int32_t begin = a.q_starts[0], end = a.q_starts[a.sequences];
     // a lane for each piece (there are at most 64): its weight, 0 for one without keys (a sum that is a NaN is not 0 and stays)
     const float4 none = sum_of(neg_inf(), 0.0f, 0.0f, 0.0f);
     const float4 mine = lane < a.splits ? a.part_ml[lane * cells + cell] : none;
+    float x[N][2];
+    const auto fetch = [&](int p0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                x[u][e] = p0 + u < a.splits && lane + 64 * e < D ? a.part_o[((p0 + u) * cells + cell) * D + lane + 64 * e] : 0.0f;
+    };
+    fetch(0);
+    if (row < begin || row >= end) return;  // no sequence's (its pieces hold anything)
     float4 top = mine.z != 0.0f ? mine : none;
     for (int d = 1; d < 64; d <<= 1) {
         const float4 other = sum_of(__shfl_xor(top.x, d, 64), __shfl_xor(top.y, d, 64), 0.0f, 0.0f);
@@ -803,25 +815,19 @@ __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
     const float w = mine.z != 0.0f ? weight_of(mine, top) * mine.z : 0.0f;
     float total = w, o[2] = {0.0f, 0.0f};
     for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d, 64);
-    // parts are divided by their sums: theirs are the weights, as shares of the whole, so that means stay finite
+    // parts are divided by their sums (zeros where there were no keys): theirs are the weights, as shares of the whole, so that
+    // means stay finite
     const float share = total == 0.0f ? 0.0f : w / total;
-    for (uint64_t left = __ballot(mine.z != 0.0f); left;) {
-        float wp[4], x[4][2];
+    for (int p0 = 0;;) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int p = left ? __builtin_ctzll(left) : -1;
-            left &= left - 1;
-            wp[u] = x[u][0] = x[u][1] = 0.0f;
-            if (p < 0) continue;
-            wp[u] = __shfl(share, p, 64);
+        for (int u = 0; u < N; ++u) {
+            const float wp = __shfl(share, p0 + u, 64);
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (lane + 64 * e < D) x[u][e] = a.part_o[(p * cells + cell) * D + lane + 64 * e];
+            for (int e = 0; e < 2; ++e) o[e] += wp * x[u][e];
         }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) o[e] += wp[u] * x[u][e];
+        p0 += N;
+        if (p0 >= a.splits) break;
+        fetch(p0);
     }
     T *to = static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(head) * D;
 #pragma unroll
@@ -840,10 +846,12 @@ struct Cut {
 Cut cut_of(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, int64_t max_k, int32_t window, int32_t sinks) {
     constexpr int64_t kGroups = 256 * 2;
     const int64_t rows = total_q * (heads / kv_heads), each = std::max<int64_t>(sequences, 1), per = (rows + each - 1) / each;
-    const int32_t tile = per <= 16 ? 16 : per <= 64 ? 32 : 128;
-    // (of sequences of one length, which take fewer than the bound)
-    const int64_t groups = std::max<int64_t>(each * ((per + tile - 1) / tile) * kv_heads, 1);
     const int64_t keys = window ? std::min<int64_t>(max_k, static_cast<int64_t>(window) + sinks + per + 2 * kStep) : max_k;
+    // workgroups (of sequences of one length, which take fewer tiles than the bound)
+    const auto groups_of = [&](int32_t tile) { return std::max<int64_t>(each * ((per + tile - 1) / tile) * kv_heads, 1); };
+    // 32 rows, too, where tiles of 128 with four steps a piece would leave compute units without one
+    const int32_t tile = per <= 16 ? 16 : per <= 64 || groups_of(128) * std::max<int64_t>(keys / (4 * kStep), 1) < 256 ? 32 : 128;
+    const int64_t groups = groups_of(tile);
     int32_t splits = 1;
     while (splits < 64 && groups * splits * 2 <= kGroups && keys >= (tile == 128 ? 4 : 16) * kStep * splits) splits *= 2;
     return {rows / tile + sequences, splits, tile};

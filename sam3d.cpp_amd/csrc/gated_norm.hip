@@ -25,107 +25,137 @@ struct NormArgs {
 // Rows whose squares' sum passes 2^128 are summed again smaller; eps is nothing beside them.
 constexpr float kLess = 0x1p-70f;
 
-// Sum over a row's threads: 2^lanes_log2 lanes of a wave, or all of a workgroup.
+// Sum over a row's threads: 2^lanes_log2 lanes of a wave, or all of a workgroup (`turn`: of sums so far, so that a place in
+// LDS is written again only after a barrier behind its last reader).
 template <bool WIDE>
-__device__ __forceinline__ float row_sum(float v, int lanes_log2, float *across) {
+__device__ __forceinline__ float row_sum(float v, int lanes_log2, float (*across)[16], int &turn) {
     for (int o = 1; o < (WIDE ? 64 : 1 << lanes_log2); o <<= 1) v += __shfl_xor(v, o, 64);
     if constexpr (WIDE) {
-        __syncthreads();  // the last sum's is read
-        if ((threadIdx.x & 63) == 0) across[threadIdx.x >> 6] = v;
+        float *mine = across[turn++ & 1];
+        if ((threadIdx.x & 63) == 0) mine[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = (across[0] + across[1]) + (across[2] + across[3]);
+        v = 0.0f;
+        for (int w = 0; w < static_cast<int>(blockDim.x >> 6); ++w) v += mine[w];
     }
     return v;
 }
 
-// Piece p of a thread's: 8 channels side by side where rows are whole 16-byte pieces; else the p-th run of 8
-// times the threads, a thread's channels as far apart as there are threads.
-template <int PPL, bool WIDE, bool VEC>
-__global__ void __launch_bounds__(256) gated_norm_kernel(NormArgs a) {
-    __shared__ float across[4];
-    const int threads = WIDE ? 256 : 1 << a.lanes_log2;
-    const int t = threadIdx.x & (threads - 1), rows = 256 / threads;
+// Four words side by side at any element's address.
+struct __attribute__((packed, aligned(2))) Words {
+    uint32_t w[4];
+};
+__device__ __forceinline__ void load8(const uint16_t *p, float (&v)[8]) {
+    const Words t = *reinterpret_cast<const Words *>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __builtin_bit_cast(float, e & 1 ? t.w[e >> 1] & 0xffff0000u : t.w[e >> 1] << 16);
+}
+__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const Words t = reinterpret_cast<const Words *>(p)[h];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * h + e] = __builtin_bit_cast(float, t.w[e]);
+    }
+}
+__device__ __forceinline__ void store8(uint16_t *p, const float (&v)[8]) {
+    Words t;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t.w[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
+    *reinterpret_cast<Words *>(p) = t;
+}
+__device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        Words t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t.w[e] = __builtin_bit_cast(uint32_t, v[4 * h + e]);
+        reinterpret_cast<Words *>(p)[h] = t;
+    }
+}
+
+// A thread holds PPL pieces of 8 channels, `threads` pieces apart.  Rows need not begin at whole 16 bytes: memory takes
+// 16-byte accesses at any element.  A last, shorter piece begins earlier instead, at the row's last 8 channels; it counts none
+// of its neighbour's in sums, and both store the same (20,000 rows of 333 channels: 31 us element by element).  REST: rows that
+// have one.  Rows of fewer than 8 channels go one by one.
+// WIDE: a row for each workgroup, of as many waves as leave its threads one piece, two beyond 8,192 channels (registers of more cost
+// the others' places: 20,000 rows of 2,048 channels 136 us in a wave, 86 us so).
+template <int PPL, bool WIDE, bool REST>
+__global__ void __launch_bounds__(WIDE ? 1024 : 256) gated_norm_kernel(NormArgs a) {
+    __shared__ float across[2][16];
+    const int threads = WIDE ? blockDim.x : 1 << a.lanes_log2;
+    const int t = WIDE ? threadIdx.x : threadIdx.x & (threads - 1), rows = WIDE ? 1 : 256 / threads;
     const int64_t row = a.first + static_cast<int64_t>(blockIdx.x) * rows + (WIDE ? 0 : threadIdx.x >> a.lanes_log2);
     if (row >= a.n) return;  // WIDE: the whole workgroup
-    const auto channel = [&](int p, int e) { return VEC ? (p * threads + t) * 8 + e : (p * 8 + e) * threads + t; };
+    const bool tiny = REST && a.c < 8;
+    // a piece's first channel, and how many of them are another's (8: all, there is no such piece)
+    const auto channel = [&](int p) {
+        const int c = (p * threads + t) * 8;
+        return REST && !tiny && c < a.c ? min(c, a.c - 8) : c;
+    };
+    const auto others = [&](int p) {
+        const int c = (p * threads + t) * 8;
+        return c >= a.c ? 8 : REST && !tiny ? c - min(c, a.c - 8) : 0;
+    };
+    const auto pieces = [&](auto &&whole, auto &&single) __attribute__((always_inline)) {
+        if (tiny) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (t == 0 && e < a.c) single(0, e, e);
+            return;
+        }
+#pragma unroll
+        for (int p = 0; p < PPL; ++p)
+            if ((p * threads + t) * 8 < a.c) whole(p, channel(p));
+    };
     const auto load = [&](const void *base, int64_t at, bool bf, float (&v)[PPL][8]) __attribute__((always_inline)) {
-        if (VEC) {
-#pragma unroll
-            for (int p = 0; p < PPL; ++p) {
-                const int c = channel(p, 0);
-                if (c >= a.c) continue;
-                if (bf) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + at + c);
-                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[p][e] = __builtin_bit_cast(float, e & 1 ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16);
-                } else {
-                    const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at + c);
-                    const float4 lo = f[0], hi = f[1];
-                    v[p][0] = lo.x, v[p][1] = lo.y, v[p][2] = lo.z, v[p][3] = lo.w;
-                    v[p][4] = hi.x, v[p][5] = hi.y, v[p][6] = hi.z, v[p][7] = hi.w;
-                }
-            }
+        if (bf) {
+            const uint16_t *x = static_cast<const uint16_t *>(base) + at;
+            pieces([&](int p, int c) { load8(x + c, v[p]); }, [&](int p, int e, int c) { v[p][e] = bf16_to_f32(x[c]); });
         } else {
-#pragma unroll
-            for (int p = 0; p < PPL; ++p)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int c = channel(p, e);
-                    if (c < a.c) v[p][e] = bf ? bf16_to_f32(static_cast<const uint16_t *>(base)[at + c]) : static_cast<const float *>(base)[at + c];
-                }
+            const float *x = static_cast<const float *>(base) + at;
+            pieces([&](int p, int c) { load8(x + c, v[p]); }, [&](int p, int e, int c) { v[p][e] = x[c]; });
         }
     };
     const auto store = [&](void *base, int64_t at, bool bf, const float (&v)[PPL][8]) __attribute__((always_inline)) {
-        if (VEC) {
-#pragma unroll
-            for (int p = 0; p < PPL; ++p) {
-                const int c = channel(p, 0);
-                if (c >= a.c) continue;
-                if (bf) {
-                    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(base) + at + c) =
-                        make_uint4(pack_bf16x2(v[p][0], v[p][1]), pack_bf16x2(v[p][2], v[p][3]), pack_bf16x2(v[p][4], v[p][5]),
-                                   pack_bf16x2(v[p][6], v[p][7]));
-                } else {
-                    float4 *f = reinterpret_cast<float4 *>(static_cast<float *>(base) + at + c);
-                    f[0] = make_float4(v[p][0], v[p][1], v[p][2], v[p][3]);
-                    f[1] = make_float4(v[p][4], v[p][5], v[p][6], v[p][7]);
-                }
-            }
+        if (bf) {
+            uint16_t *x = static_cast<uint16_t *>(base) + at;
+            pieces([&](int p, int c) { store8(x + c, v[p]); }, [&](int p, int e, int c) { x[c] = f32_to_bf16(v[p][e]); });
         } else {
-#pragma unroll
-            for (int p = 0; p < PPL; ++p)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int c = channel(p, e);
-                    if (c >= a.c) continue;
-                    if (bf) static_cast<uint16_t *>(base)[at + c] = f32_to_bf16(v[p][e]);
-                    else static_cast<float *>(base)[at + c] = v[p][e];
-                }
+            float *x = static_cast<float *>(base) + at;
+            pieces([&](int p, int c) { store8(x + c, v[p]); }, [&](int p, int e, int c) { x[c] = v[p][e]; });
         }
     };
     const auto each = [&](auto &&f) __attribute__((always_inline)) {
 #pragma unroll
         for (int p = 0; p < PPL; ++p)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (channel(p, e) < a.c) f(p, e);
+            for (int e = 0; e < 8; ++e) f(p, e);
+    };
+    // Sum of f over the row's channels, each once.
+    int turn = 0;
+    const auto sum = [&](auto &&f) __attribute__((always_inline)) {
+        float all = 0.0f;
+#pragma unroll
+        for (int p = 0; p < PPL; ++p) {
+            const int skip = others(p), end = tiny ? a.c : 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = f(p, e);
+                all += (REST ? e >= skip && e < end : skip == 0) ? x : 0.0f;
+            }
+        }
+        return row_sum<WIDE>(all, a.lanes_log2, across, turn);
     };
     const auto norm = [&](float (&v)[PPL][8], int kind, const float *w, const float *b) __attribute__((always_inline)) {
         if (kind == S3DX_NORM_NONE) return;
         float less = 1.0f, mean, rstd;
         for (;;) {
             mean = 0.0f;
-            if (kind == S3DX_NORM_LAYER) {
-                each([&](int p, int e) { mean += v[p][e] * less; });
-                mean = row_sum<WIDE>(mean, a.lanes_log2, across) / static_cast<float>(a.c);
-            }
-            float q = 0.0f;
-            each([&](int p, int e) {
+            if (kind == S3DX_NORM_LAYER) mean = sum([&](int p, int e) { return v[p][e] * less; }) / static_cast<float>(a.c);
+            const float q = sum([&](int p, int e) {
                 const float d = v[p][e] * less - mean;
-                q += d * d;
+                return d * d;
             });
-            q = row_sum<WIDE>(q, a.lanes_log2, across);
             // the same for the row's threads (a wave may hold several rows: those that are through wait)
             if (q < __builtin_inff() || less != 1.0f) {
                 rstd = rsqrtf(q / static_cast<float>(a.c) + (less == 1.0f ? a.eps : 0.0f));
@@ -151,6 +181,7 @@ __global__ void __launch_bounds__(256) gated_norm_kernel(NormArgs a) {
     float v[PPL][8], y[PPL][8], g[PPL][8];
     load(a.branch, row * a.branch_stride, a.branch_bf, v);
     load(a.x, row * a.x_stride, a.x_bf, y);
+    if (WIDE && REST) __syncthreads();  // y or h may take the place of what a neighbour's shorter piece reads as well
     norm(v, a.post, a.post_w, a.post_b);
     if (a.gate) {
         load(a.gate, mods, false, g);
@@ -174,12 +205,9 @@ __global__ void __launch_bounds__(256) gated_norm_kernel(NormArgs a) {
 constexpr int32_t kMostChannels = 16384;
 
 using NormFn = void (*)(NormArgs);
-template <bool WIDE, bool VEC>
+template <bool WIDE, bool REST>
 NormFn pick_pieces(int per) {
-    if (per <= 1) return gated_norm_kernel<1, WIDE, VEC>;
-    if (per <= 2) return gated_norm_kernel<2, WIDE, VEC>;
-    if (per <= 4) return gated_norm_kernel<4, WIDE, VEC>;
-    return gated_norm_kernel<8, WIDE, VEC>;
+    return per <= 1 ? gated_norm_kernel<1, WIDE, REST> : gated_norm_kernel<2, WIDE, REST>;
 }
 
 void check_rows(const void *p, int64_t stride, int64_t n, int32_t c, int32_t dtype, const char *what) {
@@ -188,7 +216,6 @@ void check_rows(const void *p, int64_t stride, int64_t n, int32_t c, int32_t dty
     require(stride >= c && stride <= (INT64_C(1) << 40), (name + ": the row stride is out of range (channels to 2^40)").c_str());
     require(n == 0 || (p && aligned(p, dtype_size(dtype))), (name + " is NULL or not aligned to its elements").c_str());
 }
-bool whole_pieces(const void *p, int64_t stride, int32_t dtype) { return aligned(p, 16) && stride * dtype_size(dtype) % 16 == 0; }
 
 }  // namespace
 }  // namespace s3dx
@@ -240,19 +267,17 @@ S3DX_API s3dx_status s3dx_gated_norm_rows(const void *x, int32_t x_dtype, int64_
         NormArgs a = {x, branch, y, h, post_w, post_b, pre_w, pre_b, gate, mod_scale, mod_shift, sets, 0, n, x_stride, branch_stride,
                       y_stride, h_stride, sets ? mod_stride : 0, set_stride, c, sets ? set_count : 1, post, pre, x_dtype == S3DX_BF16,
                       branch_dtype == S3DX_BF16, h_dtype == S3DX_BF16, 0, eps, residual_scale};
-        bool vec = c % 8 == 0 && whole_pieces(x, x_stride, x_dtype) && whole_pieces(branch, branch_stride, branch_dtype) &&
-                   whole_pieces(y, y_stride, x_dtype) && (!h || whole_pieces(h, h_stride, h_dtype)) && a.mod_stride % 4 == 0;
-        for (const float *p : {post_w, post_b, pre_w, pre_b, gate, mod_scale, mod_shift}) vec = vec && aligned(p, 16);
-        const bool wide = c > 64 * 8 * 4;
+        const bool wide = c > 64 * 8 * 2, rest = c % 8 != 0;
         while (!wide && a.lanes_log2 < 6 && (8 << a.lanes_log2) < c) ++a.lanes_log2;
-        const int threads = wide ? 256 : 1 << a.lanes_log2, per = (c + 8 * threads - 1) / (8 * threads), rows = 256 / threads;
-        const NormFn fn = wide ? (vec ? pick_pieces<true, true>(per) : pick_pieces<true, false>(per))
-                               : (vec ? pick_pieces<false, true>(per) : pick_pieces<false, false>(per));
+        const int threads = !wide ? 1 << a.lanes_log2 : std::min((c + 511) / 512 * 64, 1024);
+        const int per = (c + 8 * threads - 1) / (8 * threads), rows = wide ? 1 : 256 / threads, group = wide ? threads : 256;
+        const NormFn fn = wide ? (rest ? pick_pieces<true, true>(per) : pick_pieces<true, false>(per))
+                               : (rest ? pick_pieces<false, true>(per) : pick_pieces<false, false>(per));
         // a launch's threads stay below 2^32
-        const int64_t most = rows * (INT64_C(1) << 23);
+        const int64_t most = rows * (INT64_C(1) << 21);
         for (; a.first < n; a.first += most) {
             a.n = std::min(n, a.first + most);
-            fn<<<dim3(static_cast<unsigned>((a.n - a.first + rows - 1) / rows)), dim3(256), 0, as_stream(stream)>>>(a);
+            fn<<<dim3(static_cast<unsigned>((a.n - a.first + rows - 1) / rows)), dim3(group), 0, as_stream(stream)>>>(a);
         }
         launch_check("gated norm");
     });

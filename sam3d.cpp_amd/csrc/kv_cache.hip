@@ -30,15 +30,13 @@ struct Part {
 // room for the blocks that its rows can lie in, wherever they begin.
 __device__ __forceinline__ Part part_of(const RowArgs &a, int64_t unit) {
     const int log2 = a.cache.block_log2, block = 1 << log2;
-    const int64_t s = last_sequence(a.sequences, unit, [&](int64_t at) {
-        return (min(max(static_cast<int64_t>(a.starts[at]), INT64_C(0)), a.total) >> log2) + 2 * at;
-    });
-    const Span rows = sequence_span(a.starts, s, a.total);
-    const int32_t first = cached_rows(a.cache, s) - rows.rows;  // the first row's place, below 0 where there is no room for it
-    const int64_t j = (first >> log2) + unit - ((rows.begin >> log2) + 2 * s);
-    const int64_t lo = max(static_cast<int64_t>(first), j << log2), hi = min(static_cast<int64_t>(first) + rows.rows, (j + 1) << log2);
-    if (unit < (rows.begin >> log2) + 2 * s || hi <= lo) return {s, 0, 0, 0, 0};
-    return {s, rows.begin + (lo - first), static_cast<int32_t>(j), static_cast<int32_t>(lo & (block - 1)), static_cast<int32_t>(hi - lo)};
+    const Sequence q = sequence_at(a.starts, a.cache.lengths, a.sequences, a.total, 1, log2, 2, unit);
+    const int64_t base = (q.rows.begin >> log2) + 2 * q.s;
+    const int32_t first = cached_rows(a.cache, q.entry) - q.rows.rows;  // the first row's place, below 0 where there is no room for it
+    const int64_t j = (first >> log2) + unit - base;
+    const int64_t lo = max(static_cast<int64_t>(first), j << log2), hi = min(static_cast<int64_t>(first) + q.rows.rows, (j + 1) << log2);
+    if (unit < base || hi <= lo) return {q.s, 0, 0, 0, 0};
+    return {q.s, q.rows.begin + (lo - first), static_cast<int32_t>(j), static_cast<int32_t>(lo & (block - 1)), static_cast<int32_t>(hi - lo)};
 }
 
 template <class T>
@@ -107,6 +105,7 @@ __global__ void __launch_bounds__(256) write_kernel(RowArgs a) {
     if (page < 0) return;
     const int64_t cell = static_cast<int64_t>(page) * a.cache.kv_heads + head;
     uint8_t *kc = a.cache.codes + cell * (2 * BLOCK * D), *vc = kc + BLOCK * D;
+    const float2 was = p.slot > 0 ? a.cache.steps[cell] : make_float2(0.0f, 0.0f);  // read before anyone writes it (barriers below)
     if (tid < 2) most[tid] = 0;
     __syncthreads();
     uint32_t x[2][NP][8], big[2] = {0, 0};
@@ -137,8 +136,6 @@ __global__ void __launch_bounds__(256) write_kernel(RowArgs a) {
     __syncthreads();
     float step[2] = {step_of(most[0]), step_of(most[1])};
     if (p.slot > 0) {
-        const float2 was = a.cache.steps[cell];
-        __syncthreads();  // all have read it
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const float old = w ? was.y : was.x;

@@ -52,9 +52,9 @@ inline void check_table(const s3dx_cache *c, const int32_t *table, int32_t table
     require(lengths && aligned(lengths, 4), "lengths is NULL or not aligned");
 }
 
-// Rows that sequence s keeps: cut to what its table has room for.
-__device__ __forceinline__ int32_t cached_rows(const CacheView &a, int64_t s) {
-    return min(max(a.lengths[s], 0), a.table_stride << a.block_log2);
+// Rows that a sequence of length `length` keeps: cut to what its table has room for.
+__device__ __forceinline__ int32_t cached_rows(const CacheView &a, int32_t length) {
+    return min(max(length, 0), a.table_stride << a.block_log2);
 }
 // The page of block j of sequence s, or -1.
 __device__ __forceinline__ int32_t page_of(const CacheView &a, int64_t s, int32_t j) {

@@ -49,6 +49,30 @@ __device__ __forceinline__ int64_t sequence_of_row(const int32_t *starts, int64_
     return starts[s] <= row && row < starts[s + 1] ? s : -1;
 }
 
+// A sequence, its rows, and its entry of another list by sequence.
+struct Sequence {
+    int64_t s;
+    Span rows;
+    int32_t entry;
+};
+// The sequence of unit `unit`, where sequence s begins at unit (starts[s] * mul >> shift) + apart * s, by the whole wave: of up to
+// 64 sequences a lane fetches one's numbers, all in one trip to memory.
+__device__ __forceinline__ Sequence sequence_at(const int32_t *starts, const int32_t *list, int64_t sequences, int64_t total,
+                                                int64_t mul, int shift, int apart, int64_t unit) {
+    const auto cut = [&](int32_t at) { return min(max(static_cast<int64_t>(at), INT64_C(0)), total); };
+    if (sequences > 64) {
+        const int64_t s = last_sequence(sequences, unit, [&](int64_t at) { return (cut(starts[at]) * mul >> shift) + apart * at; });
+        return {s, sequence_span(starts, s, total), list[s]};
+    }
+    const int lane = threadIdx.x & 63, mine = min(lane, static_cast<int>(sequences) - 1);
+    const int32_t lo = starts[mine], hi = starts[mine + 1], entry = list[mine];
+    const bool before = lane == 0 || (lane < sequences && (cut(lo) * mul >> shift) + apart * lane <= unit);
+    const int s = __popcll(__builtin_amdgcn_ballot_w64(before)) - 1;
+    const int64_t begin = cut(__builtin_amdgcn_readlane(lo, s));
+    const int64_t end = max(begin, cut(__builtin_amdgcn_readlane(hi, s)));
+    return {s, {begin, static_cast<int32_t>(end - begin)}, __builtin_amdgcn_readlane(entry, s)};
+}
+
 // ---------------------------------------------------------------------------
 // Lanes of a 16x16 product
 // ---------------------------------------------------------------------------

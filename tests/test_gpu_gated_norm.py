@@ -93,6 +93,21 @@ def test_in_place(s3dx, types, place):
         check(s3dx, types[0], types[2], *run(s3dx, x, b, *types, 1, 2, place=place), what=place)
 
 
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("c", [9, 333, 1025, 2601, 5003, 16381])
+def test_sums_in_place_of_odd_rows(s3dx, dtype, c):
+    # a row's last piece shares channels with its neighbour's, of another wave in wide rows
+    rng = np.random.default_rng(c)
+    for place in ("y=x", "y=branch"):
+        x, b = rng.standard_normal((40, c)).astype(np.float32), rng.standard_normal((40, c)).astype(np.float32)
+        dx, x64 = R.dev(s3dx, R.stored(s3dx, x, dtype)[0]), R.stored(s3dx, x, dtype)[1]
+        db, b64 = R.dev(s3dx, R.stored(s3dx, b, dtype)[0]), R.stored(s3dx, b, dtype)[1]
+        y = dx if place == "y=x" else db
+        s3dx.gated_norm_rows(dx, dtype, db, dtype, 40, c, EPS, y)
+        want = x64 + b64
+        assert np.all(np.abs(R.values(s3dx, y, dtype) - want) <= (R.half_step(s3dx, dtype) + R.U32) * np.abs(want))
+
+
 @pytest.mark.parametrize("kind", [1, 2])
 @pytest.mark.parametrize("power", [-70, -40, 40, 64, 100, 120])
 @pytest.mark.parametrize("c", [96, 1024, 2900])
