@@ -218,6 +218,10 @@ class DeviceArray:
             call("s3dx_memcpy_d2h", out.ctypes.data_as(_vp), _vp(self.ptr), _u64(self.nbytes), _sptr(stream))
         return out
 
+    @property
+    def _as_parameter_(self):  # as ctypes takes it where an address is asked for
+        return self.ptr
+
     def free(self):
         if self.ptr:
             lib().s3dx_free(_vp(self.ptr))
@@ -789,7 +793,7 @@ class KvCache:
     def __init__(self, buffer, pages: int, kv_heads: int, head_dim: int, block: int = 64):
         self.handle = None
         p = _vp()
-        call("s3dx_cache_create", _addr(buffer), pages, kv_heads, head_dim, block, C.byref(p))
+        call("s3dx_cache_create", buffer, pages, kv_heads, head_dim, block, C.byref(p))
         self.handle = p.value
         self.buffer, self.pages, self.kv_heads, self.head_dim, self.block = buffer, pages, kv_heads, head_dim, block
 
@@ -802,15 +806,15 @@ class KvCache:
     def write(self, k, v, dtype, total, starts, table, table_stride, lengths, sequences, k_stride=None, v_stride=None, stream=None):
         """Quantises new rows into their sequences' last places (s3dx_cache_write)."""
         row = self.kv_heads * self.head_dim
-        call("s3dx_cache_write", self.handle, _addr(k), row if k_stride is None else k_stride, _addr(v),
-             row if v_stride is None else v_stride, dtype, total, _addr(starts), _addr(table), table_stride, _addr(lengths),
+        call("s3dx_cache_write", self.handle, k, row if k_stride is None else k_stride, v,
+             row if v_stride is None else v_stride, dtype, total, starts, table, table_stride, lengths,
              sequences, _handle(stream))
 
     def read(self, k, v, dtype, total, starts, table, table_stride, lengths, sequences, k_stride=None, v_stride=None, stream=None):
         """The values of each sequence's last rows, into k and v (s3dx_cache_read)."""
         row = self.kv_heads * self.head_dim
-        call("s3dx_cache_read", self.handle, _addr(k), row if k_stride is None else k_stride, _addr(v),
-             row if v_stride is None else v_stride, dtype, total, _addr(starts), _addr(table), table_stride, _addr(lengths),
+        call("s3dx_cache_read", self.handle, k, row if k_stride is None else k_stride, v,
+             row if v_stride is None else v_stride, dtype, total, starts, table, table_stride, lengths,
              sequences, _handle(stream))
 
     def attention_workspace_size(self, total_q, heads, sequences, max_k, window=0, sinks=0) -> int:
@@ -825,10 +829,10 @@ class KvCache:
         if workspace_bytes is None:
             workspace_bytes = workspace.nbytes if isinstance(workspace, DeviceArray) else 0
         row = heads * self.head_dim
-        call("s3dx_cache_attention", self.handle, _addr(q), dtype, total_q, heads, row if q_stride is None else q_stride,
-             _addr(q_starts), _addr(table), table_stride, _addr(lengths), sequences, max_k, window, sinks,
-             self.head_dim ** -0.5 if scale is None else scale, BLOCK_CAUSAL if causal else 0, _addr(o),
-             row if o_stride is None else o_stride, _addr(lse), _addr(workspace), workspace_bytes, _handle(stream))
+        call("s3dx_cache_attention", self.handle, q, dtype, total_q, heads, row if q_stride is None else q_stride,
+             q_starts, table, table_stride, lengths, sequences, max_k, window, sinks,
+             self.head_dim ** -0.5 if scale is None else scale, BLOCK_CAUSAL if causal else 0, o,
+             row if o_stride is None else o_stride, lse, workspace, workspace_bytes, _handle(stream))
 
     def __del__(self):
         try:
@@ -845,10 +849,10 @@ def gated_norm_rows(x, x_dtype, branch, branch_dtype, n, c, eps, y=None, h=None,
     """y (default: x itself) = x + residual_scale * gate * post(branch), h = pre(y) * (1 + mod_scale) + mod_shift
     (s3dx_gated_norm_rows)."""
     xs = c if x_stride is None else x_stride
-    call("s3dx_gated_norm_rows", _addr(x), x_dtype, xs, _addr(branch), branch_dtype, c if branch_stride is None else branch_stride,
-         n, c, post, _addr(post_w), _addr(post_b), residual_scale, _addr(gate), pre, _addr(pre_w), _addr(pre_b), _addr(mod_scale),
-         _addr(mod_shift), c if mod_stride is None else mod_stride, _addr(sets), set_stride, set_count, eps,
-         _addr(x if y is None else y), y_stride if y_stride is not None else (xs if y is None else c), _addr(h),
+    call("s3dx_gated_norm_rows", x, x_dtype, xs, branch, branch_dtype, c if branch_stride is None else branch_stride,
+         n, c, post, post_w, post_b, residual_scale, gate, pre, pre_w, pre_b, mod_scale,
+         mod_shift, c if mod_stride is None else mod_stride, sets, set_stride, set_count, eps,
+         x if y is None else y, y_stride if y_stride is not None else (xs if y is None else c), h,
          branch_dtype if h_dtype is None else h_dtype, c if h_stride is None else h_stride, _handle(stream))
 
 

@@ -621,7 +621,8 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
     // consecutive workgroups of one XCD run neighbouring tiles of a head: its L2 holds their keys
     const int id = xcd_tile(blockIdx.x, gridDim.x);
     const int split = id / a.tile_groups % a.splits, kvh = id / a.tile_groups / a.splits;
-    const Tile t = tile_of(a, id % a.tile_groups, 128, 7);
+    // causal rows see more keys the later they stand: the longest first
+    const Tile t = tile_of(a, a.causal ? a.tile_groups - 1 - id % a.tile_groups : id % a.tile_groups, 128, 7);
     if (t.nrows == 0) return;
     const int r0 = t.r0 + 32 * wave;
     Q q;
@@ -783,30 +784,69 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
     put<T, D, 32>(a, t, split, r0 + c, kvh, y, r.base, column_sum<32>(r.sum), r.unit);
 }
 
-// Joins the pieces of each (row, head), in their order; a wave each.
+// The pieces' weights: shares of the whole, so that means of finite values stay finite.  Parts are divided by their sums,
+// zeros where there were no keys; a sum that is a NaN is not 0 and stays.
+constexpr int kFewPieces = 8;
+
+// Joins up to kFewPieces pieces of each (row, head), in their order: D / 4 lanes of four channels each, and each for itself the
+// pieces' weights (2,048 rows x 16 heads x 64 in two pieces: 19 us with a wave for each).
 template <class T, int D>
-__global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
-    constexpr int N = 8;  // pieces on their way at a time
-    const int lane = threadIdx.x & 63;
-    const int64_t cell = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ void __launch_bounds__(256) cache_join_few_kernel(AttendArgs a) {
+    constexpr int LANES = D == 32 ? 8 : D == 64 ? 16 : 32;
+    const int lane = threadIdx.x & (LANES - 1);
+    const int64_t cell = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     const int64_t cells = a.total_q * a.heads;
-    if (cell >= cells) return;
+    if (cell >= cells || 4 * lane >= D) return;
     const int64_t row = cell / a.heads;
     const int head = static_cast<int>(cell - row * a.heads);
-    const int32_t begin = a.q_starts[0], end = a.q_starts[a.sequences];
-    // a lane for each piece (there are at most 64): its weight, 0 for one without keys (a sum that is a NaN is not 0 and stays)
+    if (row < a.q_starts[0] || row >= a.q_starts[a.sequences]) return;  // no sequence's (its pieces hold anything)
+    float4 ml[kFewPieces];
+    f32x4 x[kFewPieces];
+#pragma unroll
+    for (int p = 0; p < kFewPieces; ++p) {
+        const int64_t at = min(p, a.splits - 1) * cells + cell;
+        ml[p] = a.part_ml[at];
+        x[p] = *reinterpret_cast<const f32x4 *>(a.part_o + at * D + 4 * lane);
+    }
+    float4 top = sum_of(neg_inf(), 0.0f, 0.0f, 0.0f);
+    float w[kFewPieces], total = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kFewPieces; ++p)
+        if (p < a.splits && ml[p].z != 0.0f && above_of(ml[p], top)) top = ml[p];
+#pragma unroll
+    for (int p = 0; p < kFewPieces; ++p) {
+        w[p] = p < a.splits && ml[p].z != 0.0f ? weight_of(ml[p], top) * ml[p].z : 0.0f;
+        total += w[p];
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+    for (int p = 0; p < kFewPieces; ++p)
+        if (p < a.splits) o += x[p] * (w[p] * inv);
+    T *to = static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(head) * D + 4 * lane;
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2 *>(to) = u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+    else *reinterpret_cast<f32x4 *>(to) = o;
+    if (a.lse && lane == 0) a.lse[cell] = log_of(top.x, top.y, total);
+}
+
+// Joins up to 64 pieces of each (row, head): a workgroup each, whose waves take a quarter of the pieces, all on their way at once.
+template <class T, int D>
+__global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
+    constexpr int N = 16;
+    __shared__ float part[4][2][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t cell = blockIdx.x, cells = a.total_q * a.heads, row = cell / a.heads;
+    const int head = static_cast<int>(cell - row * a.heads);
+    // a lane for each piece: its weight
     const float4 none = sum_of(neg_inf(), 0.0f, 0.0f, 0.0f);
     const float4 mine = lane < a.splits ? a.part_ml[lane * cells + cell] : none;
     float x[N][2];
-    const auto fetch = [&](int p0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < N; ++u)
+    for (int u = 0; u < N; ++u)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                x[u][e] = p0 + u < a.splits && lane + 64 * e < D ? a.part_o[((p0 + u) * cells + cell) * D + lane + 64 * e] : 0.0f;
-    };
-    fetch(0);
-    if (row < begin || row >= end) return;  // no sequence's (its pieces hold anything)
+        for (int e = 0; e < 2; ++e)
+            x[u][e] = N * wave + u < a.splits && lane + 64 * e < D ? a.part_o[((N * wave + u) * cells + cell) * D + lane + 64 * e] : 0.0f;
+    if (row < a.q_starts[0] || row >= a.q_starts[a.sequences]) return;  // no sequence's (its pieces hold anything)
     float4 top = mine.z != 0.0f ? mine : none;
     for (int d = 1; d < 64; d <<= 1) {
         const float4 other = sum_of(__shfl_xor(top.x, d, 64), __shfl_xor(top.y, d, 64), 0.0f, 0.0f);
@@ -815,24 +855,22 @@ __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
     const float w = mine.z != 0.0f ? weight_of(mine, top) * mine.z : 0.0f;
     float total = w, o[2] = {0.0f, 0.0f};
     for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d, 64);
-    // parts are divided by their sums (zeros where there were no keys): theirs are the weights, as shares of the whole, so that
-    // means stay finite
     const float share = total == 0.0f ? 0.0f : w / total;
-    for (int p0 = 0;;) {
 #pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const float wp = __shfl(share, p0 + u, 64);
+    for (int u = 0; u < N; ++u) {
+        const float wp = __shfl(share, N * wave + u, 64);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) o[e] += wp * x[u][e];
-        }
-        p0 += N;
-        if (p0 >= a.splits) break;
-        fetch(p0);
+        for (int e = 0; e < 2; ++e) o[e] += wp * x[u][e];
     }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) part[wave][e][lane] = o[e];
+    __syncthreads();
+    if (wave != 0) return;
     T *to = static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(head) * D;
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-        if (lane + 64 * e < D) store_from_f32<T>(to + lane + 64 * e, o[e]);
+        if (lane + 64 * e < D)
+            store_from_f32<T>(to + lane + 64 * e, (part[0][e][lane] + part[1][e][lane]) + (part[2][e][lane] + part[3][e][lane]));
     if (a.lse && lane == 0) a.lse[cell] = log_of(top.x, top.y, total);
 }
 
@@ -853,7 +891,7 @@ Cut cut_of(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, 
     const int32_t tile = per <= 16 ? 16 : per <= 64 || groups_of(128) * std::max<int64_t>(keys / (4 * kStep), 1) < 256 ? 32 : 128;
     const int64_t groups = groups_of(tile);
     int32_t splits = 1;
-    while (splits < 64 && groups * splits * 2 <= kGroups && keys >= (tile == 128 ? 4 : 16) * kStep * splits) splits *= 2;
+    while (splits < 64 && groups * splits * 2 <= kGroups && keys >= (tile == 128 ? 4 : 8) * kStep * splits) splits *= 2;
     return {rows / tile + sequences, splits, tile};
 }
 
@@ -867,7 +905,8 @@ AttendFn pick_attend(int32_t d, const Cut &cut) {
     return d == 32 ? pick_tile<T, 32>(cut) : d == 64 ? pick_tile<T, 64>(cut) : d == 96 ? pick_tile<T, 96>(cut) : pick_tile<T, 128>(cut);
 }
 template <class T>
-AttendFn pick_join(int32_t d) {
+AttendFn pick_join(int32_t d, bool few) {
+    if (few) return d == 32 ? cache_join_few_kernel<T, 32> : d == 64 ? cache_join_few_kernel<T, 64> : d == 96 ? cache_join_few_kernel<T, 96> : cache_join_few_kernel<T, 128>;
     return d == 32 ? cache_join_kernel<T, 32> : d == 64 ? cache_join_kernel<T, 64> : d == 96 ? cache_join_kernel<T, 96> : cache_join_kernel<T, 128>;
 }
 
@@ -944,8 +983,11 @@ S3DX_API s3dx_status s3dx_cache_attention(const s3dx_cache *cache, const void *q
             dim3(static_cast<unsigned>(grid)), dim3(256), 0, as_stream(stream)>>>(a);
         launch_check("cache attention");
         if (cut.splits > 1) {
-            (bf ? pick_join<uint16_t>(cache->head_dim) : pick_join<float>(cache->head_dim))<<<
-                dim3(static_cast<unsigned>((total_q * heads + 3) / 4)), dim3(256), 0, as_stream(stream)>>>(a);
+            const bool few = cut.splits <= kFewPieces;
+            const int64_t cells = total_q * heads, each = !few ? 1 : cache->head_dim == 32 ? 32 : cache->head_dim == 64 ? 16 : 8;
+            require((cells + each - 1) / each <= 0xffffffffll / 256, "too many rows and heads");
+            (bf ? pick_join<uint16_t>(cache->head_dim, few) : pick_join<float>(cache->head_dim, few))<<<
+                dim3(static_cast<unsigned>((cells + each - 1) / each)), dim3(256), 0, as_stream(stream)>>>(a);
             launch_check("cache attention join");
         }
     });
