@@ -23,7 +23,7 @@ struct AttendArgs {
     float *lse;
     const int32_t *q_starts;
     int64_t total_q, q_stride, o_stride, sequences;
-    int32_t heads, group, causal, window, sinks, splits, tile_groups;
+    int32_t heads, group, causal, window, sinks, splits, tile_groups, at_once;
     float scale;
     float *part_o;    // [splits][total_q][heads][d], divided by their sums
     float4 *part_ml;  // [splits][total_q][heads]: see sum_of
@@ -113,13 +113,55 @@ struct Sight {
 __device__ __forceinline__ Sight sight_of(const AttendArgs &a, const Tile &t, int tok) {
     return {a.causal ? max(0, min(t.keys, tok + t.lag + 1)) : t.keys, a.window ? tok + t.lag - a.window + 1 : 0};
 }
-// Rows [r0, r0 + rows) of sequence s; rows == 0: none.
-__device__ __forceinline__ Tile tile_of(const AttendArgs &a, int64_t tile, int rows, int rows_log2) {
+// What a workgroup computes: tile i of `all` tiles of rows, or none, by a piece of a head's keys.  Of eight (head, piece) each XCD takes one,
+// whose keys its L2 then holds; the tiles of those left over are dealt out to all XCDs in turn.
+// Workgroups without work stand behind all others.  An XCD's dispatcher fills its shader engines in turn and in order: one without
+// work before it holds a workgroup back until the engine whose turn it is has room (8 sequences of 64 rows x 4 over 20,000 keys: 320 us
+// with one behind every two for 225).
+struct Work {
+    int64_t i;
+    int split, kvh;
+};
+__device__ __forceinline__ Work work_of(const AttendArgs &a, int n, bool ordered) {
+    constexpr int kUnits = 32;  // compute units of an XCD: an XCD's workgroups x, x + 32, x + 64 are one's
+    const int xcd = blockIdx.x % 8, x = blockIdx.x / 8, heads = a.cache.kv_heads * a.splits, each = heads / 8, left = heads - 8 * each;
+    const int own = each * n, shared = (left * n - xcd + 7) / 8, mine = own + shared;
+    if (x >= mine) return {n, 0, 0};
+    int head, i;
+    if (ordered && a.at_once) {
+        // Causal rows see more keys the later they stand.  Where all workgroups run at once, the shortest tiles share compute units, the
+        // longest of those with the shortest: by the tile's rank, 0 the longest.  (2,048 rows of 8 x 4 x 128 from the first on: 71 us
+        // in order, longest first, for 65.)
+        const int round = x / kUnits, over = min(max(mine - kUnits, 0), kUnits);
+        const int rank = round == 0 ? (x < over ? kUnits - over + x : x - over) : round == 1 ? kUnits + over - 1 - (x - kUnits) : x;
+        const int l = rank * shared / mine, o = rank - l;
+        if ((rank + 1) * shared / mine > l) {
+            const int q = 8 * l + xcd;
+            head = 8 * each + q % left, i = n - 1 - q / left;
+        } else {
+            head = xcd * each + o % each, i = n - 1 - o / each;
+        }
+    } else {
+        const int q = 8 * (x - own) + xcd;
+        head = x < own ? xcd * each + x / n : 8 * each + q / n;
+        i = x < own ? x % n : q % n;
+        if (ordered) i = n - 1 - i;  // the longest first
+    }
+    return {i, head % a.splits, head / a.splits};
+}
+
+// A workgroup's rows [r0, r0 + rows) of sequence s; nrows == 0: none.
+__device__ __forceinline__ Tile tile_of(const AttendArgs &a, Work &w, int rows, int rows_log2) {
     Tile t = {};
-    const Sequence q = sequence_at(a.q_starts, a.cache.lengths, a.sequences, a.total_q, a.group, rows_log2, 1, tile);
+    const Sequence q = sequence_at(a.q_starts, a.cache.lengths, a.sequences, a.total_q, a.group, rows_log2, 1, a.tile_groups,
+                                   [&](int32_t n, int32_t) { return (n * a.group >> rows_log2) + ((n * a.group & (rows - 1)) != 0); },
+                                   [&](int64_t all) {
+                                       w = work_of(a, static_cast<int>(min(all, static_cast<int64_t>(a.tile_groups))), a.causal && rows == 128);
+                                       return w.i;
+                                   });
     t.s = q.s;
     t.qs = q.rows;
-    const int64_t first = (tile - ((t.qs.begin * a.group >> rows_log2) + t.s)) << rows_log2;
+    const int64_t first = (q.unit - q.first) << rows_log2;
     t.nrows = t.qs.rows * a.group;  // total_q * heads < 2^31
     if (first < 0 || first >= t.nrows) {
         t.nrows = 0;
@@ -491,9 +533,9 @@ __global__ void __launch_bounds__(256, 2) cache_rows_kernel(AttendArgs a) {
     __shared__ float4 part_ml[4][COLUMNS];
     const int lane = threadIdx.x & 63, c = lane % COLUMNS, g = lane / COLUMNS;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = xcd_tile(blockIdx.x, gridDim.x);
-    const int split = id / a.tile_groups % a.splits, kvh = id / a.tile_groups / a.splits;
-    const Tile t = tile_of(a, id % a.tile_groups, COLUMNS, COLUMNS == 16 ? 4 : 5);
+    Work work;
+    const Tile t = tile_of(a, work, COLUMNS, COLUMNS == 16 ? 4 : 5);
+    const int split = work.split, kvh = work.kvh;
     if (t.nrows == 0) return;
     Q q;
     q.load(a, t, t.r0, kvh);
@@ -618,11 +660,9 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
     __shared__ u32x4 key_rows[2][2 * PIECES][64], value_rows[2][2 * PIECES][64];
     const int lane = threadIdx.x & 63, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // consecutive workgroups of one XCD run neighbouring tiles of a head: its L2 holds their keys
-    const int id = xcd_tile(blockIdx.x, gridDim.x);
-    const int split = id / a.tile_groups % a.splits, kvh = id / a.tile_groups / a.splits;
-    // causal rows see more keys the later they stand: the longest first
-    const Tile t = tile_of(a, a.causal ? a.tile_groups - 1 - id % a.tile_groups : id % a.tile_groups, 128, 7);
+    Work work;
+    const Tile t = tile_of(a, work, 128, 7);
+    const int split = work.split, kvh = work.kvh;
     if (t.nrows == 0) return;
     const int r0 = t.r0 + 32 * wave;
     Q q;
@@ -880,8 +920,9 @@ __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
 struct Cut {
     int64_t tile_groups;
     int32_t splits, rows;  // of a tile
+    bool at_once;          // all workgroups run at once (of sequences of one length; three a unit up to 64 channels, two beyond)
 };
-Cut cut_of(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, int64_t max_k, int32_t window, int32_t sinks) {
+Cut cut_of(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, int64_t max_k, int32_t window, int32_t sinks, int32_t head_dim) {
     constexpr int64_t kGroups = 256 * 2;
     const int64_t rows = total_q * (heads / kv_heads), each = std::max<int64_t>(sequences, 1), per = (rows + each - 1) / each;
     const int64_t keys = window ? std::min<int64_t>(max_k, static_cast<int64_t>(window) + sinks + per + 2 * kStep) : max_k;
@@ -892,7 +933,7 @@ Cut cut_of(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, 
     const int64_t groups = groups_of(tile);
     int32_t splits = 1;
     while (splits < 64 && groups * splits * 2 <= kGroups && keys >= (tile == 128 ? 4 : 8) * kStep * splits) splits *= 2;
-    return {rows / tile + sequences, splits, tile};
+    return {rows / tile + sequences, splits, tile, groups * splits <= 256 * (head_dim <= 64 ? 3 : 2)};
 }
 
 using AttendFn = void (*)(AttendArgs);
@@ -934,7 +975,7 @@ S3DX_API s3dx_status s3dx_cache_attention_workspace_size(const s3dx_cache *cache
     return boundary(error, error_capacity, [&] {
         require(bytes, "bytes is NULL");
         check_call(cache, total_q, heads, sequences, max_k, window, sinks);
-        const Cut cut = cut_of(total_q, heads, cache->kv_heads, sequences, max_k, window, sinks);
+        const Cut cut = cut_of(total_q, heads, cache->kv_heads, sequences, max_k, window, sinks, cache->head_dim);
         *bytes = 0;
         if (cut.splits == 1) return;
         Sizer z;
@@ -966,10 +1007,10 @@ S3DX_API s3dx_status s3dx_cache_attention(const s3dx_cache *cache, const void *q
         }
         require(q_starts && aligned(q_starts, 4), "starts is NULL or not aligned");
         require(!lse || aligned(lse, 4), "lse is not aligned");
-        const Cut cut = cut_of(total_q, heads, cache->kv_heads, sequences, max_k, window, sinks);
+        const Cut cut = cut_of(total_q, heads, cache->kv_heads, sequences, max_k, window, sinks, cache->head_dim);
         AttendArgs a = {view_of(cache, table, table_stride, lengths), q, o, lse, q_starts, total_q, q_stride, o_stride, sequences,
                         heads, heads / cache->kv_heads, flags & S3DX_BLOCK_CAUSAL, window, sinks, cut.splits,
-                        static_cast<int32_t>(cut.tile_groups), softmax_scale, nullptr, nullptr};
+                        static_cast<int32_t>(cut.tile_groups), cut.at_once, softmax_scale, nullptr, nullptr};
         if (cut.splits > 1) {
             require(workspace && aligned(workspace, 16), "workspace is NULL or not 16-byte aligned");
             Carver w(workspace, workspace_bytes);

@@ -33,16 +33,18 @@ struct Part {
     int64_t s, row;
     int32_t j, slot, count;
 };
-// Blocks are dealt out by unit: sequence s begins at unit starts[s] / block + 2 s, which leaves
-// room for the blocks that its rows can lie in, wherever they begin.
+// Blocks are dealt out by unit.  (Beyond 64 sequences: s begins at unit starts[s] / block + 2 s, which leaves
+// room for the blocks that its rows can lie in, wherever they begin.)
 __device__ __forceinline__ Part part_of(const RowArgs &a, int64_t unit) {
     const int log2 = a.cache.block_log2, block = 1 << log2;
-    const Sequence q = sequence_at(a.starts, a.cache.lengths, a.sequences, a.total, 1, log2, 2, unit);
-    const int64_t base = (q.rows.begin >> log2) + 2 * q.s;
+    const Sequence q = sequence_at(a.starts, a.cache.lengths, a.sequences, a.total, 1, log2, 2, 0, [&](int32_t n, int32_t entry) {
+        const int32_t end = cached_rows(a.cache, entry);
+        return n == 0 ? 0 : ((end - 1) >> log2) - ((end - n) >> log2) + 1;
+    }, [&](int64_t) { return unit; });
     const int32_t first = cached_rows(a.cache, q.entry) - q.rows.rows;  // the first row's place, below 0 where there is no room for it
-    const int64_t j = (first >> log2) + unit - base;
+    const int64_t j = (first >> log2) + unit - q.first;
     const int64_t lo = max(static_cast<int64_t>(first), j << log2), hi = min(static_cast<int64_t>(first) + q.rows.rows, (j + 1) << log2);
-    if (unit < base || hi <= lo) return {q.s, 0, 0, 0, 0};
+    if (unit < q.first || hi <= lo) return {q.s, 0, 0, 0, 0};
     return {q.s, q.rows.begin + (lo - first), static_cast<int32_t>(j), static_cast<int32_t>(lo & (block - 1)), static_cast<int32_t>(hi - lo)};
 }
 

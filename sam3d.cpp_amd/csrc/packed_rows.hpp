@@ -49,28 +49,39 @@ __device__ __forceinline__ int64_t sequence_of_row(const int32_t *starts, int64_
     return starts[s] <= row && row < starts[s + 1] ? s : -1;
 }
 
-// A sequence, its rows, and its entry of another list by sequence.
+// A unit's sequence, its rows, its entry of another list by sequence, and its first unit.
 struct Sequence {
     int64_t s;
     Span rows;
     int32_t entry;
+    int64_t first, unit;
 };
-// The sequence of unit `unit`, where sequence s begins at unit (starts[s] * mul >> shift) + apart * s, by the whole wave: of up to
-// 64 sequences a lane fetches one's numbers, all in one trip to memory.
+// Of a launch that gives sequence s its units(rows, entry): the sequence of unit at(all), all being how many there are or may be
+// (bound), by the whole wave.  Up to 64 sequences' units follow each other; a lane fetches one's numbers, all in one
+// trip to memory.  More sequences begin where a bound says: s at unit (starts[s] * mul >> shift) + apart * s.
+template <class Units, class At>
 __device__ __forceinline__ Sequence sequence_at(const int32_t *starts, const int32_t *list, int64_t sequences, int64_t total,
-                                                int64_t mul, int shift, int apart, int64_t unit) {
+                                                int64_t mul, int shift, int apart, int64_t bound, Units units, At at) {
     const auto cut = [&](int32_t at) { return min(max(static_cast<int64_t>(at), INT64_C(0)), total); };
     if (sequences > 64) {
-        const int64_t s = last_sequence(sequences, unit, [&](int64_t at) { return (cut(starts[at]) * mul >> shift) + apart * at; });
-        return {s, sequence_span(starts, s, total), list[s]};
+        const auto first = [&](int64_t s) { return (cut(starts[s]) * mul >> shift) + apart * s; };
+        const int64_t unit = at(bound), s = last_sequence(sequences, unit, first);
+        return {s, sequence_span(starts, s, total), list[s], first(s), unit};
     }
     const int lane = threadIdx.x & 63, mine = min(lane, static_cast<int>(sequences) - 1);
-    const int32_t lo = starts[mine], hi = starts[mine + 1], entry = list[mine];
-    const bool before = lane == 0 || (lane < sequences && (cut(lo) * mul >> shift) + apart * lane <= unit);
-    const int s = __popcll(__builtin_amdgcn_ballot_w64(before)) - 1;
-    const int64_t begin = cut(__builtin_amdgcn_readlane(lo, s));
-    const int64_t end = max(begin, cut(__builtin_amdgcn_readlane(hi, s)));
-    return {s, {begin, static_cast<int32_t>(end - begin)}, __builtin_amdgcn_readlane(entry, s)};
+    const int64_t lo = cut(starts[mine]), hi = max(lo, cut(starts[mine + 1]));
+    const int32_t entry = list[mine], rows = static_cast<int32_t>(hi - lo);
+    int32_t end = units(rows, entry);
+    for (int o = 1; o < sequences; o <<= 1) {
+        const int32_t before = __shfl_up(end, o, 64);
+        end += lane >= o ? before : 0;
+    }
+    // (the last one takes the units behind all)
+    const int64_t unit = at(static_cast<int64_t>(__builtin_amdgcn_readlane(end, static_cast<int>(sequences) - 1)));
+    const int s = min(__popcll(__builtin_amdgcn_ballot_w64(lane < sequences && end <= unit)), static_cast<int>(sequences) - 1);
+    const int32_t first = s == 0 ? 0 : __builtin_amdgcn_readlane(end, s - 1);
+    return {s, {__builtin_amdgcn_readlane(static_cast<int32_t>(lo), s), __builtin_amdgcn_readlane(rows, s)},
+            __builtin_amdgcn_readlane(entry, s), first, unit};
 }
 
 // ---------------------------------------------------------------------------

@@ -83,6 +83,25 @@ def test_attention(s3dx, dtype, case):
     K.check(s3dx, dtype, got, lse, want)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("new,lens,heads,kv,d", [
+    ([300, 0, 700, 129], [300, 5, 900, 4000], 10, 10, 32),           # two heads beyond eight
+    ([300, 0, 700, 129], [300, 5, 900, 4000], 3, 1, 128),
+    ([0, 500, 1, 0, 260], [9, 700, 2, 0, 300], 12, 6, 64),
+    ([200, 390], [1000, 390], 38, 19, 32),
+    ([100] * 70, [100 + 2 * s for s in range(70)], 3, 3, 32),        # tiles by a bound
+    ([100] * 70, [100 + 2 * s for s in range(70)], 12, 12, 32),      # ... more than run at once
+    ([130] * 33, [150 + s for s in range(33)], 13, 13, 64),
+    ([0] * 20 + [90] * 44, [64] * 64, 9, 9, 96),                     # 64 sequences, more queries than keys
+])
+def test_every_tile_is_computed(s3dx, new, lens, heads, kv, d, causal):
+    rng = np.random.default_rng(sum(lens))
+    held, table = K.filled(rng, kv, d, 64, lens)
+    q = rng.standard_normal((sum(new), heads, d)).astype(np.float32)
+    got, lse, want = run(s3dx, q, held, table, s3dx.BF16, new, lens, causal, behind=2)
+    K.check(s3dx, s3dx.BF16, got, lse, want)
+
+
 @pytest.mark.parametrize("dtype", [0, 1])
 @pytest.mark.parametrize("new,lens,heads,kv,d", [([1, 1], [2000, 300], 8, 2, 64), ([90], [260], 4, 2, 128), ([200], [200], 4, 4, 32)])
 def test_work_is_cut_by_max_k_and_results_are_not(s3dx, dtype, new, lens, heads, kv, d):
