@@ -915,25 +915,27 @@ __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
 }
 
 // How a call is cut: by sequences' mean rows into tiles of 16 or 32 (four waves share a tile's keys) or of 128 (four waves share
-// its rows), an upper bound of each, as the lengths are on the device; and, where there would be fewer than two waves for each
-// SIMD, every tile's keys over several workgroups, with at least four steps a wave.
+// its rows), an upper bound of each, as the lengths are on the device; and every tile's keys over as many workgroups as run at once:
+// two a compute unit, three for tiles of 128 up to 64 channels (1,300 rows of 12 x 64 over 3,000 keys: 44 us with two for 32), with at
+// least four steps of keys each, two in tiles of 128, whose waves each take all of them.  (Powers of two alone: 500 rows of 8 x 4 x 128
+// over 6,000 keys 116 us for 87, 3 rows of 12 x 128 over 30,000 each 74 for 59.)
 struct Cut {
     int64_t tile_groups;
     int32_t splits, rows;  // of a tile
     bool at_once;          // all workgroups run at once (of sequences of one length; three a unit up to 64 channels, two beyond)
 };
 Cut cut_of(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, int64_t max_k, int32_t window, int32_t sinks, int32_t head_dim) {
-    constexpr int64_t kGroups = 256 * 2;
     const int64_t rows = total_q * (heads / kv_heads), each = std::max<int64_t>(sequences, 1), per = (rows + each - 1) / each;
     const int64_t keys = window ? std::min<int64_t>(max_k, static_cast<int64_t>(window) + sinks + per + 2 * kStep) : max_k;
     // workgroups (of sequences of one length, which take fewer tiles than the bound)
     const auto groups_of = [&](int32_t tile) { return std::max<int64_t>(each * ((per + tile - 1) / tile) * kv_heads, 1); };
     // 32 rows, too, where tiles of 128 with four steps a piece would leave compute units without one
     const int32_t tile = per <= 16 ? 16 : per <= 64 || groups_of(128) * std::max<int64_t>(keys / (4 * kStep), 1) < 256 ? 32 : 128;
-    const int64_t groups = groups_of(tile);
-    int32_t splits = 1;
-    while (splits < 64 && groups * splits * 2 <= kGroups && keys >= (tile == 128 ? 4 : 8) * kStep * splits) splits *= 2;
-    return {rows / tile + sequences, splits, tile, groups * splits <= 256 * (head_dim <= 64 ? 3 : 2)};
+    const int64_t groups = groups_of(tile), most = 256 * (tile == 128 && head_dim <= 64 ? 3 : 2);
+    int32_t splits = static_cast<int32_t>(std::clamp<int64_t>(std::min(most / groups, keys / ((tile == 128 ? 2 : 4) * kStep)), 1, 64));
+    // few pieces join faster: of many rows 9 to 15 cost more than they gain (512 of 12 x 64 over 4,000 keys: 37 us with 10 for 31)
+    if (tile > 16 && splits > kFewPieces && splits < 2 * kFewPieces) splits = kFewPieces;
+    return {rows / tile + sequences, splits, tile, groups * splits <= most};
 }
 
 using AttendFn = void (*)(AttendArgs);
