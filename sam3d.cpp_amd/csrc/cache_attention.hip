@@ -7,8 +7,10 @@
 // power of two that fits its row, as one half-precision number (bfloat16 rows: exact) or
 // as two (float32 rows: 22 bits).  Steps are of a whole block and multiply results.
 //
-// What bounds it: the codes, read once, for few rows; for many the vector
-// instructions beside the products: exponentials, and the codes' way to half precision.
+// What bounds it: few rows, the codes, read once (8 rows over 65,536 keys each, 32 / 8 heads x 128: 188 us, 5.7 TB/s, what a
+// kernel that reads alone reaches); many, products and the vector work beside them (exponentials, maxima, the codes' way to half
+// precision), which hardly overlap: 4 chunks of 1,024 rows behind 8,192 keys, 32 / 8 heads x 128, take 640 us, 0.9 PFLOP/s,
+// matrix units busy 39% and vector issue 50% of a SIMD's cycles.
 #include <cmath>
 
 #include "kv_cache.hpp"
@@ -113,7 +115,7 @@ struct Sight {
 __device__ __forceinline__ Sight sight_of(const AttendArgs &a, const Tile &t, int tok) {
     return {a.causal ? max(0, min(t.keys, tok + t.lag + 1)) : t.keys, a.window ? tok + t.lag - a.window + 1 : 0};
 }
-// What a workgroup computes: tile i of `all` tiles of rows, or none, by a piece of a head's keys.  Of eight (head, piece) each XCD takes one,
+// What a workgroup computes: tile i of n tiles of rows (n: none) by a piece of a head's keys.  Of eight (head, piece) each XCD takes one,
 // whose keys its L2 then holds; the tiles of those left over are dealt out to all XCDs in turn.
 // Workgroups without work stand behind all others.  An XCD's dispatcher fills its shader engines in turn and in order: one without
 // work before it holds a workgroup back until the engine whose turn it is has room (8 sequences of 64 rows x 4 over 20,000 keys: 320 us
@@ -521,8 +523,9 @@ __device__ __forceinline__ uint4 fetch_values32(const uint8_t *codes, int block_
 }
 
 // Few rows: a tile of 16 or 32 of one sequence.  The workgroup's four waves take every fourth step each, and join through LDS.
-// Codes go from memory to a product's registers through two instructions for every four, without LDS; the next step's
-// keys are on their way from the first product on, its values from the last.
+// Memory bounds it, so codes go from there to a product's registers through two instructions for every four, without LDS; the
+// next step's keys are on their way from the first product on, its values from the last.  16 or 32 columns, by the rows there are: 40
+// rows x 4 over 8 x 20,000 keys take 72 us (4.6 TB/s) in tiles of 32 and took 165 in the chunks' of 128.
 template <class T, int D, int COLUMNS>
 __global__ void __launch_bounds__(256, 2) cache_rows_kernel(AttendArgs a) {
     using Q = Query<T, D, COLUMNS>;
@@ -650,8 +653,9 @@ __global__ void __launch_bounds__(256, 2) cache_rows_kernel(AttendArgs a) {
 
 // Many rows: a tile of 128 of one sequence, 32 of them for each of the workgroup's four waves.  A step's codes
 // become half precision once, a quarter of them by each wave, and lie in LDS (two buffers, one barrier a step) as the
-// products' operands, lane by lane: reads and writes are whole rows of 1 KiB.
-//
+// products' operands, lane by lane: reads and writes are whole rows of 1 KiB.  (Straight from memory, as above, every wave turns all
+// codes itself: 4 chunks of 1,024 rows 4,172 us for 640.)  Products of 32x32x16: one holds its SIMD from vector work for about 8
+// cycles whatever its size (of 16x16x32: 686 for 654 us at the time).  Rare cases stand behind the loop, so that nothing in it spills.
 template <class T, int D>
 __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
     using Q = Query<T, D, 32>;
@@ -802,17 +806,13 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
     }
     for (; now.is; advance()) {
         share();
-        __builtin_amdgcn_s_setprio(1);  // products before the other wave's vector work: 677 -> 667 us
         scores(key_rows[buffer]);
-        __builtin_amdgcn_s_setprio(0);
         f = score_unit(q.unit, now.step_k);
         if (t.cut(now.at)) r.hide(w, now.at, q.sight, t.sinks);
         r.settle(w, f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) r.weigh(i, w, f, pw);
-        __builtin_amdgcn_s_setprio(1);
         meet(value_rows[buffer], now.step_v);
-        __builtin_amdgcn_s_setprio(0);
     }
     if (r.again) {
         for (int i = r0; i < min(r0 + 32, t.nrows); ++i) row_by_keys<T, D>(a, t, split, 1, i, kvh);
