@@ -615,7 +615,7 @@ S3DX_API s3dx_status s3dx_block_attention(const void *q, const void *k, const vo
  *   codes  uint8 [pages][kv_heads][2][block * head_dim]: of each head first the keys'
  *          ([block][head_dim]), then the values' ([head_dim][block])
  *   steps  float32 [pages][kv_heads][2] (keys', values'), behind the codes
- * and a code u stands for (u - 128) * step.  head_dim is 32, 64, 96 or 128.  The object is
+ * and a code u stands for (u - 128) * step, 1 <= u <= 255, steps powers of two or 0, from 2^-106 to 2^121.  head_dim is 32, 64, 96 or 128.  The object is
  * host memory alone and may be used by any number of calls at once.
  *
  * Which pages a sequence has is the caller's: table is a DEVICE int32 [sequences][table_stride],
@@ -663,7 +663,8 @@ S3DX_API s3dx_status s3dx_cache_read(const s3dx_cache *cache, void *k, int64_t k
  * Keys and values enter the products as they are held.  A query's channels do so in units of 2^-38 of its row's largest
  * power of two, BF16 ones exactly from 2^-31 of it on, FP32 ones to 22 bits (2^-22 off at most).  Weights meet the values
  * rounded to 11 bits (2^-11 off at most, of either sign), with FP32 queries to 22, and in steps of 2^-31 of the row's largest
- * at most; their sum and lse are of the weights before that.
+ * at most; their sum and lse are of the weights before that.  Rows that meet values' steps more than 2^24 apart, or a score beyond
+ * 2^20 binary orders (7.2e5), are computed again key by key: no less exact, and slower.
  * max_k, the keys of the longest sequence, decides how the work is cut and not what is computed.  The
  * workspace holds partial results where there are too few rows to fill the GPU
  * (s3dx_cache_attention_workspace_size of the same arguments, 0 bytes where none are needed); calls that may run at

@@ -6,7 +6,9 @@
 //   y = x + residual_scale gate . post(branch),   h = pre(y) . (1 + scale) + shift
 //
 // What bounds it: memory.  A row is held in registers between its parts, so that x and
-// branch are read once and y and h written once.
+// branch are read once and y and h written once: 42,000 rows of 768 channels, float32 and
+// bfloat16, take 80 us, 4.8 TB/s of the 5.16 that a large copy reaches; 5,086 rows of 1,024 in bfloat16 11 us of 8,
+// as a launch this short ends in one round of workgroups; a single row is the call.
 #include "common.hpp"
 
 namespace s3dx {
@@ -75,10 +77,10 @@ __device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
 
 // A thread holds PPL pieces of 8 channels, `threads` pieces apart.  Rows need not begin at whole 16 bytes: memory takes
 // 16-byte accesses at any element.  A last, shorter piece begins earlier instead, at the row's last 8 channels; it counts none
-// of its neighbour's in sums, and both store the same (20,000 rows of 333 channels: 31 us element by element).  REST: rows that
+// of its neighbour's in sums, and both store the same (20,000 rows of 333 channels: 21 us, 31 element by element).  REST: rows that
 // have one.  Rows of fewer than 8 channels go one by one.
 // WIDE: a row for each workgroup, of as many waves as leave its threads one piece, two beyond 8,192 channels (registers of more cost
-// the others' places: 20,000 rows of 2,048 channels 136 us in a wave, 86 us so).
+// the others' places: 20,000 rows of 2,048 channels 136 us in a wave, 83 us so).
 template <int PPL, bool WIDE, bool REST>
 __global__ void __launch_bounds__(WIDE ? 1024 : 256) gated_norm_kernel(NormArgs a) {
     __shared__ float across[2][16];
