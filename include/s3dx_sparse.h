@@ -659,7 +659,7 @@ S3DX_API s3dx_status s3dx_cache_read(const s3dx_cache *cache, void *k, int64_t k
  * cache's count for nothing.  o [total_q][heads][head_dim] in dtype by o_stride, overlapping no input;
  * lse (may be NULL): float32 [total_q][heads], the natural logarithm of the row's sum of exp(score).  A row that sees no
  * key, or only scores of -inf, gets zeros and lse -inf; one with a query that is not finite, or with a score past float32's
- * range, NaN.
+ * range, NaN.  softmax_scale is above 0 and below 2^13.
  * Keys and values enter the products as they are held.  A query's channels do so in units of 2^-38 of its row's largest
  * power of two, BF16 ones exactly from 2^-31 of it on, FP32 ones to 22 bits (2^-22 off at most).  Weights meet the values
  * rounded to 11 bits (2^-11 off at most, of either sign), with FP32 queries to 22, and in steps of 2^-31 of the row's largest

@@ -999,7 +999,8 @@ S3DX_API s3dx_status s3dx_cache_attention(const s3dx_cache *cache, const void *q
         require_dtype(dtype);
         require((flags & ~S3DX_BLOCK_CAUSAL) == 0, "unknown flags");
         require(window == 0 || (flags & S3DX_BLOCK_CAUSAL), "a window needs S3DX_BLOCK_CAUSAL");
-        require(softmax_scale > 0.0f && softmax_scale < 1e6f, "softmax_scale must be above 0 and below 1e6");
+        // (a query's unit stays within float32's range)
+        require(softmax_scale > 0.0f && softmax_scale < 8192.0f, "softmax_scale must be above 0 and below 2^13");
         if (total_q == 0 || sequences == 0) return;
         for (const auto &[p, stride] : {std::pair(q, q_stride), std::pair(static_cast<const void *>(o), o_stride)}) {
             require(p && aligned(p, 16), "a row pointer is NULL or not 16-byte aligned");

@@ -63,7 +63,7 @@ ATTEND = dict(cache=0, q=P, dtype=1, total_q=10, heads=4, q_stride=256, q_starts
     (dict(table=None), "table"), (dict(table_stride=2 ** 30), "table_stride"), (dict(lengths=None), "lengths"),
     (dict(sequences=-1), "sequences"), (dict(max_k=-1), "max_k"), (dict(max_k=2 ** 29 + 1), "max_k"), (dict(window=-1), "window"),
     (dict(window=2 ** 29 + 1), "window"), (dict(window=5, flags=0), "CAUSAL"), (dict(sinks=4), "sinks"), (dict(window=9, sinks=-1), "sinks"),
-    (dict(softmax_scale=0.0), "softmax_scale"), (dict(softmax_scale=float("nan")), "softmax_scale"), (dict(softmax_scale=1e6), "softmax_scale"),
+    (dict(softmax_scale=0.0), "softmax_scale"), (dict(softmax_scale=float("nan")), "softmax_scale"), (dict(softmax_scale=1e6), "softmax_scale"), (dict(softmax_scale=8192.0), "softmax_scale"),
     (dict(flags=2), "flags"), (dict(lse=P + 2), "lse"), (dict(total_q=1, max_k=2 ** 20, workspace=None), "workspace"),
     (dict(total_q=1, max_k=2 ** 20, workspace=P + 4), "workspace"), (dict(total_q=1, max_k=2 ** 20, workspace_bytes=64), "workspace"),
     (dict(total_q=2 ** 28, sequences=2 ** 24), "too many")])

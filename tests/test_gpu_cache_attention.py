@@ -294,6 +294,29 @@ def test_other_streams_graphs_and_shared_pages(s3dx):
     graph.close()
 
 
+@pytest.mark.parametrize("new,lens,d", [([1, 1], [3000, 70], 64), ([20], [500], 96), ([150, 3], [200, 900], 128), ([2] * 66, [90] * 66, 32)])
+def test_sequences_that_begin_behind_the_first_row(s3dx, new, lens, d):
+    # rows before the first sequence, as those behind the last, stay as they were
+    rng = np.random.default_rng(d)
+    held, table = K.filled(rng, 2, d, 64, lens)
+    n, before, behind, heads = sum(new), 5, 4, 4
+    q = rng.standard_normal((n, heads, d)).astype(np.float32)
+    bits, q64 = R.stored(s3dx, q, s3dx.BF16)
+    wide = np.full((before + n + behind, heads * d), 0x7FC0, bits.dtype)
+    wide[before:before + n] = bits.reshape(n, -1)
+    cache = s3dx.KvCache(R.dev(s3dx, held.buffer()), held.pages, 2, d, 64)
+    o, lse = R.filled(s3dx, wide.shape, np.uint16, 0x5A), R.filled(s3dx, (len(wide), heads), np.float32, 0x5A)
+    ws = R.filled(s3dx, max(1, cache.attention_workspace_size(len(wide), heads, len(new), max(lens))), np.uint8, 0xFF)
+    cache.attention(R.dev(s3dx, wide), s3dx.BF16, len(wide), heads, R.dev(s3dx, K.starts(new) + before), R.dev(s3dx, table), table.shape[1],
+                    R.dev(s3dx, np.asarray(lens, np.int32)), len(new), max(lens), o, lse, causal=True, workspace=ws)
+    s3dx.synchronize()
+    got, l, raw = R.values(s3dx, o, s3dx.BF16), lse.download(), o.download()
+    for rest in (slice(0, before), slice(before + n, None)):
+        assert np.all(raw[rest] == 0x5A5A) and np.all(l[rest].view(np.uint32) == 0x5A5A5A5A)
+    want = K.attend(q64, held, table, new, lens, float(np.float32(d ** -0.5)), True, 0, 0, True)
+    K.check(s3dx, s3dx.BF16, got[before:before + n].reshape(n, heads, d), l[before:before + n].astype(np.float64), want)
+
+
 def test_the_same_call_gives_the_same_bits(s3dx):
     rng = np.random.default_rng(4)
     for new, lens, heads, kv, d in (([1, 1], [3000, 777], 8, 2, 128), ([60], [900], 4, 2, 64)):

@@ -83,6 +83,40 @@ def test_write_and_read(s3dx, dtype, new, lens, kv, d, block):
         assert np.all(raw[n - 2:].view(np.uint8) == 0x5A) and np.all(np.ascontiguousarray(raw[:, kv * d:]).view(np.uint8) == 0x5A)
 
 
+@pytest.mark.parametrize("seqs", [64, 65])
+@pytest.mark.parametrize("first", [0, 7])
+def test_sequences_by_count_and_by_bound(s3dx, seqs, first):
+    # as many sequences as lanes and one more, some empty, rows before the first one; what none of them has is neither written nor read
+    rng = np.random.default_rng(seqs + first)
+    kv, d = 2, 32
+    new = [int(n) for n in rng.choice([0, 1, 5, 63, 64, 65, 130], seqs)]
+    lens = [n + int(m) for n, m in zip(new, rng.choice([0, 1, 63, 64, 100], seqs))]
+    width = -(-max(lens) // 64)
+    side = Side(s3dx, width * seqs + 1, kv, d, 64)
+    table = rng.permutation(side.held.pages)[: width * seqs].reshape(seqs, width).astype(np.int32)
+    before = [m - n for n, m in zip(new, lens)]
+    side.write(K.rows(rng, sum(before), kv, d), K.rows(rng, sum(before), kv, d), s3dx.BF16, before, before, table)
+    total = first + sum(new) + 3
+    k, v = (K.rows(rng, total, kv, d) for _ in range(2))
+    (kb, k64), (vb, v64) = (R.stored(s3dx, x, s3dx.BF16) for x in (k, v))
+    ds, dt, dl = R.dev(s3dx, K.starts(new) + first), R.dev(s3dx, table), R.dev(s3dx, np.asarray(lens, np.int32))
+    side.cache.write(R.dev(s3dx, kb), R.dev(s3dx, vb), s3dx.BF16, total, ds, dt, width, dl, seqs)
+    out = [R.filled(s3dx, (total, kv * d), np.uint16, 0x5A) for _ in range(2)]
+    side.cache.read(out[0], out[1], s3dx.BF16, total, ds, dt, width, dl, seqs)
+    s3dx.synchronize()
+    here = slice(first, first + sum(new))
+    side.held.write(k64[here], v64[here], new, lens, table)
+    for s, m in enumerate(lens):
+        for j in range(-(-m // 64)):
+            side.touched[:, table[s, j], :, max(0, m - j * 64):] = True
+    side.check()
+    for w in (0, 1):
+        got, raw = R.values(s3dx, out[w], s3dx.BF16), out[w].download()
+        want = np.concatenate([side.held.values(s, m, table)[w][m - n:] for s, (n, m) in enumerate(zip(new, lens))])
+        assert np.array_equal(got[here].reshape(want.shape), want)
+        assert np.all(raw[:first] == 0x5A5A) and np.all(raw[first + sum(new):] == 0x5A5A)
+
+
 @pytest.mark.parametrize("dtype", [0, 1])
 @pytest.mark.parametrize("block", [64, 128])
 def test_row_by_row(s3dx, dtype, block):
