@@ -79,8 +79,8 @@ __device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
 // 16-byte accesses at any element.  A last, shorter piece begins earlier instead, at the row's last 8 channels; it counts none
 // of its neighbour's in sums, and both store the same (20,000 rows of 333 channels: 21 us, 31 element by element).  REST: rows that
 // have one.  Rows of fewer than 8 channels go one by one.
-// WIDE: a row for each workgroup, of as many waves as leave its threads one piece, two beyond 8,192 channels (registers of more cost
-// the others' places: 20,000 rows of 2,048 channels 136 us in a wave, 83 us so).
+// WIDE: a row for each workgroup, of as many waves as leave its threads one piece, two beyond 2,048 channels (20,000 rows of 2,048
+// channels in bfloat16: 136 us in a wave, 86 with two pieces, 83 with one; of 2,600 122 with two, 136 with one).
 template <int PPL, bool WIDE, bool REST>
 __global__ void __launch_bounds__(WIDE ? 1024 : 256) gated_norm_kernel(NormArgs a) {
     __shared__ float across[2][16];
@@ -271,7 +271,7 @@ S3DX_API s3dx_status s3dx_gated_norm_rows(const void *x, int32_t x_dtype, int64_
                       branch_dtype == S3DX_BF16, h_dtype == S3DX_BF16, 0, eps, residual_scale};
         const bool wide = c > 64 * 8 * 2, rest = c % 8 != 0;
         while (!wide && a.lanes_log2 < 6 && (8 << a.lanes_log2) < c) ++a.lanes_log2;
-        const int threads = !wide ? 1 << a.lanes_log2 : std::min((c + 511) / 512 * 64, 1024);
+        const int threads = !wide ? 1 << a.lanes_log2 : c <= 2048 ? (c + 511) / 512 * 64 : (c + 1023) / 1024 * 64;
         const int per = (c + 8 * threads - 1) / (8 * threads), rows = wide ? 1 : 256 / threads, group = wide ? threads : 256;
         const NormFn fn = wide ? (rest ? pick_pieces<true, true>(per) : pick_pieces<true, false>(per))
                                : (rest ? pick_pieces<false, true>(per) : pick_pieces<false, false>(per));
