@@ -25,7 +25,7 @@ struct AttendArgs {
     float *lse;
     const int32_t *q_starts;
     int64_t total_q, q_stride, o_stride, sequences;
-    int32_t heads, group, causal, window, sinks, splits, tile_groups, at_once;
+    int32_t heads, group, causal, window, sinks, splits, tile_groups, at_once, slots;
     float scale;
     float *part_o;    // [splits][total_q][heads][d], divided by their sums
     float4 *part_ml;  // [splits][total_q][heads]: see sum_of
@@ -104,6 +104,7 @@ struct Tile {
     int r0, nrows, keys, lag;            // its first row, the sequence's rows, keys, their difference
     int least, low_all, sinks;           // keys that all rows see: below `least`, and from `low_all` on or below `sinks`
     int steps, sink_steps, skip;
+    int pieces;                          // workgroups that share its keys
     __device__ __forceinline__ int key_of(int step) const { return (step < sink_steps ? step : step + skip) * kStep; }
     // Whether some row of the tile does not see all keys of the step at key `at`.
     __device__ __forceinline__ bool cut(int at) const { return at + kStep > least || (at < low_all && at + kStep > sinks); }
@@ -152,18 +153,61 @@ __device__ __forceinline__ Work work_of(const AttendArgs &a, int n, bool ordered
     return {i, head % a.splits, head / a.splits};
 }
 
+// Few rows of several sequences: workgroups are shared out by the sequences' lengths, each gets about as many steps (a piece a
+// workgroup, `slots` for each head, up to a.splits pieces a tile).  Every lane tries a length of pieces, from the least that could do on,
+// and the first is taken with which all tiles find room; the last lane's is one piece for every tile.  (Reciprocals of hardware are
+// the same in every wave.)
+__device__ __forceinline__ int pieces_of(float steps, float per_length, int most) {
+    return max(1, min(static_cast<int>(ceilf(steps * per_length)), most));
+}
+__device__ __forceinline__ int shared_pieces(const AttendArgs &a, int tiles, float steps) {
+    const int lane = threadIdx.x & 63;
+    float all = 0.0f, longest = 0.0f;
+    const auto of = [](float v, int s) { return as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, v), s)); };
+    for (int s = 0; s < static_cast<int>(a.sequences); ++s) {
+        all += static_cast<float>(__builtin_amdgcn_readlane(tiles, s)) * of(steps, s);
+        longest = fmaxf(longest, of(steps, s));
+    }
+    const float least = fmaxf(4.0f, fmaxf(all * __builtin_amdgcn_rcpf(static_cast<float>(a.slots)), longest * __builtin_amdgcn_rcpf(static_cast<float>(a.splits))));
+    const float per = lane == 63 ? 0.0f : __builtin_amdgcn_rcpf(least * (1.0f + static_cast<float>(lane) * 0.0625f));
+    int room = a.slots;
+    for (int s = 0; s < static_cast<int>(a.sequences); ++s)
+        room -= __builtin_amdgcn_readlane(tiles, s) * pieces_of(of(steps, s), per, a.splits);
+    const int taken = __builtin_ctzll(__builtin_amdgcn_ballot_w64(room >= 0 || lane == 63));
+    return pieces_of(steps, of(per, taken), a.splits);
+}
+
 // A workgroup's rows [r0, r0 + rows) of sequence s; nrows == 0: none.
 __device__ __forceinline__ Tile tile_of(const AttendArgs &a, Work &w, int rows, int rows_log2) {
     Tile t = {};
-    const Sequence q = sequence_at(a.q_starts, a.cache.lengths, a.sequences, a.total_q, a.group, rows_log2, 1, a.tile_groups,
-                                   [&](int32_t n, int32_t) { return (n * a.group >> rows_log2) + ((n * a.group & (rows - 1)) != 0); },
-                                   [&](int64_t all) {
-                                       w = work_of(a, static_cast<int>(min(all, static_cast<int64_t>(a.tile_groups))), a.causal && rows == 128);
-                                       return w.i;
-                                   });
+    int pieces = a.splits;
+    const bool shared = rows != 128 && a.slots > 0;
+    const Sequence q = sequence_at(
+        a.q_starts, a.cache.lengths, a.sequences, a.total_q, a.group, rows_log2, 1, a.tile_groups,
+        [&](int32_t n, int32_t length) {
+            const int tiles = (n * a.group >> rows_log2) + ((n * a.group & (rows - 1)) != 0);
+            if (!shared) return tiles;
+            int keys = cached_rows(a.cache, length);
+            if (a.window) keys = static_cast<int>(min(static_cast<int64_t>(keys), static_cast<int64_t>(a.window) + a.sinks + n + 2 * kStep));
+            pieces = shared_pieces(a, tiles, ceilf(static_cast<float>(keys) * (1.0f / kStep)));
+            return tiles * pieces;
+        },
+        [&](int64_t all) {
+            if (shared) w = {blockIdx.x / a.cache.kv_heads, 0, static_cast<int>(blockIdx.x % a.cache.kv_heads)};
+            else w = work_of(a, static_cast<int>(min(all, static_cast<int64_t>(a.tile_groups))), a.causal && rows == 128);
+            return w.i;
+        });
+    int64_t place = q.unit - q.first;  // (below 2^31 where workgroups are shared out)
+    t.pieces = a.splits;
+    if (shared) {
+        t.pieces = __builtin_amdgcn_readlane(pieces, static_cast<int>(q.s));
+        const int i = static_cast<int>(place) / t.pieces;
+        w.split = static_cast<int>(place) - i * t.pieces;
+        place = i;
+    }
     t.s = q.s;
     t.qs = q.rows;
-    const int64_t first = (q.unit - q.first) << rows_log2;
+    const int64_t first = place << rows_log2;
     t.nrows = t.qs.rows * a.group;  // total_q * heads < 2^31
     if (first < 0 || first >= t.nrows) {
         t.nrows = 0;
@@ -347,8 +391,8 @@ struct Place {
         to = static_cast<T *>(a.o) + token * a.o_stride + static_cast<int64_t>(head) * D;
     }
     // (base + lo: what weights are relative to)
-    __device__ __forceinline__ void sums(const AttendArgs &a, float base, float lo, float total) const {
-        if (a.splits > 1) a.part_ml[part] = sum_of(base, lo, total, 1.0f);
+    __device__ __forceinline__ void sums(const AttendArgs &a, const Tile &t, float base, float lo, float total) const {
+        if (a.splits > 1) a.part_ml[part] = sum_of(base, lo, total, static_cast<float>(t.pieces));
         else if (a.lse) a.lse[cell] = log_of(base, lo, total);
     }
 };
@@ -370,7 +414,7 @@ __device__ __forceinline__ void put(const AttendArgs &a, const Tile &t, int spli
         else if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2 *>(place.to + ch) = u32x2{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3])};
         else *reinterpret_cast<f32x4 *>(place.to + ch) = z;
     }
-    if (g == 0) place.sums(a, base, 0.0f, total);
+    if (g == 0) place.sums(a, t, base, 0.0f, total);
 }
 
 // One row by the whole wave, key by key: of every `splits`-th run of `run` steps, scores with a key per lane, values with a
@@ -394,7 +438,7 @@ __device__ void row_by_keys(const AttendArgs &a, const Tile &t, int split, int r
     for (int w = 0; w < 2; ++w) x[w] = ldexpf(x[w], 14 - e);
     const int room = 32 - __builtin_clz(t.keys | 1);  // weights add up to 1 at most, so that sums of finite values stay finite
     for (int i = 0; i < t.steps; ++i) {
-        if (i / run % a.splits != split) continue;
+        if (i / run % t.pieces != split) continue;
         const int k0 = t.key_of(i), page = page_of(a.cache, t.s, k0 >> a.cache.block_log2);
         if (page < 0) continue;
         const int64_t cell = static_cast<int64_t>(page) * a.cache.kv_heads + kvh;
@@ -447,7 +491,7 @@ __device__ void row_by_keys(const AttendArgs &a, const Tile &t, int split, int r
         if (a.splits > 1) a.part_o[place.part * D + lane + 64 * w] = o[w] * inv;
         else store_from_f32<T>(place.to + lane + 64 * w, o[w] * inv);
     }
-    if (lane == 0) place.sums(a, hi, lo + static_cast<float>(room), total);
+    if (lane == 0) place.sums(a, t, hi, lo + static_cast<float>(room), total);
 }
 
 // A wave's walk over its steps of a tile: pages and steps of 64 of them at a time, one a lane.
@@ -544,7 +588,7 @@ __global__ void __launch_bounds__(256, 2) cache_rows_kernel(AttendArgs a) {
     q.load(a, t, t.r0, kvh);
     S r;
     r.clear();
-    const int piece = split * 4 + wave, pieces = a.splits * 4, block = 1 << a.cache.block_log2, head_bytes = 2 * block * D;
+    const int piece = split * 4 + wave, pieces = t.pieces * 4, block = 1 << a.cache.block_log2, head_bytes = 2 * block * D;
     Walk walk = {-1, 0, 0, 0, make_float2(0.0f, 0.0f), nullptr};
     uint32_t kr[KT][2 * QV];  // two dwords a product
     uint32_t vr[C][W / 4];    // a dword for four keys
@@ -685,7 +729,7 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
         float step_k, step_v;
     };
     const auto next = [&]() __attribute__((always_inline)) {  // the same for all waves
-        Step x = {walk.next(a, t, kvh, split, a.splits, head_bytes), walk.codes, walk.k0, 0.0f, 0.0f};
+        Step x = {walk.next(a, t, kvh, split, t.pieces, head_bytes), walk.codes, walk.k0, 0.0f, 0.0f};
         if (x.is) x.step_k = walk.step_k(), x.step_v = walk.step_v();
         return x;
     };
@@ -826,11 +870,11 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
 
 // The pieces' weights: shares of the whole, so that means of finite values stay finite.  Parts are divided by their sums,
 // zeros where there were no keys; a sum that is a NaN is not 0 and stays.
-constexpr int kFewPieces = 8;
+constexpr int kFewPieces = 16;
 
-// Joins up to kFewPieces pieces of each (row, head), in their order: D / 4 lanes of four channels each, and each for itself the
+// Joins up to N pieces (8 or kFewPieces) of each (row, head), in their order: D / 4 lanes of four channels each, and each for itself the
 // pieces' weights (2,048 rows x 16 heads x 64 in two pieces: 19 us with a wave for each).
-template <class T, int D>
+template <class T, int D, int N>
 __global__ void __launch_bounds__(256) cache_join_few_kernel(AttendArgs a) {
     constexpr int LANES = D == 32 ? 8 : D == 64 ? 16 : 32;
     const int lane = threadIdx.x & (LANES - 1);
@@ -840,29 +884,30 @@ __global__ void __launch_bounds__(256) cache_join_few_kernel(AttendArgs a) {
     const int64_t row = cell / a.heads;
     const int head = static_cast<int>(cell - row * a.heads);
     if (row < a.q_starts[0] || row >= a.q_starts[a.sequences]) return;  // no sequence's (its pieces hold anything)
-    float4 ml[kFewPieces];
-    f32x4 x[kFewPieces];
+    float4 ml[N];
+    f32x4 x[N];
 #pragma unroll
-    for (int p = 0; p < kFewPieces; ++p) {
+    for (int p = 0; p < N; ++p) {
         const int64_t at = min(p, a.splits - 1) * cells + cell;
         ml[p] = a.part_ml[at];
         x[p] = *reinterpret_cast<const f32x4 *>(a.part_o + at * D + 4 * lane);
     }
+    const int pieces = static_cast<int>(ml[0].w);
     float4 top = sum_of(neg_inf(), 0.0f, 0.0f, 0.0f);
-    float w[kFewPieces], total = 0.0f;
+    float w[N], total = 0.0f;
 #pragma unroll
-    for (int p = 0; p < kFewPieces; ++p)
-        if (p < a.splits && ml[p].z != 0.0f && above_of(ml[p], top)) top = ml[p];
+    for (int p = 0; p < N; ++p)
+        if (p < pieces && ml[p].z != 0.0f && above_of(ml[p], top)) top = ml[p];
 #pragma unroll
-    for (int p = 0; p < kFewPieces; ++p) {
-        w[p] = p < a.splits && ml[p].z != 0.0f ? weight_of(ml[p], top) * ml[p].z : 0.0f;
+    for (int p = 0; p < N; ++p) {
+        w[p] = p < pieces && ml[p].z != 0.0f ? weight_of(ml[p], top) * ml[p].z : 0.0f;
         total += w[p];
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     f32x4 o = {0, 0, 0, 0};
 #pragma unroll
-    for (int p = 0; p < kFewPieces; ++p)
-        if (p < a.splits) o += x[p] * (w[p] * inv);
+    for (int p = 0; p < N; ++p)
+        if (p < pieces) o += x[p] * (w[p] * inv);
     T *to = static_cast<T *>(a.o) + row * a.o_stride + static_cast<int64_t>(head) * D + 4 * lane;
     if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2 *>(to) = u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
     else *reinterpret_cast<f32x4 *>(to) = o;
@@ -879,7 +924,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
     const int head = static_cast<int>(cell - row * a.heads);
     // a lane for each piece: its weight
     const float4 none = sum_of(neg_inf(), 0.0f, 0.0f, 0.0f);
-    const float4 mine = lane < a.splits ? a.part_ml[lane * cells + cell] : none;
+    float4 mine = lane < a.splits ? a.part_ml[lane * cells + cell] : none;
     float x[N][2];
 #pragma unroll
     for (int u = 0; u < N; ++u)
@@ -887,6 +932,8 @@ __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
         for (int e = 0; e < 2; ++e)
             x[u][e] = N * wave + u < a.splits && lane + 64 * e < D ? a.part_o[((N * wave + u) * cells + cell) * D + lane + 64 * e] : 0.0f;
     if (row < a.q_starts[0] || row >= a.q_starts[a.sequences]) return;  // no sequence's (its pieces hold anything)
+    const int pieces = static_cast<int>(as_float(__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, mine.w))));
+    if (lane >= pieces) mine = none;
     float4 top = mine.z != 0.0f ? mine : none;
     for (int d = 1; d < 64; d <<= 1) {
         const float4 other = sum_of(__shfl_xor(top.x, d, 64), __shfl_xor(top.y, d, 64), 0.0f, 0.0f);
@@ -900,7 +947,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
     for (int u = 0; u < N; ++u) {
         const float wp = __shfl(share, N * wave + u, 64);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) o[e] += wp * x[u][e];
+        for (int e = 0; e < 2; ++e) o[e] += N * wave + u < pieces ? wp * x[u][e] : 0.0f;
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) part[wave][e][lane] = o[e];
@@ -922,6 +969,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a) {
 struct Cut {
     int64_t tile_groups;
     int32_t splits, rows;  // of a tile
+    int32_t slots;         // workgroups for each key head, shared out by lengths among up to `splits` pieces a tile (0: no such cut)
     bool at_once;          // all workgroups run at once (of sequences of one length; three a unit up to 64 channels, two beyond)
 };
 Cut cut_of(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, int64_t max_k, int32_t window, int32_t sinks, int32_t head_dim) {
@@ -933,9 +981,18 @@ Cut cut_of(int64_t total_q, int32_t heads, int32_t kv_heads, int64_t sequences, 
     const int32_t tile = per <= 16 ? 16 : per <= 64 || groups_of(128) * std::max<int64_t>(keys / (4 * kStep), 1) < 256 ? 32 : 128;
     const int64_t groups = groups_of(tile), most = 256 * (tile == 128 && head_dim <= 64 ? 3 : 2);
     int32_t splits = static_cast<int32_t>(std::clamp<int64_t>(std::min(most / groups, keys / ((tile == 128 ? 2 : 4) * kStep)), 1, 64));
-    // few pieces join faster: of many rows 9 to 15 cost more than they gain (512 of 12 x 64 over 4,000 keys: 37 us with 10 for 31)
+    // single rows of several sequences share workgroups out by length, the long ones up to twice as many as if all were alike, as long
+    // as few are joined, and from 160 MB of codes on (about 30 us).  8 rows over 65,536 keys at most, 32 / 8 heads x 128: lengths
+    // apart 139 us without for 121, alike 190 for 193; 16 x 12 heads x 64 over 8,192 at most 34 for 29; below, 24 x 3,000 x 8 x 32
+    // 17.5 without for 19.6.
+    int64_t slots = 0;
+    if (tile == 16 && splits > 1 && splits <= kFewPieces / 2 && sequences > 1 && sequences <= 64 && groups * keys * 2 * head_dim >= (INT64_C(160) << 20)) {
+        slots = std::max(most / kv_heads, rows / tile + sequences);
+        splits = static_cast<int32_t>(std::min<int64_t>(2 * splits, keys / (4 * kStep)));
+    }
+    // few pieces join faster, a wave's lanes for several rows
     if (tile > 16 && splits > kFewPieces && splits < 2 * kFewPieces) splits = kFewPieces;
-    return {rows / tile + sequences, splits, tile, groups * splits <= most};
+    return {rows / tile + sequences, splits, tile, static_cast<int32_t>(slots), groups * splits <= most};
 }
 
 using AttendFn = void (*)(AttendArgs);
@@ -947,10 +1004,13 @@ template <class T>
 AttendFn pick_attend(int32_t d, const Cut &cut) {
     return d == 32 ? pick_tile<T, 32>(cut) : d == 64 ? pick_tile<T, 64>(cut) : d == 96 ? pick_tile<T, 96>(cut) : pick_tile<T, 128>(cut);
 }
+template <class T, int D>
+AttendFn pick_join_of(int32_t pieces) {
+    return pieces <= 8 ? cache_join_few_kernel<T, D, 8> : pieces <= kFewPieces ? cache_join_few_kernel<T, D, kFewPieces> : cache_join_kernel<T, D>;
+}
 template <class T>
-AttendFn pick_join(int32_t d, bool few) {
-    if (few) return d == 32 ? cache_join_few_kernel<T, 32> : d == 64 ? cache_join_few_kernel<T, 64> : d == 96 ? cache_join_few_kernel<T, 96> : cache_join_few_kernel<T, 128>;
-    return d == 32 ? cache_join_kernel<T, 32> : d == 64 ? cache_join_kernel<T, 64> : d == 96 ? cache_join_kernel<T, 96> : cache_join_kernel<T, 128>;
+AttendFn pick_join(int32_t d, int32_t pieces) {
+    return d == 32 ? pick_join_of<T, 32>(pieces) : d == 64 ? pick_join_of<T, 64>(pieces) : d == 96 ? pick_join_of<T, 96>(pieces) : pick_join_of<T, 128>(pieces);
 }
 
 void check_call(const s3dx_cache *c, int64_t total_q, int32_t heads, int64_t sequences, int64_t max_k, int32_t window, int32_t sinks) {
@@ -1013,14 +1073,14 @@ S3DX_API s3dx_status s3dx_cache_attention(const s3dx_cache *cache, const void *q
         const Cut cut = cut_of(total_q, heads, cache->kv_heads, sequences, max_k, window, sinks, cache->head_dim);
         AttendArgs a = {view_of(cache, table, table_stride, lengths), q, o, lse, q_starts, total_q, q_stride, o_stride, sequences,
                         heads, heads / cache->kv_heads, flags & S3DX_BLOCK_CAUSAL, window, sinks, cut.splits,
-                        static_cast<int32_t>(cut.tile_groups), cut.at_once, softmax_scale, nullptr, nullptr};
+                        static_cast<int32_t>(cut.tile_groups), cut.at_once, cut.slots, softmax_scale, nullptr, nullptr};
         if (cut.splits > 1) {
             require(workspace && aligned(workspace, 16), "workspace is NULL or not 16-byte aligned");
             Carver w(workspace, workspace_bytes);
             a.part_o = w.take<float>(static_cast<uint64_t>(cut.splits) * total_q * heads * cache->head_dim);
             a.part_ml = w.take<float4>(static_cast<uint64_t>(cut.splits) * total_q * heads);
         }
-        const int64_t grid = cut.tile_groups * cache->kv_heads * cut.splits;
+        const int64_t grid = cut.slots ? static_cast<int64_t>(cut.slots) * cache->kv_heads : cut.tile_groups * cache->kv_heads * cut.splits;
         require(grid <= 0xffffffffll / 256, "too many rows and sequences");
         const bool bf = dtype == S3DX_BF16;
         (bf ? pick_attend<uint16_t>(cache->head_dim, cut) : pick_attend<float>(cache->head_dim, cut))<<<
@@ -1030,7 +1090,7 @@ S3DX_API s3dx_status s3dx_cache_attention(const s3dx_cache *cache, const void *q
             const bool few = cut.splits <= kFewPieces;
             const int64_t cells = total_q * heads, each = !few ? 1 : cache->head_dim == 32 ? 32 : cache->head_dim == 64 ? 16 : 8;
             require((cells + each - 1) / each <= 0xffffffffll / 256, "too many rows and heads");
-            (bf ? pick_join<uint16_t>(cache->head_dim, few) : pick_join<float>(cache->head_dim, few))<<<
+            (bf ? pick_join<uint16_t>(cache->head_dim, cut.splits) : pick_join<float>(cache->head_dim, cut.splits))<<<
                 dim3(static_cast<unsigned>((cells + each - 1) / each)), dim3(256), 0, as_stream(stream)>>>(a);
             launch_check("cache attention join");
         }

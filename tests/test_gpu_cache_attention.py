@@ -114,6 +114,30 @@ def test_work_is_cut_by_max_k_and_results_are_not(s3dx, dtype, new, lens, heads,
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("new,lens,heads,kv,d,window,sinks", [
+    ([1] * 8, [5, 0, 3000, 64, 700, 129, 1, 2000], 16, 8, 64, 0, 0),
+    ([1] * 8, [9000] + [100] * 7, 32, 8, 128, 0, 0),                          # one that would take all
+    ([2, 0, 3, 1, 0, 4, 1, 1], [700, 50, 2, 1500, 0, 900, 64, 333], 16, 8, 96, 0, 0),
+    ([40] + [1] * 20, [2000] + [90 * s for s in range(20)], 12, 3, 32, 0, 0),   # several tiles of one
+    ([1] * 64, [1 + 37 * (s * s % 61) for s in range(64)], 4, 1, 64, 0, 0),
+    ([1] * 8, [5000, 40, 3000, 700, 64, 129, 1, 2000], 16, 8, 64, 600, 70),     # (a short window: pieces of one size)
+    ([1] * 8, [14000, 12500, 300, 40, 700, 64, 129, 2000], 8, 8, 128, 11000, 70),
+])
+def test_workgroups_are_shared_out_by_lengths(s3dx, dtype, new, lens, heads, kv, d, window, sinks):
+    # a max_k that speaks of long sequences; then with values' steps that make one sequence's rows go key by key
+    rng = np.random.default_rng(sum(lens))
+    held, table = K.filled(rng, kv, d, 64, lens)
+    q = rng.standard_normal((sum(new), heads, d)).astype(np.float32)
+    got, lse, want = run(s3dx, q, held, table, dtype, new, lens, True, window, sinks, max_k=2 ** 20, behind=2)
+    K.check(s3dx, dtype, got, lse, want)
+    longest = int(np.argmax(lens))
+    blocks = -(-lens[longest] // 64)
+    held.steps[table[longest, :blocks], :, 1] = np.ldexp(1.0, rng.choice([-60, -30, 0], (blocks, 1)))
+    got, lse, want = run(s3dx, q, held, table, dtype, new, lens, True, window, sinks, max_k=2 ** 20, behind=2)
+    K.check(s3dx, dtype, got, lse, want, "far")
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
 @pytest.mark.parametrize("new,lens,d", [([1], [1500], 64), ([40], [700], 128), ([100], [300], 96)])
 def test_pages_that_are_none_count_for_nothing(s3dx, dtype, new, lens, d):
     rng = np.random.default_rng(9)
