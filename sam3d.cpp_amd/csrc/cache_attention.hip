@@ -7,9 +7,9 @@
 // power of two that fits its row, as one half-precision number (bfloat16 rows: exact) or
 // as two (float32 rows: 22 bits).  Steps are of a whole block and multiply results.
 //
-// What bounds it: few rows, the codes, read once (8 rows over 65,536 keys each, 32 / 8 heads x 128: 188 us, 5.7 TB/s, what a
+// What bounds it: few rows, the codes, read once (8 rows over 65,536 keys each, 32 / 8 heads x 128: 191 us, 5.6 TB/s, nearly what a
 // kernel that reads alone reaches); many, products and the vector work beside them (exponentials, maxima, the codes' way to half
-// precision), which hardly overlap: 4 chunks of 1,024 rows behind 8,192 keys, 32 / 8 heads x 128, take 640 us, 0.9 PFLOP/s,
+// precision), which hardly overlap: 4 chunks of 1,024 rows behind 8,192 keys, 32 / 8 heads x 128, take 643 us, 0.9 PFLOP/s,
 // matrix units busy 39% and vector issue 50% of a SIMD's cycles.
 #include <cmath>
 
