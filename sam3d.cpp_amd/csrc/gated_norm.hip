@@ -24,8 +24,9 @@ struct NormArgs {
     float eps, residual_scale;
 };
 
-// Rows whose squares' sum passes 2^128 are summed again smaller; eps is nothing beside them.
-constexpr float kLess = 0x1p-70f;
+// Rows whose sums pass 2^128 are summed again smaller.  They hold a channel, or a difference from the mean, of 2^57 at least (2^14 squares),
+// beside which eps is nothing: 2^-23 then, up to 2^49, and the sums of squares stay from 2^-46 to 2^112.
+constexpr float kLess = 0x1p-80f;
 
 // Sum over a row's threads: 2^lanes_log2 lanes of a wave, or all of a workgroup (`turn`: of sums so far, so that a place in
 // LDS is written again only after a barrier behind its last reader).
@@ -150,23 +151,28 @@ __global__ void __launch_bounds__(WIDE ? 1024 : 256) gated_norm_kernel(NormArgs 
     };
     const auto norm = [&](float (&v)[PPL][8], int kind, const float *w, const float *b) __attribute__((always_inline)) {
         if (kind == S3DX_NORM_NONE) return;
-        float less = 1.0f, mean, rstd;
-        for (;;) {
-            mean = 0.0f;
-            if (kind == S3DX_NORM_LAYER) mean = sum([&](int p, int e) { return v[p][e] * less; }) / static_cast<float>(a.c);
-            const float q = sum([&](int p, int e) {
-                const float d = v[p][e] * less - mean;
+        const float count = static_cast<float>(a.c);
+        const auto mean_of = [&](float times) { return kind == S3DX_NORM_LAYER ? sum([&](int p, int e) { return v[p][e] * times; }) / count : 0.0f; };
+        float mean = mean_of(1.0f), eps = a.eps;
+        const auto squares = [&] {
+            return sum([&](int p, int e) {
+                const float d = v[p][e] - mean;
                 return d * d;
             });
-            // the same for the row's threads (a wave may hold several rows: those that are through wait)
-            if (q < __builtin_inff() || less != 1.0f) {
-                rstd = rsqrtf(q / static_cast<float>(a.c) + (less == 1.0f ? a.eps : 0.0f));
-                break;
-            }
-            less = kLess;
+        };
+        float q = squares();
+        // the same for the row's threads (a wave may hold several rows: those that are through wait)
+        if (!(q < __builtin_inff())) {
+            // the mean in two parts, as the rounding of one may be all the difference that a row of equal channels has
+            const float part = mean_of(kLess);
+            each([&](int p, int e) { v[p][e] = v[p][e] * kLess - part; });
+            mean = mean_of(1.0f);
+            q = squares();
+            eps = 0.0f;
         }
+        const float var = q / count + eps, rstd = var == 0.0f ? 0.0f : rsqrtf(var);
         float g[PPL][8];
-        each([&](int p, int e) { v[p][e] = (v[p][e] * less - mean) * rstd; });
+        each([&](int p, int e) { v[p][e] = (v[p][e] - mean) * rstd; });
         if (w) {
             load(w, 0, false, g);
             each([&](int p, int e) { v[p][e] *= g[p][e]; });

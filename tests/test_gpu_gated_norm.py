@@ -123,6 +123,36 @@ def test_values_of_any_size(s3dx, kind, power, c):
     check(s3dx, 0, 0, *run(s3dx, x, 0.0 * b, 0, 0, 0, 0, kind, mod=False), what=str(power))
 
 
+# The norms of rows whose sums pass float32.  Equal channels have a norm of 0 exactly: their mean is off by at most 39 u of them (sums of
+# 38 terms in a chain, one division), so that channels less this mean are exact and alike, these differences' own mean is off by (39 u)^2 of a
+# channel, far below half its last bit, and they are their mean when it is taken off them in turn.
+@pytest.mark.parametrize("kind", [1, 2])
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("c", [7, 333, 1024, 4097, 5000, 8192, 16384])
+def test_values_up_to_the_types_largest(s3dx, kind, dtype, c):
+    rng = np.random.default_rng(c + kind)
+    n, top = 10, 3.38e38
+    b = rng.standard_normal((n, c)).astype(np.float32)
+    b[1], b[2] = top * rng.choice([-1, 1], c), 1.8e38 * rng.choice([-1, 1], c)
+    b[4], b[5] = top * rng.random(c), np.where(np.arange(c) % 97 == 5, -top, top)
+    b[6], b[7] = 2.0 ** 120 * rng.standard_normal(c), 1e25 * rng.standard_normal(c)
+    b[8] = np.where(np.arange(c) == c // 2, top, 1.0)
+    x = rng.standard_normal((n, c)).astype(np.float32)
+    check(s3dx, dtype, dtype, *run(s3dx, x, b, dtype, dtype, dtype, kind, kind, mod=False, gate=False), what="branch")
+    check(s3dx, dtype, dtype, *run(s3dx, b, 0.0 * b, dtype, dtype, dtype, 0, kind, mod=False), what="stream")
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("c", [1, 200, 333, 1000, 1024, 2600, 5000, 16384])
+def test_equal_channels_beyond_float32s_sums(s3dx, dtype, c):
+    x = np.array([2.0 ** 120, -1.1e36, 3.3e38, -(2.0 ** 127), 1.7e34, 3.0], np.float32)[:, None] * np.ones((6, c), np.float32)
+    zero = np.zeros_like(x)
+    y, h, _ = run(s3dx, x, zero, dtype, dtype, dtype, 0, 1, bias=False, mod=False)
+    assert np.array_equal(y, R.stored(s3dx, x, dtype)[1]) and not h.any()
+    y, h, _ = run(s3dx, zero, x, dtype, dtype, dtype, 1, 1, bias=False, mod=False)
+    assert not y.any() and not h.any()
+
+
 def test_rows_that_are_alike_or_not_finite(s3dx):
     c = 200
     x, b = np.zeros((6, c), np.float32), np.ones((6, c), np.float32)
