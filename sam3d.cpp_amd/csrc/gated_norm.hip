@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(WIDE ? 1024 : 256) gated_norm_kernel(NormArgs 
     if (WIDE && REST) __syncthreads();  // y or h may take the place of what a neighbour's shorter piece reads as well
     norm(v, a.post, a.post_w, a.post_b);
     if (a.gate) {
-        load(a.gate, mods, false, g);
+        if (in) load(a.gate, mods, false, g);  // (there may be no set at all)
         each([&](int p, int e) { v[p][e] *= in ? g[p][e] : 0.0f; });
     }
     each([&](int p, int e) { y[p][e] = fmaf(v[p][e], a.residual_scale, y[p][e]); });

@@ -153,6 +153,27 @@ def test_equal_channels_beyond_float32s_sums(s3dx, dtype, c):
     assert not y.any() and not h.any()
 
 
+@pytest.mark.parametrize("count", [0, 2])
+@pytest.mark.parametrize("c", [5, 96, 1001, 3000])
+def test_rows_of_no_set_fetch_no_vectors(s3dx, count, c):
+    # a table of no sets holds nothing to be fetched: rows outside take gate, scale and shift as 0
+    rng = np.random.default_rng(c + count)
+    n = 21
+    x, b = rng.standard_normal((n, c)).astype(np.float32), rng.standard_normal((n, c)).astype(np.float32)
+    sets = rng.choice([-1, count, 2 ** 31 - 1, -(2 ** 31)] + list(range(count)), n).astype(np.int32)
+    table = (1 + rng.random((max(count, 1), 3, c)) if count else np.ones(1)).astype(np.float32)
+    dx, db, dm, ds = (R.dev(s3dx, a) for a in (x, b, table, sets))
+    y, h = (s3dx.DeviceArray((n, c), np.float32) for _ in range(2))
+    at = lambda j: dm.ptr + 4 * j * c if count else dm.ptr  # noqa: E731
+    s3dx.gated_norm_rows(dx, 0, db, 0, n, c, EPS, y, h, 0, post=1, pre=1, gate=at(0), mod_scale=at(1), mod_shift=at(2), mod_stride=3 * c,
+                         sets=ds, set_count=count)
+    inside = (sets >= 0) & (sets < count)
+    m = np.zeros((n, 3, c)) if not count else np.where(inside[:, None, None], table.astype(np.float64)[np.where(inside, sets, 0)], 0.0)
+    want = K.gated(x.astype(np.float64), b.astype(np.float64), 1, None, None, 1.0, m[:, 0], 1, None, None, m[:, 1], m[:, 2], EPS)
+    check(s3dx, 0, 0, y.download(), h.download(), want, "%d sets" % count)
+    assert np.array_equal(y.download()[~inside], x[~inside])
+
+
 def test_rows_that_are_alike_or_not_finite(s3dx):
     c = 200
     x, b = np.zeros((6, c), np.float32), np.ones((6, c), np.float32)
