@@ -40,6 +40,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = 64;  // keys of a step: half or all of a block
+constexpr uint32_t kInfBits = 0x7f800000u;
 
 // Weights are 2^(score - base), score in binary orders.  A base stands 2^7 below the largest score when it is set
 // and moves once a weight would pass 2^15: half precision keeps its 11 bits of weights down to 2^-21 of the
@@ -261,16 +262,17 @@ struct Query {
             }
         }
         // the row's power: its largest magnitude to [2^14, 2^15).  Magnitudes' bits rise with them, infinities and NaN above
-        // all; their rows keep them, and give NaN.
+        // all; their rows are NaN throughout, so that they give NaN (an infinity alone can make all scores -inf, which weigh nothing).
         if constexpr (G == 4) big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 16, 64)));
         big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 32, 64)));
         const int e = min(max(static_cast<int>(big >> 23) - 127, -100), 127);
         unit = ldexpf(a.scale * kLog2e, e - 14);
+        const float none = big < kInfBits ? 0.0f : __builtin_nanf("");
 #pragma unroll
         for (int j = 0; j < QV; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float u = ldexpf(x[j][2 * i], 14 - e), v = ldexpf(x[j][2 * i + 1], 14 - e);
+                const float u = ldexpf(x[j][2 * i], 14 - e) + none, v = ldexpf(x[j][2 * i + 1], 14 - e) + none;
                 f[j][0][i] = pack_f16x2(u, v);
                 if constexpr (P == 2) {
                     const f32x2 h = unpack_f16x2(f[j][0][i]);
@@ -435,7 +437,7 @@ __device__ void row_by_keys(const AttendArgs &a, const Tile &t, int split, int r
     for (int d = 1; d < 64; d <<= 1) big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), d, 64)));
     const int e = min(max(static_cast<int>(big >> 23) - 127, -100), 127);
 #pragma unroll
-    for (int w = 0; w < 2; ++w) x[w] = ldexpf(x[w], 14 - e);
+    for (int w = 0; w < 2; ++w) x[w] = big < kInfBits ? ldexpf(x[w], 14 - e) : __builtin_nanf("");
     const int room = 32 - __builtin_clz(t.keys | 1);  // weights add up to 1 at most, so that sums of finite values stay finite
     for (int i = 0; i < t.steps; ++i) {
         if (i / run % t.pieces != split) continue;

@@ -348,3 +348,31 @@ def test_the_same_call_gives_the_same_bits(s3dx):
         q = rng.standard_normal((sum(new), heads, d)).astype(np.float32)
         a, b = (run(s3dx, q, held, table, s3dx.BF16, new, lens) for _ in range(2))
         assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("new,lens,d", [([1], [300], 64), ([1, 1], [3000, 64], 128), ([40], [200], 96), ([200], [500], 64)])
+def test_infinite_queries_whose_products_are_all_negative(s3dx, dtype, far, new, lens, d):
+    # their scores are all -inf, and the rows NaN all the same; far: rows that go key by key
+    rng = np.random.default_rng(11)
+    held, table = K.filled(rng, 2, d, 64, lens)
+    held.codes[0, ..., 3] = -1 - np.abs(held.codes[0, ..., 3]) % 127
+    if far:
+        held.steps[..., 1] = np.ldexp(1.0, rng.choice([-60, 0], held.steps[..., 1].shape))
+        held.steps[table[0, 0], :, 1], held.steps[table[0, 1], :, 1] = 2.0 ** -60, 1.0
+    q = rng.standard_normal((sum(new), 4, d)).astype(np.float32)
+    clean = run(s3dx, q, held, table, dtype, new, lens)
+    K.check(s3dx, dtype, *clean)
+    bad = np.zeros((sum(new), 4), bool)
+    for r, h, x in ((0, 1, 1.0), (sum(new) - 1, 2, 1.0), (sum(new) // 2, 3, 1.0)):
+        q[r, h, 3] = x * np.inf
+        bad[r, h] = True
+    with np.errstate(invalid="ignore"):
+        got, lse, _ = run(s3dx, q, held, table, dtype, new, lens)
+    assert np.array_equal(got[~bad], clean[0][~bad]) and np.array_equal(lse[~bad], clean[1][~bad])
+    assert np.all(np.isnan(got[bad])) and np.all(np.isnan(lse[bad]))
+    # pages that are none: nothing is seen, and the rows are zeros
+    with np.errstate(invalid="ignore"):
+        got, lse, _ = run(s3dx, q, held, np.full_like(table, -1), dtype, new, lens)
+    assert not got.any() and np.all(lse == -np.inf)
