@@ -153,6 +153,23 @@ def test_equal_channels_beyond_float32s_sums(s3dx, dtype, c):
     assert not y.any() and not h.any()
 
 
+@pytest.mark.parametrize("c", [5, 200, 333, 1000, 1024, 2600, 5000, 16384])
+def test_channels_that_are_nearly_alike(s3dx, c):
+    size = np.array([100.7, -3.7, 1e-3, 12345.678, -1e10, 1.3e20, 1e30, 1e-30], np.float32)
+    x = size[:, None] * np.ones((8, c), np.float32)
+    zero = np.zeros_like(x)
+    for dtype in (s3dx.F32, s3dx.BF16):
+        y, h, _ = run(s3dx, x, zero, dtype, dtype, dtype, 0, 1, bias=False, mod=False)
+        assert np.array_equal(y, R.stored(s3dx, x, dtype)[1]) and not h.any()  # as above
+    # Channels apart by a few of their last bits.  Differences from a first mean are exact, whole last bits, and what is left to round is
+    # their own mean, their differences from that and the root: no more than the bound of these rows less one of their channels.
+    rng = np.random.default_rng(c)
+    near = np.ldexp(1.0 + 2.0 ** -23 * rng.integers(5, 12, (8, c)), rng.integers(-20, 90, (8, 1)))
+    got = run(s3dx, near.astype(np.float32), zero, 0, 0, 0, 0, 1, gain=False, bias=False, mod=False)[1]
+    want, off = K.normed(near - near[:, :1], K.LAYER, None, None, EPS)
+    assert np.all(np.abs(got - want) <= off + R.U32 * (np.abs(want) + off) + 1e-37)
+
+
 @pytest.mark.parametrize("count", [0, 2])
 @pytest.mark.parametrize("c", [5, 96, 1001, 3000])
 def test_rows_of_no_set_fetch_no_vectors(s3dx, count, c):
