@@ -262,21 +262,23 @@ struct Query {
             }
         }
         // the row's power: its largest magnitude to [2^14, 2^15).  Magnitudes' bits rise with them, infinities and NaN above
-        // all; their rows are NaN throughout, so that they give NaN (an infinity alone can make all scores -inf, which weigh nothing).
+        // all; their rows give NaN: one term is NaN throughout (an infinity alone can make all scores -inf, which weigh nothing), of two the
+        // second is where they stand.
         if constexpr (G == 4) big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 16, 64)));
         big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 32, 64)));
         const int e = min(max(static_cast<int>(big >> 23) - 127, -100), 127);
         unit = ldexpf(a.scale * kLog2e, e - 14);
-        const float none = big < kInfBits ? 0.0f : __builtin_nanf("");
 #pragma unroll
         for (int j = 0; j < QV; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float u = ldexpf(x[j][2 * i], 14 - e) + none, v = ldexpf(x[j][2 * i + 1], 14 - e) + none;
+                const float u = ldexpf(x[j][2 * i], 14 - e), v = ldexpf(x[j][2 * i + 1], 14 - e);
                 f[j][0][i] = pack_f16x2(u, v);
                 if constexpr (P == 2) {
                     const f32x2 h = unpack_f16x2(f[j][0][i]);
                     f[j][1][i] = pack_f16x2(u - h[0], v - h[1]);
+                } else {
+                    f[j][0][i] = big < kInfBits ? f[j][0][i] : 0x7e007e00u;
                 }
             }
     }
