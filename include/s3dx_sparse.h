@@ -657,9 +657,10 @@ S3DX_API s3dx_status s3dx_cache_read(const s3dx_cache *cache, void *k, int64_t k
  * reading key head h / (heads / kv_heads).  With S3DX_BLOCK_CAUSAL a row at place p sees places up to p; with
  * window > 0 (causal only) those from p - window + 1 on, and of the ones before them the first `sinks`.  Keys on pages that are not the
  * cache's count for nothing.  o [total_q][heads][head_dim] in dtype by o_stride, overlapping no input;
- * lse (may be NULL): float32 [total_q][heads], the natural logarithm of the row's sum of exp(score).  A row that sees no
- * key, or only scores of -inf, gets zeros and lse -inf; one with a query that is not finite, or with a score past float32's
- * range, NaN.  softmax_scale is above 0 and below 2^13.
+ * lse (may be NULL): float32 [total_q][heads], the natural logarithm of the row's sum of exp(score).  Scores are float32: one
+ * below its range counts as -inf and weighs nothing.  A row that sees no key, or only scores of -inf, gets zeros and lse -inf; one
+ * that sees a key and has a query that is not finite, or a score above float32's range, NaN (also for a score of 0 in a block
+ * where 2^(e-14) * softmax_scale / ln 2 * step, 2^e the query's largest power of two, is above it).  softmax_scale is above 0 and below 2^13.
  * Keys and values enter the products as they are held.  A query's channels do so in units of 2^-38 of its row's largest
  * power of two, BF16 ones exactly from 2^-31 of it on, FP32 ones to 22 bits (2^-22 off at most).  Weights meet the values
  * rounded to 11 bits (2^-11 off at most, of either sign), with FP32 queries to 22, and in steps of 2^-31 of the row's largest

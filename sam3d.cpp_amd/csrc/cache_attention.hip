@@ -471,7 +471,7 @@ __device__ void row_by_keys(const AttendArgs &a, const Tile &t, int split, int r
             hi = h;
             lo = l;
         }
-        const float p = hidden ? 0.0f : exp2f(hi == neg_inf() ? s : (fmaf(s, f, -hi) - lo) - static_cast<float>(room));
+        const float p = hidden ? 0.0f : exp2f(hi == neg_inf() ? s * f : (fmaf(s, f, -hi) - lo) - static_cast<float>(room));
         float all = p;
         for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d, 64);
         total += all;

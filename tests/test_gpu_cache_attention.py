@@ -376,3 +376,42 @@ def test_infinite_queries_whose_products_are_all_negative(s3dx, dtype, far, new,
     with np.errstate(invalid="ignore"):
         got, lse, _ = run(s3dx, q, held, np.full_like(table, -1), dtype, new, lens)
     assert not got.any() and np.all(lse == -np.inf)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("new,lens,d", [([1], [300], 64), ([1, 1], [3000, 64], 128), ([40], [200], 96), ([200], [500], 64)])
+def test_scores_beyond_float32(s3dx, dtype, far, new, lens, d):
+    # products of -1 and -2 in units of 2^200: below float32's range they weigh nothing, above it they make a row NaN; far: rows that go
+    # key by key
+    rng = np.random.default_rng(13)
+    held, table = K.filled(rng, 2, d, 64, lens)
+    held.codes[0], held.steps[..., 0] = 0, 2.0 ** 100
+    held.codes[0, ..., 1] = -rng.integers(1, 3, held.codes.shape[1:4])
+    held.codes[0, ..., 2] = 0
+    if far:
+        held.steps[..., 1] = np.ldexp(1.0, rng.choice([-60, 0], held.steps[..., 1].shape))
+        held.steps[table[0, 0], :, 1], held.steps[table[0, 1], :, 1] = 2.0 ** -60, 1.0
+    q = np.zeros((sum(new), 4, d), np.float32)
+    q[..., 0], q[..., 1] = 2.0 ** 120, 2.0 ** 100
+    with np.errstate(all="ignore"):
+        got, lse, _ = run(s3dx, q, held, table, dtype, new, lens)
+        assert not got.any() and np.all(lse == -np.inf)
+        q[0, 1, 1] = -(2.0 ** 100)
+        got, lse, _ = run(s3dx, q, held, table, dtype, new, lens)
+        assert np.all(np.isnan(got[0, 1])) and np.isnan(lse[0, 1])
+        got[0, 1], lse[0, 1] = 0.0, -np.inf
+        assert not got.any() and np.all(lse == -np.inf)
+        # beside keys whose scores float32 holds they count for nothing: the mean of those keys' values
+        here = table[0, 0]
+        held.codes[0, here], held.steps[here, :, 0] = 0, 2.0 ** -6
+        got, lse, _ = run(s3dx, q, held, table, dtype, new, lens, causal=False)
+    mean = (held.codes[1, here, :, : min(64, lens[0])] * held.steps[here, :, 1, None, None]).mean(1)
+    size = (np.abs(held.codes[1, here, :, : min(64, lens[0])]) * held.steps[here, :, 1, None, None]).mean(1)
+    for r in range(new[0]):
+        for h in range(4):
+            if (r, h) == (0, 1):
+                continue
+            # weights are equal powers of two; sums of 64 terms; a logarithm of up to 16 to its last bit, times ln 2, and a sum
+            assert np.all(np.abs(got[r, h] - mean[h // 2]) <= R.half_step(s3dx, dtype) * np.abs(mean[h // 2]) * 1.01 + 80 * R.U32 * size[h // 2])
+            assert abs(lse[r, h] - np.log(64)) <= 2.0 ** -20 + 2.0 ** -21 + 4 * R.U32
