@@ -81,10 +81,10 @@ __device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
 
 // A thread holds PPL pieces of 8 channels, `threads` pieces apart.  Rows need not begin at whole 16 bytes: memory takes
 // 16-byte accesses at any element.  A last, shorter piece begins earlier instead, at the row's last 8 channels; it counts none
-// of its neighbour's in sums, and both store the same (20,000 rows of 333 channels: 21 us, 31 element by element).  REST: rows that
+// of its neighbour's in sums, and both store the same (20,000 rows of 333 channels: 20 us, 31 element by element).  REST: rows that
 // have one.  Rows of fewer than 8 channels go one by one.
 // WIDE: a row for each workgroup, of as many waves as leave its threads one piece, two beyond 2,048 channels (20,000 rows of 2,048
-// channels in bfloat16: 136 us in a wave, 86 with two pieces, 83 with one; of 2,600 122 with two, 136 with one).
+// channels in bfloat16: 136 us in a wave, 86 with two pieces, 83 with one; of 2,600 121 with two, 136 with one).
 template <int PPL, bool WIDE, bool REST>
 __global__ void __launch_bounds__(WIDE ? 1024 : 256) gated_norm_kernel(NormArgs a) {
     __shared__ float across[2][16];
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(WIDE ? 1024 : 256) gated_norm_kernel(NormArgs 
         // the same for the row's threads (a wave may hold several rows: those that are through wait)
         const bool over = !(q < __builtin_inff());
         const float beside = mean * kAlike;
-        if (over || q / count < beside * beside) {
+        if (over || (kind == S3DX_NORM_LAYER && q / count <= beside * beside)) {
             // the mean in two parts, as the rounding of one may be all the difference that channels have
             const float less = over ? kLess : 1.0f, part = mean_of(less);
             each([&](int p, int e) { v[p][e] = v[p][e] * less - part; });

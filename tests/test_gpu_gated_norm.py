@@ -155,8 +155,8 @@ def test_equal_channels_beyond_float32s_sums(s3dx, dtype, c):
 
 @pytest.mark.parametrize("c", [5, 200, 333, 1000, 1024, 2600, 5000, 16384])
 def test_channels_that_are_nearly_alike(s3dx, c):
-    size = np.array([100.7, -3.7, 1e-3, 12345.678, -1e10, 1.3e20, 1e30, 1e-30], np.float32)
-    x = size[:, None] * np.ones((8, c), np.float32)
+    size = np.array([100.7, -3.7, 1e-3, 12345.678, -1e10, 1.3e20, 1e30, 1e-30, 1.37e-30, -1.9e-20, 7.3e-13, 1.1e-37], np.float32)
+    x = size[:, None] * np.ones((len(size), c), np.float32)
     zero = np.zeros_like(x)
     for dtype in (s3dx.F32, s3dx.BF16):
         y, h, _ = run(s3dx, x, zero, dtype, dtype, dtype, 0, 1, bias=False, mod=False)
@@ -165,7 +165,7 @@ def test_channels_that_are_nearly_alike(s3dx, c):
     # their own mean, their differences from that and the root: no more than the bound of these rows less one of their channels.
     rng = np.random.default_rng(c)
     near = np.ldexp(1.0 + 2.0 ** -23 * rng.integers(5, 12, (8, c)), rng.integers(-20, 90, (8, 1)))
-    got = run(s3dx, near.astype(np.float32), zero, 0, 0, 0, 0, 1, gain=False, bias=False, mod=False)[1]
+    got = run(s3dx, near.astype(np.float32), zero[:8], 0, 0, 0, 0, 1, gain=False, bias=False, mod=False)[1]
     want, off = K.normed(near - near[:, :1], K.LAYER, None, None, EPS)
     assert np.all(np.abs(got - want) <= off + R.U32 * (np.abs(want) + off) + 1e-37)
 
