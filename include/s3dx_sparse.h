@@ -690,8 +690,9 @@ S3DX_API s3dx_status s3dx_cache_attention(const s3dx_cache *cache, const void *q
  * that they may lie side by side in one projection's output; a row's set is
  * sets[row*set_stride] (int32; the batch of voxel coordinates: coords, stride 4), or 0 for all
  * rows where sets is NULL.  Rows with a set outside [0, set_count) take gate, scale and shift as 0 (those that
- * are given).  x and y are in x_dtype, 1 <= c <= 16384; strides in elements, any.  h is
- * of y before its rounding; h NULL: the sum alone, without pre.  All in float32, each output rounded once.  y and h may
+ * are given; no channel of theirs is read).  x and y are in x_dtype, 1 <= c <= 16384; strides in elements, any.  h is
+ * of y before its rounding; h NULL: the sum alone, without pre.  All in float32, each output rounded once; norms hold for finite rows of any
+ * size (rows whose sums pass float32 without eps, which is nothing beside them), and equal channels have a layer norm of 0.  y and h may
  * be x or branch (same dtype and stride) and overlap nothing otherwise. */
 #define S3DX_NORM_NONE 0
 #define S3DX_NORM_LAYER 1

@@ -7,9 +7,9 @@
 // power of two that fits its row, as one half-precision number (bfloat16 rows: exact) or
 // as two (float32 rows: 22 bits).  Steps are of a whole block and multiply results.
 //
-// What bounds it: few rows, the codes, read once (8 rows over 65,536 keys each, 32 / 8 heads x 128: 191 us, 5.6 TB/s, nearly what a
+// What bounds it: few rows, the codes, read once (8 rows over 65,536 keys each, 32 / 8 heads x 128: 193 us, 5.6 TB/s, nearly what a
 // kernel that reads alone reaches); many, products and the vector work beside them (exponentials, maxima, the codes' way to half
-// precision), which hardly overlap: 4 chunks of 1,024 rows behind 8,192 keys, 32 / 8 heads x 128, take 643 us, 0.9 PFLOP/s,
+// precision), which hardly overlap: 4 chunks of 1,024 rows behind 8,192 keys, 32 / 8 heads x 128, take 640 us, 0.9 PFLOP/s,
 // matrix units busy 39% and vector issue 50% of a SIMD's cycles.
 #include <cmath>
 
@@ -573,7 +573,8 @@ __device__ __forceinline__ uint4 fetch_values32(const uint8_t *codes, int block_
 // Few rows: a tile of 16 or 32 of one sequence.  The workgroup's four waves take every fourth step each, and join through LDS.
 // Memory bounds it, so codes go from there to a product's registers through two instructions for every four, without LDS; the
 // next step's keys are on their way from the first product on, its values from the last.  16 or 32 columns, by the rows there are: 40
-// rows x 4 over 8 x 20,000 keys take 72 us (4.6 TB/s) in tiles of 32 and took 165 in the chunks' of 128.
+// rows x 4 over 8 x 20,000 keys take 73 us (4.5 TB/s) in tiles of 32 and took 165 in the chunks' of 128.  (At 128 channels tiles of 32 fill the
+// registers and spill 10 of them, 39 of float32 rows, which take 101 us.)
 template <class T, int D, int COLUMNS>
 __global__ void __launch_bounds__(256, 2) cache_rows_kernel(AttendArgs a) {
     using Q = Query<T, D, COLUMNS>;
@@ -877,7 +878,7 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
 constexpr int kFewPieces = 16;
 
 // Joins up to N pieces (8 or kFewPieces) of each (row, head), in their order: D / 4 lanes of four channels each, and each for itself the
-// pieces' weights (2,048 rows x 16 heads x 64 in two pieces: 19 us with a wave for each).
+// pieces' weights.  Places of all pieces that there may be are fetched at once, those that a row has not (by its first one) then left out (2,048 rows x 16 heads x 64 in two pieces: 19 us with a wave for each).
 template <class T, int D, int N>
 __global__ void __launch_bounds__(256) cache_join_few_kernel(AttendArgs a) {
     constexpr int LANES = D == 32 ? 8 : D == 64 ? 16 : 32;
