@@ -878,7 +878,8 @@ __global__ void __launch_bounds__(256, 2) cache_chunk_kernel(AttendArgs a) {
 constexpr int kFewPieces = 16;
 
 // Joins up to N pieces (8 or kFewPieces) of each (row, head), in their order: D / 4 lanes of four channels each, and each for itself the
-// pieces' weights.  Places of all pieces that there may be are fetched at once, those that a row has not (by its first one) then left out (2,048 rows x 16 heads x 64 in two pieces: 19 us with a wave for each).
+// pieces' weights (2,048 rows x 16 heads x 64 in two pieces: 19 us with a wave for each).  Places of all pieces that there may be are
+// fetched at once; those that a row has not, as its first one says, are left out.
 template <class T, int D, int N>
 __global__ void __launch_bounds__(256) cache_join_few_kernel(AttendArgs a) {
     constexpr int LANES = D == 32 ? 8 : D == 64 ? 16 : 32;

@@ -25,7 +25,8 @@ struct NormArgs {
 };
 
 // Rows whose sums pass 2^128 are summed again smaller.  They hold a channel, or a difference from the mean, of 2^57 at least (2^14 squares),
-// beside which eps is nothing: 2^-23 then, up to 2^49, and the sums of squares stay from 2^-46 to 2^112.
+// beside which eps is nothing: 2^-23 then, up to 2^49, and the sums of squares stay from 2^-46 to 2^112.  (Where the difference was the mean's
+// rounding alone, channels are 2^75 at least and differ, if they do, by 2^52: 2^-28 then.)
 constexpr float kLess = 0x1p-80f;
 // A mean is off by some 2^-24 of itself, which rows whose channels differ by less than this share of it take for a difference: of equal
 // channels of 100.7 the norm came out as 0.015 and of 1e10 as 1, for 0.
